@@ -30,12 +30,16 @@
 /* 1: first release; 2: plan options xcd_split .. hot_rows, reorder minhash, wider plan stats;
  * 3: struct_size fields and the stats size argument; 4: the GPU format builder
  * (trs_build_online_device, trs_dformat_*) and plans from its output (trs_plan_create_dformat,
- * trs_plan_create_sddmm_dformat); struct layouts as in 3. */
-#define TRSPMM_ABI_VERSION 4
+ * trs_plan_create_sddmm_dformat); struct layouts as in 3; 5: the dense operators (trs_embed ..
+ * trs_matmul_i8), struct layouts as in 3. */
+#define TRSPMM_ABI_VERSION 5
 
 #ifdef __cplusplus
 extern "C" {
 #endif
+
+/* element types of the dense operators */
+typedef enum trs_dtype { TRS_F32 = 0, TRS_F16 = 1, TRS_BF16 = 2 } trs_dtype;
 
 typedef enum trs_status {
   TRS_OK = 0,
@@ -467,6 +471,67 @@ int trs_spmm_f16_kernel_ms(const trs_plan* p, const uint16_t* B, int64_t ldb, in
 int trs_sddmm_f16_kernel_ms(const trs_plan* p, const uint16_t* X, int64_t ldx, const uint16_t* Y,
                             int64_t ldy, int32_t K, float* out, void* workspace, int64_t workspace_bytes,
                             void* stream, int32_t iters, float* ms);
+
+/* ---------------------------------------------------------------------------------------------
+ * Dense operators beside the sparse products: what a layer does to the features before and after
+ * the SpMM.  No reference counterparts (the reference multiplies by the graph only).
+ *
+ * Matrices are row-major with a leading dimension (elements between rows, at least the width) and
+ * start at any element; types are trs_dtype.  Sums, norms and scales are held in 32 bits and
+ * rounded once when written.  Calls launch kernels only (no memset nodes, no allocation, no
+ * synchronisation), so they can be captured in a HIP graph; equal inputs give equal bits.  They run
+ * on the current device, which must hold the operands.  A call with no rows or no width launches
+ * nothing it need not.
+ * ------------------------------------------------------------------------------------------- */
+/* out[t] = scale * table[ids[t]] for t < count: table [rows, width], out [count, width].  ids are
+ * int32 (id_bits 32) or int64 (64); one outside [0, rows) (a padded slot) gives a row of zeros.
+ * out must not overlap table.  scale is finite (TRS_EINVAL otherwise). */
+int trs_embed(const void* table, int32_t table_type, int64_t ldt, int64_t rows, const void* ids, int32_t id_bits,
+              int64_t count, int32_t width, float scale, void* out, int32_t out_type, int64_t ldo, void* stream);
+
+/* The gradient of trs_embed towards its table: out[v] = scale * sum over t with ids[t] = v of
+ * grad[t], for every row v < rows (zeros where no id names it; ids outside [0, rows) take no part).
+ * out is written whole.  The ids are sorted in the workspace, equal ones summed in the order they
+ * come in, in 32 bits.  count and rows below 2^31 - 1 (TRS_ERANGE otherwise). */
+int64_t trs_embed_grad_workspace_bytes(int64_t count, int64_t rows, int32_t width);
+int trs_embed_grad(const void* grad, int32_t grad_type, int64_t ldg, const void* ids, int32_t id_bits, int64_t count,
+                   int64_t rows, int32_t width, float scale, void* out, int32_t out_type, int64_t ldo, void* workspace,
+                   int64_t workspace_bytes, void* stream);
+
+/* h = x + residual, r_out = h in the residual's type, y = h / sqrt(mean(h^2) + eps) * weight, row by
+ * row.  The norm is that of the 32-bit sum, before its rounding to r_out.  residual may be NULL,
+ * r_out then too.  x and residual are of the same type, or one of them is TRS_F32; weight and y are
+ * of any type.  r_out may be residual itself; no other output may overlap an input.  eps > 0. */
+int trs_rms_norm(const void* x, int32_t x_type, int64_t ldx, const void* residual, int32_t r_type, int64_t ldr,
+                 const void* weight, int32_t w_type, float eps, int64_t rows, int32_t width, void* y, int32_t y_type,
+                 int64_t ldy, void* r_out, int64_t ldro, void* stream);
+
+/* trs_rms_norm with y in 8 bits: scale[row] = max|y| / 127, q = y / scale rounded to nearest even, in
+ * [-127, 127].  A row of zeros (or below 2^-119) has scale 0 and codes 0; a row that holds a NaN or
+ * an infinity has scale NaN and codes 0. */
+int trs_rms_norm_i8(const void* x, int32_t x_type, int64_t ldx, const void* residual, int32_t r_type, int64_t ldr,
+                    const void* weight, int32_t w_type, float eps, int64_t rows, int32_t width, int8_t* q, int64_t ldq,
+                    float* scale, void* r_out, int64_t ldro, void* stream);
+
+/* The gradient of trs_rms_norm from grad (that of y) and r (r_out of the forward call, or its x where
+ * it had no residual): dr, of r's type, is the gradient of x and of the residual alike, with grad_r
+ * (that of r_out, of r's type; NULL: none) added; dweight [width] in float32 is summed over the rows
+ * in a fixed order.  grad and r are of the same type, or one of them is TRS_F32.  dr must not
+ * overlap an input, but may be grad_r. */
+int64_t trs_rms_norm_grad_workspace_bytes(int64_t rows, int32_t width);
+int trs_rms_norm_grad(const void* grad, int32_t grad_type, int64_t ldg, const void* r, int32_t r_type, int64_t ldr,
+                      const void* weight, int32_t w_type, const void* grad_r, int64_t ldgr, float eps, int64_t rows,
+                      int32_t width, void* dr, int64_t lddr, float* dweight, void* workspace, int64_t workspace_bytes,
+                      void* stream);
+
+/* out[i, j] = a_scale[i] * w_scale[j] * sum over k of a[i, k] * w[j, k] + bias[j]: codes a [m, k] (what
+ * trs_rms_norm_i8 writes) and weights w [n, k] in int8, scales in float32, bias in float32 or NULL.
+ * The sums are exact 32-bit integers (any codes, -128 too); k at most 131071 (TRS_ERANGE
+ * otherwise).  The workspace, where its size is not 0, holds sums of shares of k. */
+int64_t trs_matmul_i8_workspace_bytes(int64_t m, int32_t n, int32_t k);
+int trs_matmul_i8(const int8_t* a, int64_t lda, const float* a_scale, const int8_t* w, int64_t ldw, const float* w_scale,
+                  const float* bias, int64_t m, int32_t n, int32_t k, void* out, int32_t out_type, int64_t ldo,
+                  void* workspace, int64_t workspace_bytes, void* stream);
 
 const char* trs_last_error(void);
 

@@ -1,0 +1,103 @@
+// Shared by the dense operators beside the sparse products (embed.hip, norm.hip, matmul_i8.hip):
+// element types, eight-element chunks of a row at any address, argument checks.
+//
+// Rows are handled in chunks of 8 elements.  A row whose width 8 does not divide ends in a chunk that
+// starts at width - 8 and overlaps its neighbour: both compute the same values for the shared
+// elements and store them twice, and a sum leaves the duplicates out (chunk_at).  So every load and
+// store is a whole vector; only rows narrower than 8 go element by element.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+#include <cstdint>
+#include <string>
+
+#include "trspmm.h"
+
+namespace trs {
+void set_error(const std::string& msg);
+
+namespace dense {
+
+inline int fail(int code, const std::string& msg) {
+  set_error(msg);
+  return code;
+}
+
+inline int launched(const char* where) {
+  const hipError_t e = hipGetLastError();
+  if (e == hipSuccess) return TRS_OK;
+  return fail(TRS_EDEVICE, std::string(where) + ": kernel launch failed: " + hipGetErrorString(e));
+}
+
+inline bool known_type(int32_t t) { return t == TRS_F32 || t == TRS_F16 || t == TRS_BF16; }
+
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+inline int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
+
+// A launch holds less than 2^32 threads along a dimension.
+inline bool fits_grid(int64_t blocks, int threads = 256) { return blocks * threads <= (int64_t)UINT32_MAX; }
+
+// Storage types.  bfloat16 is kept as its bits; float -> bfloat16 rounds to nearest even (the
+// compiler's own conversion instruction on gfx950).
+struct f32_t { using raw = float; static constexpr int code = TRS_F32; };
+struct f16_t { using raw = _Float16; static constexpr int code = TRS_F16; };
+struct bf16_t { using raw = __bf16; static constexpr int code = TRS_BF16; };
+
+template <class T, int N>
+struct vec_of { typedef typename T::raw type __attribute__((ext_vector_type(N))); };
+
+// N consecutive elements at any element address (gfx950 loads and stores vectors at their element's
+// alignment).
+template <class T, int N>
+__device__ __forceinline__ void load_vec(const typename T::raw* p, float (&v)[N]) {
+  typedef typename vec_of<T, N>::type V;
+  typedef V U __attribute__((aligned(sizeof(typename T::raw))));
+  const V x = *reinterpret_cast<const U*>(p);
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = (float)x[i];
+}
+
+template <class T, int N>
+__device__ __forceinline__ void store_vec(typename T::raw* p, const float (&v)[N]) {
+  typedef typename vec_of<T, N>::type V;
+  typedef V U __attribute__((aligned(sizeof(typename T::raw))));
+  V x;
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i] = (typename T::raw)v[i];
+  *reinterpret_cast<U*>(p) = x;
+}
+
+// A chunk of 8 elements of a row of `width`; narrower rows (n < 8 elements) element by element, the
+// rest of the chunk zero.
+template <class T>
+__device__ __forceinline__ void load_chunk(const typename T::raw* p, int n, float (&v)[8]) {
+  if (n >= 8) {
+    load_vec<T, 8>(p, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? (float)p[i] : 0.f;
+  }
+}
+
+template <class T>
+__device__ __forceinline__ void store_chunk(typename T::raw* p, int n, const float (&v)[8]) {
+  if (n >= 8) {
+    store_vec<T, 8>(p, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) p[i] = (typename T::raw)v[i];
+  }
+}
+
+// First element of chunk c of a row of `width`, and how many of its elements the chunk before holds too.
+__device__ __forceinline__ int chunk_at(int c, int width, int& shared) {
+  const int at = 8 * c, last = width - 8;
+  const int s = at > last ? (last > 0 ? last : 0) : at;
+  shared = at - s;
+  return s;
+}
+
+}  // namespace dense
+}  // namespace trs
