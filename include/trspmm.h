@@ -527,11 +527,10 @@ int trs_rms_norm_grad(const void* grad, int32_t grad_type, int64_t ldg, const vo
 /* out[i, j] = a_scale[i] * w_scale[j] * sum over k of a[i, k] * w[j, k] + bias[j]: codes a [m, k] (what
  * trs_rms_norm_i8 writes) and weights w [n, k] in int8, scales in float32, bias in float32 or NULL.
  * The sums are exact 32-bit integers (any codes, -128 too); k at most 131071 (TRS_ERANGE
- * otherwise).  The workspace, where its size is not 0, holds sums of shares of k. */
-int64_t trs_matmul_i8_workspace_bytes(int64_t m, int32_t n, int32_t k);
+ * otherwise). */
 int trs_matmul_i8(const int8_t* a, int64_t lda, const float* a_scale, const int8_t* w, int64_t ldw, const float* w_scale,
                   const float* bias, int64_t m, int32_t n, int32_t k, void* out, int32_t out_type, int64_t ldo,
-                  void* workspace, int64_t workspace_bytes, void* stream);
+                  void* stream);
 
 const char* trs_last_error(void);
 

@@ -7,7 +7,6 @@ import torch
 
 import trspmm
 from trspmm import _native as nat
-from trspmm import dense
 
 pytestmark = pytest.mark.gpu
 
@@ -78,7 +77,9 @@ def test_channels(n):
 
 
 @pytest.mark.parametrize("m,n,k", [(2048, 2048, 512), (2000, 2100, 1000), (2049, 1030, 256), (513, 4097, 2049), (70_000, 96, 64),
-                                   (33_000, 256, 128), (4096, 8192, 256), (1, 16_000, 8192), (8, 8192, 16_384), (64, 4096, 4096)])
+                                   (33_000, 256, 128), (66_001, 200, 100), (70_000, 41, 128), (40_001, 100, 77), (4096, 8192, 256),
+                                   (5000, 3000, 600), (5000, 3001, 601), (1500, 1500, 1031), (200, 4096, 4096), (500, 4096, 4095),
+                                   (250, 4000, 2049), (60_000, 256, 200), (1, 16_000, 8192), (8, 8192, 16_384), (64, 4096, 4096)])
 def test_large(m, n, k):
     say("large", m, n, k)
     run(m, n, k, torch.bfloat16)
@@ -156,20 +157,18 @@ def test_graph_replays_and_streams(m, n, k):
     say("graph", m, n, k)
     a, w, sa, sw = codes(m, k, 1), codes(n, k, 2), scales(m, 3), scales(n, 4)
     out = torch.empty((m, n), dtype=torch.float16, device="cuda")
-    ws = torch.empty(max(1, dense.matmul_i8_workspace_bytes(m, n, k)), dtype=torch.uint8, device="cuda")
     s = torch.cuda.Stream()
     s.wait_stream(torch.cuda.current_stream())
     other = trspmm.matmul_i8(a, sa, w, sw, stream=s)
     s.synchronize()
-    assert torch.equal(other, trspmm.matmul_i8(a, sa, w, sw, out=out, workspace=ws))
+    assert torch.equal(other, trspmm.matmul_i8(a, sa, w, sw, out=out))
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
-        trspmm.matmul_i8(a, sa, w, sw, out=out, workspace=ws)
+        trspmm.matmul_i8(a, sa, w, sw, out=out)
     for i in range(4):
         a.copy_(codes(m, k, 30 + i))
         out.fill_(float("nan"))
-        ws.fill_(255)
         torch.cuda.synchronize()
         graph.replay()
         torch.cuda.synchronize()
@@ -189,7 +188,7 @@ def test_refusals():
         trspmm.matmul_i8(long, sa[:1], long, sw[:1])
     assert e.value.code == 5
     lib, out = nat.lib(), torch.empty((4, 6), device="cuda")
-    good = (a.data_ptr(), 32, sa.data_ptr(), w.data_ptr(), 32, sw.data_ptr(), None, 4, 6, 32, out.data_ptr(), 0, 6, None, 0, None)
+    good = (a.data_ptr(), 32, sa.data_ptr(), w.data_ptr(), 32, sw.data_ptr(), None, 4, 6, 32, out.data_ptr(), 0, 6, None)
     for k, v in [(0, None), (1, 31), (2, None), (3, None), (4, 31), (5, None), (7, -1), (8, -1), (9, -1), (10, None), (11, 5), (12, 5)]:
         call = list(good)
         call[k] = v

@@ -91,6 +91,12 @@ __device__ __forceinline__ void store_chunk(typename T::raw* p, int n, const flo
   }
 }
 
+// Orders a wave's LDS accesses: lanes read what other lanes of the wave wrote.
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 // First element of chunk c of a row of `width`, and how many of its elements the chunk before holds too.
 __device__ __forceinline__ int chunk_at(int c, int width, int& shared) {
   const int at = 8 * c, last = width - 8;

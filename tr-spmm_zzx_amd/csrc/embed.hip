@@ -108,12 +108,6 @@ __global__ __launch_bounds__(kThreads) void k_digit_offsets(uint32_t* __restrict
   if (lane == 0) totals[digit] = before;
 }
 
-// Orders a wave's LDS accesses: lanes read what other lanes of the wave wrote.
-__device__ __forceinline__ void wave_fence() {
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-}
-
 template <class I, bool FIRST>
 __global__ __launch_bounds__(kThreads) void k_digit_move(const I* __restrict__ ids, const uint32_t* __restrict__ at_in,
                                                          uint32_t count, uint32_t rows, int shift, int bits, uint32_t blocks,

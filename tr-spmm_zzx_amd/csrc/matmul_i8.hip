@@ -11,7 +11,6 @@ namespace trs {
 namespace dense {
 namespace {
 
-constexpr int kThreads = 256;
 constexpr int32_t kMostK = 131071;   // 128 * 128 * k stays below 2^31
 
 typedef int int4_v __attribute__((ext_vector_type(4)));
@@ -26,95 +25,539 @@ struct MatArgs {
   int n, k, out_type;
 };
 
-// 16 codes of a row from column `at` on; zeros past the row's end (zeros add nothing to the sums)
+// 16 codes of a row from column `at` on; zeros past the row's end (zeros add nothing to the sums).  A piece that
+// the end cuts is the row's last 16 codes, shifted.
 __device__ __forceinline__ int4_v load_codes(const int8_t* row, int at, int k) {
   if (at + 16 <= k) return *reinterpret_cast<const int4_u*>(row + at);
-  union { int8_t c[16]; int4_v v; } u;
+  union { int8_t c[16]; uint64_t q[2]; int4_v v; } u;
   u.v = int4_v{0, 0, 0, 0};
+  if (at >= k) return u.v;
+  if (k >= 16) {
+    u.v = *reinterpret_cast<const int4_u*>(row + k - 16);
+    const int bits = 8 * (at + 16 - k);   // 8 .. 120
+    if (bits >= 64) {
+      u.q[0] = u.q[1] >> (bits - 64);
+      u.q[1] = 0;
+    } else {
+      u.q[0] = u.q[0] >> bits | u.q[1] << (64 - bits);
+      u.q[1] >>= bits;
+    }
+  } else {
 #pragma unroll
-  for (int i = 0; i < 16; ++i)
-    if (at + i < k) u.c[i] = row[at + i];
+    for (int i = 0; i < 16; ++i)
+      if (at + i < k) u.c[i] = row[at + i];
+  }
   return u.v;
 }
 
-// Four neighbouring columns of one output row.
-__device__ __forceinline__ void store_columns(const MatArgs& p, int64_t m, int n, const float (&v)[4]) {
-  const int64_t at = m * p.ldo + n;
-  const int left = p.n - n;
-  if (left >= 4) {
-    if (p.out_type == TRS_F32) store_vec<f32_t, 4>(static_cast<float*>(p.out) + at, v);
-    else if (p.out_type == TRS_F16) store_vec<f16_t, 4>(static_cast<_Float16*>(p.out) + at, v);
-    else store_vec<bf16_t, 4>(static_cast<__bf16*>(p.out) + at, v);
-  } else {
+// A wave's sums, 32 rows and (up to) 64 columns at a time, through LDS (a wave's own part: `lds`, 32 rows of
+// kOutPitch integers), so that a lane holds 8 neighbouring columns of a row, and rows leave in whole vectors.
+template <int FN>
+constexpr int kOutPitch = (FN > 1 ? 64 : 32) + 4;
+
+// The scales of the rows that a lane of store_wave writes, read together: one wait for all.
+template <int FM, int FN>
+struct RowScales {
+  static constexpr int kRowLanes = FN > 1 ? 8 : 4, kRows = 64 / kRowLanes, kTurns = 32 / kRows;
+  float of[FM][kTurns];
+  __device__ __forceinline__ void load(const MatArgs& p, int64_t m0, int lane) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (i >= left) break;
-      if (p.out_type == TRS_F32) static_cast<float*>(p.out)[at + i] = v[i];
-      else if (p.out_type == TRS_F16) static_cast<_Float16*>(p.out)[at + i] = (_Float16)v[i];
-      else static_cast<__bf16*>(p.out)[at + i] = (__bf16)v[i];
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int t = 0; t < kTurns; ++t) {
+        const int64_t m = m0 + i * 32 + t * kRows + lane / kRowLanes;
+        of[i][t] = p.a_scale[m < p.m ? m : p.m - 1];
+      }
+  }
+};
+
+template <int FM, int FN>
+__device__ __forceinline__ void store_wave(const MatArgs& p, const int16_v (&acc)[FM][FN], const RowScales<FM, FN>& sa, int* lds,
+                                           int64_t m0, int n0, int lane) {
+  using S = RowScales<FM, FN>;
+  constexpr int FJ = FN > 1 ? 2 : 1, kPitch = kOutPitch<FN>;
+  const int first = lane % S::kRowLanes * 8;
+#pragma unroll
+  for (int j0 = 0; j0 < FN; j0 += FJ) {
+    // A lane whose 8 columns the matrix's end cuts takes the last 8 instead, if its wave has them: they are written
+    // twice, the same.
+    const int end = p.n - n0 - j0 * 32;   // columns there are from the part's first on
+    const int column = first + 8 > end && first < end && end >= 8 ? end - 8 : first;
+    const int n = n0 + j0 * 32 + column, left = first < end ? end - column : 0;
+    float sw[8], bias[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sw[e] = bias[e] = 0.f;
+    if (left > 0) {
+      load_chunk<f32_t>(p.w_scale + n, left, sw);
+      if (p.bias) load_chunk<f32_t>(p.bias + n, left, bias);
+    }
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+#pragma unroll
+      for (int j = 0; j < FJ; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int16_v& part = acc[i][j0 + j];
+          *reinterpret_cast<int4_v*>(lds + (lane & 31) * kPitch + j * 32 + 8 * q + 4 * (lane >> 5)) =
+              int4_v{part[4 * q], part[4 * q + 1], part[4 * q + 2], part[4 * q + 3]};
+        }
+      wave_fence();
+#pragma unroll
+      for (int t = 0; t < S::kTurns; ++t) {
+        const int r = t * S::kRows + lane / S::kRowLanes;
+        const int64_t m = m0 + i * 32 + r;
+        const int* from = lds + r * kPitch + column;
+        int got[8];
+        if (column % 4 == 0) {
+          *reinterpret_cast<int4_v*>(got) = *reinterpret_cast<const int4_v*>(from);
+          *reinterpret_cast<int4_v*>(got + 4) = *reinterpret_cast<const int4_v*>(from + 4);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) got[e] = from[e];
+        }
+        if (m >= p.m || left <= 0) continue;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = (float)got[e] * sa.of[i][t] * sw[e] + bias[e];
+        const int64_t at = m * p.ldo + n;
+        if (p.out_type == TRS_F32) store_chunk<f32_t>(static_cast<float*>(p.out) + at, left, v);
+        else if (p.out_type == TRS_F16) store_chunk<f16_t>(static_cast<_Float16*>(p.out) + at, left, v);
+        else store_chunk<bf16_t>(static_cast<__bf16*>(p.out) + at, left, v);
+      }
+      wave_fence();
     }
   }
 }
 
-// 128 x 128 outputs a workgroup, 64 x 64 a wave, 64 codes of k a step, any alignment.  The weights are the
-// matrix instruction's first operand, so a lane's registers run along n and a row of the output is written in
-// vectors.
-constexpr int kTile = 128, kStep = 64, kPitch = kStep + 16;
+// ---------------------------------------------------------------------------------------------
+// Tiles: TM x TN outputs a workgroup, WM x WN a wave, 128 codes of k a step, the next step's operands on their
+// way while this one's are multiplied.  A tile's row is 128 bytes, eight pieces of 16; piece c of row r lies in
+// place c ^ (r & 7), so that the 16-byte reads of neighbouring rows spread over the banks.
+//
+// DIRECT: rows on 16-byte boundaries and k a multiple of 16; the pieces go from memory to LDS without
+// registers.  Otherwise any address, through registers.  KS groups of waves split a workgroup's steps, each
+// with its own tiles, and the first adds the sums up: for few workgroups and a long k.
+constexpr int kDepth = 128;
 
-__global__ __launch_bounds__(kThreads) void k_matmul_tiles(MatArgs p) {
-  __shared__ __align__(16) int8_t tile[2][kTile * kPitch];
-  const int64_t m0 = (int64_t)blockIdx.y * kTile;
-  const int n0 = (int)blockIdx.x * kTile;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
-  int16_v acc[2][2] = {};
-  for (int k0 = 0; k0 < p.k; k0 += kStep) {
+typedef __attribute__((address_space(3))) void* lds_ptr;
+
+// A barrier that also waits for the wave's own LDS reads: what is written after it (by another wave's copy from
+// memory) must not reach them.  __syncthreads alone has been compiled to a barrier before which reads into
+// registers were still on their way.
+__device__ __forceinline__ void barrier_and_wait() {
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+}
+
+// A buffer that ends with the operand's last code.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t operand(const int8_t* from, int64_t rows, int64_t ld, int k) {
+  const int64_t bytes = (rows - 1) * ld + k;
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(from), 0, (int)(bytes < UINT32_MAX ? bytes : UINT32_MAX), 0x00020000);
+}
+
+// Workgroup b of `total` as a tile: the workgroups of one XCD (b mod 8) take neighbouring tiles, in bands of 8
+// rows of tiles, so that an XCD's L2 serves the operands they share.
+__device__ __forceinline__ void tile_of(uint32_t b, uint32_t tiles_m, uint32_t tiles_n, uint32_t& tm, uint32_t& tn) {
+  const uint32_t total = tiles_m * tiles_n;
+  const uint32_t xcd = b & 7, q = total >> 3, r = total & 7;
+  const uint32_t t = xcd * q + (xcd < r ? xcd : r) + (b >> 3);
+  const uint32_t band = 8 * tiles_n, first = t / band * 8, in = t % band;
+  const uint32_t high = tiles_m - first < 8 ? tiles_m - first : 8;
+  tm = first + in % high;
+  tn = in / high;
+}
+
+template <int TM, int TN, int WM, int WN, int KS, bool DIRECT, class Offset>
+__device__ __forceinline__ void matmul_tile(const MatArgs& p, uint32_t tiles_m, uint32_t tiles_n) {
+  constexpr int kWaveRows = TM / WM, kWavesOf = kWaveRows * (TN / WN), kAll = kWavesOf * 64;   // of a group
+  constexpr int FM = WM / 32, FN = WN / 32;
+  constexpr int kLoadsA = TM * 8 / kAll, kLoadsW = TN * 8 / kAll;
+  __shared__ __align__(1024) int8_t a_even[KS * TM * kDepth], a_odd[KS * TM * kDepth], w_even[KS * TN * kDepth],
+      w_odd[KS * TN * kDepth];
+  uint32_t tm, tn;
+  tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn);
+  const int64_t m0 = (int64_t)tm * TM;
+  const int n0 = (int)tn * TN;
+  const int any_wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int group = KS > 1 ? any_wave / kWavesOf : 0, wave = any_wave - group * kWavesOf;
+  const int thread = wave * 64 + lane;
+  const int wm = wave % kWaveRows * WM, wn = wave / kWaveRows * WN;
+  int8_t *const a0 = a_even + group * (TM * kDepth), *const a1 = a_odd + group * (TM * kDepth);
+  int8_t *const w0 = w_even + group * (TN * kDepth), *const w1 = w_odd + group * (TN * kDepth);
+
+  // Where this thread's pieces come from: `row0` and every kAll / 8 rows on, which agree in r / 2 & 7.  Rows past the
+  // operand's end are its last row again; their outputs are not stored.
+  const int row0 = thread >> 3, my_k = ((thread & 7) ^ (row0 >> 1 & 7)) * 16;
+  const int8_t *base_a = p.a + m0 * p.lda, *base_w = p.w + n0 * p.ldw;
+  Offset at_a[kLoadsA], at_w[kLoadsW];
+#pragma unroll
+  for (int u = 0; u < kLoadsA; ++u) {
+    const int r = u * (kAll / 8) + row0;
+    at_a[u] = (m0 + r < p.m ? r : (int)(p.m - 1 - m0)) * (Offset)p.lda + my_k;
+  }
+#pragma unroll
+  for (int u = 0; u < kLoadsW; ++u) {
+    const int r = u * (kAll / 8) + row0;
+    at_w[u] = (n0 + r < p.n ? r : p.n - 1 - n0) * (Offset)p.ldw + my_k;
+  }
+
+  int4_v held[DIRECT ? 1 : kLoadsA + kLoadsW];
+  auto fetch = [&](int8_t* a, int8_t* w, int at) {
+    const int k0 = __builtin_amdgcn_readfirstlane(at);   // the same in every lane
+    if constexpr (DIRECT) {
+      const __amdgpu_buffer_rsrc_t buf_a = operand(base_a, p.m - m0, p.lda, p.k), buf_w = operand(base_w, p.n - n0, p.ldw, p.k);
+#pragma unroll
+      for (int u = 0; u < kLoadsA; ++u)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(buf_a, (lds_ptr)(a + (u * kAll + wave * 64) * 16), 16, at_a[u], k0, 0, 0);
+#pragma unroll
+      for (int u = 0; u < kLoadsW; ++u)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(buf_w, (lds_ptr)(w + (u * kAll + wave * 64) * 16), 16, at_w[u], k0, 0, 0);
+    } else {
+#pragma unroll
+      for (int u = 0; u < kLoadsA; ++u) held[u] = *reinterpret_cast<const int4_u*>(base_a + at_a[u] + k0);
+#pragma unroll
+      for (int u = 0; u < kLoadsW; ++u) held[kLoadsA + u] = *reinterpret_cast<const int4_u*>(base_w + at_w[u] + k0);
+    }
+  };
+  auto put = [&](int8_t* a, int8_t* w) {
+    if constexpr (!DIRECT) {
+#pragma unroll
+      for (int u = 0; u < kLoadsA; ++u) *reinterpret_cast<int4_v*>(a + (u * kAll + thread) * 16) = held[u];
+#pragma unroll
+      for (int u = 0; u < kLoadsW; ++u) *reinterpret_cast<int4_v*>(w + (u * kAll + thread) * 16) = held[kLoadsA + u];
+    }
+  };
+  // The last step where 128 does not divide k: codes past k are zeros.
+  auto fetch_rest = [&](int8_t* a, int8_t* w, int k0) {
+#pragma unroll
+    for (int u = 0; u < kLoadsA; ++u)
+      *reinterpret_cast<int4_v*>(a + (u * kAll + thread) * 16) = load_codes(base_a + at_a[u] - my_k, k0 + my_k, p.k);
+#pragma unroll
+    for (int u = 0; u < kLoadsW; ++u)
+      *reinterpret_cast<int4_v*>(w + (u * kAll + thread) * 16) = load_codes(base_w + at_w[u] - my_k, k0 + my_k, p.k);
+  };
+
+  int16_v acc[FM][FN] = {};
+  const int swz = lane >> 1 & 7, row = lane & 31, half = lane >> 5;
+  // Two sets of fragments: one is read from LDS while the other is multiplied.
+  int4_v fa[2][FM] = {}, fw[2][FN] = {};
+  auto read = [&](int set, const int8_t* a, const int8_t* w, int h) {
+    const int at = ((2 * h + half) ^ swz) * 16;
+#pragma unroll
+    for (int i = 0; i < FM; ++i) fa[set][i] = *reinterpret_cast<const int4_v*>(a + (wm + i * 32 + row) * kDepth + at);
+#pragma unroll
+    for (int j = 0; j < FN; ++j) fw[set][j] = *reinterpret_cast<const int4_v*>(w + (wn + j * 32 + row) * kDepth + at);
+  };
+  // The weights are the matrix instruction's first operand, so a lane's registers run along n.
+  auto multiply = [&](int set) {
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[set][j], fa[set][i], acc[i][j], 0, 0, 0);
+  };
+  // A step: the products of the last quarter of the step before are made while the first of this one is read,
+  // with one read of LDS after each product as far as they go.
+  auto step = [&](const int8_t* a, const int8_t* w) {
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      read(h & 1, a, w, h);
+      multiply((h & 1) ^ 1);
+      constexpr int kReads = FM * FN > 1 ? 2 : 1, kPairs = FM * FN < (FM + FN) / kReads ? FM * FN : (FM + FN) / kReads;
+#pragma unroll
+      for (int k = 0; k < kPairs; ++k) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, kReads, 0);
+      }
+      if constexpr (FM * FN > kPairs) __builtin_amdgcn_sched_group_barrier(0x008, FM * FN - kPairs, 0);
+      if constexpr (FM + FN > kPairs * kReads) __builtin_amdgcn_sched_group_barrier(0x100, FM + FN - kPairs * kReads, 0);
+    }
+  };
+
+  const int whole = p.k / kDepth;                       // steps of 128
+  const int turns = (whole + KS - 1) / KS, first = group * turns;
+  const int mine = whole - first < turns ? whole - first : turns;   // this group's; not positive: none
+  if (whole > 0) {
+    if (mine > 0) {
+      fetch(a0, w0, first * kDepth);
+      put(a0, w0);
+    }
+    for (int t = 0;;) {
+      barrier_and_wait();
+      if (t + 1 < mine) fetch(a1, w1, (first + t + 1) * kDepth);
+      if (KS == 1 || t < mine) step(a0, w0);
+      if (t + 1 < mine) put(a1, w1);
+      if (++t == turns) break;
+      barrier_and_wait();
+      if (t + 1 < mine) fetch(a0, w0, (first + t + 1) * kDepth);
+      if (KS == 1 || t < mine) step(a1, w1);
+      if (t + 1 < mine) put(a0, w0);
+      if (++t == turns) break;
+    }
+    multiply(1);
+  }
+  if (const int rest = p.k - whole * kDepth) {
+    barrier_and_wait();
+    if (group == 0) fetch_rest(a0, w0, whole * kDepth);
+    barrier_and_wait();
+    if (group == 0) {
+#pragma unroll 1
+      for (int h = 0; h < (rest + 31) / 32; ++h) {
+        read(0, a0, w0, h);
+        multiply(0);
+      }
+    }
+  }
+  barrier_and_wait();
+  if constexpr (KS > 1) {
+    // each group's sums in its own tiles of a, a register of the 64 lanes after the other
+    constexpr int kRegs = FM * FN * 16, kHalf = TM * kDepth / 4 / kAll;
+    static_assert(kRegs <= 2 * kHalf, "sums fit");
+    auto place = [&](int g, int r) {
+      return reinterpret_cast<int*>((r < kHalf ? a_even : a_odd) + g * (TM * kDepth)) + (r % kHalf) * kAll + thread;
+    };
+    if (group > 0) {
+#pragma unroll
+      for (int r = 0; r < kRegs; ++r) *place(group, r) = acc[r / 16 / FN][r / 16 % FN][r % 16];
+    }
+    barrier_and_wait();
+    if (group > 0) return;
+    for (int g = 1; g < KS; ++g)
+#pragma unroll
+      for (int r = 0; r < kRegs; ++r) acc[r / 16 / FN][r / 16 % FN][r % 16] += *place(g, r);
+  }
+  constexpr int kPerArray = kAll / 256, kPart = 32 * kOutPitch<FN>;   // waves that share one of the four arrays
+  static_assert(kPerArray * kPart * 4 <= (TM < TN ? TM : TN) * kDepth, "outputs fit");
+  int8_t* const array = wave < kPerArray ? a0 : wave < 2 * kPerArray ? a1 : wave < 3 * kPerArray ? w0 : w1;
+  RowScales<FM, FN> sa;
+  sa.load(p, m0 + wm, lane);
+  store_wave<FM, FN>(p, acc, sa, reinterpret_cast<int*>(array) + wave % kPerArray * kPart, m0 + wm, n0 + wn, lane);
+}
+
+template <int TM, int TN, int WM, int WN, int KS, bool DIRECT, class Offset>
+__global__ __launch_bounds__((TM / WM) * (TN / WN) * 64 * KS, 2) void k_matmul_tile(MatArgs p, uint32_t tiles_m,
+                                                                                    uint32_t tiles_n) {
+  matmul_tile<TM, TN, WM, WN, KS, DIRECT, Offset>(p, tiles_m, tiles_n);
+}
+
+// ---------------------------------------------------------------------------------------------
+// k of one step (at most 128): a tile is read once and its outputs, the bytes that count here, are written; with one
+// set of tiles in LDS several workgroups share a CU, and some read while others write.
+template <int TM, int TN, int WM, int WN>
+__global__ __launch_bounds__((TM / WM) * (TN / WN) * 64, 4) void k_matmul_once(MatArgs p, uint32_t tiles_m, uint32_t tiles_n) {
+  constexpr int kWaveRows = TM / WM, kWavesOf = kWaveRows * (TN / WN), kAll = kWavesOf * 64;
+  constexpr int FM = WM / 32, FN = WN / 32, kPart = 32 * kOutPitch<FN>;
+  constexpr int kIn = (TM + TN) * kDepth, kOut = kWavesOf * kPart * 4;
+  __shared__ __align__(1024) int8_t lds[kIn > kOut ? kIn : kOut];
+  uint32_t tm, tn;
+  tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn);
+  const int64_t m0 = (int64_t)tm * TM;
+  const int n0 = (int)tn * TN;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int wm = wave % kWaveRows * WM, wn = wave / kWaveRows * WN;
+  const int row0 = threadIdx.x >> 3, my_k = ((threadIdx.x & 7) ^ (row0 >> 1 & 7)) * 16;
+  RowScales<FM, FN> sa;
+  sa.load(p, m0 + wm, lane);
+  constexpr int kLoads = (TM + TN) * 8 / kAll, kPerLoad = kAll / 8;
+  static_assert(TM % kPerLoad == 0 && TN % kPerLoad == 0, "a load is of one operand");
+#pragma unroll
+  for (int u = 0; u < kLoads; ++u) {
+    const int r = u * kPerLoad + row0;
+    const int8_t* from;
+    if (u * kPerLoad < TM) from = p.a + (m0 + r < p.m ? m0 + r : p.m - 1) * p.lda;
+    else from = p.w + (int64_t)(n0 + r - TM < p.n ? n0 + r - TM : p.n - 1) * p.ldw;
+    *reinterpret_cast<int4_v*>(lds + (u * kAll + threadIdx.x) * 16) = load_codes(from, my_k, p.k);
+  }
+  __syncthreads();
+  int16_v acc[FM][FN] = {};
+  const int swz = lane >> 1 & 7, row = lane & 31, half = lane >> 5;
+  const int8_t *a = lds, *w = lds + TM * kDepth;
+  for (int h = 0; h * 32 < p.k; ++h) {
+    const int at = ((2 * h + half) ^ swz) * 16;
+    int4_v fa[FM], fw[FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i) fa[i] = *reinterpret_cast<const int4_v*>(a + (wm + i * 32 + row) * kDepth + at);
+#pragma unroll
+    for (int j = 0; j < FN; ++j) fw[j] = *reinterpret_cast<const int4_v*>(w + (wn + j * 32 + row) * kDepth + at);
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[j], fa[i], acc[i][j], 0, 0, 0);
+  }
+  barrier_and_wait();
+  store_wave<FM, FN>(p, acc, sa, reinterpret_cast<int*>(lds) + wave * kPart, m0 + wm, n0 + wn, lane);
+}
+
+// ---------------------------------------------------------------------------------------------
+// Few rows: 16 FM rows and 16 output channels a workgroup, its waves taking turns at 128 codes of k each, so that
+// the weights -- the bytes that count here -- arrive by as many loads in flight as fit.  The waves' sums are
+// added up in LDS.
+template <int FM>
+__global__ __launch_bounds__(1024) void k_matmul_rows(MatArgs p, uint32_t blocks_n) {
+  __shared__ int sums[16][FM * 256];
+  const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6, lane = threadIdx.x & 63;
+  const int n0 = (int)(blockIdx.x % blocks_n) * 16;
+  const int64_t m0 = (int64_t)(blockIdx.x / blocks_n) * (16 * FM);
+  const int row = lane & 15, piece = (lane >> 4) * 16;
+  const int8_t* w = p.w + (int64_t)(n0 + row < p.n ? n0 + row : p.n - 1) * p.ldw;
+  const int8_t* a[FM];
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+    const int64_t m = m0 + i * 16 + row;
+    a[i] = p.a + (m < p.m ? m : p.m - 1) * p.lda;
+  }
+  int4_v acc[FM] = {};
+  constexpr int kAhead = FM > 2 ? 1 : 2;   // pieces of 128 codes on their way together
+  const int whole = p.k / 128;
+  int t = wave;
+  for (; t + (kAhead - 1) * waves < whole; t += kAhead * waves) {
+    int4_v fw[2 * kAhead], fa[2 * kAhead][FM];
+#pragma unroll
+    for (int u = 0; u < 2 * kAhead; ++u) {
+      const int at = (t + u / 2 * waves) * 128 + u % 2 * 64 + piece;
+      fw[u] = *reinterpret_cast<const int4_u*>(w + at);
+#pragma unroll
+      for (int i = 0; i < FM; ++i) fa[u][i] = *reinterpret_cast<const int4_u*>(a[i] + at);
+    }
+#pragma unroll
+    for (int u = 0; u < 2 * kAhead; ++u)
+#pragma unroll
+      for (int i = 0; i < FM; ++i) acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[u], fa[u][i], acc[i], 0, 0, 0);
+  }
+  for (; t * 128 < p.k; t += waves) {   // what is left, the end of k among it
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int j = u * kThreads + threadIdx.x, row = j >> 2, at = (j & 3) * 16;
-      int4_v va = {0, 0, 0, 0}, vw = {0, 0, 0, 0};
-      if (m0 + row < p.m) va = load_codes(p.a + (m0 + row) * p.lda, k0 + at, p.k);
-      if (n0 + row < p.n) vw = load_codes(p.w + (int64_t)(n0 + row) * p.ldw, k0 + at, p.k);
-      *reinterpret_cast<int4_v*>(&tile[0][row * kPitch + at]) = va;
-      *reinterpret_cast<int4_v*>(&tile[1][row * kPitch + at]) = vw;
+      const int at = t * 128 + u * 64 + piece;
+      const int4_v fw = load_codes(w, at, p.k);
+#pragma unroll
+      for (int i = 0; i < FM; ++i) acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw, load_codes(a[i], at, p.k), acc[i], 0, 0, 0);
     }
-    __syncthreads();
-#pragma unroll
-    for (int h = 0; h < kStep; h += 32) {
-      int4_v fa[2], fw[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int at = h + (lane >> 5) * 16;
-        fa[i] = *reinterpret_cast<const int4_v*>(&tile[0][(wm + i * 32 + (lane & 31)) * kPitch + at]);
-        fw[i] = *reinterpret_cast<const int4_v*>(&tile[1][(wn + i * 32 + (lane & 31)) * kPitch + at]);
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[j], fa[i], acc[i][j], 0, 0, 0);
-    }
-    __syncthreads();
   }
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int64_t m = m0 + wm + i * 32 + (lane & 31);
-    if (m >= p.m) continue;
-    const float sa = p.a_scale[m];
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int n = n0 + wn + j * 32 + 8 * q + 4 * (lane >> 5);
-        if (n >= p.n) continue;
-        float v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int nn = n + e < p.n ? n + e : p.n - 1;
-          v[e] = (float)acc[i][j][4 * q + e] * sa * p.w_scale[nn] + (p.bias ? p.bias[nn] : 0.f);
-        }
-        store_columns(p, m, n, v);
-      }
+  for (int i = 0; i < FM; ++i)
+    *reinterpret_cast<int4_v*>(&sums[wave][(i * 16 + row) * 16 + (lane >> 4) * 4]) = acc[i];
+  __syncthreads();
+  for (int o = threadIdx.x; o < FM * 256; o += blockDim.x) {
+    const int64_t m = m0 + o / 16;
+    const int n = n0 + o % 16;
+    if (m >= p.m || n >= p.n) continue;
+    int sum = 0;
+    for (int v = 0; v < waves; ++v) sum += sums[v][o];
+    const float v = (float)sum * p.a_scale[m] * p.w_scale[n] + (p.bias ? p.bias[n] : 0.f);
+    const int64_t at = m * p.ldo + n;
+    if (p.out_type == TRS_F32) static_cast<float*>(p.out)[at] = v;
+    else if (p.out_type == TRS_F16) static_cast<_Float16*>(p.out)[at] = (_Float16)v;
+    else static_cast<__bf16*>(p.out)[at] = (__bf16)v;
   }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Host side: which kernel.  Times in us measured on the MI355X with operands that change from call to call.
+constexpr int kCus = 256;
+
+template <int T, int WM, int WN, int KS, bool DIRECT, class Offset>
+void launch_tile(const MatArgs& p, hipStream_t s) {
+  const uint32_t tm = (uint32_t)ceil_div(p.m, T), tn = (uint32_t)ceil_div(p.n, T);
+  k_matmul_tile<T, T, WM, WN, KS, DIRECT, Offset><<<dim3(tm * tn), (T / WM) * (T / WN) * 64 * KS, 0, s>>>(p, tm, tn);
+}
+
+template <int TM, int TN, int WM, int WN>
+void launch_once(const MatArgs& p, hipStream_t s) {
+  const uint32_t tm = (uint32_t)ceil_div(p.m, TM), tn = (uint32_t)ceil_div(p.n, TN);
+  k_matmul_once<TM, TN, WM, WN><<<dim3(tm * tn), (TM / WM) * (TN / WN) * 64, 0, s>>>(p, tm, tn);
+}
+
+template <int FM>
+void launch_rows(const MatArgs& p, hipStream_t s) {
+  const uint32_t bn = (uint32_t)ceil_div(p.n, 16), bm = (uint32_t)ceil_div(p.m, 16 * FM);
+  const int pieces = (p.k + 127) / 128, waves = pieces >= 16 ? 16 : pieces >= 8 ? 8 : 4;
+  k_matmul_rows<FM><<<dim3(bn * bm), 64 * waves, 0, s>>>(p, bn);
+}
+
+int64_t tiles(const MatArgs& p, int tm, int tn) { return ceil_div(p.m, tm) * ceil_div(p.n, tn); }
+
+// k_matmul_rows reads 16 FM rows and 16 channels a workgroup, at some 39 bytes/ns a CU (rows past m are the last
+// one again and cost nothing); 64 x 64 tiles read 128 rows at some 75.  By rounds over the CUs, relative:
+//   m x n x k          FM = 1   2     4    tiles
+//   1 x 4096 x 4096      5.5   -     -     10.8
+//   32 x 4096 x 4096    10.1   8.3   9.3   11.3
+//   64 x 4096 x 4096    17.3  13.5  11.9   11.9
+//   200 x 300 x 1000     3.5   4.0   5.3    6.2
+//   32 x 16384 x 8192   66    51     -     32.6
+// Returns FM, or 0 for tiles.
+int rows_kernel(const MatArgs& p) {
+  double best = ceil_div(tiles(p, 64, 64), kCus) * 128 / 75.0;
+  int fm = 0;
+  for (int f : {1, 2, 4}) {
+    const int64_t rows = p.m < 16 * f ? p.m : 16 * f;
+    const double cost = ceil_div(tiles(p, 16 * f, 16), kCus) * (16 + rows) / 39.0;
+    if (cost < best || (fm == 0 && p.m <= 8)) {
+      best = cost;
+      fm = f;
+    }
+  }
+  return fm;
+}
+
+// The tile's side, by us a round of workgroups over the CUs: so much a step of 128 codes and so much around the steps
+// (128: two workgroups share a CU; 64: five).
+//   m x n x k               256    128    64
+//   8192 x 8192 x 8192      460    550    -
+//   4096 x 4096 x 4096       62     71   102
+//   16384 x 1024 x 512       18     24    22
+//   2048 x 2048 x 2048       27     16    16
+//   512 x 4096 x 4096        42     23    18
+//   1000003 x 128 x 256     190    132   157
+// Through registers (odd strides) a step takes a third longer in tiles of 256, less in the others.
+int tile_side(const MatArgs& p, bool direct) {
+  const double steps = p.k / (double)kDepth, more = direct ? 1.0 : 1.2;
+  const int64_t r256 = ceil_div(tiles(p, 256, 256), kCus), r128 = ceil_div(tiles(p, 128, 128), kCus),
+                r64 = ceil_div(tiles(p, 64, 64), kCus);
+  const double t256 = r256 * (steps * (direct ? 1.65 : 2.2) + 9), t128 = r128 * (steps * 0.53 * more + 2.7),
+               t64 = (r64 < 3 ? 0.42 : r64 * 0.2) * steps * more + r64 * 0.65;
+  return t256 < t128 && t256 < t64 ? 256 : t128 < t64 ? 128 : 64;
+}
+
+template <bool DIRECT, class Offset>
+void launch_small_tiles(const MatArgs& p, hipStream_t s) {
+  // Few workgroups: groups of waves share out the steps (256 x 4096 x 4096: 17.1 us with 1 group, 13.5 with 2, 12.1 with
+  // 4; 512 x 4096 x 4096: 17.8, 16.4, 22.1; 1000^3: 6.8, 7.4, 7.6).
+  const int64_t t = tiles(p, 64, 64);
+  if (t <= kCus && p.k >= 16 * kDepth) launch_tile<64, 32, 32, 4, DIRECT, Offset>(p, s);
+  else if (t <= 2 * kCus && p.k >= 8 * kDepth) launch_tile<64, 32, 32, 2, DIRECT, Offset>(p, s);
+  else launch_tile<64, 32, 32, 1, DIRECT, Offset>(p, s);
+}
+
+void launch(const MatArgs& p, hipStream_t s) {
+  switch (rows_kernel(p)) {
+    case 1: return launch_rows<1>(p, s);
+    case 2: return launch_rows<2>(p, s);
+    case 4: return launch_rows<4>(p, s);
+  }
+  if (p.k <= kDepth) {
+    // 1000003 x 256 x 128: 240 us with tiles of 64 x 64, 213 of 128 x 128, 171 of 128 x 256; x 128: 120, 106, 136;
+    // x 64: 61, 87, 118.  Below two workgroups a CU the smallest (2000 x 500 x 128: 4.1, 6.5, 7.0).
+    if (p.n > 128 && tiles(p, 128, 256) >= 2 * kCus) launch_once<128, 256, 64, 64>(p, s);
+    else if (p.n > 64 && tiles(p, 128, 128) >= 2 * kCus) launch_once<128, 128, 64, 64>(p, s);
+    else launch_once<64, 64, 32, 32>(p, s);
+    return;
+  }
+  const bool direct = ((reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.w) | (uintptr_t)p.lda | (uintptr_t)p.ldw |
+                        (uintptr_t)p.k) & 15) == 0;
+  const int64_t ld = p.lda > p.ldw ? p.lda : p.ldw;
+  if (ld * 256 > INT32_MAX) return launch_small_tiles<false, int64_t>(p, s);   // a tile's offsets pass 32 bits
+  switch (tile_side(p, direct)) {
+    case 256:
+      if (direct) launch_tile<256, 128, 64, 1, true, int>(p, s);
+      else launch_tile<256, 128, 64, 1, false, int>(p, s);
+      return;
+    case 128:
+      if (direct) launch_tile<128, 64, 64, 1, true, int>(p, s);
+      else launch_tile<128, 64, 64, 1, false, int>(p, s);
+      return;
+  }
+  if (direct) launch_small_tiles<true, int>(p, s);
+  else launch_small_tiles<false, int64_t>(p, s);
 }
 
 }  // namespace
@@ -123,16 +566,9 @@ __global__ __launch_bounds__(kThreads) void k_matmul_tiles(MatArgs p) {
 
 using namespace trs::dense;
 
-extern "C" int64_t trs_matmul_i8_workspace_bytes(int64_t m, int32_t n, int32_t k) {
-  (void)m;
-  (void)n;
-  (void)k;
-  return 0;
-}
-
 extern "C" int trs_matmul_i8(const int8_t* a, int64_t lda, const float* a_scale, const int8_t* w, int64_t ldw,
                              const float* w_scale, const float* bias, int64_t m, int32_t n, int32_t k, void* out,
-                             int32_t out_type, int64_t ldo, void* workspace, int64_t workspace_bytes, void* stream) {
+                             int32_t out_type, int64_t ldo, void* stream) {
   const std::string at = "trs_matmul_i8: ";
   if (m < 0 || n < 0 || k < 0) return fail(TRS_EINVAL, at + "negative m, n or k");
   if (!known_type(out_type)) return fail(TRS_EINVAL, at + "unknown element type");
@@ -140,11 +576,9 @@ extern "C" int trs_matmul_i8(const int8_t* a, int64_t lda, const float* a_scale,
   if (m == 0 || n == 0) return TRS_OK;
   if (!out || !a_scale || !w_scale || (k > 0 && (!a || !w))) return fail(TRS_EINVAL, at + "NULL operand");
   if (lda < k || ldw < k || ldo < n) return fail(TRS_EINVAL, at + "leading dimension too small");
-  if (workspace_bytes < trs_matmul_i8_workspace_bytes(m, n, k) || (trs_matmul_i8_workspace_bytes(m, n, k) > 0 && !workspace))
-    return fail(TRS_EINVAL, at + "workspace smaller than trs_matmul_i8_workspace_bytes");
   const MatArgs p{a, w, a_scale, w_scale, bias, out, lda, ldw, ldo, m, n, k, out_type};
-  hipStream_t s = static_cast<hipStream_t>(stream);
-  if (ceil_div(m, kTile) > 65535) return fail(TRS_ERANGE, at + "more rows than a launch can have workgroups");
-  k_matmul_tiles<<<dim3((uint32_t)ceil_div(n, kTile), (uint32_t)ceil_div(m, kTile)), kThreads, 0, s>>>(p);
+  // the most workgroups, of the most threads, that any of the kernels takes
+  if (!fits_grid(tiles(p, 64, 64), 1024)) return fail(TRS_ERANGE, at + "the output needs more workgroups than a launch can have");
+  launch(p, static_cast<hipStream_t>(stream));
   return launched("trs_matmul_i8");
 }

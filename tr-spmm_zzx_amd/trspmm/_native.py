@@ -116,9 +116,7 @@ PROTOTYPES = {
     "trs_rms_norm_grad_workspace_bytes": (c_i64, [c_i64, c_i32]),
     "trs_rms_norm_grad": (c_i32, [c_p, c_i32, c_i64, c_p, c_i32, c_i64, c_p, c_i32, c_p, c_i64, c_f32, c_i64, c_i32, c_p,
                                   c_i64, c_p, c_p, c_i64, c_p]),
-    "trs_matmul_i8_workspace_bytes": (c_i64, [c_i64, c_i32, c_i32]),
-    "trs_matmul_i8": (c_i32, [c_p, c_i64, c_p, c_p, c_i64, c_p, c_p, c_i64, c_i32, c_i32, c_p, c_i32, c_i64, c_p, c_i64,
-                              c_p]),
+    "trs_matmul_i8": (c_i32, [c_p, c_i64, c_p, c_p, c_i64, c_p, c_p, c_i64, c_i32, c_i32, c_p, c_i32, c_i64, c_p]),
     "trs_last_error": (ctypes.c_char_p, []),
     "trs_abi_version": (c_i32, []),
 }

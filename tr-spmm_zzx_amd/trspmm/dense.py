@@ -274,13 +274,9 @@ def rms_norm_grad(grad: torch.Tensor, r: torch.Tensor, weight: torch.Tensor, gra
     return out, dweight
 
 
-def matmul_i8_workspace_bytes(m: int, n: int, k: int) -> int:
-    return int(nat.lib().trs_matmul_i8_workspace_bytes(m, n, k))
-
-
 def matmul_i8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
               bias: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.float16,
-              out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+              out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
     """out[i, j] = a_scale[i] * w_scale[j] * (a[i] . w[j]) + bias[j] in `dtype`: codes `a` [m, k] with a scale
     for each row (of :func:`rms_norm_i8`), weights `w` [n, k] with a scale for each output channel, both
     int8; scales and bias float32.  The integer sums are exact (k at most 131071)."""
@@ -305,12 +301,9 @@ def matmul_i8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: 
     else:
         o_type = _type("out", out.dtype)
         _output("out", out, (m, n), out.dtype, dev)
-    lib = nat.lib()
-    need = lib.trs_matmul_i8_workspace_bytes(m, n, k)
-    workspace, ws_ptr = _workspace(workspace, need, stream, dev)
-    rc = lib.trs_matmul_i8(a.data_ptr(), _ld(a), a_scale.data_ptr(), w.data_ptr(), _ld(w), w_scale.data_ptr(),
-                           None if bias is None else bias.data_ptr(), m, n, k, out.data_ptr(), o_type, _ld(out), ws_ptr,
-                           need, _launch_ptr(stream, dev))
+    rc = nat.lib().trs_matmul_i8(a.data_ptr(), _ld(a), a_scale.data_ptr(), w.data_ptr(), _ld(w), w_scale.data_ptr(),
+                                 None if bias is None else bias.data_ptr(), m, n, k, out.data_ptr(), o_type, _ld(out),
+                                 _launch_ptr(stream, dev))
     if rc:
         nat.check(rc, "trs_matmul_i8")
     return out
