@@ -68,6 +68,28 @@ __device__ __forceinline__ void store_vec(typename T::raw* p, const float (&v)[N
   *reinterpret_cast<U*>(p) = x;
 }
 
+// 8 elements as they lie in memory, for loads that are to be on their way together: converted when they are
+// used, since a conversion waits for its load.
+template <class T>
+using raw8 = typename vec_of<T, 8>::type;
+
+template <class T>
+__device__ __forceinline__ raw8<T> load_raw(const typename T::raw* p) {
+  typedef raw8<T> U __attribute__((aligned(sizeof(typename T::raw))));
+  return *reinterpret_cast<const U*>(p);
+}
+
+// The same of a row narrower than 8: n elements, the rest zeros.
+template <class T>
+__device__ __forceinline__ raw8<T> load_raw_narrow(const typename T::raw* p, int n) {
+  raw8<T> v;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = p[i < n ? i : n - 1];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = i < n ? v[i] : (typename T::raw)0.f;
+  return v;
+}
+
 // A chunk of 8 elements of a row of `width`; narrower rows (n < 8 elements) element by element, the
 // rest of the chunk zero.
 template <class T>

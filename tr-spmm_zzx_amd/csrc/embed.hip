@@ -7,6 +7,8 @@
 // owner for each output row, no float atomics, and sums in a fixed order, so equal inputs give equal
 // bits: the ids are sorted (stable, by counting digits), equal ids then lie together and are summed as
 // runs, 32-bit sums, rounded once when the row is written.
+#include <type_traits>
+
 #include "dense.hpp"
 
 namespace trs {
@@ -47,123 +49,137 @@ __global__ __launch_bounds__(kThreads) void k_embed(const typename T::raw* __res
 }
 
 // ---------------------------------------------------------------------------------------------
-// Gradient: sort of the ids.  Least significant digit first; a pass counts the digits of each block of
-// ids (k_digit_count), turns each digit's counts into offsets (k_digit_offsets) and moves the ids with
-// their positions (k_digit_move).  The order of equal digits is kept: a wave ranks 64 ids at a time with
-// ballots, waves and blocks follow one another.  Ids outside the table get the key `rows`, sort last and
-// take part in nothing.
+// Gradient: sort of the ids, for many of them.  Least significant digit first; a pass counts the digits of
+// each block of ids (k_digit_count), turns each digit's counts into offsets (k_digit_offsets) and moves the ids
+// with their positions (k_digit_move).  The order of equal digits is kept: a wave ranks 64 ids at a time with
+// ballots, waves and blocks follow one another.  Ids outside the table are left out in the first pass, whose
+// move writes how many are left (`kept`).
 constexpr int kMaxBits = 11;
 constexpr int kMaxBins = 1 << kMaxBits;
-constexpr int kRounds = 8;                       // ids of a lane in a block
-constexpr int kBlockIds = kThreads * kRounds;    // 2048
-constexpr int kWaves = kThreads / 64;
+constexpr int kSortThreads = 1024;
+constexpr int kSortWaves = kSortThreads / 64;
+constexpr int kRounds = 4;                           // ids of a lane in a block
+constexpr int kBlockIds = kSortThreads * kRounds;    // 4096
 
+// An id and where it stands among the ids: moved, and read, as one word.
+struct __align__(8) Entry { uint32_t key, at; };
+
+// The i-th id (of the call, or of an earlier pass), and whether it names a row.
 template <class I>
-__device__ __forceinline__ uint32_t key_of(const I* ids, int64_t i, uint32_t rows) {
-  const int64_t id = (int64_t)ids[i];
-  return id >= 0 && id < (int64_t)rows ? (uint32_t)id : rows;
-}
-// the sorted keys of an earlier pass
-struct sorted_t { uint32_t v; };
-template <>
-__device__ __forceinline__ uint32_t key_of<sorted_t>(const sorted_t* ids, int64_t i, uint32_t) { return ids[i].v; }
-
-template <class I>
-__global__ __launch_bounds__(kThreads) void k_digit_count(const I* __restrict__ ids, uint32_t count, uint32_t rows, int shift,
-                                                          int bins, uint32_t blocks, uint32_t* __restrict__ counts,
-                                                          uint32_t* __restrict__ present, uint32_t present_words) {
-  __shared__ uint32_t bin[kMaxBins];
-  for (int b = threadIdx.x; b < bins; b += kThreads) bin[b] = 0;
-  if (present)   // the first pass clears the marks that the moves of this pass set
-    for (uint32_t w = blockIdx.x * kThreads + threadIdx.x; w < present_words; w += gridDim.x * kThreads) present[w] = 0;
-  __syncthreads();
-  const uint32_t first = blockIdx.x * kBlockIds;
-#pragma unroll
-  for (int r = 0; r < kRounds; ++r) {
-    const uint32_t i = first + r * kThreads + threadIdx.x;
-    if (i < count) atomicAdd(&bin[(key_of<I>(ids, i, rows) >> shift) & (uint32_t)(bins - 1)], 1u);
+__device__ __forceinline__ bool entry_of(const I* ids, uint32_t i, uint32_t rows, Entry& e) {
+  if constexpr (std::is_same<I, Entry>::value) {
+    e = ids[i];
+    return true;
+  } else {
+    const int64_t id = (int64_t)ids[i];
+    e = {(uint32_t)id, i};
+    return id >= 0 && id < (int64_t)rows;
   }
-  __syncthreads();
-  for (int b = threadIdx.x; b < bins; b += kThreads) counts[(size_t)b * blocks + blockIdx.x] = bin[b];
-}
-
-// counts[digit][block] becomes the number of ids with that digit in earlier blocks; totals[digit] all.
-__global__ __launch_bounds__(kThreads) void k_digit_offsets(uint32_t* __restrict__ counts, uint32_t blocks, int bins,
-                                                            uint32_t* __restrict__ totals) {
-  const int digit = blockIdx.x * kWaves + threadIdx.x / 64, lane = threadIdx.x & 63;
-  if (digit >= bins) return;
-  uint32_t* row = counts + (size_t)digit * blocks;
-  uint32_t before = 0;
-  for (uint32_t b0 = 0; b0 < blocks; b0 += 64) {
-    const uint32_t mine = b0 + lane < blocks ? row[b0 + lane] : 0;
-    uint32_t upto = mine;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const uint32_t other = __shfl_up(upto, d);
-      if (lane >= d) upto += other;
-    }
-    if (b0 + lane < blocks) row[b0 + lane] = before + upto - mine;
-    before += __shfl(upto, 63);
-  }
-  if (lane == 0) totals[digit] = before;
 }
 
 template <class I, bool FIRST>
-__global__ __launch_bounds__(kThreads) void k_digit_move(const I* __restrict__ ids, const uint32_t* __restrict__ at_in,
-                                                         uint32_t count, uint32_t rows, int shift, int bits, uint32_t blocks,
-                                                         const uint32_t* __restrict__ counts,
-                                                         const uint32_t* __restrict__ totals, uint32_t* __restrict__ key_out,
-                                                         uint32_t* __restrict__ at_out, uint32_t* __restrict__ present) {
-  __shared__ uint32_t base[kMaxBins];              // digit -> first place of this block's ids with it
-  __shared__ uint16_t seen[kWaves][kMaxBins];      // ids with the digit in this wave, then in the waves before it
-  __shared__ uint32_t wave_sum[kWaves];
-  const int bins = 1 << bits, wave = threadIdx.x / 64, lane = threadIdx.x & 63;
-  // exclusive sum of the totals: each thread takes consecutive digits
-  const int per = (bins + kThreads - 1) / kThreads;
-  uint32_t mine = 0;
-  for (int k = 0; k < per; ++k) {
-    const int b = threadIdx.x * per + k;
-    if (b < bins) mine += totals[b];
+__global__ __launch_bounds__(kSortThreads) void k_digit_count(const I* __restrict__ ids, uint32_t count, uint32_t rows,
+                                                              int shift, int bins, const uint32_t* __restrict__ kept,
+                                                              uint32_t* __restrict__ counts) {
+  __shared__ uint32_t bin[kMaxBins];
+  for (int b = threadIdx.x; b < bins; b += kSortThreads) bin[b] = 0;
+  __syncthreads();
+  const uint32_t n = FIRST ? count : *kept, first = blockIdx.x * kBlockIds;
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) {
+    const uint32_t i = first + r * kSortThreads + threadIdx.x;
+    Entry e;
+    if (i < n && entry_of<I>(ids, i, rows, e)) atomicAdd(&bin[(e.key >> shift) & (uint32_t)(bins - 1)], 1u);
   }
-  uint32_t upto = mine;
+  __syncthreads();
+  for (int b = threadIdx.x; b < bins; b += kSortThreads) counts[(size_t)blockIdx.x * bins + b] = bin[b];
+}
+
+// counts[block][digit] becomes the number of ids with that digit in earlier blocks; totals[digit] all.  A
+// workgroup takes 64 digits, a wave a share of the blocks.
+__global__ __launch_bounds__(kSortThreads) void k_digit_offsets(uint32_t* __restrict__ counts, uint32_t blocks, int bins,
+                                                                uint32_t* __restrict__ totals) {
+  __shared__ uint32_t part[kSortWaves][64];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, digit = blockIdx.x * 64 + lane;
+  const uint32_t share = (blocks + kSortWaves - 1) / kSortWaves;
+  const uint32_t b0 = wave * share, b1 = b0 + share < blocks ? b0 + share : blocks;
+  uint32_t sum = 0;
+  if (digit < bins)
+#pragma unroll 8
+    for (uint32_t b = b0; b < b1; ++b) sum += counts[(size_t)b * bins + digit];
+  part[wave][lane] = sum;
+  __syncthreads();
+  uint32_t before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kSortWaves; ++w) {
+    if (w == wave) before = all;
+    all += part[w][lane];
+  }
+  if (digit >= bins) return;
+  if (wave == 0) totals[digit] = all;
+#pragma unroll 4
+  for (uint32_t b = b0; b < b1; ++b) {
+    const uint32_t mine = counts[(size_t)b * bins + digit];
+    counts[(size_t)b * bins + digit] = before;
+    before += mine;
+  }
+}
+
+template <class I, bool FIRST>
+__global__ __launch_bounds__(kSortThreads) void k_digit_move(const I* __restrict__ ids, uint32_t count, uint32_t rows,
+                                                             int shift, int bits, const uint32_t* __restrict__ counts,
+                                                             const uint32_t* __restrict__ totals, uint32_t* __restrict__ kept,
+                                                             Entry* __restrict__ out) {
+  __shared__ uint32_t base[kMaxBins];                 // digit -> first place of this block's ids with it
+  __shared__ uint16_t seen[kSortWaves][kMaxBins];     // ids with the digit in this wave, then in the waves before it
+  __shared__ uint32_t wave_sum[kSortWaves];
+  const int bins = 1 << bits, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const uint32_t n = FIRST ? count : *kept;
+  const uint32_t first = blockIdx.x * kBlockIds + wave * (kRounds * 64);
+  Entry e[kRounds];
+  uint32_t rank[kRounds];
+  bool in[kRounds];
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) {
+    const uint32_t i = first + r * 64 + lane;
+    in[r] = i < n;
+    e[r] = {0, 0};
+    if (in[r]) in[r] = entry_of<I>(ids, i, rows, e[r]);
+  }
+  // exclusive sum of the totals: each thread takes up to two neighbouring digits
+  static_assert(kMaxBins <= 2 * kSortThreads, "two digits a thread");
+  const int d0 = 2 * threadIdx.x;
+  const uint32_t t0 = d0 < bins ? totals[d0] : 0, t1 = d0 + 1 < bins ? totals[d0 + 1] : 0;
+  const uint32_t o0 = d0 < bins ? counts[(size_t)blockIdx.x * bins + d0] : 0;
+  const uint32_t o1 = d0 + 1 < bins ? counts[(size_t)blockIdx.x * bins + d0 + 1] : 0;
+  uint32_t upto = t0 + t1;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
     const uint32_t other = __shfl_up(upto, d);
     if (lane >= d) upto += other;
   }
   if (lane == 63) wave_sum[wave] = upto;
-  for (int b = lane; b < bins; b += 64) seen[wave][b] = 0;
+  for (int b = lane; b < bins / 2; b += 64) reinterpret_cast<uint32_t*>(seen[wave])[b] = 0;
   __syncthreads();
-  uint32_t before = upto - mine;
-  for (int w = 0; w < wave; ++w) before += wave_sum[w];
-  for (int k = 0; k < per; ++k) {
-    const int b = threadIdx.x * per + k;
-    if (b < bins) {
-      base[b] = before + counts[(size_t)b * blocks + blockIdx.x];
-      before += totals[b];
-    }
-  }
+  uint32_t before = upto - t0 - t1;
+#pragma unroll
+  for (int w = 0; w < kSortWaves; ++w) before += w < wave ? wave_sum[w] : 0;
+  if (d0 < bins) base[d0] = before + o0;
+  if (d0 + 1 < bins) base[d0 + 1] = before + t0 + o1;
+  if (FIRST && blockIdx.x == 0 && threadIdx.x == kSortThreads - 1) *kept = before + t0 + t1;
   // rank of each id among the equal digits of its wave
-  const uint32_t first = blockIdx.x * kBlockIds + wave * (kRounds * 64);
-  uint32_t key[kRounds], rank[kRounds];
   const uint64_t below = (1ull << lane) - 1;
 #pragma unroll
   for (int r = 0; r < kRounds; ++r) {
-    const uint32_t i = first + r * 64 + lane;
-    key[r] = i < count ? key_of<I>(ids, i, rows) : 0;
-  }
-#pragma unroll
-  for (int r = 0; r < kRounds; ++r) {
-    const bool in = first + r * 64 + lane < count;
-    const uint32_t digit = (key[r] >> shift) & (uint32_t)(bins - 1);
-    uint64_t same = __ballot(in);
+    const uint32_t digit = (e[r].key >> shift) & (uint32_t)(bins - 1);
+    uint64_t same = __ballot(in[r]);
     for (int b = 0; b < bits; ++b) {
       const bool set = (digit >> b) & 1;
       const uint64_t ones = __ballot(set);
       same &= set ? ones : ~ones;
     }
     rank[r] = 0;
-    if (in) {
+    if (in[r]) {
       const uint32_t earlier = seen[wave][digit];
       rank[r] = earlier + __popcll(same & below);
       wave_fence();
@@ -172,29 +188,22 @@ __global__ __launch_bounds__(kThreads) void k_digit_move(const I* __restrict__ i
     wave_fence();
   }
   __syncthreads();
-  for (int b = threadIdx.x; b < bins; b += kThreads) {
+  for (int b = threadIdx.x; b < bins; b += kSortThreads) {
     uint32_t sum = 0;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const uint32_t n = seen[w][b];
+    for (int w = 0; w < kSortWaves; ++w) {
+      const uint32_t mine = seen[w][b];
       seen[w][b] = (uint16_t)sum;
-      sum += n;
+      sum += mine;
     }
   }
   __syncthreads();
 #pragma unroll
   for (int r = 0; r < kRounds; ++r) {
-    const uint32_t i = first + r * 64 + lane;
-    if (i >= count) continue;
-    const uint32_t digit = (key[r] >> shift) & (uint32_t)(bins - 1);
+    if (!in[r]) continue;
+    const uint32_t digit = (e[r].key >> shift) & (uint32_t)(bins - 1);
     const uint32_t to = base[digit] + seen[wave][digit] + rank[r];
-    key_out[to] = key[r];
-    at_out[to] = FIRST ? i : at_in[i];
-    if (FIRST && key[r] < rows) {   // mark the row; frequent ids mostly find their mark set
-      const uint32_t mark = 1u << (key[r] & 31);
-      uint32_t* word = &present[key[r] >> 5];
-      if (!(__hip_atomic_load(word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) & mark)) atomicOr(word, mark);
-    }
+    out[to] = e[r];
   }
 }
 
@@ -209,10 +218,9 @@ template <class T>
 struct RunArgs {
   const typename T::raw* grad;
   int64_t ldg;
-  const uint32_t* key;
-  const uint32_t* at;
-  const uint32_t* present;
-  uint32_t count, rows, groups_blocks;   // workgroups that walk ids; the others fill
+  const Entry* sorted;
+  const uint32_t* kept;               // how many keys there are; null: none
+  uint32_t rows, groups_blocks;       // workgroups that walk ids (enough for all that were given); the others fill
   int width, out_type;
   float scale;
   void* out;
@@ -233,48 +241,88 @@ __device__ __forceinline__ void write_row(void* out, int out_type, int64_t ldo, 
   else store_chunk<bf16_t>(static_cast<__bf16*>(out) + e, width, v);
 }
 
-__device__ __forceinline__ void fill_rows(const uint32_t* present, uint32_t rows, uint32_t first, uint32_t n, int width,
-                                          void* out, int out_type, int64_t ldo) {
+// The first of n sorted keys that is not below `row`, by the 64 lanes of a wave together.
+__device__ __forceinline__ uint32_t first_of(const Entry* sorted, uint32_t n, uint32_t row, int lane) {
+  uint32_t low = 0, high = n;   // every key before `low` is below `row`, no key from `high` on is
+  while (low < high) {
+    const uint32_t step = (high - low + 63) / 64, i = low + lane * step;
+    const uint64_t under = __ballot(i < high && sorted[i].key < row);
+    if (under == 0) break;                              // not even key[low]
+    const uint32_t top = 63 - __clzll(under);           // the lanes below stand at smaller keys
+    const uint32_t next = low + top * step + step;      // where the lane after stands: not below `row`
+    high = next < high ? next : high;
+    low = low + top * step + 1;
+  }
+  return low;
+}
+
+// Rows first .. first + rows_of_fill(width) - 1 that no key names are filled with zeros.
+constexpr int kMostFill = 2048;
+__device__ __forceinline__ void fill_rows(const Entry* sorted, uint32_t n, uint32_t rows, uint32_t first, uint32_t most,
+                                          int width, void* out, int out_type, int64_t ldo) {
+  __shared__ uint32_t range[2];
+  __shared__ uint8_t named[kMostFill];
+  const uint32_t end = first + most < rows ? first + most : rows;
+  const int wave = threadIdx.x >> 6;
+  if (wave < 2) {
+    const uint32_t found = first_of(sorted, n, wave == 0 ? first : end, threadIdx.x & 63);
+    if ((threadIdx.x & 63) == 0) range[wave] = found;
+  }
+  __syncthreads();
+  const uint32_t r0 = range[0], r1 = range[1];
+  for (uint32_t row = first + threadIdx.x; row < end; row += kThreads) {
+    uint32_t low = r0, high = r1;
+    while (low < high) {
+      const uint32_t mid = (low + high) / 2;
+      if (sorted[mid].key < row) low = mid + 1;
+      else high = mid;
+    }
+    named[row - first] = low < r1 && sorted[low].key == row;
+  }
+  __syncthreads();
   const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   const uint32_t chunks = (uint32_t)(width + 7) / 8;
-  const uint32_t end = first + n < rows ? first + n : rows;
-  // rows x chunks of a workgroup stay below 2^32 (fill_rows_of)
-  const uint32_t total = (end - first) * chunks;
+  const uint32_t total = (end - first) * chunks;   // at most 2048 rows of 8 columns, or a row
   for (uint32_t j = threadIdx.x; j < total; j += kThreads) {
-    const uint32_t dr = j / chunks, row = first + dr;
-    if (present && (present[row >> 5] >> (row & 31) & 1)) continue;   // no marks: no ids at all
+    const uint32_t dr = j / chunks;
+    if (named[dr]) continue;
     int shared;
-    write_row(out, out_type, ldo, row, chunk_at((int)(j - dr * chunks), width, shared), width, 1.f, zero);
+    write_row(out, out_type, ldo, first + dr, chunk_at((int)(j - dr * chunks), width, shared), width, 1.f, zero);
   }
 }
 
-template <class T, int L>
+__global__ __launch_bounds__(kThreads) void k_fill_rows(const Entry* sorted, const uint32_t* kept, uint32_t rows, uint32_t most,
+                                                        int width, void* out, int out_type, int64_t ldo) {
+  fill_rows(sorted, kept ? *kept : 0, rows, blockIdx.x * most, most, width, out, out_type, ldo);
+}
+
+// NARROW: rows of less than 8 columns.
+template <class T, int L, bool NARROW>
 __global__ __launch_bounds__(kThreads) void k_sum_runs(RunArgs<T> p) {
   constexpr int kGroups = kThreads / L;
   constexpr int kIds = kGroups * kPiece;
   __shared__ float part[kGroups][2][L * 8];
   __shared__ uint8_t goes_on[kGroups];   // bit 0: the group's last run goes on; bit 1: so does its only run, which came in
-  if (blockIdx.x >= p.groups_blocks) {
-    if (blockIdx.y == 0)
-      fill_rows(p.present, p.rows, (blockIdx.x - p.groups_blocks) * p.fill_rows, p.fill_rows, p.width, p.out, p.out_type,
-                p.ldo);
-    return;
-  }
+  const uint32_t count = p.kept ? *p.kept : 0;
+  const uint32_t block = blockIdx.x;
+  if (block * kIds >= count) return;
   const int group = threadIdx.x / L, lane = threadIdx.x % L;
   const int chunk = (int)blockIdx.y * L + lane;
   const bool used = chunk * 8 < p.width;
   int shared;
   const int at = chunk_at(used ? chunk : 0, p.width, shared);
-  const uint32_t e0 = blockIdx.x * kIds + group * kPiece;
+  const uint32_t e0 = block * kIds + group * kPiece;
 
-  // the piece's keys, one more on either side; `rows` (no row) past the end
+  // the piece's keys and the one after it; `rows` (no row) past the end
   uint32_t key[kPiece + 1], pos[kPiece];
 #pragma unroll
-  for (int i = 0; i <= kPiece; ++i) key[i] = e0 + i < p.count ? p.key[e0 + i] : p.rows;
-#pragma unroll
-  for (int i = 0; i < kPiece; ++i) pos[i] = key[i] < p.rows ? p.at[e0 + i] : 0;
+  for (int i = 0; i <= kPiece; ++i) {
+    const Entry e = p.sorted[e0 + i < count ? e0 + i : count - 1];
+    key[i] = e0 + i < count ? e.key : p.rows;
+    if (i < kPiece) pos[i] = e.at;
+  }
   const bool some = key[0] < p.rows;
-  bool came = some && e0 > 0 && p.key[e0 - 1] == key[0];
+  bool came = some && e0 > 0 && p.sorted[e0 - 1].key == key[0];
   const bool only = came && key[kPiece] == key[0];
   const bool starts_on = some && key[kPiece - 1] < p.rows && key[kPiece] == key[kPiece - 1] && !only;
   if (lane == 0) goes_on[group] = (uint8_t)((starts_on || only ? 1 : 0) | (only ? 2 : 0));
@@ -283,16 +331,17 @@ __global__ __launch_bounds__(kThreads) void k_sum_runs(RunArgs<T> p) {
   const bool head = came;
 #pragma unroll
   for (int half = 0; half < kPiece; half += 8) {
-    float row[8][8];
+    raw8<T> row[8];   // all on their way; one past the end is some other row, and not used
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if (used && key[half + i] < p.rows) load_chunk<T>(p.grad + (int64_t)pos[half + i] * p.ldg + at, p.width, row[i]);
+      const typename T::raw* from = p.grad + (int64_t)pos[half + i] * p.ldg + at;
+      row[i] = NARROW ? load_raw_narrow<T>(from, p.width) : load_raw<T>(from);
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       if (key[half + i] >= p.rows || !used) continue;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) acc[j] += row[i][j];
+      for (int j = 0; j < 8; ++j) acc[j] += (float)row[i][j];
       const bool last = half + i == kPiece - 1;
       if (key[half + i + 1] != key[half + i] || last) {
         const bool on = key[half + i + 1] == key[half + i];   // only at the piece's end
@@ -329,7 +378,7 @@ __global__ __launch_bounds__(kThreads) void k_sum_runs(RunArgs<T> p) {
     }
     if (!used) continue;
     if (which == 1 || on) {
-      float* to = p.parts + ((int64_t)blockIdx.x * 2 + (which == 1 ? 0 : 1)) * p.part_ld + (int64_t)blockIdx.y * (L * 8) + lane * 8;
+      float* to = p.parts + ((int64_t)block * 2 + (which == 1 ? 0 : 1)) * p.part_ld + (int64_t)blockIdx.y * (L * 8) + lane * 8;
 #pragma unroll
       for (int j = 0; j < 8; ++j) to[j] = acc[j];
     } else {
@@ -346,9 +395,10 @@ __global__ __launch_bounds__(kThreads) void k_join_runs(RunArgs<T> p) {
   constexpr uint32_t kIds = kGroups * kPiece;
   __shared__ float part[kGroups][L * 8];
   __shared__ uint32_t first_end;
-  const uint32_t s = blockIdx.x * kIds, e = s + kIds;   // e < count: the last workgroup has no launch
-  const uint32_t key = p.key[e - 1];
-  if (key >= p.rows || p.key[e] != key || (s > 0 && p.key[s - 1] == key)) return;
+  const uint32_t count = *p.kept, s = blockIdx.x * kIds, e = s + kIds;
+  if (e >= count) return;
+  const uint32_t key = p.sorted[e - 1].key;
+  if (p.sorted[e].key != key || (s > 0 && p.sorted[s - 1].key == key)) return;
   // the workgroup in which the run ends: the first whose last id is another, or is the last of the run
   if (threadIdx.x == 0) first_end = 0xffffffffu;
   __syncthreads();
@@ -356,7 +406,7 @@ __global__ __launch_bounds__(kThreads) void k_join_runs(RunArgs<T> p) {
   for (uint32_t w0 = blockIdx.x + 1; end == 0xffffffffu; w0 += kThreads) {
     const uint32_t w = w0 + threadIdx.x;
     const int64_t next = ((int64_t)w + 1) * kIds;
-    if (next >= (int64_t)p.count || p.key[next - 1] != key || p.key[next] != key) atomicMin(&first_end, w);
+    if (next >= (int64_t)count || p.sorted[next - 1].key != key || p.sorted[next].key != key) atomicMin(&first_end, w);
     __syncthreads();
     end = first_end;
     __syncthreads();
@@ -384,6 +434,182 @@ __global__ __launch_bounds__(kThreads) void k_join_runs(RunArgs<T> p) {
     for (int j = 0; j < 8; ++j) acc[j] += part[g][lane * 8 + j];
   int shared;
   write_row(p.out, p.out_type, p.ldo, key, chunk_at((int)blockIdx.y * L + lane, p.width, shared), p.width, p.scale, acc);
+}
+
+// ---------------------------------------------------------------------------------------------
+// Gradient of few ids (at most kFewIds), in one launch: each workgroup owns some of the table's rows, looks
+// all ids over for them, sorts the ones it finds in LDS and sums their runs; the rows it found none for are
+// filled.  Rows are owned in units (of at least 256 bytes) that are dealt out so that neither neighbouring
+// nor evenly spaced ids meet in one workgroup: unit q belongs to owner (q ^ q >> bits) mod 2^bits.
+constexpr int kFewThreads = 512;
+constexpr int kFewWaves = kFewThreads / 64;
+constexpr uint32_t kFewBits = 13, kFewIds = 1u << kFewBits;
+constexpr uint32_t kFewRows = 65536;     // rows of a workgroup: marks in LDS
+constexpr uint32_t kLongRun = 64;        // longer ones are summed by the whole workgroup
+
+template <class T>
+struct FewArgs {
+  const typename T::raw* grad;
+  int64_t ldg;
+  const void* ids;
+  int id_bits;
+  uint32_t count, rows;
+  int width;
+  float scale;
+  void* out;
+  int out_type;
+  int64_t ldo;
+  int owner_bits, unit_bits;
+  uint32_t local_rows;   // rows of an owner, those past the table's end among them
+};
+
+template <class T, int L>
+__global__ __launch_bounds__(kFewThreads) void k_grad_few(FewArgs<T> p) {
+  constexpr int kGroups = kFewThreads / L;
+  extern __shared__ uint32_t found[];      // count, rounded up to a power of two: local row << kFewBits | place of the id
+  __shared__ uint32_t marks[kFewRows / 32];
+  __shared__ float part[kFewWaves][L * 8];
+  __shared__ uint32_t n_found, n_long, long_at[kFewIds / kLongRun];
+  const uint32_t owner = blockIdx.x, owner_mask = (1u << p.owner_bits) - 1, unit_mask = (1u << p.unit_bits) - 1;
+  for (uint32_t k = threadIdx.x; k < (p.local_rows + 31) / 32; k += kFewThreads) marks[k] = 0;
+  if (threadIdx.x == 0) n_found = n_long = 0;
+  __syncthreads();
+  for (uint32_t i0 = threadIdx.x; i0 < p.count; i0 += 4 * kFewThreads) {
+    int64_t id[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const uint32_t i = i0 + u * kFewThreads, at = i < p.count ? i : i0;
+      id[u] = p.id_bits == 32 ? (int64_t) static_cast<const int32_t*>(p.ids)[at] : static_cast<const int64_t*>(p.ids)[at];
+      if (i >= p.count) id[u] = -1;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (id[u] < 0 || id[u] >= (int64_t)p.rows) continue;
+      const uint32_t row = (uint32_t)id[u], unit = row >> p.unit_bits, high = unit >> p.owner_bits;
+      if (((unit ^ high) & owner_mask) != owner) continue;
+      const uint32_t local = high << p.unit_bits | (row & unit_mask);
+      found[atomicAdd(&n_found, 1u)] = local << kFewBits | (i0 + u * kFewThreads);
+      atomicOr(&marks[local >> 5], 1u << (local & 31));
+    }
+  }
+  __syncthreads();
+  const uint32_t n = n_found;
+  auto row_of = [&](uint32_t local) {
+    const uint32_t high = local >> p.unit_bits;
+    return (high << p.owner_bits | ((owner ^ high) & owner_mask)) << p.unit_bits | (local & unit_mask);
+  };
+  {   // rows without ids
+    const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    const uint32_t chunks = (uint32_t)(p.width + 7) / 8;
+    for (uint64_t j = threadIdx.x; j < (uint64_t)p.local_rows * chunks; j += kFewThreads) {
+      const uint32_t local = (uint32_t)(j / chunks), row = row_of(local);
+      if (row >= p.rows || (marks[local >> 5] >> (local & 31) & 1)) continue;
+      int shared;
+      write_row(p.out, p.out_type, p.ldo, row, chunk_at((int)(j - (uint64_t)local * chunks), p.width, shared), p.width, 1.f, zero);
+    }
+  }
+  if (n == 0) return;
+  // Sort: the words are all different.  Up to a word a thread by rank, more by a bitonic network.
+  if (n <= kFewThreads) {
+    uint32_t mine = 0, rank = 0;
+    if (threadIdx.x < n) {
+      mine = found[threadIdx.x];
+      for (uint32_t j = 0; j < n; ++j) rank += found[j] < mine;
+    }
+    __syncthreads();
+    if (threadIdx.x < n) found[rank] = mine;
+    __syncthreads();
+  } else {
+    uint32_t size = kFewThreads;
+    while (size < n) size *= 2;   // at most count rounded up: found[] holds them
+    for (uint32_t j = n + threadIdx.x; j < size; j += kFewThreads) found[j] = 0xffffffffu;
+    for (uint32_t width = 2; width <= size; width *= 2)
+      for (uint32_t d = width / 2; d > 0; d /= 2) {
+        __syncthreads();
+        for (uint32_t j = threadIdx.x; j < size / 2; j += kFewThreads) {
+          const uint32_t low = j / d * 2 * d + j % d, high = low + d;
+          const uint32_t a = found[low], b = found[high];
+          if ((a > b) == ((low & width) == 0)) {
+            found[low] = b;
+            found[high] = a;
+          }
+        }
+      }
+    __syncthreads();
+  }
+  // Runs: a group of lanes each, in the order of the ids; long ones after them.
+  const int group = threadIdx.x / L, lane = threadIdx.x % L;
+  auto add = [&](uint32_t first, uint32_t end, int at, float (&acc)[8]) {
+    for (uint32_t i = first; i < end; i += 4) {
+      raw8<T> row[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const uint32_t place = found[i + u < end ? i + u : first] & (kFewIds - 1);
+        const typename T::raw* from = p.grad + (int64_t)place * p.ldg + at;
+        row[u] = L > 1 || p.width >= 8 ? load_raw<T>(from) : load_raw_narrow<T>(from, p.width);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (i + u < end)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) acc[j] += (float)row[u][j];
+    }
+  };
+  const int columns = (p.width + L * 8 - 1) / (L * 8);
+  for (uint32_t i = group; i < n; i += kGroups) {
+    const uint32_t local = found[i] >> kFewBits;
+    if (i > 0 && found[i - 1] >> kFewBits == local) continue;
+    uint32_t end = i + 1;
+    while (end < n && end - i <= kLongRun && found[end] >> kFewBits == local) ++end;
+    if (end - i > kLongRun) {
+      if (lane == 0) long_at[atomicAdd(&n_long, 1u)] = i;
+      continue;
+    }
+    for (int c = 0; c < columns; ++c) {
+      int shared;
+      const int chunk = c * L + lane, at = chunk_at(chunk * 8 < p.width ? chunk : 0, p.width, shared);
+      float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      add(i, end, at, acc);
+      if (chunk * 8 < p.width) write_row(p.out, p.out_type, p.ldo, row_of(local), at, p.width, p.scale, acc);
+    }
+  }
+  __syncthreads();
+  const uint32_t longs = n_long;
+  for (uint32_t q = 0; q < longs; ++q) {
+    const uint32_t i = long_at[q], local = found[i] >> kFewBits;
+    uint32_t low = i + kLongRun, high = n;   // its end
+    while (low < high) {
+      const uint32_t mid = (low + high) / 2;
+      if (found[mid] >> kFewBits == local) low = mid + 1;
+      else high = mid;
+    }
+    const uint32_t share = (low - i + kGroups - 1) / kGroups;
+    const uint32_t k0 = i + group * share < low ? i + group * share : low, k1 = k0 + share < low ? k0 + share : low;
+    for (int c = 0; c < columns; ++c) {
+      int shared;
+      const int chunk = c * L + lane, at = chunk_at(chunk * 8 < p.width ? chunk : 0, p.width, shared);
+      float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      add(k0, k1, at, acc);
+      // the groups of a wave, then the waves
+#pragma unroll
+      for (int d = L; d < 64; d <<= 1)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[j] += __shfl_xor(acc[j], d);
+      if ((threadIdx.x & 63) < L)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) part[threadIdx.x >> 6][lane * 8 + j] = acc[j];
+      __syncthreads();
+      if (group == 0) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[j] = part[0][lane * 8 + j];
+        for (int w = 1; w < kFewWaves; ++w)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) acc[j] += part[w][lane * 8 + j];
+        if (chunk * 8 < p.width) write_row(p.out, p.out_type, p.ldo, row_of(local), at, p.width, p.scale, acc);
+      }
+      __syncthreads();
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -422,26 +648,25 @@ int group_lanes(int width) {
 }
 
 // Rows of a filling workgroup: about 64 KB of output.
-uint32_t rows_of_fill(int width) { return (uint32_t)(width >= 16384 ? 1 : 16384 / width); }
+uint32_t rows_of_fill(int width) { return (uint32_t)(width >= 16384 ? 1 : width <= 8 ? kMostFill : 16384 / width); }
 int64_t fill_blocks(int64_t rows, int width) { return ceil_div(rows, rows_of_fill(width)); }
 
 // How the sort and the sums lie in the workspace.
 struct GradLayout {
   int lanes, bits, passes;
-  uint32_t blocks, run_blocks, words;
-  int64_t part_ld, key[2], at[2], counts, totals, present, parts, bytes;
+  uint32_t blocks, run_blocks;
+  int64_t part_ld, entries[2], counts, totals, kept, parts, bytes;
 };
 
 GradLayout grad_layout(int64_t count, int64_t rows, int width) {
   GradLayout g{};
   int need = 1;
-  while (need < 32 && (rows >> need) != 0) ++need;   // bits of the largest key, `rows`
+  while (need < 31 && (rows - 1) >> need != 0) ++need;   // bits of the largest key
   g.passes = (need + kMaxBits - 1) / kMaxBits;
   g.bits = (need + g.passes - 1) / g.passes;
   g.lanes = group_lanes(width);
   g.blocks = (uint32_t)ceil_div(count, kBlockIds);
   g.run_blocks = (uint32_t)ceil_div(count, (int64_t)(kThreads / g.lanes) * kPiece);
-  g.words = (uint32_t)ceil_div(rows, 32);
   g.part_ld = round_up(width, 8 * g.lanes);
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
@@ -449,44 +674,41 @@ GradLayout grad_layout(int64_t count, int64_t rows, int width) {
     at += round_up(bytes, 256);
     return here;
   };
-  for (int k = 0; k < (g.passes > 1 ? 2 : 1); ++k) {
-    g.key[k] = take(4 * count);
-    g.at[k] = take(4 * count);
-  }
+  for (int k = 0; k < (g.passes > 1 ? 2 : 1); ++k) g.entries[k] = take((int64_t)sizeof(Entry) * count);
   g.counts = take(((int64_t)4 << g.bits) * g.blocks);
   g.totals = take((int64_t)4 << g.bits);
-  g.present = take((int64_t)4 * g.words);
+  g.kept = take(4);
   g.parts = take((int64_t)g.run_blocks * 2 * g.part_ld * 4);
   g.bytes = at;
   return g;
 }
 
 template <class I, bool FIRST>
-void sort_pass(const GradLayout& g, const I* ids, const uint32_t* at_in, int64_t count, int64_t rows, int pass, char* ws,
-               uint32_t* key_out, uint32_t* at_out, hipStream_t s) {
+void sort_pass(const GradLayout& g, const I* ids, int64_t count, int64_t rows, int pass, char* ws, Entry* out,
+               hipStream_t s) {
   uint32_t* counts = reinterpret_cast<uint32_t*>(ws + g.counts);
   uint32_t* totals = reinterpret_cast<uint32_t*>(ws + g.totals);
-  uint32_t* present = FIRST ? reinterpret_cast<uint32_t*>(ws + g.present) : nullptr;
+  uint32_t* kept = reinterpret_cast<uint32_t*>(ws + g.kept);
   const int bins = 1 << g.bits, shift = pass * g.bits;
-  k_digit_count<I><<<dim3(g.blocks), kThreads, 0, s>>>(ids, (uint32_t)count, (uint32_t)rows, shift, bins, g.blocks, counts,
-                                                       present, g.words);
-  k_digit_offsets<<<dim3((bins + kWaves - 1) / kWaves), kThreads, 0, s>>>(counts, g.blocks, bins, totals);
-  k_digit_move<I, FIRST><<<dim3(g.blocks), kThreads, 0, s>>>(ids, at_in, (uint32_t)count, (uint32_t)rows, shift, g.bits,
-                                                             g.blocks, counts, totals, key_out, at_out, present);
+  k_digit_count<I, FIRST><<<dim3(g.blocks), kSortThreads, 0, s>>>(ids, (uint32_t)count, (uint32_t)rows, shift, bins, kept, counts);
+  k_digit_offsets<<<dim3((bins + 63) / 64), kSortThreads, 0, s>>>(counts, g.blocks, bins, totals);
+  k_digit_move<I, FIRST><<<dim3(g.blocks), kSortThreads, 0, s>>>(ids, (uint32_t)count, (uint32_t)rows, shift, g.bits, counts,
+                                                                 totals, kept, out);
 }
 
-template <class T, int L>
+template <class T, int L, bool NARROW = false>
 void launch_runs(RunArgs<T>& p, const GradLayout& g, hipStream_t s) {
   const uint32_t columns = (uint32_t)ceil_div(p.width, 8 * L);
   const uint32_t fills = (uint32_t)fill_blocks(p.rows, p.width);
-  k_sum_runs<T, L><<<dim3(g.run_blocks + fills, columns), kThreads, 0, s>>>(p);
+  k_fill_rows<<<dim3(fills), kThreads, 0, s>>>(p.sorted, p.kept, p.rows, p.fill_rows, p.width, p.out, p.out_type, p.ldo);
+  if (g.run_blocks) k_sum_runs<T, L, NARROW><<<dim3(g.run_blocks, columns), kThreads, 0, s>>>(p);
   if (g.run_blocks > 1) k_join_runs<T, L><<<dim3(g.run_blocks - 1, columns), kThreads, 0, s>>>(p);
 }
 
 template <class T>
 void launch_runs_of(RunArgs<T>& p, const GradLayout& g, hipStream_t s) {
   switch (g.lanes) {
-    case 1: return launch_runs<T, 1>(p, g, s);
+    case 1: return p.width < 8 ? launch_runs<T, 1, true>(p, g, s) : launch_runs<T, 1>(p, g, s);
     case 2: return launch_runs<T, 2>(p, g, s);
     case 4: return launch_runs<T, 4>(p, g, s);
     case 8: return launch_runs<T, 8>(p, g, s);
@@ -503,12 +725,10 @@ void grad_runs(const GradLayout& g, int sorted, const void* grad, int64_t ldg, i
   p.grad = static_cast<const typename T::raw*>(grad);
   p.ldg = ldg;
   if (count > 0) {
-    p.key = reinterpret_cast<const uint32_t*>(ws + g.key[sorted]);
-    p.at = reinterpret_cast<const uint32_t*>(ws + g.at[sorted]);
+    p.sorted = reinterpret_cast<const Entry*>(ws + g.entries[sorted]);
+    p.kept = reinterpret_cast<const uint32_t*>(ws + g.kept);
     p.parts = reinterpret_cast<float*>(ws + g.parts);
   }
-  p.present = count > 0 ? reinterpret_cast<const uint32_t*>(ws + g.present) : nullptr;
-  p.count = (uint32_t)count;
   p.rows = (uint32_t)rows;
   p.groups_blocks = g.run_blocks;
   p.width = width;
@@ -519,6 +739,41 @@ void grad_runs(const GradLayout& g, int sorted, const void* grad, int64_t ldg, i
   p.part_ld = g.part_ld;
   p.fill_rows = rows_of_fill(width);
   launch_runs_of<T>(p, g, s);
+}
+
+// How k_grad_few deals the rows out; false: too many rows for its workgroups.
+struct FewPlan { int owner_bits, unit_bits; uint32_t local_rows; };
+bool few_plan(int64_t count, int64_t rows, int width, int out_type, FewPlan& f) {
+  if (count > kFewIds) return false;
+  const int64_t bytes = (int64_t)width * (out_type == TRS_F32 ? 4 : 2);
+  f.unit_bits = 0;
+  while (bytes << f.unit_bits < 256) ++f.unit_bits;
+  const int64_t units = ceil_div(rows, 1 << f.unit_bits);
+  f.owner_bits = 0;
+  while (f.owner_bits < 9 && units >> f.owner_bits > 1) ++f.owner_bits;   // 512 workgroups at most
+  const int64_t local = ceil_div(units, 1 << f.owner_bits) << f.unit_bits;
+  f.local_rows = (uint32_t)local;
+  return local <= kFewRows;
+}
+
+template <class T>
+void launch_few(const FewPlan& f, const void* grad, int64_t ldg, const void* ids, int id_bits, int64_t count, int64_t rows,
+                int width, float scale, void* out, int32_t out_type, int64_t ldo, hipStream_t s) {
+  const FewArgs<T> p{static_cast<const typename T::raw*>(grad), ldg, ids, id_bits, (uint32_t)count, (uint32_t)rows, width,
+                     scale, out, out_type, ldo, f.owner_bits, f.unit_bits, f.local_rows};
+  uint32_t size = kFewThreads;
+  while (size < count) size *= 2;
+  const dim3 grid(1u << f.owner_bits);
+  const size_t lds = size * sizeof(uint32_t);
+  switch (group_lanes(width)) {
+    case 1: k_grad_few<T, 1><<<grid, kFewThreads, lds, s>>>(p); break;
+    case 2: k_grad_few<T, 2><<<grid, kFewThreads, lds, s>>>(p); break;
+    case 4: k_grad_few<T, 4><<<grid, kFewThreads, lds, s>>>(p); break;
+    case 8: k_grad_few<T, 8><<<grid, kFewThreads, lds, s>>>(p); break;
+    case 16: k_grad_few<T, 16><<<grid, kFewThreads, lds, s>>>(p); break;
+    case 32: k_grad_few<T, 32><<<grid, kFewThreads, lds, s>>>(p); break;
+    default: k_grad_few<T, 64><<<grid, kFewThreads, lds, s>>>(p);
+  }
 }
 
 // What both calls check of their ids and rows.
@@ -555,8 +810,11 @@ extern "C" int trs_embed(const void* table, int32_t table_type, int64_t ldt, int
   return launched("trs_embed");
 }
 
+// The size does not depend on the output's type: a call takes k_grad_few if it could with either size of one.
 extern "C" int64_t trs_embed_grad_workspace_bytes(int64_t count, int64_t rows, int32_t width) {
   if (count <= 0 || rows <= 0 || width <= 0 || count >= INT32_MAX || rows >= INT32_MAX) return 0;
+  FewPlan few;
+  if (few_plan(count, rows, width, TRS_F32, few) && few_plan(count, rows, width, TRS_F16, few)) return 0;
   return grad_layout(count, rows, width).bytes;
 }
 
@@ -571,6 +829,13 @@ extern "C" int trs_embed_grad(const void* grad, int32_t grad_type, int64_t ldg, 
   if (ldg < width || ldo < width) return fail(TRS_EINVAL, "trs_embed_grad: leading dimension < width");
   if (count >= INT32_MAX || rows >= INT32_MAX) return fail(TRS_ERANGE, "trs_embed_grad: 2^31 - 1 ids or rows at most");
   hipStream_t s = static_cast<hipStream_t>(stream);
+  FewPlan few;
+  if (trs_embed_grad_workspace_bytes(count, rows, width) == 0 && few_plan(count, rows, width, out_type, few)) {
+    if (grad_type == TRS_F32) launch_few<f32_t>(few, grad, ldg, ids, id_bits, count, rows, width, scale, out, out_type, ldo, s);
+    else if (grad_type == TRS_F16) launch_few<f16_t>(few, grad, ldg, ids, id_bits, count, rows, width, scale, out, out_type, ldo, s);
+    else launch_few<bf16_t>(few, grad, ldg, ids, id_bits, count, rows, width, scale, out, out_type, ldo, s);
+    return launched("trs_embed_grad");
+  }
   GradLayout g{};   // no ids: nothing to sort, every row is filled
   if (count > 0) {
     g = grad_layout(count, rows, width);
@@ -585,17 +850,13 @@ extern "C" int trs_embed_grad(const void* grad, int32_t grad_type, int64_t ldg, 
   int sorted = 0;
   for (int pass = 0; pass < g.passes; ++pass) {
     sorted = pass & 1;
-    uint32_t* key_out = reinterpret_cast<uint32_t*>(ws + g.key[sorted]);
-    uint32_t* at_out = reinterpret_cast<uint32_t*>(ws + g.at[sorted]);
-    if (pass > 0) {
-      const int from = sorted ^ 1;
-      sort_pass<sorted_t, false>(g, reinterpret_cast<const sorted_t*>(ws + g.key[from]),
-                                 reinterpret_cast<const uint32_t*>(ws + g.at[from]), count, rows, pass, ws, key_out, at_out, s);
-    } else if (id_bits == 32) {
-      sort_pass<int32_t, true>(g, static_cast<const int32_t*>(ids), nullptr, count, rows, 0, ws, key_out, at_out, s);
-    } else {
-      sort_pass<int64_t, true>(g, static_cast<const int64_t*>(ids), nullptr, count, rows, 0, ws, key_out, at_out, s);
-    }
+    Entry* to = reinterpret_cast<Entry*>(ws + g.entries[sorted]);
+    if (pass > 0)
+      sort_pass<Entry, false>(g, reinterpret_cast<const Entry*>(ws + g.entries[sorted ^ 1]), count, rows, pass, ws, to, s);
+    else if (id_bits == 32)
+      sort_pass<int32_t, true>(g, static_cast<const int32_t*>(ids), count, rows, 0, ws, to, s);
+    else
+      sort_pass<int64_t, true>(g, static_cast<const int64_t*>(ids), count, rows, 0, ws, to, s);
   }
   if (grad_type == TRS_F32) grad_runs<f32_t>(g, sorted, grad, ldg, count, rows, width, scale, out, out_type, ldo, ws, s);
   else if (grad_type == TRS_F16) grad_runs<f16_t>(g, sorted, grad, ldg, count, rows, width, scale, out, out_type, ldo, ws, s);

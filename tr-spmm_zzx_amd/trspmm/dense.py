@@ -79,13 +79,14 @@ def _empty(stream, shape, dtype, dev: int) -> torch.Tensor:
 
 
 def _workspace(workspace: Optional[torch.Tensor], need: int, stream, dev: int) -> Tuple[Optional[torch.Tensor], int]:
+    if workspace is not None:
+        if not (workspace.is_cuda and workspace.is_contiguous()):
+            raise ValueError("workspace must be a contiguous CUDA tensor")
+        _on_device("workspace", workspace, dev)
     if not need:
         return None, 0
     if workspace is None or workspace.numel() * workspace.element_size() < need:
         workspace = _empty(stream, need, torch.uint8, dev)
-    if not (workspace.is_cuda and workspace.is_contiguous()):
-        raise ValueError("workspace must be a contiguous CUDA tensor")
-    _on_device("workspace", workspace, dev)
     return workspace, workspace.data_ptr()
 
 
