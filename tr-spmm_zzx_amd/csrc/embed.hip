@@ -291,11 +291,6 @@ __device__ __forceinline__ void fill_rows(const Entry* sorted, uint32_t n, uint3
   }
 }
 
-__global__ __launch_bounds__(kThreads) void k_fill_rows(const Entry* sorted, const uint32_t* kept, uint32_t rows, uint32_t most,
-                                                        int width, void* out, int out_type, int64_t ldo) {
-  fill_rows(sorted, kept ? *kept : 0, rows, blockIdx.x * most, most, width, out, out_type, ldo);
-}
-
 // NARROW: rows of less than 8 columns.
 template <class T, int L, bool NARROW>
 __global__ __launch_bounds__(kThreads) void k_sum_runs(RunArgs<T> p) {
@@ -305,6 +300,11 @@ __global__ __launch_bounds__(kThreads) void k_sum_runs(RunArgs<T> p) {
   __shared__ uint8_t goes_on[kGroups];   // bit 0: the group's last run goes on; bit 1: so does its only run, which came in
   const uint32_t count = p.kept ? *p.kept : 0;
   const uint32_t block = blockIdx.x;
+  if (block >= p.groups_blocks) {
+    if (blockIdx.y == 0)
+      fill_rows(p.sorted, count, p.rows, (block - p.groups_blocks) * p.fill_rows, p.fill_rows, p.width, p.out, p.out_type, p.ldo);
+    return;
+  }
   if (block * kIds >= count) return;
   const int group = threadIdx.x / L, lane = threadIdx.x % L;
   const int chunk = (int)blockIdx.y * L + lane;
@@ -700,8 +700,7 @@ template <class T, int L, bool NARROW = false>
 void launch_runs(RunArgs<T>& p, const GradLayout& g, hipStream_t s) {
   const uint32_t columns = (uint32_t)ceil_div(p.width, 8 * L);
   const uint32_t fills = (uint32_t)fill_blocks(p.rows, p.width);
-  k_fill_rows<<<dim3(fills), kThreads, 0, s>>>(p.sorted, p.kept, p.rows, p.fill_rows, p.width, p.out, p.out_type, p.ldo);
-  if (g.run_blocks) k_sum_runs<T, L, NARROW><<<dim3(g.run_blocks, columns), kThreads, 0, s>>>(p);
+  k_sum_runs<T, L, NARROW><<<dim3(g.run_blocks + fills, columns), kThreads, 0, s>>>(p);
   if (g.run_blocks > 1) k_join_runs<T, L><<<dim3(g.run_blocks - 1, columns), kThreads, 0, s>>>(p);
 }
 

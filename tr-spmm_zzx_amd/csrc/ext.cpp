@@ -437,6 +437,8 @@ std::vector<torch::Tensor> sptc_mma_packed_online(torch::Tensor s_tile_column, t
 
 }  // namespace
 
+void bind_dense(pybind11::module_& m);   // ext_dense.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("block_sptc_2to4_online", &block_sptc_2to4_online,
         "Hybrid format builder: 16-row windows -> TC blocks, 2:4 groups, CSR residual (29 arrays + time)");
@@ -459,4 +461,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("forward_fp16_sptc_online", &sptc_online, "2:4 group SpMM, rows from s_window");
   m.def("forward_fp16_sptc_mma_online", &sptc_mma_online, "2:4 group SpMM, windows from s_offsets");
   m.def("forward_fp16_sptc_mma_packed_online", &sptc_mma_packed_online, "2:4 group SpMM from packed tiles");
+  bind_dense(m);
 }

@@ -154,7 +154,7 @@ def check(rc: int, where: str) -> None:
 
 
 def ext():
-    """The PyTorch extension with the reference operator signatures."""
+    """The PyTorch extension: the reference operator signatures, and the dense operators on tensors."""
     global _ext
     if _ext is None:
         lib()
