@@ -90,6 +90,11 @@ __device__ __forceinline__ raw8<T> load_raw_narrow(const typename T::raw* p, int
   return v;
 }
 
+template <class T>
+__device__ __forceinline__ raw8<T> load_raw_any(const typename T::raw* p, int n) {
+  return n >= 8 ? load_raw<T>(p) : load_raw_narrow<T>(p, n);
+}
+
 // A chunk of 8 elements of a row of `width`; narrower rows (n < 8 elements) element by element, the
 // rest of the chunk zero.
 template <class T>

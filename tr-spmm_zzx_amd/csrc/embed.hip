@@ -29,22 +29,28 @@ __global__ __launch_bounds__(kThreads) void k_embed(const typename T::raw* __res
   const int64_t first = (int64_t)blockIdx.x * (kThreads * kLookups);
   const int64_t t0 = first / chunks;
   const uint32_t c0 = (uint32_t)(first - t0 * chunks);
+  int64_t t[kLookups], id[kLookups];
+  int at[kLookups];
 #pragma unroll
   for (int u = 0; u < kLookups; ++u) {
     const uint32_t j = c0 + (uint32_t)(u * kThreads) + threadIdx.x;
     const uint32_t dt = j / (uint32_t)chunks;
-    const int64_t t = t0 + dt;
-    if (t >= count) continue;
     int shared;
-    const int at = chunk_at((int)(j - dt * (uint32_t)chunks), width, shared);
-    const int64_t id = (int64_t)ids[t];
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (id >= 0 && id < rows) {
-      load_chunk<T>(table + id * ldt + at, width, v);
+    at[u] = chunk_at((int)(j - dt * (uint32_t)chunks), width, shared);
+    t[u] = t0 + dt;
+    id[u] = (int64_t)ids[t[u] < count ? t[u] : count - 1];
+  }
+  raw8<T> row[kLookups] = {};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] *= scale;
-    }
-    store_chunk<O>(out + t * ldo + at, width, v);
+  for (int u = 0; u < kLookups; ++u)
+    if (id[u] >= 0 && id[u] < rows) row[u] = load_raw_any<T>(table + id[u] * ldt + at[u], width);
+#pragma unroll
+  for (int u = 0; u < kLookups; ++u) {
+    if (t[u] >= count) continue;
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (float)row[u][i] * scale;
+    store_chunk<O>(out + t[u] * ldo + at[u], width, v);
   }
 }
 
@@ -445,7 +451,7 @@ constexpr int kFewThreads = 512;
 constexpr int kFewWaves = kFewThreads / 64;
 constexpr uint32_t kFewBits = 13, kFewIds = 1u << kFewBits;
 constexpr uint32_t kFewRows = 65536;     // rows of a workgroup: marks in LDS
-constexpr uint32_t kLongRun = 64;        // longer ones are summed by the whole workgroup
+constexpr uint32_t kLongRun = 16;        // longer ones are summed by the whole workgroup
 
 template <class T>
 struct FewArgs {
@@ -538,18 +544,19 @@ __global__ __launch_bounds__(kFewThreads) void k_grad_few(FewArgs<T> p) {
     __syncthreads();
   }
   // Runs: a group of lanes each, in the order of the ids; long ones after them.
+  constexpr int kAhead = 8;   // rows on their way together
   const int group = threadIdx.x / L, lane = threadIdx.x % L;
   auto add = [&](uint32_t first, uint32_t end, int at, float (&acc)[8]) {
-    for (uint32_t i = first; i < end; i += 4) {
-      raw8<T> row[4];
+    for (uint32_t i = first; i < end; i += kAhead) {
+      raw8<T> row[kAhead];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < kAhead; ++u) {
         const uint32_t place = found[i + u < end ? i + u : first] & (kFewIds - 1);
         const typename T::raw* from = p.grad + (int64_t)place * p.ldg + at;
         row[u] = L > 1 || p.width >= 8 ? load_raw<T>(from) : load_raw_narrow<T>(from, p.width);
       }
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
+      for (int u = 0; u < kAhead; ++u)
         if (i + u < end)
 #pragma unroll
           for (int j = 0; j < 8; ++j) acc[j] += (float)row[u][j];

@@ -15,6 +15,7 @@
 #include "dense.hpp"
 
 #include <cfloat>
+#include <type_traits>
 
 namespace trs {
 namespace dense {
@@ -113,25 +114,30 @@ __global__ __launch_bounds__(kThreads) void k_norm(NormArgs p) {
   const int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / G;
   if (row >= p.rows) return;   // a whole group
   const int chunks = (p.width + 7) / 8;
+  // All loads are on their way before the first is waited for.  A lane without a chunk reads the first one, counts
+  // nothing of it and writes nothing.
+  constexpr bool kRes = !is_none<R>;
+  raw8<X> x[NC];
+  raw8<typename std::conditional<kRes, R, X>::type> res[NC];
   float h[NC][8], w[NC][8];
   int at[NC], dup[NC];
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     const int chunk = c * G + lane;
     at[c] = chunk_at(chunk < chunks ? chunk : 0, p.width, dup[c]);
-    if (chunk >= chunks) { dup[c] = 8; at[c] = -1; }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) h[c][i] = w[c][i] = 0.f;
-    if (at[c] < 0) continue;
-    load_chunk<X>(static_cast<const typename X::raw*>(p.x) + row * p.ldx + at[c], p.width, h[c]);
-    load_any(p.weight, p.w_type, at[c], p.width, w[c]);
-    if constexpr (!is_none<R>) {
-      float v[8];
-      load_chunk<R>(static_cast<const typename R::raw*>(p.res) + row * p.ldr + at[c], p.width, v);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) h[c][i] += v[i];
-    }
+    if (chunk >= chunks) dup[c] = 8;
+    x[c] = load_raw_any<X>(static_cast<const typename X::raw*>(p.x) + row * p.ldx + at[c], p.width);
+    if constexpr (kRes) res[c] = load_raw_any<R>(static_cast<const typename R::raw*>(p.res) + row * p.ldr + at[c], p.width);
   }
+#pragma unroll
+  for (int c = 0; c < NC; ++c) load_any(p.weight, p.w_type, at[c], p.width, w[c]);
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      h[c][i] = (float)x[c][i];
+      if constexpr (kRes) h[c][i] += (float)res[c][i];
+    }
   float sum = 0.f;
 #pragma unroll
   for (int c = 0; c < NC; ++c)
@@ -153,7 +159,7 @@ __global__ __launch_bounds__(kThreads) void k_norm(NormArgs p) {
   uint32_t peak = 0;
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
-    if (at[c] < 0) continue;
+    if (dup[c] == 8) continue;
     if constexpr (!is_none<R>)
       store_chunk<R>(static_cast<typename R::raw*>(p.r) + row * p.ldro + at[c], p.width, h[c]);
 #pragma unroll
@@ -171,7 +177,7 @@ __global__ __launch_bounds__(kThreads) void k_norm(NormArgs p) {
     if (lane == 0) p.scale[row] = some ? most / 127.f : finite ? 0.f : __builtin_nanf("");
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      if (at[c] < 0) continue;
+      if (dup[c] == 8) continue;
       if (!finite)
 #pragma unroll
         for (int i = 0; i < 8; ++i) h[c][i] = 0.f;
@@ -260,47 +266,77 @@ struct GradArgs {
   float* rstd;           // long rows: [rows][2], the norm's factor and the mean of g u
 };
 
+// Two sums at once.
+template <int G>
+__device__ __forceinline__ void group_sums(float& a, float& b, float* red) {
+#pragma unroll
+  for (int d = (G < 64 ? G : 64) / 2; d > 0; d >>= 1) {
+    a += __shfl_xor(a, d);
+    b += __shfl_xor(b, d);
+  }
+  if constexpr (G > 64) {
+    if ((threadIdx.x & 63) == 0) {
+      red[threadIdx.x >> 6] = a;
+      red[4 + (threadIdx.x >> 6)] = b;
+    }
+    __syncthreads();
+    a = (red[0] + red[1]) + (red[2] + red[3]);
+    b = (red[4] + red[5]) + (red[6] + red[7]);
+  }
+}
+
 template <class D, class R, int G, int NC>
 __global__ __launch_bounds__(kThreads) void k_norm_grad(GradArgs p) {
   constexpr int kRows = kThreads / G;
-  __shared__ float red[2][4][4];
+  __shared__ float red[2][2][8];
   __shared__ float joined[kRows > 1 ? kThreads * NC * 8 : 1];
   const int lane = threadIdx.x % G, group = threadIdx.x / G;
   const int chunks = (p.width + 7) / 8;
   float w[NC][8], dw[NC][8];
-  int at[NC], dup[NC];
+  int at[NC], dup[NC];   // a lane without a chunk reads the first one, counts nothing of it and writes nothing
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     const int chunk = c * G + lane;
     at[c] = chunk_at(chunk < chunks ? chunk : 0, p.width, dup[c]);
-    if (chunk >= chunks) { dup[c] = 8; at[c] = -1; }
+    if (chunk >= chunks) dup[c] = 8;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) dw[c][i] = w[c][i] = 0.f;
-    if (at[c] >= 0) load_any(p.weight, p.w_type, at[c], p.width, w[c]);
+    for (int i = 0; i < 8; ++i) dw[c][i] = 0.f;
   }
   const int64_t first = (int64_t)blockIdx.x * p.share;
   const int64_t end = first + p.share < p.rows ? first + p.share : p.rows;
+  // The next row is on its way while this one is reduced and written.
+  struct Row { raw8<R> r[NC], more[NC]; raw8<D> g[NC]; };
+  auto load = [&](Row& x, int64_t row) {
+    const typename R::raw* r = static_cast<const typename R::raw*>(p.r) + row * p.ldr;
+    const typename D::raw* g = static_cast<const typename D::raw*>(p.grad) + row * p.ldg;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) x.r[c] = load_raw_any<R>(r + at[c], p.width);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) x.g[c] = load_raw_any<D>(g + at[c], p.width);
+    if (p.grad_r) {
+      const typename R::raw* more = static_cast<const typename R::raw*>(p.grad_r) + row * p.ldgr;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) x.more[c] = load_raw_any<R>(more + at[c], p.width);
+    }
+  };
+  Row next = {};
+  if (first + group < end) load(next, first + group);
+#pragma unroll
+  for (int c = 0; c < NC; ++c) load_any(p.weight, p.w_type, at[c], p.width, w[c]);
   int turn = 0;
   for (int64_t row = first + group; row < end; row += kRows, turn ^= 1) {
-    float r[NC][8], g[NC][8];
+    const Row x = next;
+    if (row + kRows < end) load(next, row + kRows);
     float square = 0.f, dot = 0.f;
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) r[c][i] = g[c][i] = 0.f;
-      if (at[c] < 0) continue;
-      load_chunk<R>(static_cast<const typename R::raw*>(p.r) + row * p.ldr + at[c], p.width, r[c]);
-      load_chunk<D>(static_cast<const typename D::raw*>(p.grad) + row * p.ldg + at[c], p.width, g[c]);
-    }
 #pragma unroll
     for (int c = 0; c < NC; ++c)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        square += i >= dup[c] ? r[c][i] * r[c][i] : 0.f;
-        dot += i >= dup[c] ? g[c][i] * w[c][i] * r[c][i] : 0.f;
+        const float r = (float)x.r[c][i], g = (float)x.g[c][i];
+        square += i >= dup[c] ? r * r : 0.f;
+        dot += i >= dup[c] ? g * w[c][i] * r : 0.f;
       }
-    square = group_sum<G>(square, red[turn][0]);
-    dot = group_sum<G>(dot, red[turn][1]);
+    group_sums<G>(square, dot, red[turn][0]);
     float s = rstd_of(square, p.width, p.eps), f = 1.f;
     if (!(square <= FLT_MAX)) {
       f = kSmall;
@@ -309,27 +345,24 @@ __global__ __launch_bounds__(kThreads) void k_norm_grad(GradArgs p) {
       for (int c = 0; c < NC; ++c)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          r[c][i] *= f;
-          square += i >= dup[c] ? r[c][i] * r[c][i] : 0.f;
-          dot += i >= dup[c] ? g[c][i] * w[c][i] * r[c][i] : 0.f;
+          const float r = (float)x.r[c][i] * f, g = (float)x.g[c][i];
+          square += i >= dup[c] ? r * r : 0.f;
+          dot += i >= dup[c] ? g * w[c][i] * r : 0.f;
         }
-      square = group_sum<G>(square, red[turn][2]);
-      dot = group_sum<G>(dot, red[turn][3]);
+      group_sums<G>(square, dot, red[turn][1]);
       s = rstd_of(square, p.width, 0.f);
     }
     const float mean = dot * s / (float)p.width;   // of g u
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      if (at[c] < 0) continue;
-      float out[8], more[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (p.grad_r) load_chunk<R>(static_cast<const typename R::raw*>(p.grad_r) + row * p.ldgr + at[c], p.width, more);
+      float out[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float u = r[c][i] * s;
-        dw[c][i] += g[c][i] * u;
-        out[i] = (s * f) * (g[c][i] * w[c][i] - u * mean) + more[i];
+        const float u = (float)x.r[c][i] * f * s, g = (float)x.g[c][i];
+        dw[c][i] += g * u;
+        out[i] = (s * f) * (g * w[c][i] - u * mean) + (float)x.more[c][i];
       }
-      store_chunk<R>(static_cast<typename R::raw*>(p.dr) + row * p.lddr + at[c], p.width, out);
+      if (dup[c] < 8) store_chunk<R>(static_cast<typename R::raw*>(p.dr) + row * p.lddr + at[c], p.width, out);
     }
   }
   float* to = p.sums + (int64_t)blockIdx.x * chunks * 8;
@@ -348,7 +381,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_grad(GradArgs p) {
   } else {
 #pragma unroll
     for (int c = 0; c < NC; ++c)
-      if (at[c] >= 0)
+      if (dup[c] < 8)
 #pragma unroll
         for (int i = 0; i < 8; ++i) to[(c * G + lane) * 8 + i] = dw[c][i];
   }
@@ -421,28 +454,33 @@ __global__ __launch_bounds__(kThreads) void k_norm_grad_columns(GradArgs p) {
   for (int i = 0; i < 8; ++i) to[i] = dw[i];
 }
 
-// dweight[c] = sum of the workgroups' sums of column c, 16 shares in order.  `overlapped`: the last chunk of a
-// row is its last 8 elements.
-constexpr int kSumWaves = 16;
-__global__ __launch_bounds__(64 * kSumWaves) void k_column_sums(const float* __restrict__ sums, int64_t blocks, int width,
-                                                                int overlapped, float* __restrict__ out) {
-  __shared__ float part[kSumWaves][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int column = blockIdx.x * 64 + lane;
+// dweight[c] = sum of the workgroups' sums of column c: 64 shares of them side by side, then the shares, in a fixed
+// order.  `overlapped`: the last chunk of a row is its last 8 elements.
+constexpr int kSumThreads = 1024, kSumColumns = 16;
+__global__ __launch_bounds__(kSumThreads) void k_column_sums(const float* __restrict__ sums, int64_t blocks, int width,
+                                                             int overlapped, float* __restrict__ out) {
+  __shared__ float part[kSumThreads / 64][kSumColumns];
+  const int lane = threadIdx.x % kSumColumns, slice = threadIdx.x / kSumColumns;
+  constexpr int kSlices = kSumThreads / kSumColumns;
+  const int column = blockIdx.x * kSumColumns + lane;
   const int last = (width + 7) / 8 - 1;
   const int64_t ld = (int64_t)(last + 1) * 8;
   int at = column;
   if (overlapped && column >= last * 8 && width >= 8) at = last * 8 + (column - (width - 8));
-  const int64_t share = (blocks + kSumWaves - 1) / kSumWaves;
-  const int64_t b0 = wave * share, b1 = b0 + share < blocks ? b0 + share : blocks;
+  const int64_t share = (blocks + kSlices - 1) / kSlices;
+  const int64_t b0 = slice * share, b1 = b0 + share < blocks ? b0 + share : blocks;
   float sum = 0.f;
   if (column < width)
 #pragma unroll 8
     for (int64_t b = b0; b < b1; ++b) sum += sums[b * ld + at];
-  part[wave][lane] = sum;
+#pragma unroll
+  for (int d = kSumColumns; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+  if ((threadIdx.x & 63) < kSumColumns) part[threadIdx.x >> 6][lane] = sum;
   __syncthreads();
-  if (wave != 0 || column >= width) return;
-  for (int k = 1; k < kSumWaves; ++k) sum += part[k][lane];
+  if (threadIdx.x >= kSumColumns || column >= width) return;
+  sum = part[0][lane];
+#pragma unroll
+  for (int k = 1; k < kSumThreads / 64; ++k) sum += part[k][lane];
   out[column] = sum;
 }
 
@@ -458,6 +496,7 @@ void launch_norm(const NormArgs& p, hipStream_t s) {
   else if (w <= 128) k_norm<X, R, CODES, 16, 1><<<blocks(16), kThreads, 0, s>>>(p);
   else if (w <= 256) k_norm<X, R, CODES, 32, 1><<<blocks(8), kThreads, 0, s>>>(p);
   else if (w <= 512) k_norm<X, R, CODES, 64, 1><<<blocks(4), kThreads, 0, s>>>(p);
+  else if (w <= 1024 && p.rows >= 1024) k_norm<X, R, CODES, 64, 2><<<blocks(4), kThreads, 0, s>>>(p);
   else if (w <= 2048) k_norm<X, R, CODES, 256, 1><<<blocks(1), kThreads, 0, s>>>(p);
   else if (w <= 4096) k_norm<X, R, CODES, 256, 2><<<blocks(1), kThreads, 0, s>>>(p);
   else if (w <= kNormMost) k_norm<X, R, CODES, 256, 4><<<blocks(1), kThreads, 0, s>>>(p);
@@ -500,12 +539,16 @@ int norm_call(const char* where, const NormArgs& p, int x_type, int r_type, void
   return launched(where);
 }
 
-// Workgroups of the gradient: enough to fill the chip (256 CUs), each with at least a few rows.
-int64_t grad_blocks(int64_t rows) { return rows < 1024 ? rows : 1024; }
+// Workgroups of the gradient: their sums of the weight's gradient are written and read again, so wide rows get fewer
+// (16384 x 4096 with 256, 512, 1024 workgroups: 108, 113, 117 us; 4099 x 1000: 14.6, 13.5, 18.3; 262144 x 96: 65, 45, 44).
+int64_t grad_blocks(int64_t rows, int width) {
+  const int64_t most = width <= 512 ? 1024 : width <= 2048 ? 512 : 256;
+  return rows < most ? rows : most;
+}
 
 template <class D, class R>
 void launch_grad(GradArgs p, float* dweight, hipStream_t s) {
-  int64_t blocks = grad_blocks(p.rows);
+  int64_t blocks = grad_blocks(p.rows, p.width);
   p.share = ceil_div(p.rows, blocks);
   blocks = ceil_div(p.rows, p.share);
   const dim3 grid((uint32_t)blocks);
@@ -515,6 +558,7 @@ void launch_grad(GradArgs p, float* dweight, hipStream_t s) {
   else if (w <= 128) k_norm_grad<D, R, 16, 1><<<grid, kThreads, 0, s>>>(p);
   else if (w <= 256) k_norm_grad<D, R, 32, 1><<<grid, kThreads, 0, s>>>(p);
   else if (w <= 512) k_norm_grad<D, R, 64, 1><<<grid, kThreads, 0, s>>>(p);
+  else if (w <= 1024) k_norm_grad<D, R, 64, 2><<<grid, kThreads, 0, s>>>(p);
   else if (w <= 2048) k_norm_grad<D, R, 256, 1><<<grid, kThreads, 0, s>>>(p);
   else if (w <= 4096) k_norm_grad<D, R, 256, 2><<<grid, kThreads, 0, s>>>(p);
   else if (w <= kNormMost) k_norm_grad<D, R, 256, 4><<<grid, kThreads, 0, s>>>(p);
@@ -523,7 +567,7 @@ void launch_grad(GradArgs p, float* dweight, hipStream_t s) {
     k_norm_grad_long<D, R><<<dim3((uint32_t)p.rows), kThreads, 0, s>>>(p);
     k_norm_grad_columns<D, R><<<dim3((uint32_t)blocks, (uint32_t)ceil_div(w, kThreads * 8)), kThreads, 0, s>>>(p);
   }
-  k_column_sums<<<dim3((uint32_t)ceil_div(w, 64)), 64 * kSumWaves, 0, s>>>(p.sums, blocks, w, overlapped, dweight);
+  k_column_sums<<<dim3((uint32_t)ceil_div(w, kSumColumns)), kSumThreads, 0, s>>>(p.sums, blocks, w, overlapped, dweight);
 }
 
 template <class D>
@@ -564,7 +608,7 @@ extern "C" int trs_rms_norm_i8(const void* x, int32_t x_type, int64_t ldx, const
 
 extern "C" int64_t trs_rms_norm_grad_workspace_bytes(int64_t rows, int32_t width) {
   if (rows <= 0 || width <= 0) return 0;
-  const int64_t sums = round_up(grad_blocks(rows) * round_up(width, 8) * 4, 256);
+  const int64_t sums = round_up(grad_blocks(rows, width) * round_up(width, 8) * 4, 256);
   return sums + (width > kNormMost ? rows * 8 : 0);
 }
 
@@ -591,7 +635,7 @@ extern "C" int trs_rms_norm_grad(const void* grad, int32_t grad_type, int64_t ld
     return fail(TRS_EINVAL, w + "workspace smaller than trs_rms_norm_grad_workspace_bytes");
   if (dr == grad || dr == r) return fail(TRS_EINVAL, w + "dr cannot take the place of grad or r");
   char* ws = static_cast<char*>(workspace);
-  const int64_t sums = round_up(grad_blocks(rows) * round_up(width, 8) * 4, 256);
+  const int64_t sums = round_up(grad_blocks(rows, width) * round_up(width, 8) * 4, 256);
   const GradArgs p{grad, r, weight, grad_r, ldg, ldr, ldgr, w_type, width, eps, rows, 0, dr, lddr,
                    reinterpret_cast<float*>(ws), reinterpret_cast<float*>(ws + sums)};
   const bool known = grad_type == TRS_F32   ? launch_grad_r<f32_t>(p, r_type, dweight, s)
