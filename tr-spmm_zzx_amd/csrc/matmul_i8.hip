@@ -5,6 +5,8 @@
 // Both operands lie along k, as the matrix instructions (v_mfma_i32_32x32x32_i8, _16x16x64_i8) take them: 16
 // codes of a row in each lane.  The sums are 32-bit integers, exact for k <= kMostK, so their order does not
 // matter; the scales and the bias are applied in 32-bit floats and the result rounded once.
+#include <type_traits>
+
 #include "dense.hpp"
 
 namespace trs {
@@ -25,28 +27,43 @@ struct MatArgs {
   int n, k, out_type;
 };
 
-// 16 codes of a row from column `at` on; zeros past the row's end (zeros add nothing to the sums).  A piece that
-// the end cuts is the row's last 16 codes, shifted.
-__device__ __forceinline__ int4_v load_codes(const int8_t* row, int at, int k) {
-  if (at + 16 <= k) return *reinterpret_cast<const int4_u*>(row + at);
-  union { int8_t c[16]; uint64_t q[2]; int4_v v; } u;
-  u.v = int4_v{0, 0, 0, 0};
-  if (at >= k) return u.v;
-  if (k >= 16) {
-    u.v = *reinterpret_cast<const int4_u*>(row + k - 16);
-    const int bits = 8 * (at + 16 - k);   // 8 .. 120
-    if (bits >= 64) {
-      u.q[0] = u.q[1] >> (bits - 64);
-      u.q[1] = 0;
-    } else {
-      u.q[0] = u.q[0] >> bits | u.q[1] << (64 - bits);
-      u.q[1] >>= bits;
-    }
+// 16 codes at any address.  ODD: where rows do not start on 4-byte boundaries, by the 4-byte words that hold them (a
+// 16-byte load off those boundaries takes several times as long: 24 x 104 x 3545 10.7 us, with words 6.8); each word holds a
+// code of the row.
+template <bool ODD>
+__device__ __forceinline__ int4_v load16(const int8_t* p) {
+  if constexpr (!ODD) {
+    return *reinterpret_cast<const int4_u*>(p);
   } else {
+    typedef int4_v int4_w __attribute__((aligned(4)));
+    const uint32_t off = (uint32_t)(reinterpret_cast<uintptr_t>(p) & 3);
+    const int8_t* word = p - off;
+    const int4_v low = *reinterpret_cast<const int4_w*>(word);
+    const int high = *reinterpret_cast<const int*>(word + (off ? 16 : 0));   // not needed where off is 0
+    return int4_v{(int)__builtin_amdgcn_alignbyte(low[1], low[0], off), (int)__builtin_amdgcn_alignbyte(low[2], low[1], off),
+                  (int)__builtin_amdgcn_alignbyte(low[3], low[2], off), (int)__builtin_amdgcn_alignbyte(high, low[3], off)};
+  }
+}
+
+// 16 codes of a row from column `at` on; zeros past the row's end (zeros add nothing to the sums).  Without a
+// branch, so that several are on their way together: a piece that the end cuts is the row's last 16 codes, moved
+// down.
+template <bool ODD>
+__device__ __forceinline__ int4_v load_codes(const int8_t* row, int at, int k) {
+  union { int8_t c[16]; uint64_t q[2]; int4_v v; } u;
+  if (k < 16) {   // the same in every lane
+    u.v = int4_v{0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < 16; ++i)
       if (at + i < k) u.c[i] = row[at + i];
+    return u.v;
   }
+  const int from = at < k - 16 ? at : k - 16, bits = 8 * (at - from);
+  u.v = load16<ODD>(row + from);
+  const uint64_t low = u.q[0], high = u.q[1];
+  const uint64_t over = bits == 0 ? 0 : high << (64 - (bits & 63));
+  u.q[0] = bits >= 128 ? 0 : bits >= 64 ? high >> (bits & 63) : low >> (bits & 63) | over;
+  u.q[1] = bits >= 64 ? 0 : high >> (bits & 63);
   return u.v;
 }
 
@@ -135,7 +152,8 @@ __device__ __forceinline__ void store_wave(const MatArgs& p, const int16_v (&acc
 // place c ^ (r & 7), so that the 16-byte reads of neighbouring rows spread over the banks.
 //
 // DIRECT: rows on 16-byte boundaries and k a multiple of 16; the pieces go from memory to LDS without
-// registers.  Otherwise any address, through registers.  KS groups of waves split a workgroup's steps, each
+// registers.  Otherwise any address, through registers (4096 x 4096 x 4095: 85 us; by 4-byte words, put together as they
+// arrive, 134: the products wait for them).  KS groups of waves split a workgroup's steps, each
 // with its own tiles, and the first adds the sums up: for few workgroups and a long k.
 constexpr int kDepth = 128;
 
@@ -214,9 +232,9 @@ __device__ __forceinline__ void matmul_tile(const MatArgs& p, uint32_t tiles_m, 
         __builtin_amdgcn_raw_ptr_buffer_load_lds(buf_w, (lds_ptr)(w + (u * kAll + wave * 64) * 16), 16, at_w[u], k0, 0, 0);
     } else {
 #pragma unroll
-      for (int u = 0; u < kLoadsA; ++u) held[u] = *reinterpret_cast<const int4_u*>(base_a + at_a[u] + k0);
+      for (int u = 0; u < kLoadsA; ++u) held[u] = load16<false>(base_a + at_a[u] + k0);
 #pragma unroll
-      for (int u = 0; u < kLoadsW; ++u) held[kLoadsA + u] = *reinterpret_cast<const int4_u*>(base_w + at_w[u] + k0);
+      for (int u = 0; u < kLoadsW; ++u) held[kLoadsA + u] = load16<false>(base_w + at_w[u] + k0);
     }
   };
   auto put = [&](int8_t* a, int8_t* w) {
@@ -231,10 +249,10 @@ __device__ __forceinline__ void matmul_tile(const MatArgs& p, uint32_t tiles_m, 
   auto fetch_rest = [&](int8_t* a, int8_t* w, int k0) {
 #pragma unroll
     for (int u = 0; u < kLoadsA; ++u)
-      *reinterpret_cast<int4_v*>(a + (u * kAll + thread) * 16) = load_codes(base_a + at_a[u] - my_k, k0 + my_k, p.k);
+      *reinterpret_cast<int4_v*>(a + (u * kAll + thread) * 16) = load_codes<!DIRECT>(base_a + at_a[u] - my_k, k0 + my_k, p.k);
 #pragma unroll
     for (int u = 0; u < kLoadsW; ++u)
-      *reinterpret_cast<int4_v*>(w + (u * kAll + thread) * 16) = load_codes(base_w + at_w[u] - my_k, k0 + my_k, p.k);
+      *reinterpret_cast<int4_v*>(w + (u * kAll + thread) * 16) = load_codes<!DIRECT>(base_w + at_w[u] - my_k, k0 + my_k, p.k);
   };
 
   int16_v acc[FM][FN] = {};
@@ -343,7 +361,7 @@ __global__ __launch_bounds__((TM / WM) * (TN / WN) * 64 * KS, 2) void k_matmul_t
 // ---------------------------------------------------------------------------------------------
 // k of one step (at most 128): a tile is read once and its outputs, the bytes that count here, are written; with one
 // set of tiles in LDS several workgroups share a CU, and some read while others write.
-template <int TM, int TN, int WM, int WN>
+template <int TM, int TN, int WM, int WN, bool ODD>
 __global__ __launch_bounds__((TM / WM) * (TN / WN) * 64, 4) void k_matmul_once(MatArgs p, uint32_t tiles_m, uint32_t tiles_n) {
   constexpr int kWaveRows = TM / WM, kWavesOf = kWaveRows * (TN / WN), kAll = kWavesOf * 64;
   constexpr int FM = WM / 32, FN = WN / 32, kPart = 32 * kOutPitch<FN>;
@@ -366,7 +384,7 @@ __global__ __launch_bounds__((TM / WM) * (TN / WN) * 64, 4) void k_matmul_once(M
     const int8_t* from;
     if (u * kPerLoad < TM) from = p.a + (m0 + r < p.m ? m0 + r : p.m - 1) * p.lda;
     else from = p.w + (int64_t)(n0 + r - TM < p.n ? n0 + r - TM : p.n - 1) * p.ldw;
-    *reinterpret_cast<int4_v*>(lds + (u * kAll + threadIdx.x) * 16) = load_codes(from, my_k, p.k);
+    *reinterpret_cast<int4_v*>(lds + (u * kAll + threadIdx.x) * 16) = load_codes<ODD>(from, my_k, p.k);
   }
   __syncthreads();
   int16_v acc[FM][FN] = {};
@@ -392,7 +410,7 @@ __global__ __launch_bounds__((TM / WM) * (TN / WN) * 64, 4) void k_matmul_once(M
 // Few rows: 16 FM rows and 16 output channels a workgroup, its waves taking turns at 128 codes of k each, so that
 // the weights -- the bytes that count here -- arrive by as many loads in flight as fit.  The waves' sums are
 // added up in LDS.
-template <int FM>
+template <int FM, bool ODD>
 __global__ __launch_bounds__(1024) void k_matmul_rows(MatArgs p, uint32_t blocks_n) {
   __shared__ int sums[16][FM * 256];
   const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6, lane = threadIdx.x & 63;
@@ -407,32 +425,30 @@ __global__ __launch_bounds__(1024) void k_matmul_rows(MatArgs p, uint32_t blocks
     a[i] = p.a + (m < p.m ? m : p.m - 1) * p.lda;
   }
   int4_v acc[FM] = {};
-  constexpr int kAhead = FM > 2 ? 1 : 2;   // pieces of 128 codes on their way together
-  const int whole = p.k / 128;
-  int t = wave;
-  for (; t + (kAhead - 1) * waves < whole; t += kAhead * waves) {
+  // `ahead` pieces of 128 codes on their way together, the first at t
+  auto pieces = [&](auto ahead, int t, auto&& codes) {
+    constexpr int kAhead = decltype(ahead)::value;
     int4_v fw[2 * kAhead], fa[2 * kAhead][FM];
 #pragma unroll
     for (int u = 0; u < 2 * kAhead; ++u) {
       const int at = (t + u / 2 * waves) * 128 + u % 2 * 64 + piece;
-      fw[u] = *reinterpret_cast<const int4_u*>(w + at);
+      fw[u] = codes(w, at);
 #pragma unroll
-      for (int i = 0; i < FM; ++i) fa[u][i] = *reinterpret_cast<const int4_u*>(a[i] + at);
+      for (int i = 0; i < FM; ++i) fa[u][i] = codes(a[i], at);
     }
 #pragma unroll
     for (int u = 0; u < 2 * kAhead; ++u)
 #pragma unroll
       for (int i = 0; i < FM; ++i) acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[u], fa[u][i], acc[i], 0, 0, 0);
-  }
-  for (; t * 128 < p.k; t += waves) {   // what is left, the end of k among it
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int at = t * 128 + u * 64 + piece;
-      const int4_v fw = load_codes(w, at, p.k);
-#pragma unroll
-      for (int i = 0; i < FM; ++i) acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw, load_codes(a[i], at, p.k), acc[i], 0, 0, 0);
-    }
-  }
+  };
+  const auto inside = [](const int8_t* row, int at) { return load16<ODD>(row + at); };
+  const int whole = p.k / 128;
+  int t = wave;
+  if constexpr (FM <= 2)
+    for (; t + waves < whole; t += 2 * waves) pieces(std::integral_constant<int, 2>{}, t, inside);
+  for (; t < whole; t += waves) pieces(std::integral_constant<int, 1>{}, t, inside);
+  if (t * 128 < p.k)   // the end of k
+    pieces(std::integral_constant<int, 1>{}, t, [&](const int8_t* row, int at) { return load_codes<ODD>(row, at, p.k); });
 #pragma unroll
   for (int i = 0; i < FM; ++i)
     *reinterpret_cast<int4_v*>(&sums[wave][(i * 16 + row) * 16 + (lane >> 4) * 4]) = acc[i];
@@ -462,16 +478,20 @@ void launch_tile(const MatArgs& p, hipStream_t s) {
 }
 
 template <int TM, int TN, int WM, int WN>
-void launch_once(const MatArgs& p, hipStream_t s) {
+void launch_once(const MatArgs& p, bool odd, hipStream_t s) {
   const uint32_t tm = (uint32_t)ceil_div(p.m, TM), tn = (uint32_t)ceil_div(p.n, TN);
-  k_matmul_once<TM, TN, WM, WN><<<dim3(tm * tn), (TM / WM) * (TN / WN) * 64, 0, s>>>(p, tm, tn);
+  const dim3 grid(tm * tn);
+  constexpr int kAll = (TM / WM) * (TN / WN) * 64;
+  if (odd) k_matmul_once<TM, TN, WM, WN, true><<<grid, kAll, 0, s>>>(p, tm, tn);
+  else k_matmul_once<TM, TN, WM, WN, false><<<grid, kAll, 0, s>>>(p, tm, tn);
 }
 
 template <int FM>
-void launch_rows(const MatArgs& p, hipStream_t s) {
+void launch_rows(const MatArgs& p, bool odd, hipStream_t s) {
   const uint32_t bn = (uint32_t)ceil_div(p.n, 16), bm = (uint32_t)ceil_div(p.m, 16 * FM);
   const int pieces = (p.k + 127) / 128, waves = pieces >= 16 ? 16 : pieces >= 8 ? 8 : 4;
-  k_matmul_rows<FM><<<dim3(bn * bm), 64 * waves, 0, s>>>(p, bn);
+  if (odd) k_matmul_rows<FM, true><<<dim3(bn * bm), 64 * waves, 0, s>>>(p, bn);
+  else k_matmul_rows<FM, false><<<dim3(bn * bm), 64 * waves, 0, s>>>(p, bn);
 }
 
 int64_t tiles(const MatArgs& p, int tm, int tn) { return ceil_div(p.m, tm) * ceil_div(p.n, tn); }
@@ -528,36 +548,35 @@ void launch_small_tiles(const MatArgs& p, hipStream_t s) {
   else launch_tile<64, 32, 32, 1, DIRECT, Offset>(p, s);
 }
 
+template <bool DIRECT>
+void launch_tiles(const MatArgs& p, hipStream_t s) {
+  switch (tile_side(p, DIRECT)) {
+    case 256: return launch_tile<256, 128, 64, 1, DIRECT, int>(p, s);
+    case 128: return launch_tile<128, 64, 64, 1, DIRECT, int>(p, s);
+  }
+  launch_small_tiles<DIRECT, typename std::conditional<DIRECT, int, int64_t>::type>(p, s);
+}
+
 void launch(const MatArgs& p, hipStream_t s) {
+  const uintptr_t starts = reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.w) | (uintptr_t)p.lda | (uintptr_t)p.ldw;
+  const bool odd = (starts & 3) != 0;
   switch (rows_kernel(p)) {
-    case 1: return launch_rows<1>(p, s);
-    case 2: return launch_rows<2>(p, s);
-    case 4: return launch_rows<4>(p, s);
+    case 1: return launch_rows<1>(p, odd, s);
+    case 2: return launch_rows<2>(p, odd, s);
+    case 4: return launch_rows<4>(p, odd, s);
   }
   if (p.k <= kDepth) {
     // 1000003 x 256 x 128: 240 us with tiles of 64 x 64, 213 of 128 x 128, 171 of 128 x 256; x 128: 120, 106, 136;
     // x 64: 61, 87, 118.  Below two workgroups a CU the smallest (2000 x 500 x 128: 4.1, 6.5, 7.0).
-    if (p.n > 128 && tiles(p, 128, 256) >= 2 * kCus) launch_once<128, 256, 64, 64>(p, s);
-    else if (p.n > 64 && tiles(p, 128, 128) >= 2 * kCus) launch_once<128, 128, 64, 64>(p, s);
-    else launch_once<64, 64, 32, 32>(p, s);
+    if (p.n > 128 && tiles(p, 128, 256) >= 2 * kCus) launch_once<128, 256, 64, 64>(p, odd, s);
+    else if (p.n > 64 && tiles(p, 128, 128) >= 2 * kCus) launch_once<128, 128, 64, 64>(p, odd, s);
+    else launch_once<64, 64, 32, 32>(p, odd, s);
     return;
   }
-  const bool direct = ((reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.w) | (uintptr_t)p.lda | (uintptr_t)p.ldw |
-                        (uintptr_t)p.k) & 15) == 0;
   const int64_t ld = p.lda > p.ldw ? p.lda : p.ldw;
   if (ld * 256 > INT32_MAX) return launch_small_tiles<false, int64_t>(p, s);   // a tile's offsets pass 32 bits
-  switch (tile_side(p, direct)) {
-    case 256:
-      if (direct) launch_tile<256, 128, 64, 1, true, int>(p, s);
-      else launch_tile<256, 128, 64, 1, false, int>(p, s);
-      return;
-    case 128:
-      if (direct) launch_tile<128, 64, 64, 1, true, int>(p, s);
-      else launch_tile<128, 64, 64, 1, false, int>(p, s);
-      return;
-  }
-  if (direct) launch_small_tiles<true, int>(p, s);
-  else launch_small_tiles<false, int64_t>(p, s);
+  if (((starts | (uintptr_t)p.k) & 15) == 0) launch_tiles<true>(p, s);
+  else launch_tiles<false>(p, s);
 }
 
 }  // namespace

@@ -22,6 +22,7 @@ namespace dense {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kNormMost = kThreads * 8 * 4;   // widths in registers
 constexpr float kSmall = 0x1p-80f;       // brings any finite value's square, summed, into range
 constexpr float kLeastPeak = 0x1p-119f;  // below this largest |y|, 127 / max|y| overflows: the row counts as zeros
 
@@ -262,6 +263,7 @@ struct GradArgs {
   int64_t rows, share;   // share: rows of a workgroup
   void* dr;
   int64_t lddr;
+  float* dweight;
   float* sums;           // [workgroup][chunks * 8]
   float* rstd;           // long rows: [rows][2], the norm's factor and the mean of g u
 };
@@ -365,7 +367,9 @@ __global__ __launch_bounds__(kThreads) void k_norm_grad(GradArgs p) {
       if (dup[c] < 8) store_chunk<R>(static_cast<typename R::raw*>(p.dr) + row * p.lddr + at[c], p.width, out);
     }
   }
-  float* to = p.sums + (int64_t)blockIdx.x * chunks * 8;
+  // One workgroup's sums are the weight's gradient; others are laid out chunk by chunk for k_column_sums.
+  const bool alone = gridDim.x == 1;
+  float* to = alone ? p.dweight : p.sums + (int64_t)blockIdx.x * chunks * 8;
   if constexpr (kRows > 1) {
     // the groups' sums in order
 #pragma unroll
@@ -376,14 +380,17 @@ __global__ __launch_bounds__(kThreads) void k_norm_grad(GradArgs p) {
     for (int k = threadIdx.x; k < chunks * 8; k += kThreads) {
       float sum = 0.f;
       for (int q = 0; q < kRows; ++q) sum += joined[q * (NC * G * 8) + k];
-      to[k] = sum;
+      int shared;
+      const int column = chunk_at(k / 8, p.width, shared) + k % 8;   // a narrow row's chunk goes past its end
+      if (!alone) to[k] = sum;
+      else if (column < p.width) to[column] = sum;
     }
   } else {
 #pragma unroll
     for (int c = 0; c < NC; ++c)
       if (dup[c] < 8)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) to[(c * G + lane) * 8 + i] = dw[c][i];
+        for (int i = 0; i < 8; ++i) to[alone ? at[c] + i : (c * G + lane) * 8 + i] = dw[c][i];
   }
 }
 
@@ -486,7 +493,6 @@ __global__ __launch_bounds__(kSumThreads) void k_column_sums(const float* __rest
 
 // ---------------------------------------------------------------------------------------------
 // Host side.
-constexpr int kNormMost = kThreads * 8 * 4;   // widths in registers
 
 template <class X, class R, bool CODES>
 void launch_norm(const NormArgs& p, hipStream_t s) {
@@ -543,11 +549,12 @@ int norm_call(const char* where, const NormArgs& p, int x_type, int r_type, void
 // (16384 x 4096 with 256, 512, 1024 workgroups: 108, 113, 117 us; 4099 x 1000: 14.6, 13.5, 18.3; 262144 x 96: 65, 45, 44).
 int64_t grad_blocks(int64_t rows, int width) {
   const int64_t most = width <= 512 ? 1024 : width <= 2048 ? 512 : 256;
+  if (rows <= 2 && width <= kNormMost) return 1;   // and no second kernel
   return rows < most ? rows : most;
 }
 
 template <class D, class R>
-void launch_grad(GradArgs p, float* dweight, hipStream_t s) {
+void launch_grad(GradArgs p, hipStream_t s) {
   int64_t blocks = grad_blocks(p.rows, p.width);
   p.share = ceil_div(p.rows, blocks);
   blocks = ceil_div(p.rows, p.share);
@@ -567,16 +574,16 @@ void launch_grad(GradArgs p, float* dweight, hipStream_t s) {
     k_norm_grad_long<D, R><<<dim3((uint32_t)p.rows), kThreads, 0, s>>>(p);
     k_norm_grad_columns<D, R><<<dim3((uint32_t)blocks, (uint32_t)ceil_div(w, kThreads * 8)), kThreads, 0, s>>>(p);
   }
-  k_column_sums<<<dim3((uint32_t)ceil_div(w, kSumColumns)), kSumThreads, 0, s>>>(p.sums, blocks, w, overlapped, dweight);
+  if (blocks > 1 || !overlapped) k_column_sums<<<dim3((uint32_t)ceil_div(w, kSumColumns)), kSumThreads, 0, s>>>(p.sums, blocks, w, overlapped, p.dweight);
 }
 
 template <class D>
-bool launch_grad_r(const GradArgs& p, int r_type, float* dweight, hipStream_t s) {
-  if (r_type == D::code) launch_grad<D, D>(p, dweight, s);
-  else if (r_type == TRS_F32) launch_grad<D, f32_t>(p, dweight, s);
+bool launch_grad_r(const GradArgs& p, int r_type, hipStream_t s) {
+  if (r_type == D::code) launch_grad<D, D>(p, s);
+  else if (r_type == TRS_F32) launch_grad<D, f32_t>(p, s);
   else if constexpr (D::code != TRS_F32) return false;
-  else if (r_type == TRS_F16) launch_grad<D, f16_t>(p, dweight, s);
-  else launch_grad<D, bf16_t>(p, dweight, s);
+  else if (r_type == TRS_F16) launch_grad<D, f16_t>(p, s);
+  else launch_grad<D, bf16_t>(p, s);
   return true;
 }
 
@@ -636,11 +643,11 @@ extern "C" int trs_rms_norm_grad(const void* grad, int32_t grad_type, int64_t ld
   if (dr == grad || dr == r) return fail(TRS_EINVAL, w + "dr cannot take the place of grad or r");
   char* ws = static_cast<char*>(workspace);
   const int64_t sums = round_up(grad_blocks(rows, width) * round_up(width, 8) * 4, 256);
-  const GradArgs p{grad, r, weight, grad_r, ldg, ldr, ldgr, w_type, width, eps, rows, 0, dr, lddr,
+  const GradArgs p{grad, r, weight, grad_r, ldg, ldr, ldgr, w_type, width, eps, rows, 0, dr, lddr, dweight,
                    reinterpret_cast<float*>(ws), reinterpret_cast<float*>(ws + sums)};
-  const bool known = grad_type == TRS_F32   ? launch_grad_r<f32_t>(p, r_type, dweight, s)
-                     : grad_type == TRS_F16 ? launch_grad_r<f16_t>(p, r_type, dweight, s)
-                                            : launch_grad_r<bf16_t>(p, r_type, dweight, s);
+  const bool known = grad_type == TRS_F32   ? launch_grad_r<f32_t>(p, r_type, s)
+                     : grad_type == TRS_F16 ? launch_grad_r<f16_t>(p, r_type, s)
+                                            : launch_grad_r<bf16_t>(p, r_type, s);
   if (!known) return fail(TRS_EINVAL, w + "grad and r of two different 16-bit types");
   return launched("trs_rms_norm_grad");
 }
