@@ -247,6 +247,18 @@ def test_many_rows():
     check_grad(g, x, w, None, *trspmm.rms_norm_grad(g, x, w, eps=EPS))
 
 
+def test_more_rows_than_a_launch():
+    """2^24 + 1000 rows of 3: more than 2^32 threads at a workgroup a row; and at 32 rows a workgroup many."""
+    say("rows past a launch")
+    rows = (1 << 24) + 1000
+    x, w, res = rand((rows, 3), torch.float16, 1), weights(3, torch.float16, 2), rand((rows, 3), torch.float16, 3)
+    keep = torch.cat([torch.arange(50), torch.arange((1 << 24) - 50, rows)]).cuda()
+    q, scale, r = trspmm.rms_norm_i8(x, w, res, EPS)
+    check_codes(x[keep], w, res[keep], q[keep], scale[keep], r[keep])
+    y, r = trspmm.rms_norm(x, w, res, EPS)
+    check_norm(x[keep], w, res[keep], y[keep], r[keep])
+
+
 def test_no_rows_no_width():
     say("empty")
     x, w = rand((4, 24), torch.float16, 1), weights(24, torch.float16, 2)

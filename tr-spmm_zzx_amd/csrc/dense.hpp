@@ -19,15 +19,23 @@ void set_error(const std::string& msg);
 
 namespace dense {
 
-inline int fail(int code, const std::string& msg) {
-  set_error(msg);
+// Every failure of an entry point: nothing is thrown past it.
+inline int fail(int code, const char* where, const char* what) noexcept {
+  try {
+    set_error(std::string(where) + ": " + what);
+  } catch (...) {   // no memory for the message
+  }
   return code;
 }
 
-inline int launched(const char* where) {
+inline int launched(const char* where) noexcept {
   const hipError_t e = hipGetLastError();
   if (e == hipSuccess) return TRS_OK;
-  return fail(TRS_EDEVICE, std::string(where) + ": kernel launch failed: " + hipGetErrorString(e));
+  try {
+    set_error(std::string(where) + ": kernel launch failed: " + hipGetErrorString(e));
+  } catch (...) {
+  }
+  return TRS_EDEVICE;
 }
 
 inline bool known_type(int32_t t) { return t == TRS_F32 || t == TRS_F16 || t == TRS_BF16; }
@@ -122,6 +130,19 @@ __device__ __forceinline__ void store_chunk(typename T::raw* p, int n, const flo
 __device__ __forceinline__ void wave_fence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
+}
+
+// A chunk's elements from the shared ones on: for an output that takes an input's place, where an element is
+// written only by the lane whose element it is.
+template <class T>
+__device__ __forceinline__ void store_own(typename T::raw* p, int n, int shared, const float (&v)[8]) {
+  if (shared == 0) {
+    store_chunk<T>(p, n, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i >= shared) p[i] = (typename T::raw)v[i];
+  }
 }
 
 // First element of chunk c of a row of `width`, and how many of its elements the chunk before holds too.

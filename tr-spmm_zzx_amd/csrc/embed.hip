@@ -784,11 +784,10 @@ void launch_few(const FewPlan& f, const void* grad, int64_t ldg, const void* ids
 
 // What both calls check of their ids and rows.
 int check_ids(const char* where, const void* ids, int32_t id_bits, int64_t count, int64_t rows, int32_t width, float scale) {
-  const std::string w = std::string(where) + ": ";
-  if (count < 0 || rows < 0 || width < 0) return fail(TRS_EINVAL, w + "negative count, rows or width");
-  if (id_bits != 32 && id_bits != 64) return fail(TRS_EINVAL, w + "id_bits must be 32 or 64");
-  if (count > 0 && !ids) return fail(TRS_EINVAL, w + "NULL ids");
-  if (!std::isfinite(scale)) return fail(TRS_EINVAL, w + "scale must be finite");
+  if (count < 0 || rows < 0 || width < 0) return fail(TRS_EINVAL, where, "negative count, rows or width");
+  if (id_bits != 32 && id_bits != 64) return fail(TRS_EINVAL, where, "id_bits must be 32 or 64");
+  if (count > 0 && !ids) return fail(TRS_EINVAL, where, "NULL ids");
+  if (!std::isfinite(scale)) return fail(TRS_EINVAL, where, "scale must be finite");
   return TRS_OK;
 }
 
@@ -803,12 +802,12 @@ extern "C" int trs_embed(const void* table, int32_t table_type, int64_t ldt, int
                          void* stream) {
   const int rc = check_ids("trs_embed", ids, id_bits, count, rows, width, scale);
   if (rc) return rc;
-  if (!known_type(table_type) || !known_type(out_type)) return fail(TRS_EINVAL, "trs_embed: unknown element type");
+  if (!known_type(table_type) || !known_type(out_type)) return fail(TRS_EINVAL, "trs_embed", "unknown element type");
   if (count == 0 || width == 0) return TRS_OK;
-  if (!out || (rows > 0 && !table)) return fail(TRS_EINVAL, "trs_embed: NULL table or out");
-  if (ldt < width || ldo < width) return fail(TRS_EINVAL, "trs_embed: leading dimension < width");
-  if (!fits_grid(ceil_div(count, kThreads * kLookups) * ((width + 7) / 8)))
-    return fail(TRS_ERANGE, "trs_embed: the output needs more workgroups than a launch can have");
+  if (!out || (rows > 0 && !table)) return fail(TRS_EINVAL, "trs_embed", "NULL table or out");
+  if (ldt < width || ldo < width) return fail(TRS_EINVAL, "trs_embed", "leading dimension < width");
+  if (count > (int64_t)1 << 42 || !fits_grid(ceil_div(count, kThreads * kLookups) * ((width + 7) / 8)))
+    return fail(TRS_ERANGE, "trs_embed", "the output needs more workgroups than a launch can have");
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (table_type == TRS_F32) launch_embed_out<f32_t>(out_type, table, ldt, rows, ids, id_bits, count, width, scale, out, ldo, s);
   else if (table_type == TRS_F16) launch_embed_out<f16_t>(out_type, table, ldt, rows, ids, id_bits, count, width, scale, out, ldo, s);
@@ -829,11 +828,11 @@ extern "C" int trs_embed_grad(const void* grad, int32_t grad_type, int64_t ldg, 
                               void* workspace, int64_t workspace_bytes, void* stream) {
   const int rc = check_ids("trs_embed_grad", ids, id_bits, count, rows, width, scale);
   if (rc) return rc;
-  if (!known_type(grad_type) || !known_type(out_type)) return fail(TRS_EINVAL, "trs_embed_grad: unknown element type");
+  if (!known_type(grad_type) || !known_type(out_type)) return fail(TRS_EINVAL, "trs_embed_grad", "unknown element type");
   if (rows == 0 || width == 0) return TRS_OK;
-  if (!out || (count > 0 && !grad)) return fail(TRS_EINVAL, "trs_embed_grad: NULL grad or out");
-  if (ldg < width || ldo < width) return fail(TRS_EINVAL, "trs_embed_grad: leading dimension < width");
-  if (count >= INT32_MAX || rows >= INT32_MAX) return fail(TRS_ERANGE, "trs_embed_grad: 2^31 - 1 ids or rows at most");
+  if (!out || (count > 0 && !grad)) return fail(TRS_EINVAL, "trs_embed_grad", "NULL grad or out");
+  if (ldg < width || ldo < width) return fail(TRS_EINVAL, "trs_embed_grad", "leading dimension < width");
+  if (count >= INT32_MAX || rows >= INT32_MAX) return fail(TRS_ERANGE, "trs_embed_grad", "2^31 - 1 ids or rows, or more");
   hipStream_t s = static_cast<hipStream_t>(stream);
   FewPlan few;
   if (trs_embed_grad_workspace_bytes(count, rows, width) == 0 && few_plan(count, rows, width, out_type, few)) {
@@ -846,12 +845,12 @@ extern "C" int trs_embed_grad(const void* grad, int32_t grad_type, int64_t ldg, 
   if (count > 0) {
     g = grad_layout(count, rows, width);
     if (!workspace || workspace_bytes < g.bytes)
-      return fail(TRS_EINVAL, "trs_embed_grad: workspace smaller than trs_embed_grad_workspace_bytes");
+      return fail(TRS_EINVAL, "trs_embed_grad", "workspace smaller than trs_embed_grad_workspace_bytes");
   } else {
     g.lanes = group_lanes(width);
   }
   if (!fits_grid((int64_t)g.run_blocks + fill_blocks(rows, width)) || ceil_div(width, 8 * g.lanes) > 65535)
-    return fail(TRS_ERANGE, "trs_embed_grad: the output needs more workgroups than a launch can have");
+    return fail(TRS_ERANGE, "trs_embed_grad", "the output needs more workgroups than a launch can have");
   char* ws = static_cast<char*>(workspace);
   int sorted = 0;
   for (int pass = 0; pass < g.passes; ++pass) {

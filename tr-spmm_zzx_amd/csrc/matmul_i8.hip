@@ -588,16 +588,16 @@ using namespace trs::dense;
 extern "C" int trs_matmul_i8(const int8_t* a, int64_t lda, const float* a_scale, const int8_t* w, int64_t ldw,
                              const float* w_scale, const float* bias, int64_t m, int32_t n, int32_t k, void* out,
                              int32_t out_type, int64_t ldo, void* stream) {
-  const std::string at = "trs_matmul_i8: ";
-  if (m < 0 || n < 0 || k < 0) return fail(TRS_EINVAL, at + "negative m, n or k");
-  if (!known_type(out_type)) return fail(TRS_EINVAL, at + "unknown element type");
-  if (k > kMostK) return fail(TRS_ERANGE, at + "k beyond 131071: the 32-bit sums could overflow");
+  const char* where = "trs_matmul_i8";
+  if (m < 0 || n < 0 || k < 0) return fail(TRS_EINVAL, where, "negative m, n or k");
+  if (!known_type(out_type)) return fail(TRS_EINVAL, where, "unknown element type");
+  if (k > kMostK) return fail(TRS_ERANGE, where, "k beyond 131071: the 32-bit sums could overflow");
   if (m == 0 || n == 0) return TRS_OK;
-  if (!out || !a_scale || !w_scale || (k > 0 && (!a || !w))) return fail(TRS_EINVAL, at + "NULL operand");
-  if (lda < k || ldw < k || ldo < n) return fail(TRS_EINVAL, at + "leading dimension too small");
+  if (!out || !a_scale || !w_scale || (k > 0 && (!a || !w))) return fail(TRS_EINVAL, where, "NULL operand");
+  if (lda < k || ldw < k || ldo < n) return fail(TRS_EINVAL, where, "leading dimension too small");
   const MatArgs p{a, w, a_scale, w_scale, bias, out, lda, ldw, ldo, m, n, k, out_type};
   // the most workgroups, of the most threads, that any of the kernels takes
-  if (!fits_grid(tiles(p, 64, 64), 1024)) return fail(TRS_ERANGE, at + "the output needs more workgroups than a launch can have");
+  if (!fits_grid(tiles(p, 64, 64), 1024)) return fail(TRS_ERANGE, where, "the output needs more workgroups than a launch can have");
   launch(p, static_cast<hipStream_t>(stream));
   return launched("trs_matmul_i8");
 }

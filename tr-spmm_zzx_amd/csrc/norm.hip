@@ -364,7 +364,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_grad(GradArgs p) {
         dw[c][i] += g * u;
         out[i] = (s * f) * (g * w[c][i] - u * mean) + (float)x.more[c][i];
       }
-      if (dup[c] < 8) store_chunk<R>(static_cast<typename R::raw*>(p.dr) + row * p.lddr + at[c], p.width, out);
+      if (dup[c] < 8) store_own<R>(static_cast<typename R::raw*>(p.dr) + row * p.lddr + at[c], p.width, dup[c], out);
     }
   }
   // One workgroup's sums are the weight's gradient; others are laid out chunk by chunk for k_column_sums.
@@ -522,26 +522,48 @@ bool launch_norm_res(const NormArgs& p, int r_type, hipStream_t s) {
   return true;
 }
 
+constexpr int64_t kMostRows = (int64_t)1 << 38;
+
+const void* at_row(const void* p, int64_t elements, int type) {
+  return static_cast<const char*>(p) + elements * (type == TRS_F32 ? 4 : 2);
+}
+
 template <bool CODES>
 int norm_call(const char* where, const NormArgs& p, int x_type, int r_type, void* stream) {
-  const std::string w = std::string(where) + ": ";
-  if (p.rows < 0 || p.width < 0) return fail(TRS_EINVAL, w + "negative rows or width");
+  if (p.rows < 0 || p.width < 0) return fail(TRS_EINVAL, where, "negative rows or width");
   if (!known_type(x_type) || !known_type(p.w_type) || (!CODES && !known_type(p.y_type)) ||
       (p.res && !known_type(r_type)))
-    return fail(TRS_EINVAL, w + "unknown element type");
-  if (!(p.eps > 0.f) || !std::isfinite(p.eps)) return fail(TRS_EINVAL, w + "eps must be positive and finite");
+    return fail(TRS_EINVAL, where, "unknown element type");
+  if (!(p.eps > 0.f) || !std::isfinite(p.eps)) return fail(TRS_EINVAL, where, "eps must be positive and finite");
   if (p.rows == 0 || p.width == 0) return TRS_OK;
-  if (!p.x || !p.weight || !p.y || (CODES && !p.scale)) return fail(TRS_EINVAL, w + "NULL operand");
-  if ((p.res == nullptr) != (p.r == nullptr)) return fail(TRS_EINVAL, w + "residual and its output go together");
+  if (!p.x || !p.weight || !p.y || (CODES && !p.scale)) return fail(TRS_EINVAL, where, "NULL operand");
+  if ((p.res == nullptr) != (p.r == nullptr)) return fail(TRS_EINVAL, where, "residual and its output go together");
   if (p.ldx < p.width || p.ldy < p.width || (p.res && (p.ldr < p.width || p.ldro < p.width)))
-    return fail(TRS_EINVAL, w + "leading dimension < width");
-  if (!fits_grid(p.rows)) return fail(TRS_ERANGE, w + "more rows than a launch can have workgroups");
+    return fail(TRS_EINVAL, where, "leading dimension < width");
+  if (p.rows > kMostRows) return fail(TRS_ERANGE, where, "too many rows");
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (!p.res) r_type = kNoResidual;
-  const bool known = x_type == TRS_F32   ? launch_norm_res<f32_t, CODES>(p, r_type, s)
-                     : x_type == TRS_F16 ? launch_norm_res<f16_t, CODES>(p, r_type, s)
-                                         : launch_norm_res<bf16_t, CODES>(p, r_type, s);
-  if (!known) return fail(TRS_EINVAL, w + "x and residual of two different 16-bit types");
+  // as many rows a launch as it can have workgroups
+  constexpr int64_t kSlice = UINT32_MAX / kThreads;
+  for (int64_t first = 0; first < p.rows; first += kSlice) {
+    NormArgs q = p;
+    q.rows = p.rows - first < kSlice ? p.rows - first : kSlice;
+    q.x = at_row(p.x, first * p.ldx, x_type);
+    if (p.res) {
+      q.res = at_row(p.res, first * p.ldr, r_type);
+      q.r = const_cast<void*>(at_row(p.r, first * p.ldro, r_type));
+    }
+    if (CODES) {
+      q.y = static_cast<int8_t*>(p.y) + first * p.ldy;
+      q.scale = p.scale + first;
+    } else {
+      q.y = const_cast<void*>(at_row(p.y, first * p.ldy, p.y_type));
+    }
+    const bool known = x_type == TRS_F32   ? launch_norm_res<f32_t, CODES>(q, r_type, s)
+                       : x_type == TRS_F16 ? launch_norm_res<f16_t, CODES>(q, r_type, s)
+                                           : launch_norm_res<bf16_t, CODES>(q, r_type, s);
+    if (!known) return fail(TRS_EINVAL, where, "x and residual of two different 16-bit types");
+  }
   return launched(where);
 }
 
@@ -623,24 +645,24 @@ extern "C" int trs_rms_norm_grad(const void* grad, int32_t grad_type, int64_t ld
                                  const void* weight, int32_t w_type, const void* grad_r, int64_t ldgr, float eps, int64_t rows,
                                  int32_t width, void* dr, int64_t lddr, float* dweight, void* workspace,
                                  int64_t workspace_bytes, void* stream) {
-  const std::string w = "trs_rms_norm_grad: ";
-  if (rows < 0 || width < 0) return fail(TRS_EINVAL, w + "negative rows or width");
-  if (!known_type(grad_type) || !known_type(r_type) || !known_type(w_type)) return fail(TRS_EINVAL, w + "unknown element type");
-  if (!(eps > 0.f) || !std::isfinite(eps)) return fail(TRS_EINVAL, w + "eps must be positive and finite");
+  const char* where = "trs_rms_norm_grad";
+  if (rows < 0 || width < 0) return fail(TRS_EINVAL, where, "negative rows or width");
+  if (!known_type(grad_type) || !known_type(r_type) || !known_type(w_type)) return fail(TRS_EINVAL, where, "unknown element type");
+  if (!(eps > 0.f) || !std::isfinite(eps)) return fail(TRS_EINVAL, where, "eps must be positive and finite");
   if (width == 0) return TRS_OK;
-  if (!dweight) return fail(TRS_EINVAL, w + "NULL operand");
+  if (!dweight) return fail(TRS_EINVAL, where, "NULL operand");
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (rows == 0) {
     k_zero<<<dim3((uint32_t)ceil_div(width, kThreads)), kThreads, 0, s>>>(dweight, width);
     return launched("trs_rms_norm_grad");
   }
-  if (!grad || !r || !weight || !dr) return fail(TRS_EINVAL, w + "NULL operand");
+  if (!grad || !r || !weight || !dr) return fail(TRS_EINVAL, where, "NULL operand");
   if (ldg < width || ldr < width || lddr < width || (grad_r && ldgr < width))
-    return fail(TRS_EINVAL, w + "leading dimension < width");
-  if (!fits_grid(rows)) return fail(TRS_ERANGE, w + "more rows than a launch can have workgroups");
+    return fail(TRS_EINVAL, where, "leading dimension < width");
+  if (rows > kMostRows || (width > kNormMost && !fits_grid(rows))) return fail(TRS_ERANGE, where, "too many rows");
   if (!workspace || workspace_bytes < trs_rms_norm_grad_workspace_bytes(rows, width))
-    return fail(TRS_EINVAL, w + "workspace smaller than trs_rms_norm_grad_workspace_bytes");
-  if (dr == grad || dr == r) return fail(TRS_EINVAL, w + "dr cannot take the place of grad or r");
+    return fail(TRS_EINVAL, where, "workspace smaller than trs_rms_norm_grad_workspace_bytes");
+  if (dr == grad || dr == r) return fail(TRS_EINVAL, where, "dr cannot take the place of grad or r");
   char* ws = static_cast<char*>(workspace);
   const int64_t sums = round_up(grad_blocks(rows, width) * round_up(width, 8) * 4, 256);
   const GradArgs p{grad, r, weight, grad_r, ldg, ldr, ldgr, w_type, width, eps, rows, 0, dr, lddr, dweight,
@@ -648,6 +670,6 @@ extern "C" int trs_rms_norm_grad(const void* grad, int32_t grad_type, int64_t ld
   const bool known = grad_type == TRS_F32   ? launch_grad_r<f32_t>(p, r_type, s)
                      : grad_type == TRS_F16 ? launch_grad_r<f16_t>(p, r_type, s)
                                             : launch_grad_r<bf16_t>(p, r_type, s);
-  if (!known) return fail(TRS_EINVAL, w + "grad and r of two different 16-bit types");
+  if (!known) return fail(TRS_EINVAL, where, "grad and r of two different 16-bit types");
   return launched("trs_rms_norm_grad");
 }
