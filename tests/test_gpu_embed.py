@@ -252,6 +252,18 @@ def test_graph_replays(count):
         assert torch.equal(back, trspmm.embed_grad(grad, ids, 999, 2.0)), f"replay {i}"
 
 
+@pytest.mark.parametrize("o", TYPES)
+def test_large_outputs(o):
+    """Outputs of more than 16 MB, which leave past the caches where their rows allow it."""
+    say("large", o)
+    for width in (128, 132, 131):
+        ids = some_ids(70_001, 90_000, torch.int32, 3, skew=2)
+        table, grad = rand((90_000, width), torch.float16, 2), rand((70_001, width), torch.float16, 3)
+        check_embed(trspmm.embed(table, ids, 0.7, o), table, ids, 0.7)
+        check_grad(trspmm.embed_grad(grad, ids, 90_000, 0.7, o), grad, ids, 90_000, 0.7)
+        check_grad(trspmm.embed_grad(grad[:900], ids[:900], 90_000, 0.7, o), grad[:900], ids[:900], 90_000, 0.7)
+
+
 def test_gradient_against_differences():
     """The lookup is linear in the table: <embed(table + v) - embed(table), g> = <embed_grad(g), v>."""
     say("differences")

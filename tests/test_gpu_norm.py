@@ -247,6 +247,17 @@ def test_many_rows():
     check_grad(g, x, w, None, *trspmm.rms_norm_grad(g, x, w, eps=EPS))
 
 
+@pytest.mark.parametrize("width", [512, 516])
+def test_large_outputs(width):
+    """Outputs of more than 128 MB, which leave past the caches where their rows allow it."""
+    say("large", width)
+    rows = 270_000
+    x, w, res = rand((rows, width), torch.bfloat16, 1), weights(width, torch.float16, 2), rand((rows, width), torch.bfloat16, 3)
+    check_codes(x, w, res, *trspmm.rms_norm_i8(x, w, res, EPS))
+    check_norm(x, w, res, *trspmm.rms_norm(x, w, res, EPS))
+    check_grad(x, res, w, x, *trspmm.rms_norm_grad(x, res, w, x, EPS))
+
+
 def test_more_rows_than_a_launch():
     """2^24 + 1000 rows of 3: more than 2^32 threads at a workgroup a row; and at 32 rows a workgroup many."""
     say("rows past a launch")

@@ -25,6 +25,7 @@ struct MatArgs {
   void* out;
   int64_t lda, ldw, ldo, m;
   int n, k, out_type;
+  bool past;   // out is written past the caches
 };
 
 // 16 codes at any address.  ODD: where rows do not start on 4-byte boundaries, by the 4-byte words that hold them (a
@@ -137,9 +138,9 @@ __device__ __forceinline__ void store_wave(const MatArgs& p, const int16_v (&acc
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = (float)got[e] * sa.of[i][t] * sw[e] + bias[e];
         const int64_t at = m * p.ldo + n;
-        if (p.out_type == TRS_F32) store_chunk<f32_t>(static_cast<float*>(p.out) + at, left, v);
-        else if (p.out_type == TRS_F16) store_chunk<f16_t>(static_cast<_Float16*>(p.out) + at, left, v);
-        else store_chunk<bf16_t>(static_cast<__bf16*>(p.out) + at, left, v);
+        if (p.out_type == TRS_F32) store_chunk<f32_t>(static_cast<float*>(p.out) + at, left, v, p.past);
+        else if (p.out_type == TRS_F16) store_chunk<f16_t>(static_cast<_Float16*>(p.out) + at, left, v, p.past);
+        else store_chunk<bf16_t>(static_cast<__bf16*>(p.out) + at, left, v, p.past);
       }
       wave_fence();
     }
@@ -595,7 +596,8 @@ extern "C" int trs_matmul_i8(const int8_t* a, int64_t lda, const float* a_scale,
   if (m == 0 || n == 0) return TRS_OK;
   if (!out || !a_scale || !w_scale || (k > 0 && (!a || !w))) return fail(TRS_EINVAL, where, "NULL operand");
   if (lda < k || ldw < k || ldo < n) return fail(TRS_EINVAL, where, "leading dimension too small");
-  const MatArgs p{a, w, a_scale, w_scale, bias, out, lda, ldw, ldo, m, n, k, out_type};
+  const bool past = streams(out, ldo, out_type == TRS_F32 ? 4 : 2, m, n);
+  const MatArgs p{a, w, a_scale, w_scale, bias, out, lda, ldw, ldo, m, n, k, out_type, past};
   // the most workgroups, of the most threads, that any of the kernels takes
   if (!fits_grid(tiles(p, 64, 64), 1024)) return fail(TRS_ERANGE, where, "the output needs more workgroups than a launch can have");
   launch(p, static_cast<hipStream_t>(stream));

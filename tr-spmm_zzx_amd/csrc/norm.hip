@@ -22,6 +22,9 @@ namespace dense {
 namespace {
 
 constexpr int kThreads = 256;
+// Rows are written past the caches from this size on (16384 x 4096 in 16 bits: 97 -> 92 us, its gradient 109 -> 104; half of
+// that, 41 -> 46 and 56 -> 57).
+constexpr int64_t kNormStreams = (int64_t)128 << 20;
 constexpr int kNormMost = kThreads * 8 * 4;   // widths in registers
 constexpr float kSmall = 0x1p-80f;       // brings any finite value's square, summed, into range
 constexpr float kLeastPeak = 0x1p-119f;  // below this largest |y|, 127 / max|y| overflows: the row counts as zeros
@@ -39,10 +42,10 @@ __device__ __forceinline__ void load_any(const void* p, int type, int64_t at, in
   else load_chunk<bf16_t>(static_cast<const __bf16*>(p) + at, n, v);
 }
 
-__device__ __forceinline__ void store_any(void* p, int type, int64_t at, int n, const float (&v)[8]) {
-  if (type == TRS_F32) store_chunk<f32_t>(static_cast<float*>(p) + at, n, v);
-  else if (type == TRS_F16) store_chunk<f16_t>(static_cast<_Float16*>(p) + at, n, v);
-  else store_chunk<bf16_t>(static_cast<__bf16*>(p) + at, n, v);
+__device__ __forceinline__ void store_any(void* p, int type, int64_t at, int n, const float (&v)[8], bool past = false) {
+  if (type == TRS_F32) store_chunk<f32_t>(static_cast<float*>(p) + at, n, v, past);
+  else if (type == TRS_F16) store_chunk<f16_t>(static_cast<_Float16*>(p) + at, n, v, past);
+  else store_chunk<bf16_t>(static_cast<__bf16*>(p) + at, n, v, past);
 }
 
 // Sum (or largest) over a group of G lanes, the same value in each of them and in every run.  `red` is LDS of
@@ -76,13 +79,19 @@ __device__ __forceinline__ uint32_t group_max(uint32_t v, float* red) {
 __device__ __forceinline__ uint32_t size_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 constexpr uint32_t kInfBits = 0x7f800000u;
 
-__device__ __forceinline__ void store_codes(int8_t* q, int n, const float (&v)[8], float inv) {
+__device__ __forceinline__ void store_codes(int8_t* q, int n, const float (&v)[8], float inv, bool past = false) {
   union { int8_t c[8]; uint64_t w; } u;
 #pragma unroll
   for (int i = 0; i < 8; ++i) u.c[i] = (int8_t)(int)__builtin_rintf(v[i] * inv);
   if (n >= 8) {
     typedef uint64_t word __attribute__((aligned(1)));
-    *reinterpret_cast<word*>(q) = u.w;
+    if (past) {
+      keep_apart();
+      __builtin_nontemporal_store(u.w, reinterpret_cast<word*>(q));
+      keep_apart();
+    } else {
+      *reinterpret_cast<word*>(q) = u.w;
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -101,6 +110,7 @@ struct NormArgs {
   float* scale;
   void* r;
   int64_t ldro;
+  bool past_y, past_r;   // written past the caches
 };
 
 // 1/sqrt of the mean square, of a row whose sum of squares is not finite: from the values at a smaller scale.
@@ -162,13 +172,13 @@ __global__ __launch_bounds__(kThreads) void k_norm(NormArgs p) {
   for (int c = 0; c < NC; ++c) {
     if (dup[c] == 8) continue;
     if constexpr (!is_none<R>)
-      store_chunk<R>(static_cast<typename R::raw*>(p.r) + row * p.ldro + at[c], p.width, h[c]);
+      store_chunk<R>(static_cast<typename R::raw*>(p.r) + row * p.ldro + at[c], p.width, h[c], p.past_r);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       h[c][i] = (h[c][i] * f) * s * w[c][i];
       if (CODES) peak = max(peak, size_bits(h[c][i]));
     }
-    if constexpr (!CODES) store_any(p.y, p.y_type, row * p.ldy + at[c], p.width, h[c]);
+    if constexpr (!CODES) store_any(p.y, p.y_type, row * p.ldy + at[c], p.width, h[c], p.past_y);
   }
   if constexpr (CODES) {
     peak = group_max<G>(peak, red[2]);
@@ -182,7 +192,7 @@ __global__ __launch_bounds__(kThreads) void k_norm(NormArgs p) {
       if (!finite)
 #pragma unroll
         for (int i = 0; i < 8; ++i) h[c][i] = 0.f;
-      store_codes(static_cast<int8_t*>(p.y) + row * p.ldy + at[c], p.width, h[c], inv);
+      store_codes(static_cast<int8_t*>(p.y) + row * p.ldy + at[c], p.width, h[c], inv, p.past_y);
     }
   }
 }
@@ -263,6 +273,7 @@ struct GradArgs {
   int64_t rows, share;   // share: rows of a workgroup
   void* dr;
   int64_t lddr;
+  bool past;             // dr is written past the caches
   float* dweight;
   float* sums;           // [workgroup][chunks * 8]
   float* rstd;           // long rows: [rows][2], the norm's factor and the mean of g u
@@ -364,7 +375,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_grad(GradArgs p) {
         dw[c][i] += g * u;
         out[i] = (s * f) * (g * w[c][i] - u * mean) + (float)x.more[c][i];
       }
-      if (dup[c] < 8) store_own<R>(static_cast<typename R::raw*>(p.dr) + row * p.lddr + at[c], p.width, dup[c], out);
+      if (dup[c] < 8) store_own<R>(static_cast<typename R::raw*>(p.dr) + row * p.lddr + at[c], p.width, dup[c], out, p.past);
     }
   }
   // One workgroup's sums are the weight's gradient; others are laid out chunk by chunk for k_column_sums.
@@ -547,6 +558,8 @@ int norm_call(const char* where, const NormArgs& p, int x_type, int r_type, void
   constexpr int64_t kSlice = UINT32_MAX / kThreads;
   for (int64_t first = 0; first < p.rows; first += kSlice) {
     NormArgs q = p;
+    q.past_y = streams(p.y, p.ldy, CODES ? 1 : p.y_type == TRS_F32 ? 4 : 2, p.rows, p.width, kNormStreams);
+    q.past_r = p.res && streams(p.r, p.ldro, r_type == TRS_F32 ? 4 : 2, p.rows, p.width, kNormStreams);
     q.rows = p.rows - first < kSlice ? p.rows - first : kSlice;
     q.x = at_row(p.x, first * p.ldx, x_type);
     if (p.res) {
@@ -624,14 +637,14 @@ using namespace trs::dense;
 extern "C" int trs_rms_norm(const void* x, int32_t x_type, int64_t ldx, const void* residual, int32_t r_type, int64_t ldr,
                             const void* weight, int32_t w_type, float eps, int64_t rows, int32_t width, void* y,
                             int32_t y_type, int64_t ldy, void* r_out, int64_t ldro, void* stream) {
-  const NormArgs p{x, residual, weight, ldx, ldr, w_type, y_type, width, eps, rows, y, ldy, nullptr, r_out, ldro};
+  const NormArgs p{x, residual, weight, ldx, ldr, w_type, y_type, width, eps, rows, y, ldy, nullptr, r_out, ldro, false, false};
   return norm_call<false>("trs_rms_norm", p, x_type, r_type, stream);
 }
 
 extern "C" int trs_rms_norm_i8(const void* x, int32_t x_type, int64_t ldx, const void* residual, int32_t r_type, int64_t ldr,
                                const void* weight, int32_t w_type, float eps, int64_t rows, int32_t width, int8_t* q,
                                int64_t ldq, float* scale, void* r_out, int64_t ldro, void* stream) {
-  const NormArgs p{x, residual, weight, ldx, ldr, w_type, 0, width, eps, rows, q, ldq, scale, r_out, ldro};
+  const NormArgs p{x, residual, weight, ldx, ldr, w_type, 0, width, eps, rows, q, ldq, scale, r_out, ldro, false, false};
   return norm_call<true>("trs_rms_norm_i8", p, x_type, r_type, stream);
 }
 
@@ -665,7 +678,7 @@ extern "C" int trs_rms_norm_grad(const void* grad, int32_t grad_type, int64_t ld
   if (dr == grad || dr == r) return fail(TRS_EINVAL, where, "dr cannot take the place of grad or r");
   char* ws = static_cast<char*>(workspace);
   const int64_t sums = round_up(grad_blocks(rows, width) * round_up(width, 8) * 4, 256);
-  const GradArgs p{grad, r, weight, grad_r, ldg, ldr, ldgr, w_type, width, eps, rows, 0, dr, lddr, dweight,
+  const GradArgs p{grad, r, weight, grad_r, ldg, ldr, ldgr, w_type, width, eps, rows, 0, dr, lddr, streams(dr, lddr, r_type == TRS_F32 ? 4 : 2, rows, width, kNormStreams), dweight,
                    reinterpret_cast<float*>(ws), reinterpret_cast<float*>(ws + sums)};
   const bool known = grad_type == TRS_F32   ? launch_grad_r<f32_t>(p, r_type, s)
                      : grad_type == TRS_F16 ? launch_grad_r<f16_t>(p, r_type, s)
