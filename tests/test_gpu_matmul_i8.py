@@ -79,7 +79,8 @@ def test_channels(n):
 @pytest.mark.parametrize("m,n,k", [(2048, 2048, 512), (2000, 2100, 1000), (2049, 1030, 256), (513, 4097, 2049), (70_000, 96, 64),
                                    (33_000, 256, 128), (66_001, 200, 100), (70_000, 41, 128), (40_001, 100, 77), (4096, 8192, 256),
                                    (5000, 3000, 600), (5000, 3001, 601), (1500, 1500, 1031), (200, 4096, 4096), (500, 4096, 4095),
-                                   (250, 4000, 2049), (60_000, 256, 200), (1, 16_000, 8192), (8, 8192, 16_384), (64, 4096, 4096)])
+                                   (250, 4000, 2049), (60_000, 256, 200),
+                                   (800_001, 200, 120), (790_000, 300, 127), (740_000, 1000, 128), (5_900_001, 136, 16), (1, 16_000, 8192), (8, 8192, 16_384), (64, 4096, 4096)])
 def test_large(m, n, k):
     say("large", m, n, k)
     run(m, n, k, torch.bfloat16)

@@ -46,12 +46,12 @@ inline int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
 // A launch holds less than 2^32 threads along a dimension.
 inline bool fits_grid(int64_t blocks, int threads = 256) { return blocks * threads <= (int64_t)UINT32_MAX; }
 
-// Whether an output is written past the caches: one of at most 16 bits an element, whose whole 16-byte pieces fill lines,
-// and of `least` bytes, more than the L2s (8 of 4 MB) could keep for its reader.  (Lookups of 256 MB: 86 -> 76 us; a product
-// of 16384 x 4096 x 1024: 100 -> 85; of 1,000,003 x 250 x 100, whose rows start off the lines, 181 -> 218 if it were; float32,
-// two pieces a lane, half as fast.)
+// Whether an output is written past the caches: one of at most 16 bits an element, whose rows fill 64-byte lines, and of
+// `least` bytes, more than the L2s (8 of 4 MB) could keep for its reader.  (Lookups of 256 MB: 86 -> 76 us; a product of
+// 16384 x 4096 x 1024: 100 -> 85; of 1,000,003 x 250 x 100, whose rows start off the lines, 181 -> 218 if it were; float32, two
+// pieces a lane, half as fast.)
 inline bool streams(const void* p, int64_t ld, int bytes, int64_t rows, int64_t width, int64_t least = 16 << 20) {
-  return bytes <= 2 && width % 8 == 0 && ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * bytes)) & 15) == 0 &&
+  return bytes <= 2 && ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * bytes) | (uintptr_t)(width * bytes)) & 63) == 0 &&
          rows * width * bytes >= least;
 }
 

@@ -46,26 +46,32 @@ __device__ __forceinline__ int4_v load16(const int8_t* p) {
   }
 }
 
-// 16 codes of a row from column `at` on; zeros past the row's end (zeros add nothing to the sums).  Without a
-// branch, so that several are on their way together: a piece that the end cuts is the row's last 16 codes, moved
-// down.
+// Where the 16 codes of a row of k >= 16 that hold its codes from `at` on start, and those codes of them: the end may cut
+// them (then they are the row's last 16, moved down) or lie before them.
+__device__ __forceinline__ int start_of(int at, int k) { return at < k - 16 ? at : k - 16; }
+__device__ __forceinline__ int4_v settle(int4_v codes, int at, int k) {
+  const int bits = 8 * (at - start_of(at, k));
+  union { uint64_t q[2]; int4_v v; } u;
+  u.v = codes;
+  const uint64_t low = u.q[0], high = u.q[1];
+  const uint64_t over = bits == 0 ? 0 : high << (64 - (bits & 63));
+  u.q[0] = bits >= 128 ? 0 : bits >= 64 ? high >> (bits & 63) : low >> (bits & 63) | over;
+  u.q[1] = bits >= 64 ? 0 : high >> (bits & 63);
+  return u.v;
+}
+
+// 16 codes of a row from column `at` on; zeros past the row's end (zeros add nothing to the sums).
 template <bool ODD>
 __device__ __forceinline__ int4_v load_codes(const int8_t* row, int at, int k) {
-  union { int8_t c[16]; uint64_t q[2]; int4_v v; } u;
   if (k < 16) {   // the same in every lane
+    union { int8_t c[16]; int4_v v; } u;
     u.v = int4_v{0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < 16; ++i)
       if (at + i < k) u.c[i] = row[at + i];
     return u.v;
   }
-  const int from = at < k - 16 ? at : k - 16, bits = 8 * (at - from);
-  u.v = load16<ODD>(row + from);
-  const uint64_t low = u.q[0], high = u.q[1];
-  const uint64_t over = bits == 0 ? 0 : high << (64 - (bits & 63));
-  u.q[0] = bits >= 128 ? 0 : bits >= 64 ? high >> (bits & 63) : low >> (bits & 63) | over;
-  u.q[1] = bits >= 64 ? 0 : high >> (bits & 63);
-  return u.v;
+  return settle(load16<ODD>(row + start_of(at, k)), at, k);
 }
 
 // A wave's sums, 32 rows and (up to) 64 columns at a time, through LDS (a wave's own part: `lds`, 32 rows of
@@ -368,8 +374,9 @@ __global__ __launch_bounds__((TM / WM) * (TN / WN) * 64, 4) void k_matmul_once(M
   constexpr int FM = WM / 32, FN = WN / 32, kPart = 32 * kOutPitch<FN>;
   constexpr int kIn = (TM + TN) * kDepth, kOut = kWavesOf * kPart * 4;
   __shared__ __align__(1024) int8_t lds[kIn > kOut ? kIn : kOut];
-  uint32_t tm, tn;
-  tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn);
+  // A row of tiles stays on one XCD, neighbouring rows go to different ones: so the XCDs' streams lie side by side in memory.
+  const uint32_t octet = blockIdx.x >> 3, tn = octet % tiles_n, tm = octet / tiles_n * 8 + (blockIdx.x & 7);
+  if (tm >= tiles_m) return;
   const int64_t m0 = (int64_t)tm * TM;
   const int n0 = (int)tn * TN;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -405,6 +412,120 @@ __global__ __launch_bounds__((TM / WM) * (TN / WN) * 64, 4) void k_matmul_once(M
   }
   barrier_and_wait();
   store_wave<FM, FN>(p, acc, sa, reinterpret_cast<int*>(lds) + wave * kPart, m0 + wm, n0 + wn, lane);
+}
+
+// The same for many rows: a workgroup keeps 256 channels' weights in LDS and walks tiles of 128 rows, the next tile's
+// codes on their way while this one's outputs are written.  Outputs pass through LDS 16 rows at a time (in the place
+// of the codes), so that two workgroups share a CU.  1,000,003 x 256 x 128: 145 us, 4.4 TB/s of codes read and outputs
+// written.
+constexpr int kPanelRows = 128, kPanelColumns = 256, kPanelThreads = 512;
+
+__global__ __launch_bounds__(kPanelThreads, 4) void k_matmul_panel(MatArgs p, uint32_t tiles_m, uint32_t tiles_n, uint32_t walkers) {
+  constexpr int kWaves = kPanelThreads / 64, kPitch = 68, kPart = 16 * kPitch;
+  constexpr int kOut = kWaves * kPart * 4, kIn = kPanelRows * kDepth;
+  __shared__ __align__(1024) int8_t w_lds[kPanelColumns * kDepth], lds[kOut > kIn ? kOut : kIn];
+  __shared__ float scales[2][kPanelRows], channel[2][kPanelColumns + 8];   // the channels' scales and biases
+  const uint32_t octet = blockIdx.x >> 3, tn = octet % tiles_n;
+  uint32_t tm = octet / tiles_n * 8 + (blockIdx.x & 7);   // an XCD's walkers of the same rows follow one another
+  if (tm >= tiles_m) return;
+  const int n0 = (int)tn * kPanelColumns;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int wm = (wave & 1) * 64, wn = (wave >> 1) * 64;
+  const int row0 = threadIdx.x >> 3, my_k = ((threadIdx.x & 7) ^ (row0 >> 1 & 7)) * 16;
+  int4_v held[2];
+  float held_scale = 0.f;
+  auto fetch = [&](uint32_t tile) {
+    const int64_t mine = (int64_t)tile * kPanelRows + (threadIdx.x & (kPanelRows - 1));
+    held_scale = p.a_scale[mine < p.m ? mine : p.m - 1];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int64_t m = (int64_t)tile * kPanelRows + u * 64 + row0;
+      held[u] = load16<false>(p.a + (m < p.m ? m : p.m - 1) * p.lda + start_of(my_k, p.k));
+    }
+  };
+  fetch(tm);
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int n = n0 + u * 64 + row0;
+    *reinterpret_cast<int4_v*>(w_lds + (u * kPanelThreads + threadIdx.x) * 16) =
+        load_codes<false>(p.w + (int64_t)(n < p.n ? n : p.n - 1) * p.ldw, my_k, p.k);
+  }
+  // the lane's 8 columns, as in store_wave
+  const int first = (lane & 7) * 8, end = p.n - n0 - wn;
+  const int column = first + 8 > end && first < end && end >= 8 ? end - 8 : first;
+  const int n = n0 + wn + column, left = first < end ? end - column : 0;
+  if (threadIdx.x < kPanelColumns) {
+    const int c = n0 + (int)threadIdx.x;
+    channel[0][threadIdx.x] = c < p.n ? p.w_scale[c] : 0.f;
+    channel[1][threadIdx.x] = c < p.n && p.bias ? p.bias[c] : 0.f;
+  }
+  const int swz = lane >> 1 & 7, row = lane & 31, half = lane >> 5;
+  int* const out = reinterpret_cast<int*>(lds) + wave * kPart;
+  for (int turn = 0; tm < tiles_m; tm += walkers, turn ^= 1) {
+    const int64_t m0 = (int64_t)tm * kPanelRows + wm;
+    if (threadIdx.x < kPanelRows) scales[turn][threadIdx.x] = held_scale;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) *reinterpret_cast<int4_v*>(lds + (u * kPanelThreads + threadIdx.x) * 16) = settle(held[u], my_k, p.k);
+    __syncthreads();
+    if (tm + walkers < tiles_m) fetch(tm + walkers);
+    int16_v acc[2][2] = {};
+#pragma unroll 1
+    for (int h = 0; h * 32 < p.k; ++h) {
+      const int at = ((2 * h + half) ^ swz) * 16;
+      int4_v fa[2], fw[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) fa[i] = *reinterpret_cast<const int4_v*>(lds + (wm + i * 32 + row) * kDepth + at);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) fw[j] = *reinterpret_cast<const int4_v*>(w_lds + (wn + j * 32 + row) * kDepth + at);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[j], fa[i], acc[i][j], 0, 0, 0);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)");   // the codes are read: outputs take their place (the next tile's stay on their way)
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll 1
+      for (int s = 0; s < 2; ++s) {   // rows 16 s .. of the 32
+        if ((row >> 4) == s) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const int16_v& part = acc[i][j];
+              *reinterpret_cast<int4_v*>(out + (row & 15) * kPitch + j * 32 + 8 * q + 4 * half) =
+                  int4_v{part[4 * q], part[4 * q + 1], part[4 * q + 2], part[4 * q + 3]};
+            }
+        }
+        wave_fence();
+#pragma unroll 1
+        for (int t = 0; t < 2; ++t) {
+          const int r = t * 8 + (lane >> 3);
+          const int64_t m = m0 + i * 32 + s * 16 + r;
+          const float sa = scales[turn][wm + i * 32 + s * 16 + r];
+          const int* from = out + r * kPitch + column;
+          int got[8];
+          if (column % 4 == 0) {
+            *reinterpret_cast<int4_v*>(got) = *reinterpret_cast<const int4_v*>(from);
+            *reinterpret_cast<int4_v*>(got + 4) = *reinterpret_cast<const int4_v*>(from + 4);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) got[e] = from[e];
+          }
+          if (m >= p.m || left <= 0) continue;
+          float v[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = (float)got[e] * sa * channel[0][wn + column + e] + channel[1][wn + column + e];
+          const int64_t at = m * p.ldo + n;
+          if (p.out_type == TRS_F32) store_chunk<f32_t>(static_cast<float*>(p.out) + at, left, v, p.past);
+          else if (p.out_type == TRS_F16) store_chunk<f16_t>(static_cast<_Float16*>(p.out) + at, left, v, p.past);
+          else store_chunk<bf16_t>(static_cast<__bf16*>(p.out) + at, left, v, p.past);
+        }
+        wave_fence();
+      }
+    __syncthreads();   // the outputs are read from LDS: the next codes take their place
+  }
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -481,10 +602,17 @@ void launch_tile(const MatArgs& p, hipStream_t s) {
 template <int TM, int TN, int WM, int WN>
 void launch_once(const MatArgs& p, bool odd, hipStream_t s) {
   const uint32_t tm = (uint32_t)ceil_div(p.m, TM), tn = (uint32_t)ceil_div(p.n, TN);
-  const dim3 grid(tm * tn);
+  const dim3 grid((uint32_t)round_up(tm, 8) * tn);
   constexpr int kAll = (TM / WM) * (TN / WN) * 64;
   if (odd) k_matmul_once<TM, TN, WM, WN, true><<<grid, kAll, 0, s>>>(p, tm, tn);
   else k_matmul_once<TM, TN, WM, WN, false><<<grid, kAll, 0, s>>>(p, tm, tn);
+}
+
+void launch_panel(const MatArgs& p, hipStream_t s) {
+  const uint32_t tm = (uint32_t)ceil_div(p.m, kPanelRows), tn = (uint32_t)ceil_div(p.n, kPanelColumns);
+  const uint32_t walkers = 2 * kCus / tn / 8 * 8;   // of a panel; all run at once
+  const dim3 grid(walkers * tn);
+  k_matmul_panel<<<grid, kPanelThreads, 0, s>>>(p, tm, tn, walkers);
 }
 
 template <int FM>
@@ -567,9 +695,13 @@ void launch(const MatArgs& p, hipStream_t s) {
     case 4: return launch_rows<4>(p, odd, s);
   }
   if (p.k <= kDepth) {
-    // 1000003 x 256 x 128: 240 us with tiles of 64 x 64, 213 of 128 x 128, 171 of 128 x 256; x 128: 120, 106, 136;
-    // x 64: 61, 87, 118.  Below two workgroups a CU the smallest (2000 x 500 x 128: 4.1, 6.5, 7.0).
-    if (p.n > 128 && tiles(p, 128, 256) >= 2 * kCus) launch_once<128, 256, 64, 64>(p, odd, s);
+    // Rows that do not come from the MALL (256 MB) are read ahead by k_matmul_panel: 1000003 x 256 x 128: 145 us, with tiles of
+    // 128 x 256 168; x 96: 139, 166; but x 80: 137, 122; 262144 x 512 x 128: 75, 68.
+    // Otherwise, without large outputs' way past the caches: 1000003 x 256 x 128: 240 us with tiles of 64 x 64, 213 of
+    // 128 x 128, 171 of 128 x 256; x 128: 120, 106, 136; x 64: 61, 87, 118.  Below two workgroups a CU the smallest
+    // (2000 x 500 x 128: 4.1, 6.5, 7.0).
+    if (p.n > 128 && p.n <= 64 * kPanelColumns && p.k >= 16 && p.m * p.k >= (int64_t)90 << 20) launch_panel(p, s);
+    else if (p.n > 128 && tiles(p, 128, 256) >= 2 * kCus) launch_once<128, 256, 64, 64>(p, odd, s);
     else if (p.n > 64 && tiles(p, 128, 128) >= 2 * kCus) launch_once<128, 128, 64, 64>(p, odd, s);
     else launch_once<64, 64, 32, 32>(p, odd, s);
     return;
