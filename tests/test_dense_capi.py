@@ -51,6 +51,12 @@ def test_refused(name, arg, value, status):
     assert lib.trs_last_error().startswith(name.encode() + b": ")
 
 
+@pytest.mark.parametrize("m,n", [(1 << 62, 2 ** 31 - 1), (64, 2 ** 31 - 1), (1, 2 ** 27 + 1)])
+def test_products_past_a_launch_are_refused(m, n):
+    lib = nat.lib()
+    assert lib.trs_matmul_i8(*{**MATMUL, "m": m, "n": n, "ldo": n}.values()) == 5, lib.trs_last_error()
+
+
 @pytest.mark.parametrize("first,second", [(1, 2), (2, 1)])
 def test_two_different_16_bit_types_are_refused(first, second):
     lib = nat.lib()

@@ -44,7 +44,7 @@ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
 
 // A launch holds less than 2^32 threads along a dimension.
-inline bool fits_grid(int64_t blocks, int threads = 256) { return blocks * threads <= (int64_t)UINT32_MAX; }
+inline bool fits_grid(int64_t blocks, int threads = 256) { return blocks <= (int64_t)UINT32_MAX / threads; }
 
 // Whether an output is written past the caches: one of at most 16 bits an element, whose rows fill 64-byte lines, and of
 // `least` bytes, more than the L2s (8 of 4 MB) could keep for its reader.  (Lookups of 256 MB: 86 -> 76 us; a product of

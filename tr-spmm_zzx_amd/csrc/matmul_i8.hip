@@ -156,12 +156,16 @@ __device__ __forceinline__ void store_wave(const MatArgs& p, const int16_v (&acc
 // ---------------------------------------------------------------------------------------------
 // Tiles: TM x TN outputs a workgroup, WM x WN a wave, 128 codes of k a step, the next step's operands on their
 // way while this one's are multiplied.  A tile's row is 128 bytes, eight pieces of 16; piece c of row r lies in
-// place c ^ (r & 7), so that the 16-byte reads of neighbouring rows spread over the banks.
+// place c ^ (r / 2 & 7), so that the 16-byte reads of neighbouring rows spread over the banks.
 //
 // DIRECT: rows on 16-byte boundaries and k a multiple of 16; the pieces go from memory to LDS without
 // registers.  Otherwise any address, through registers (4096 x 4096 x 4095: 85 us; by 4-byte words, put together as they
 // arrive, 134: the products wait for them).  KS groups of waves split a workgroup's steps, each
 // with its own tiles, and the first adds the sums up: for few workgroups and a long k.
+//
+// Bound by arithmetic: 8192 x 8192 x 8192 454 us, 2.42 POP/s, the matrix units busy 75% of the cycles (at the 1.6 GHz that
+// the card holds under them), 2% of the LDS cycles lost to conflicts.  A wave owns 128 x 64 of a 256 x 256 tile; with
+// 64 x 64 (a tile of 256 x 128) it reads more LDS for each product (645 us), 128 x 128 spilled registers (2375).
 constexpr int kDepth = 128;
 
 typedef __attribute__((address_space(3))) void* lds_ptr;
@@ -416,8 +420,8 @@ __global__ __launch_bounds__((TM / WM) * (TN / WN) * 64, 4) void k_matmul_once(M
 
 // The same for many rows: a workgroup keeps 256 channels' weights in LDS and walks tiles of 128 rows, the next tile's
 // codes on their way while this one's outputs are written.  Outputs pass through LDS 16 rows at a time (in the place
-// of the codes), so that two workgroups share a CU.  1,000,003 x 256 x 128: 145 us, 4.4 TB/s of codes read and outputs
-// written.
+// of the codes), so that two workgroups share a CU.  Bound by memory: 1,000,003 x 256 x 128 145 to 158 us by card, 0.64 GB
+// at 4.1 to 4.4 TB/s, each byte moved once.
 constexpr int kPanelRows = 128, kPanelColumns = 256, kPanelThreads = 512;
 
 __global__ __launch_bounds__(kPanelThreads, 4) void k_matmul_panel(MatArgs p, uint32_t tiles_m, uint32_t tiles_n, uint32_t walkers) {
@@ -531,7 +535,7 @@ __global__ __launch_bounds__(kPanelThreads, 4) void k_matmul_panel(MatArgs p, ui
 // ---------------------------------------------------------------------------------------------
 // Few rows: 16 FM rows and 16 output channels a workgroup, its waves taking turns at 128 codes of k each, so that
 // the weights -- the bytes that count here -- arrive by as many loads in flight as fit.  The waves' sums are
-// added up in LDS.
+// added up in LDS.  Bound by memory and a launch: 1 x 4096 x 4096 5.2 us, 16.8 MB at 3.2 TB/s.
 template <int FM, bool ODD>
 __global__ __launch_bounds__(1024) void k_matmul_rows(MatArgs p, uint32_t blocks_n) {
   __shared__ int sums[16][FM * 256];
@@ -638,6 +642,7 @@ int rows_kernel(const MatArgs& p) {
   double best = ceil_div(tiles(p, 64, 64), kCus) * 128 / 75.0;
   int fm = 0;
   for (int f : {1, 2, 4}) {
+    if (!fits_grid(tiles(p, 16 * f, 16), 1024)) continue;
     const int64_t rows = p.m < 16 * f ? p.m : 16 * f;
     const double cost = ceil_div(tiles(p, 16 * f, 16), kCus) * (16 + rows) / 39.0;
     if (cost < best || (fm == 0 && p.m <= 8)) {
@@ -728,10 +733,11 @@ extern "C" int trs_matmul_i8(const int8_t* a, int64_t lda, const float* a_scale,
   if (m == 0 || n == 0) return TRS_OK;
   if (!out || !a_scale || !w_scale || (k > 0 && (!a || !w))) return fail(TRS_EINVAL, where, "NULL operand");
   if (lda < k || ldw < k || ldo < n) return fail(TRS_EINVAL, where, "leading dimension too small");
+  // the most threads that any of the kernels takes but k_matmul_rows, which rows_kernel leaves out where it needs more
+  if (m > (int64_t)1 << 42 || !fits_grid(round_up(ceil_div(m, 64), 8) * ceil_div(n, 64)))
+    return fail(TRS_ERANGE, where, "the output needs more workgroups than a launch can have");
   const bool past = streams(out, ldo, out_type == TRS_F32 ? 4 : 2, m, n);
   const MatArgs p{a, w, a_scale, w_scale, bias, out, lda, ldw, ldo, m, n, k, out_type, past};
-  // the most workgroups, of the most threads, that any of the kernels takes
-  if (!fits_grid(tiles(p, 64, 64), 1024)) return fail(TRS_ERANGE, where, "the output needs more workgroups than a launch can have");
   launch(p, static_cast<hipStream_t>(stream));
   return launched("trs_matmul_i8");
 }
