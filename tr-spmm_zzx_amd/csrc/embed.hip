@@ -18,8 +18,9 @@ namespace {
 constexpr int kThreads = 256;
 
 // ---------------------------------------------------------------------------------------------
-// Lookup.  One thread per chunk of 8 elements, kUnroll chunks a thread: the id and the row are two
-// dependent loads, so several such chains are kept in flight.
+// Lookup.  One thread per chunk of 8 elements, kLookups chunks a thread: the id and the row are two
+// dependent loads, so several such chains are kept in flight.  Bound by memory: 1,000,003 rows of 128 16-bit
+// elements 75 us, 0.26 GB written and 0.25 GB read by L2 misses (6.7 TB/s); 256 ids 3 us, a launch.
 constexpr int kLookups = 4;
 
 template <class T, class O, class I>
@@ -59,7 +60,9 @@ __global__ __launch_bounds__(kThreads) void k_embed(const typename T::raw* __res
 // each block of ids (k_digit_count), turns each digit's counts into offsets (k_digit_offsets) and moves the ids
 // with their positions (k_digit_move).  The order of equal digits is kept: a wave ranks 64 ids at a time with
 // ballots, waves and blocks follow one another.  Ids outside the table are left out in the first pass, whose
-// move writes how many are left (`kept`).
+// move writes how many are left (`kept`).  Digits of 11 bits, the most whose counts for each wave fit in LDS, as
+// every pass costs three launches.  Bound by their latency and scattered 8-byte writes: 1,000,003 ids of 2^20
+// rows, two passes, 52 us (a pass: counts 5, offsets 5, moves 16).
 constexpr int kMaxBits = 11;
 constexpr int kMaxBins = 1 << kMaxBits;
 constexpr int kSortThreads = 1024;
@@ -217,7 +220,8 @@ __global__ __launch_bounds__(kSortThreads) void k_digit_move(const I* __restrict
 // Gradient: sums of runs.  L lanes (a group) hold 8 L columns and walk kPiece consecutive sorted ids; a
 // run inside one piece is written at once.  A run that crosses pieces leaves a part in LDS, and the group
 // where it starts adds the parts up in order; one that crosses workgroups leaves a part in the workspace
-// for k_join_runs.  Workgroups past the ids write the rows that no id names.
+// for k_join_runs.  Workgroups past the ids write the rows that no id names.  Bound by memory: 1,000,003
+// 16-bit rows of 128 into 2^20 float32 rows 156 us, 0.54 GB written and 0.29 GB read (5.3 TB/s).
 constexpr int kPiece = 16;
 
 // How rows of zeros are written: chunk by chunk, or (`pieces` of 16 bytes a row, not 0) past the caches: of any type, as a
@@ -414,7 +418,8 @@ __global__ __launch_bounds__(kThreads) void k_sum_runs(RunArgs<T> p) {
 }
 
 // Runs that cross workgroups: the workgroup where one starts adds its parts, a share of them for each
-// group, then the groups' sums in order.
+// group, then the groups' sums in order.  Bound by the longest run, whose parts one workgroup reads (12 us in the call
+// above, whose most frequent id comes thousands of times).
 template <class T, int L>
 __global__ __launch_bounds__(kThreads) void k_join_runs(RunArgs<T> p) {
   constexpr int kGroups = kThreads / L;
@@ -466,7 +471,8 @@ __global__ __launch_bounds__(kThreads) void k_join_runs(RunArgs<T> p) {
 // Gradient of few ids (at most kFewIds), in one launch: each workgroup owns some of the table's rows, looks
 // all ids over for them, sorts the ones it finds in LDS and sums their runs; the rows it found none for are
 // filled.  Rows are owned in units (of at least 256 bytes) that are dealt out so that neither neighbouring
-// nor evenly spaced ids meet in one workgroup: unit q belongs to owner (q ^ q >> bits) mod 2^bits.
+// nor evenly spaced ids meet in one workgroup: unit q belongs to owner (q ^ q >> bits) mod 2^bits.  Bound by
+// latency: 4096 ids into 16,384 float32 rows of 64: 9 us, where the launches of the sort and the sums take 35.
 constexpr int kFewThreads = 512;
 constexpr int kFewWaves = kFewThreads / 64;
 constexpr uint32_t kFewBits = 13, kFewIds = 1u << kFewBits;
