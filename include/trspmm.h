@@ -508,7 +508,7 @@ int trs_rms_norm(const void* x, int32_t x_type, int64_t ldx, const void* residua
 
 /* trs_rms_norm with y in 8 bits: scale[row] = max|y| / 127, q = y / scale rounded to nearest even, in
  * [-127, 127].  A row of zeros (or below 2^-119) has scale 0 and codes 0; a row that holds a NaN or
- * an infinity has scale NaN and codes 0. */
+ * an infinity has scale NaN and codes 0.  width = 0: nothing is written, scale neither. */
 int trs_rms_norm_i8(const void* x, int32_t x_type, int64_t ldx, const void* residual, int32_t r_type, int64_t ldr,
                     const void* weight, int32_t w_type, float eps, int64_t rows, int32_t width, int8_t* q, int64_t ldq,
                     float* scale, void* r_out, int64_t ldro, void* stream);

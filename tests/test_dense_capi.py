@@ -43,7 +43,11 @@ BAD = {
 }
 
 
-@pytest.mark.parametrize("name,arg,value,status", [(n, *b) for n, (_, bad) in BAD.items() for b in bad])
+REFUSED = [(n, *b) for n, (_, bad) in BAD.items() for b in bad]
+
+
+# named by their place in the list: an address is another in each process
+@pytest.mark.parametrize("name,arg,value,status", REFUSED, ids=[f"{n}-{arg}-{i}" for i, (n, arg, _, _) in enumerate(REFUSED)])
 def test_refused(name, arg, value, status):
     lib = nat.lib()
     rc = getattr(lib, name)(*{**BAD[name][0], arg: value}.values())

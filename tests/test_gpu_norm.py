@@ -281,6 +281,20 @@ def test_no_rows_no_width():
     assert dr.shape == (0, 24) and not dw.any()
 
 
+def test_codes_of_rows_without_width():
+    """The scale of an empty row is a row of zeros' own, also in a scale that is given and holds something else; a product of
+    such codes is the bias alone."""
+    say("no width")
+    x, w = rand((4, 24), torch.float16, 1)[:, :0], weights(24, torch.float16, 2)[:0]
+    given = torch.full((4,), float("nan"), device="cuda")
+    for kw in ({}, {"scale": given}):
+        q, scale, _ = trspmm.rms_norm_i8(x, w, **kw)
+        assert q.shape == (4, 0) and scale.tolist() == [0.0] * 4
+    codes, bias = torch.empty((3, 0), dtype=torch.int8, device="cuda"), rand((3,), torch.float32, 3)
+    out = trspmm.matmul_i8(q, scale, codes, torch.ones(3, device="cuda"), bias, torch.float32)
+    assert torch.equal(out, bias.expand(4, 3))
+
+
 def test_graph_replays_and_streams():
     say("graph")
     x, res, w = rand((500, 384), torch.float16, 1), rand((500, 384), torch.float16, 2), weights(384, torch.float16, 3)

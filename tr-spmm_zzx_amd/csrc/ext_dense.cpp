@@ -185,6 +185,7 @@ std::tuple<Tensor, Tensor, Given> rms_norm_i8(const Tensor& x, const Tensor& wei
   const NormOperands n(x, weight, residual, r_out, dev);
   const Tensor out = output("out", out_in, n.rows, n.width, at::kChar, dev);
   const Tensor scale = scale_in ? floats("scale", *scale_in, n.rows, dev) : fresh({n.rows}, at::kFloat, dev);
+  if (n.width == 0) scale.zero_();   // the C entry has nothing to do then, but an empty row is a row of zeros
   ok(trs_rms_norm_i8(n.x.data_ptr(), n.x_type, ld(n.x), data(n.residual), n.r_type, n.ldr(), weight.data_ptr(), n.w_type,
                      (float)eps, n.rows, n.width, static_cast<int8_t*>(out.data_ptr()), ld(out),
                      static_cast<float*>(scale.data_ptr()), data(n.r), n.ldro(), stream_of(stream)),

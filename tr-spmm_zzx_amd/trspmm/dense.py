@@ -75,7 +75,7 @@ def rms_norm_i8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.
                 ) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
     """(q, scale, r): :func:`rms_norm` with y in 8 bits, y[t] = q[t] * scale[t], q int8 in [-127, 127] and
     scale float32 [rows] = max|y[t]| / 127.  A row of zeros has scale 0; a row that holds a NaN or an
-    infinity has scale NaN and codes 0."""
+    infinity has scale NaN and codes 0; without a width every scale is 0."""
     return _call("rms_norm_i8", stream, x, weight, residual, eps, out, scale, r_out)
 
 
