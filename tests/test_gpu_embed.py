@@ -105,6 +105,41 @@ def test_three_digit_tables(rows):
     check_grad(trspmm.embed_grad(grad, ids, rows), grad, ids, rows, 1.0)
 
 
+@pytest.mark.parametrize("rows", [2000, 4_194_303, 4_194_304, 5_000_001])
+@pytest.mark.parametrize("count", [20_000, 262_144, 262_145])
+def test_sorted_tables(rows, count):
+    """One to three sorting passes, with the blocks' counts added up where they are used (at most 64 blocks of 4096) and before."""
+    say("sorted", rows, count)
+    ids = some_ids(count, rows, torch.int64, 6, skew=2)
+    ids[:3] = torch.tensor([rows - 1, 0, rows - 1], device="cuda")
+    grad = rand((count, 8), torch.float32, 4)
+    check_grad(trspmm.embed_grad(grad, ids, rows), grad, ids, rows, 1.0)
+
+
+@pytest.mark.parametrize("count", [16_383, 16_384, 16_385])
+@pytest.mark.parametrize("width", [3, 8, 120, 128, 129])
+@pytest.mark.parametrize("rows", [1, 40, 3000, 300_000])
+def test_most_ids_of_one_launch(count, width, rows):
+    """Around the most ids and columns that one launch takes; few rows make each workgroup's list of ids long."""
+    say("most", count, width, rows)
+    grad = rand((count, width), torch.bfloat16, 1)
+    for skew in (1, 4):
+        ids = some_ids(count, rows, torch.int32, count + skew, skew=skew)
+        check_grad(trspmm.embed_grad(grad, ids, rows, 0.25), grad, ids, rows, 0.25)
+
+
+@pytest.mark.parametrize("found", [511, 512, 513, 1024, 1025, 2048, 2049, 4096, 5000, 8192, 8193])
+def test_lists_of_one_workgroup(found):
+    """Lists of ids around each size of the sort in LDS, all different runs and places: row 0's neighbours share its workgroup."""
+    say("list", found)
+    ids = torch.full((max(found, 9000),), -1, dtype=torch.int64, device="cuda")
+    ids[:found] = torch.randint(0, 4, (found,), generator=gen(found), device="cuda")
+    ids = ids[torch.randperm(ids.shape[0], generator=gen(1), device="cuda")]
+    grad = rand((ids.shape[0], 16), torch.float16, 2)
+    check_grad(trspmm.embed_grad(grad, ids, 10_000), grad, ids, 10_000, 1.0)
+    assert torch.equal(trspmm.embed_grad(grad, ids, 10_000), trspmm.embed_grad(grad, ids, 10_000))
+
+
 @pytest.mark.parametrize("count", [300, 5000, 300_001])
 @pytest.mark.parametrize("width", [8, 128, 600])
 def test_one_frequent_row(count, width):

@@ -61,7 +61,7 @@ __global__ __launch_bounds__(kThreads) void k_embed(const typename T::raw* __res
 // with their positions (k_digit_move).  The order of equal digits is kept: a wave ranks 64 ids at a time with
 // ballots, waves and blocks follow one another.  Ids outside the table are left out in the first pass, whose
 // move writes how many are left (`kept`).  Digits of 11 bits, the most whose counts for each wave fit in LDS, as
-// every pass costs three launches.  Bound by their latency and scattered 8-byte writes: 1,000,003 ids of 2^20
+// every pass costs two or three launches.  Bound by their latency and scattered 8-byte writes: 1,000,003 ids of 2^20
 // rows, two passes, 52 us (a pass: counts 5, offsets 5, moves 16).
 constexpr int kMaxBits = 11;
 constexpr int kMaxBins = 1 << kMaxBits;
@@ -69,6 +69,9 @@ constexpr int kSortThreads = 1024;
 constexpr int kSortWaves = kSortThreads / 64;
 constexpr int kRounds = 4;                           // ids of a lane in a block
 constexpr int kBlockIds = kSortThreads * kRounds;    // 4096
+// Up to so many blocks, k_digit_move adds the blocks' counts up itself, and k_digit_offsets is not launched (9000 to 65,536
+// ids 3.5 us less a call, 262,144 ids 1; of 524,288 it would take 6 more).
+constexpr uint32_t kFewBlocks = 64;
 
 // An id and where it stands among the ids: moved, and read, as one word.
 struct __align__(8) Entry { uint32_t key, at; };
@@ -158,9 +161,24 @@ __global__ __launch_bounds__(kSortThreads) void k_digit_move(const I* __restrict
   // exclusive sum of the totals: each thread takes up to two neighbouring digits
   static_assert(kMaxBins <= 2 * kSortThreads, "two digits a thread");
   const int d0 = 2 * threadIdx.x;
-  const uint32_t t0 = d0 < bins ? totals[d0] : 0, t1 = d0 + 1 < bins ? totals[d0 + 1] : 0;
-  const uint32_t o0 = d0 < bins ? counts[(size_t)blockIdx.x * bins + d0] : 0;
-  const uint32_t o1 = d0 + 1 < bins ? counts[(size_t)blockIdx.x * bins + d0 + 1] : 0;
+  uint32_t t0 = 0, t1 = 0, o0 = 0, o1 = 0;
+  if (d0 < bins) {   // bins is even
+    if (gridDim.x <= kFewBlocks) {   // the blocks' own counts
+#pragma unroll 8
+      for (uint32_t b = 0; b < gridDim.x; ++b) {
+        const uint32_t c0 = counts[(size_t)b * bins + d0], c1 = counts[(size_t)b * bins + d0 + 1];
+        t0 += c0;
+        t1 += c1;
+        o0 += b < blockIdx.x ? c0 : 0;
+        o1 += b < blockIdx.x ? c1 : 0;
+      }
+    } else {
+      t0 = totals[d0];
+      t1 = totals[d0 + 1];
+      o0 = counts[(size_t)blockIdx.x * bins + d0];
+      o1 = counts[(size_t)blockIdx.x * bins + d0 + 1];
+    }
+  }
   uint32_t upto = t0 + t1;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
@@ -475,7 +493,11 @@ __global__ __launch_bounds__(kThreads) void k_join_runs(RunArgs<T> p) {
 // latency: 4096 ids into 16,384 float32 rows of 64: 9 us, where the launches of the sort and the sums take 35.
 constexpr int kFewThreads = 512;
 constexpr int kFewWaves = kFewThreads / 64;
-constexpr uint32_t kFewBits = 13, kFewIds = 1u << kFewBits;
+constexpr uint32_t kFewBits = 14, kFewIds = 1u << kFewBits;
+// Wider rows than this only up to half as many ids (16,384 of them against the sort's launches: 16,384 rows of 64 17 us, not
+// 34; 2^20 rows of 128 118, not 135; but 4096 rows of 256 with hubs 40, not 33, of 1024 57, not 36).  Where all
+// ids name one row, which one workgroup then sums, the launches would be faster: 64 columns, 8192 ids 76 us to 38.
+constexpr int kFewWidth = 128;
 constexpr uint32_t kFewRows = 65536;     // rows of a workgroup: marks in LDS
 constexpr uint32_t kLongRun = 16;        // longer ones are summed by the whole workgroup
 
@@ -494,6 +516,32 @@ struct FewArgs {
   int owner_bits, unit_bits;
   uint32_t local_rows;   // rows of an owner, those past the table's end among them
 };
+
+// LEVELS steps of the bitonic network at once, at distances from `least` << (LEVELS - 1) down to `least`: 2^LEVELS words a
+// thread in registers, read and written once (8192 ids of one row of 64: 128 -> 91 us, as a step's
+// words are on their way together).
+template <int LEVELS>
+__device__ __forceinline__ void exchange(uint32_t* words, uint32_t size, uint32_t width, uint32_t least) {
+  constexpr int kWords = 1 << LEVELS;
+  for (uint32_t j = threadIdx.x; j < size >> LEVELS; j += kFewThreads) {
+    const uint32_t first = (j / least * least << LEVELS) + j % least;
+    const bool up = (first & width) == 0;   // the same for all the thread's words: they lie in one stretch of `width`
+    uint32_t v[kWords];
+#pragma unroll
+    for (int e = 0; e < kWords; ++e) v[e] = words[first + e * least];
+#pragma unroll
+    for (int d = kWords / 2; d > 0; d /= 2)
+#pragma unroll
+      for (int e = 0; e < kWords; ++e)
+        if ((e & d) == 0) {
+          const uint32_t low = min(v[e], v[e + d]), high = max(v[e], v[e + d]);
+          v[e] = up ? low : high;
+          v[e + d] = up ? high : low;
+        }
+#pragma unroll
+    for (int e = 0; e < kWords; ++e) words[first + e * least] = v[e];
+  }
+}
 
 template <class T, int L>
 __global__ __launch_bounds__(kFewThreads) void k_grad_few(FewArgs<T> p) {
@@ -555,15 +603,17 @@ __global__ __launch_bounds__(kFewThreads) void k_grad_few(FewArgs<T> p) {
     while (size < n) size *= 2;   // at most count rounded up: found[] holds them
     for (uint32_t j = n + threadIdx.x; j < size; j += kFewThreads) found[j] = 0xffffffffu;
     for (uint32_t width = 2; width <= size; width *= 2)
-      for (uint32_t d = width / 2; d > 0; d /= 2) {
+      for (uint32_t d = width / 2; d > 0;) {
         __syncthreads();
-        for (uint32_t j = threadIdx.x; j < size / 2; j += kFewThreads) {
-          const uint32_t low = j / d * 2 * d + j % d, high = low + d;
-          const uint32_t a = found[low], b = found[high];
-          if ((a > b) == ((low & width) == 0)) {
-            found[low] = b;
-            found[high] = a;
-          }
+        if (d >= 4) {
+          exchange<3>(found, size, width, d / 4);
+          d /= 8;
+        } else if (d == 2) {
+          exchange<2>(found, size, width, 1);
+          d = 0;
+        } else {
+          exchange<1>(found, size, width, 1);
+          d = 0;
         }
       }
     __syncthreads();
@@ -588,21 +638,26 @@ __global__ __launch_bounds__(kFewThreads) void k_grad_few(FewArgs<T> p) {
     }
   };
   const int columns = (p.width + L * 8 - 1) / (L * 8);
-  for (uint32_t i = group; i < n; i += kGroups) {
-    const uint32_t local = found[i] >> kFewBits;
-    if (i > 0 && found[i - 1] >> kFewBits == local) continue;
-    uint32_t end = i + 1;
-    while (end < n && end - i <= kLongRun && found[end] >> kFewBits == local) ++end;
-    if (end - i > kLongRun) {
-      if (lane == 0) long_at[atomicAdd(&n_long, 1u)] = i;
-      continue;
-    }
-    for (int c = 0; c < columns; ++c) {
-      int shared;
-      const int chunk = c * L + lane, at = chunk_at(chunk * 8 < p.width ? chunk : 0, p.width, shared);
-      float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      add(i, end, at, acc);
-      if (chunk * 8 < p.width) write_row(p.out, p.out_type, p.ldo, row_of(local), at, p.width, p.scale, acc, false);
+  for (uint32_t base = 0; base < n; base += kFewThreads) {
+    // A group's lanes look for the runs' starts together (8192 ids of one row of 64: 91 -> 76 us; of 256: 174 -> 127).
+    const uint32_t look = base + lane * kGroups + group;
+    const bool start = look < n && (look == 0 || found[look - 1] >> kFewBits != found[look] >> kFewBits);
+    uint64_t starts = __ballot(start) >> ((threadIdx.x & 63) - lane) & (~0ull >> (64 - L));
+    for (; starts != 0; starts &= starts - 1) {
+      const uint32_t i = base + (uint32_t)__builtin_ctzll(starts) * kGroups + group, local = found[i] >> kFewBits;
+      uint32_t end = i + 1;
+      while (end < n && end - i <= kLongRun && found[end] >> kFewBits == local) ++end;
+      if (end - i > kLongRun) {
+        if (lane == 0) long_at[atomicAdd(&n_long, 1u)] = i;
+        continue;
+      }
+      for (int c = 0; c < columns; ++c) {
+        int shared;
+        const int chunk = c * L + lane, at = chunk_at(chunk * 8 < p.width ? chunk : 0, p.width, shared);
+        float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        add(i, end, at, acc);
+        if (chunk * 8 < p.width) write_row(p.out, p.out_type, p.ldo, row_of(local), at, p.width, p.scale, acc, false);
+      }
     }
   }
   __syncthreads();
@@ -731,7 +786,8 @@ void sort_pass(const GradLayout& g, const I* ids, int64_t count, int64_t rows, i
   uint32_t* kept = reinterpret_cast<uint32_t*>(ws + g.kept);
   const int bins = 1 << g.bits, shift = pass * g.bits;
   k_digit_count<I, FIRST><<<dim3(g.blocks), kSortThreads, 0, s>>>(ids, (uint32_t)count, (uint32_t)rows, shift, bins, kept, counts);
-  k_digit_offsets<<<dim3((bins + 63) / 64), kSortThreads, 0, s>>>(counts, g.blocks, bins, totals);
+  if (g.blocks > kFewBlocks)
+    k_digit_offsets<<<dim3((bins + 63) / 64), kSortThreads, 0, s>>>(counts, g.blocks, bins, totals);
   k_digit_move<I, FIRST><<<dim3(g.blocks), kSortThreads, 0, s>>>(ids, (uint32_t)count, (uint32_t)rows, shift, g.bits, counts,
                                                                  totals, kept, out);
 }
@@ -785,7 +841,7 @@ void grad_runs(const GradLayout& g, int sorted, const void* grad, int64_t ldg, i
 // How k_grad_few deals the rows out; false: too many rows for its workgroups.
 struct FewPlan { int owner_bits, unit_bits; uint32_t local_rows; };
 bool few_plan(int64_t count, int64_t rows, int width, int out_type, FewPlan& f) {
-  if (count > kFewIds) return false;
+  if (count > (width <= kFewWidth ? kFewIds : kFewIds / 2)) return false;
   const int64_t bytes = (int64_t)width * (out_type == TRS_F32 ? 4 : 2);
   f.unit_bits = 0;
   while (bytes << f.unit_bits < 256) ++f.unit_bits;
