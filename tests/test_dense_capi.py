@@ -91,3 +91,26 @@ def test_workspace_sizes():
     assert norm(0, 8) == norm(8, 0) == 0
     assert norm(10_000, 4096) >= 256 * 4096 * 4
     assert norm(10, 10_000) >= 10 * 10_000 * 4 + 10 * 8         # long rows keep two numbers a row
+
+
+WIDEST, FAR = 2 ** 31 - 65536, 1 << 31   # the most columns whose indexes, a step past the last among them, are 32-bit integers
+
+
+@pytest.mark.parametrize("width", [WIDEST + 1, 2 ** 31 - 2048, 2 ** 31 - 7, 2 ** 31 - 1])
+def test_columns_past_32_bit_indexes_are_refused(width):
+    lib = nat.lib()
+    for count in (3, 100_000):      # the one launch's sums and the sorted ones
+        for name, args in [("trs_embed", {**EMBED, "ldt": FAR, "ldo": FAR}), ("trs_embed_grad", {**EMBED_GRAD, "ldg": FAR, "ldo": FAR})]:
+            assert getattr(lib, name)(*{**args, "width": width, "count": count}.values()) == 5, (name, lib.trs_last_error())
+    for name, args in [("trs_rms_norm", {**NORM, "ldx": FAR, "ldr": FAR, "ldy": FAR, "ldro": FAR}),
+                       ("trs_rms_norm_i8", {**NORM_I8, "ldx": FAR, "ldr": FAR, "ldq": FAR, "ldro": FAR})]:
+        assert getattr(lib, name)(*{**args, "width": width}.values()) == 5, (name, lib.trs_last_error())
+
+
+@pytest.mark.parametrize("width", [65535 * 2048 + 1, WIDEST, 2 ** 31 - 1])
+@pytest.mark.parametrize("rows", [0, 3])
+def test_gradients_of_more_columns_than_a_grid_are_refused(width, rows):
+    """Before the first of its launches, and where there are no rows and dweight alone is written."""
+    lib = nat.lib()
+    args = {**NORM_GRAD, "ldg": FAR, "ldr": FAR, "lddr": FAR, "width": width, "rows": rows, "ws_bytes": 1 << 60}
+    assert lib.trs_rms_norm_grad(*args.values()) == 5, lib.trs_last_error()

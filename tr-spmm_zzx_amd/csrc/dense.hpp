@@ -46,6 +46,10 @@ inline int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
 // A launch holds less than 2^32 threads along a dimension.
 inline bool fits_grid(int64_t blocks, int threads = 256) { return blocks <= (int64_t)UINT32_MAX / threads; }
 
+// Columns of a row at most: kernels hold a column's index, and that of a step (up to 2048 columns) past the last one, in
+// 32 bits.
+constexpr int32_t kMostWidth = INT32_MAX - 65535;
+
 // Whether an output is written past the caches: one of at most 16 bits an element, whose rows fill 64-byte lines, and of
 // `least` bytes, more than the L2s (8 of 4 MB) could keep for its reader.  (Lookups of 256 MB: 86 -> 76 us; a product of
 // 16384 x 4096 x 1024: 100 -> 85; of 1,000,003 x 250 x 100, whose rows start off the lines, 181 -> 218 if it were; float32, two

@@ -897,6 +897,7 @@ extern "C" int trs_embed(const void* table, int32_t table_type, int64_t ldt, int
   if (count == 0 || width == 0) return TRS_OK;
   if (!out || (rows > 0 && !table)) return fail(TRS_EINVAL, "trs_embed", "NULL table or out");
   if (ldt < width || ldo < width) return fail(TRS_EINVAL, "trs_embed", "leading dimension < width");
+  if (width > kMostWidth) return fail(TRS_ERANGE, "trs_embed", "more than 2^31 - 65536 columns");
   if (count > (int64_t)1 << 42 || !fits_grid(ceil_div(count, kThreads * kLookups) * ((width + 7) / 8)))
     return fail(TRS_ERANGE, "trs_embed", "the output needs more workgroups than a launch can have");
   hipStream_t s = static_cast<hipStream_t>(stream);
@@ -924,6 +925,7 @@ extern "C" int trs_embed_grad(const void* grad, int32_t grad_type, int64_t ldg, 
   if (!out || (count > 0 && !grad)) return fail(TRS_EINVAL, "trs_embed_grad", "NULL grad or out");
   if (ldg < width || ldo < width) return fail(TRS_EINVAL, "trs_embed_grad", "leading dimension < width");
   if (count >= INT32_MAX || rows >= INT32_MAX) return fail(TRS_ERANGE, "trs_embed_grad", "2^31 - 1 ids or rows, or more");
+  if (width > kMostWidth) return fail(TRS_ERANGE, "trs_embed_grad", "more than 2^31 - 65536 columns");
   hipStream_t s = static_cast<hipStream_t>(stream);
   FewPlan few;
   if (trs_embed_grad_workspace_bytes(count, rows, width) == 0 && few_plan(count, rows, width, out_type, few)) {

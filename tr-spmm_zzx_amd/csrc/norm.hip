@@ -538,6 +538,9 @@ bool launch_norm_res(const NormArgs& p, int r_type, hipStream_t s) {
 }
 
 constexpr int64_t kMostRows = (int64_t)1 << 38;
+// k_norm_grad_columns takes its columns along the grid's second dimension.
+constexpr int32_t kMostGradWidth = 65535 * kThreads * 8;
+static_assert(kMostGradWidth <= kMostWidth, "column indexes of 32 bits");
 
 const void* at_row(const void* p, int64_t elements, int type) {
   return static_cast<const char*>(p) + elements * (type == TRS_F32 ? 4 : 2);
@@ -556,6 +559,7 @@ int norm_call(const char* where, const NormArgs& p, int x_type, int r_type, void
   if (p.ldx < p.width || p.ldy < p.width || (p.res && (p.ldr < p.width || p.ldro < p.width)))
     return fail(TRS_EINVAL, where, "leading dimension < width");
   if (p.rows > kMostRows) return fail(TRS_ERANGE, where, "too many rows");
+  if (p.width > kMostWidth) return fail(TRS_ERANGE, where, "more than 2^31 - 65536 columns");
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (!p.res) r_type = kNoResidual;
   // as many rows a launch as it can have workgroups
@@ -668,6 +672,7 @@ extern "C" int trs_rms_norm_grad(const void* grad, int32_t grad_type, int64_t ld
   if (!(eps > 0.f) || !std::isfinite(eps)) return fail(TRS_EINVAL, where, "eps must be positive and finite");
   if (width == 0) return TRS_OK;
   if (!dweight) return fail(TRS_EINVAL, where, "NULL operand");
+  if (width > kMostGradWidth) return fail(TRS_ERANGE, where, "more than 134215680 columns");
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (rows == 0) {
     k_zero<<<dim3((uint32_t)ceil_div(width, kThreads)), kThreads, 0, s>>>(dweight, width);
