@@ -199,6 +199,21 @@ def test_grad_of_special_rows(width):
     assert bool(torch.isnan(dw).all())
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("width", [5, 40, 127, 600, 2100, 5000, 9001])
+def test_grad_where_products_pass_32_bits(width, dtype):
+    """dr is ordinary where grad is as large as r, while their products are not: with squares in 32 bits and beyond, beside
+    ordinary rows, and with a residual's own gradient."""
+    say("large products", width, dtype)
+    r, w, g, more = (rand((9, width), dtype, 1), weights(width, torch.float32, 2), rand((9, width), dtype, 3), rand((9, width), dtype, 4))
+    for row, of_r, of_g in [(1, 1e17, 1e22), (2, 1e18, 1e24), (4, 3e37, 1e37), (5, 1e-3, 1e34), (7, 1e30, 1e30)]:
+        r[row] *= of_r
+        g[row] *= of_g
+    dr, dw = trspmm.rms_norm_grad(g, r, w, more, EPS)
+    assert bool(torch.isfinite(dr).all())
+    check_grad(g, r, w, more, dr, dw)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("width", [13, 43, 130, 1001, 8199])
 def test_strides_offsets_and_place(dtype, width):

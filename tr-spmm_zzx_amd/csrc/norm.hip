@@ -11,7 +11,7 @@
 // A row is held in registers between its reduction and its output, so each operand is read once and each
 // output written once: the kernels are bound by memory.  A group of lanes (8 .. 64, or the workgroup) owns a
 // row; 8 elements are one load.  The sum of squares of a row whose values are too large for 32-bit squares
-// is taken again at a smaller scale (kSmall).
+// is taken again at a smaller scale (kSmall), and so is the gradient's sum of g r where it passes 32 bits.
 #include "dense.hpp"
 
 #include <cfloat>
@@ -305,6 +305,7 @@ __device__ __forceinline__ void group_sums(float& a, float& b, float* red) {
 template <class D, class R, int G, int NC>
 __global__ __launch_bounds__(kThreads) void k_norm_grad(GradArgs p) {
   constexpr int kRows = kThreads / G;
+  constexpr bool kHalf = std::is_same<R, f16_t>::value;
   __shared__ float red[2][2][8];
   __shared__ float joined[kRows > 1 ? kThreads * NC * 8 : 1];
   const int lane = threadIdx.x % G, group = threadIdx.x / G;
@@ -355,21 +356,27 @@ __global__ __launch_bounds__(kThreads) void k_norm_grad(GradArgs p) {
       }
     group_sums<G>(square, dot, red[turn][0]);
     float s = rstd_of(square, p.width, p.eps), f = 1.f;
-    if (!(square <= FLT_MAX)) {
-      f = kSmall;
+    float mean = dot * s / (float)p.width;   // of g u
+    // Products pass 32 bits beside an r of at most 65504 only where dr passes 65504 too.
+    const bool fits = kHalf || fabsf(dot * s) <= FLT_MAX;
+    if (!(square <= FLT_MAX && fits)) {   // squares or products beyond 32 bits, or a value that is not finite
+      const bool large = !(square <= FLT_MAX);
+      const float q = fits ? 1.f : kSmall;
+      if (large) f = kSmall;
       square = dot = 0.f;
+      // Unrolled, this would take a lane of one chunk past 128 registers (bfloat16 and float32, 262144 x 300: 235 -> 271 us).
 #pragma unroll
       for (int c = 0; c < NC; ++c)
-#pragma unroll
+#pragma unroll(NC == 1 && !kHalf ? 1 : 8)
         for (int i = 0; i < 8; ++i) {
           const float r = (float)x.r[c][i] * f, g = (float)x.g[c][i];
           square += i >= dup[c] ? r * r : 0.f;
-          dot += i >= dup[c] ? g * w[c][i] * r : 0.f;
+          dot += i >= dup[c] ? g * w[c][i] * (r * q) : 0.f;
         }
       group_sums<G>(square, dot, red[turn][1]);
-      s = rstd_of(square, p.width, 0.f);
+      s = rstd_of(square, p.width, large ? 0.f : p.eps);
+      mean = dot * s / (float)p.width / q;
     }
-    const float mean = dot * s / (float)p.width;   // of g u
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       float out[8];
@@ -413,7 +420,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_grad(GradArgs p) {
 // for the weight.
 template <class D, class R>
 __global__ __launch_bounds__(kThreads) void k_norm_grad_long(GradArgs p) {
-  __shared__ float red[4][4];
+  __shared__ float red[5][4];
   const int64_t row = blockIdx.x;
   const typename R::raw* r_row = static_cast<const typename R::raw*>(p.r) + row * p.ldr;
   const typename D::raw* g_row = static_cast<const typename D::raw*>(p.grad) + row * p.ldg;
@@ -437,7 +444,19 @@ __global__ __launch_bounds__(kThreads) void k_norm_grad_long(GradArgs p) {
     if (square <= FLT_MAX) break;
     f = kSmall;
   }
-  const float mean = dot * s / (float)p.width;
+  float mean = dot * s / (float)p.width;
+  if (!(fabsf(dot * s) <= FLT_MAX)) {   // products beyond 32 bits, or a value that is not finite
+    dot = 0.f;
+    for (int at = threadIdx.x * 8; at < p.width; at += kThreads * 8) {
+      const int n = p.width - at;
+      load_chunk<R>(r_row + at, n, r);
+      load_chunk<D>(g_row + at, n, g);
+      load_any(p.weight, p.w_type, at, n, w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) dot += g[i] * w[i] * (r[i] * f * kSmall);
+    }
+    mean = group_sum<kThreads>(dot, red[4]) * s / (float)p.width / kSmall;
+  }
   if (threadIdx.x == 0) {
     p.rstd[2 * row] = s;
     p.rstd[2 * row + 1] = f;
