@@ -214,6 +214,19 @@ def test_grad_where_products_pass_32_bits(width, dtype):
     check_grad(g, r, w, more, dr, dw)
 
 
+@pytest.mark.parametrize("eps", [1e-5, 1e36, 1e38])
+@pytest.mark.parametrize("width", [6, 40, 600, 4000, 9001])
+def test_eps_beside_squares_beyond_32_bits(width, eps):
+    """eps counts at every size of it and of the rows, also where squares pass 32 bits."""
+    say("large eps", width, eps)
+    x, w, g = rand((6, width), torch.float32, 1), weights(width, torch.float32, 2), rand((6, width), torch.float32, 3)
+    for row, size in enumerate([1.0, 3e17, 1e19, 3e19, 1e21, 3e37]):
+        x[row] *= size
+    check_norm(x, w, None, *trspmm.rms_norm(x, w, eps=eps), eps=eps)
+    check_codes(x, w, None, *trspmm.rms_norm_i8(x, w, eps=eps), eps=eps)
+    check_grad(g, x, w, None, *trspmm.rms_norm_grad(g, x, w, eps=eps), eps=eps)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("width", [13, 43, 130, 1001, 8199])
 def test_strides_offsets_and_place(dtype, width):

@@ -113,9 +113,11 @@ struct NormArgs {
   bool past_y, past_r;   // written past the caches
 };
 
-// 1/sqrt of the mean square.  Where 32-bit squares overflow, `sum` is that of the values times kSmall, and eps, nothing beside
-// them, is left out; a row with an infinity or a NaN then gives NaN or 0.
-__device__ __forceinline__ float rstd_of(float sum, int width, float eps) { return rsqrtf(sum / (float)width + eps); }
+// 1/sqrt of the mean square.  Where 32-bit squares overflow, `sum` is that of the values times f = kSmall, and eps is taken down
+// with them; a row with an infinity or a NaN then gives NaN or 0.
+__device__ __forceinline__ float rstd_of(float sum, int width, float eps, float f = 1.f) {
+  return rsqrtf(sum / (float)width + eps * f * f);
+}
 
 // A row by G lanes, NC chunks a lane.  2^20 x 128, float32 and a 16-bit residual to 8 bits: 201 us, 1.21 GB, 6.0 TB/s;
 // 16384 x 4096, all bfloat16: 83 us, 0.54 GB, 6.5 TB/s; one row of 4096 3.6 us, a launch and two reductions.
@@ -167,7 +169,7 @@ __global__ __launch_bounds__(kThreads) void k_norm(NormArgs p) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) sum += i >= dup[c] ? (h[c][i] * f) * (h[c][i] * f) : 0.f;
     sum = group_sum<G>(sum, red[1]);
-    s = rstd_of(sum, p.width, 0.f);
+    s = rstd_of(sum, p.width, p.eps, f);
   }
   uint32_t peak = 0;
 #pragma unroll
@@ -233,7 +235,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_long(NormArgs p) {
       for (int i = 0; i < 8; ++i) sum += (h[i] * f) * (h[i] * f);
     }
     sum = group_sum<kThreads>(sum, red[1]);
-    s = rstd_of(sum, p.width, 0.f);
+    s = rstd_of(sum, p.width, p.eps, f);
   }
   bool finite = true;
   float inv = 0.f;
@@ -360,9 +362,8 @@ __global__ __launch_bounds__(kThreads) void k_norm_grad(GradArgs p) {
     // Products pass 32 bits beside an r of at most 65504 only where dr passes 65504 too.
     const bool fits = kHalf || fabsf(dot * s) <= FLT_MAX;
     if (!(square <= FLT_MAX && fits)) {   // squares or products beyond 32 bits, or a value that is not finite
-      const bool large = !(square <= FLT_MAX);
       const float q = fits ? 1.f : kSmall;
-      if (large) f = kSmall;
+      if (!(square <= FLT_MAX)) f = kSmall;
       square = dot = 0.f;
       // Unrolled, this would take a lane of one chunk past 128 registers (bfloat16 and float32, 262144 x 300: 235 -> 271 us).
 #pragma unroll
@@ -374,7 +375,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_grad(GradArgs p) {
           dot += i >= dup[c] ? g * w[c][i] * (r * q) : 0.f;
         }
       group_sums<G>(square, dot, red[turn][1]);
-      s = rstd_of(square, p.width, large ? 0.f : p.eps);
+      s = rstd_of(square, p.width, kHalf ? 0.f : p.eps, f);   // float16: here for a value that is not finite alone
       mean = dot * s / (float)p.width / q;
     }
 #pragma unroll
@@ -440,7 +441,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_grad_long(GradArgs p) {
     }
     square = group_sum<kThreads>(square, red[again * 2]);
     dot = group_sum<kThreads>(dot, red[again * 2 + 1]);
-    s = rstd_of(square, p.width, again ? 0.f : p.eps);
+    s = rstd_of(square, p.width, p.eps, f);
     if (square <= FLT_MAX) break;
     f = kSmall;
   }
