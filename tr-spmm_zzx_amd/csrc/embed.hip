@@ -490,16 +490,25 @@ __global__ __launch_bounds__(kThreads) void k_join_runs(RunArgs<T> p) {
 // all ids over for them, sorts the ones it finds in LDS and sums their runs; the rows it found none for are
 // filled.  Rows are owned in units (of at least 256 bytes) that are dealt out so that neither neighbouring
 // nor evenly spaced ids meet in one workgroup: unit q belongs to owner (q ^ q >> bits) mod 2^bits.  Bound by
-// latency: 4096 ids into 16,384 float32 rows of 64: 9 us, where the launches of the sort and the sums take 35.
+// latency: 4096 ids into 16,384 float32 rows of 64: 7 us, where the launches of the sort and the sums take 29.
 constexpr int kFewThreads = 512;
 constexpr int kFewWaves = kFewThreads / 64;
 constexpr uint32_t kFewBits = 14, kFewIds = 1u << kFewBits;
-// Wider rows than this only up to half as many ids (16,384 of them against the sort's launches: 16,384 rows of 64 17 us, not
-// 34; 2^20 rows of 128 118, not 135; but 4096 rows of 256 with hubs 40, not 33, of 1024 57, not 36).  Where all
-// ids name one row, which one workgroup then sums, the launches would be faster: 64 columns, 8192 ids 76 us to 38.
+// Wider rows than this only up to half as many ids, as the gain over the sort's launches shrinks with the width (16,384 ids into
+// 16,384 rows of 64: 11 us, not 34; of 128: 22, not 35; 8192 ids, rows of 1024: 32, not 41).
 constexpr int kFewWidth = 128;
 constexpr uint32_t kFewRows = 65536;     // rows of a workgroup: marks in LDS
 constexpr uint32_t kLongRun = 16;        // longer ones are summed by the whole workgroup
+// Frequent rows (a hub, a padding id that is a real row): of 64 ids spread over the call's, kFrequent or more.  They are summed
+// by columns: each workgroup finds the same ones, takes some of their columns and walks all ids for them, with no list to sort
+// and no parts to join.  Into 16,384 rows, us, beside the sort's launches and, in brackets, one workgroup's list and sum:
+//   16,384 ids, rows of 64     all of one row 44, 36 (152)    half of them 38, 37 (93)    a tenth (not frequent) 32, 35
+//   8192 ids, rows of 1024     all 46, 45 (463)               30% 45, 43 (166)            8192 ids, rows of 64, all: 25, 35 (78)
+// A walk takes about as long whatever the row's share is, and a list of a sixth of the ids as long as a walk.
+constexpr uint32_t kSampled = 1024;         // from more ids than this on
+constexpr uint32_t kFrequent = 10, kMostFrequent = 64 / kFrequent;
+constexpr uint32_t kFrequentBlocks = 128;   // workgroups that there are for it at least
+constexpr uint32_t kNoRow = 0xffffffffu;
 
 template <class T>
 struct FewArgs {
@@ -543,42 +552,106 @@ __device__ __forceinline__ void exchange(uint32_t* words, uint32_t size, uint32_
   }
 }
 
+// Sums of a chunk from all groups of L lanes of the workgroup, in order: whole in the first group.
+template <int L, int W>
+__device__ __forceinline__ void join_groups(float (&acc)[8], float (&part)[kFewWaves][W]) {
+  const int lane = threadIdx.x % L;
+  // the groups of a wave, then the waves
+#pragma unroll
+  for (int d = L; d < 64; d <<= 1)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[j] += __shfl_xor(acc[j], d);
+  if ((threadIdx.x & 63) < L)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) part[threadIdx.x >> 6][lane * 8 + j] = acc[j];
+  __syncthreads();
+  if (threadIdx.x >= L) return;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) acc[j] = part[0][lane * 8 + j];
+  for (int w = 1; w < kFewWaves; ++w)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[j] += part[w][lane * 8 + j];
+}
+
 template <class T, int L>
-__global__ __launch_bounds__(kFewThreads) void k_grad_few(FewArgs<T> p) {
+__global__ __launch_bounds__(kFewThreads, 4) void k_grad_few(FewArgs<T> p) {
   constexpr int kGroups = kFewThreads / L;
   extern __shared__ uint32_t found[];      // count, rounded up to a power of two: local row << kFewBits | place of the id
   __shared__ uint32_t marks[kFewRows / 32];
   __shared__ float part[kFewWaves][L * 8];
   __shared__ uint32_t n_found, n_long, long_at[kFewIds / kLongRun];
+  __shared__ uint32_t bins[64], frequent[kMostFrequent], n_frequent, n_listed;
   const uint32_t owner = blockIdx.x, owner_mask = (1u << p.owner_bits) - 1, unit_mask = (1u << p.unit_bits) - 1;
+  const bool owns = owner <= owner_mask;   // other workgroups are there for frequent rows
+  auto id_at = [&](uint32_t i) {
+    return p.id_bits == 32 ? (int64_t) static_cast<const int32_t*>(p.ids)[i] : static_cast<const int64_t*>(p.ids)[i];
+  };
+  const bool looks = p.count > kSampled && threadIdx.x >= kFewThreads - 64;   // the last wave, for frequent rows
+  int64_t seen = -1;
+  if (looks) seen = id_at((threadIdx.x & 63) * p.count / 64);
   for (uint32_t k = threadIdx.x; k < (p.local_rows + 31) / 32; k += kFewThreads) marks[k] = 0;
-  if (threadIdx.x == 0) n_found = n_long = 0;
+  if (threadIdx.x < 64) bins[threadIdx.x] = 0;
+  if (threadIdx.x == 0) n_found = n_long = n_frequent = n_listed = 0;
   __syncthreads();
-  for (uint32_t i0 = threadIdx.x; i0 < p.count; i0 += 4 * kFewThreads) {
-    int64_t id[4];
+  if (owns)
+    for (uint32_t i0 = threadIdx.x; i0 < p.count; i0 += 4 * kFewThreads) {
+      int64_t id[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const uint32_t i = i0 + u * kFewThreads, at = i < p.count ? i : i0;
-      id[u] = p.id_bits == 32 ? (int64_t) static_cast<const int32_t*>(p.ids)[at] : static_cast<const int64_t*>(p.ids)[at];
-      if (i >= p.count) id[u] = -1;
-    }
+      for (int u = 0; u < 4; ++u) {
+        const uint32_t i = i0 + u * kFewThreads, at = i < p.count ? i : i0;
+        id[u] = id_at(at);
+        if (i >= p.count) id[u] = -1;
+      }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      if (id[u] < 0 || id[u] >= (int64_t)p.rows) continue;
-      const uint32_t row = (uint32_t)id[u], unit = row >> p.unit_bits, high = unit >> p.owner_bits;
-      if (((unit ^ high) & owner_mask) != owner) continue;
-      const uint32_t local = high << p.unit_bits | (row & unit_mask);
-      found[atomicAdd(&n_found, 1u)] = local << kFewBits | (i0 + u * kFewThreads);
-      atomicOr(&marks[local >> 5], 1u << (local & 31));
+      for (int u = 0; u < 4; ++u) {
+        if (id[u] < 0 || id[u] >= (int64_t)p.rows) continue;
+        const uint32_t row = (uint32_t)id[u], unit = row >> p.unit_bits, high = unit >> p.owner_bits;
+        if (((unit ^ high) & owner_mask) != owner) continue;
+        const uint32_t local = high << p.unit_bits | (row & unit_mask);
+        found[atomicAdd(&n_found, 1u)] = local << kFewBits | (i0 + u * kFewThreads);
+        atomicOr(&marks[local >> 5], 1u << (local & 31));
+      }
     }
+  if (looks) {
+    const uint32_t row = seen >= 0 && seen < (int64_t)p.rows ? (uint32_t)seen : kNoRow;
+    uint32_t some = 0;
+    atomicAdd(&bins[row & 63], row != kNoRow);
+    wave_fence();
+    uint64_t left = __ballot(row != kNoRow && bins[row & 63] >= kFrequent);   // hardly ever any where no row is frequent
+    while (left != 0) {
+      const uint32_t candidate = (uint32_t)__builtin_amdgcn_readlane((int)row, __builtin_ctzll(left));
+      const uint64_t same = __ballot(row == candidate);
+      if ((uint32_t)__popcll(same) >= kFrequent) frequent[some++] = candidate;
+      left &= ~same;
+    }
+    n_frequent = some;
   }
   __syncthreads();
-  const uint32_t n = n_found;
+  const uint32_t hubs = n_frequent;
+  uint32_t n = n_found;
   auto row_of = [&](uint32_t local) {
     const uint32_t high = local >> p.unit_bits;
     return (high << p.owner_bits | ((owner ^ high) & owner_mask)) << p.unit_bits | (local & unit_mask);
   };
-  {   // rows without ids (not past the caches: 2^20 rows of 128 with 4096 ids take 102 us, 110 if they were)
+  if (hubs > 0) {   // frequent rows leave the list
+    for (uint32_t base = 0; base < n; base += 4 * kFewThreads) {
+      uint32_t word[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const uint32_t j = base + u * kFewThreads + threadIdx.x;
+        word[u] = j < n ? found[j] : kNoRow;
+        const uint32_t row = row_of(word[u] >> kFewBits);
+        for (uint32_t h = 0; h < hubs; ++h) word[u] = frequent[h] == row ? kNoRow : word[u];
+      }
+      __syncthreads();   // read: the places so far are free
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (word[u] != kNoRow) found[atomicAdd(&n_listed, 1u)] = word[u];
+    }
+    __syncthreads();
+    n = n_listed;
+  }
+  if (owns) {   // rows without ids (not past the caches: 2^20 rows of 128 with 4096 ids take 102 us, 110 if they were)
     const Zeros chunks{0};
     const uint32_t parts = parts_of(chunks, p.width);
     for (uint64_t j = threadIdx.x; j < (uint64_t)p.local_rows * parts; j += kFewThreads) {
@@ -587,7 +660,7 @@ __global__ __launch_bounds__(kFewThreads) void k_grad_few(FewArgs<T> p) {
         write_zeros(chunks, p.out, p.out_type, p.ldo, row, (uint32_t)(j - (uint64_t)local * parts), p.width);
     }
   }
-  if (n == 0) return;
+  if (n == 0 && hubs == 0) return;
   // Sort: the words are all different.  Up to a word a thread by rank, more by a bitonic network.
   if (n <= kFewThreads) {
     uint32_t mine = 0, rank = 0;
@@ -677,25 +750,42 @@ __global__ __launch_bounds__(kFewThreads) void k_grad_few(FewArgs<T> p) {
       const int chunk = c * L + lane, at = chunk_at(chunk * 8 < p.width ? chunk : 0, p.width, shared);
       float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
       add(k0, k1, at, acc);
-      // the groups of a wave, then the waves
-#pragma unroll
-      for (int d = L; d < 64; d <<= 1)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) acc[j] += __shfl_xor(acc[j], d);
-      if ((threadIdx.x & 63) < L)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) part[threadIdx.x >> 6][lane * 8 + j] = acc[j];
-      __syncthreads();
-      if (group == 0) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) acc[j] = part[0][lane * 8 + j];
-        for (int w = 1; w < kFewWaves; ++w)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) acc[j] += part[w][lane * 8 + j];
-        if (chunk * 8 < p.width) write_row(p.out, p.out_type, p.ldo, row_of(local), at, p.width, p.scale, acc, false);
-      }
+      join_groups<L>(acc, part);
+      if (group == 0 && chunk * 8 < p.width) write_row(p.out, p.out_type, p.ldo, row_of(local), at, p.width, p.scale, acc, false);
       __syncthreads();
     }
+  }
+  // Frequent rows: H lanes hold 8 H columns of the row, and walk the ids with the workgroup's other groups.  From the last
+  // workgroup on, as a table's first rows, often its frequent ones, are in the first.
+  constexpr int H = L < 16 ? 1 : L / 16, kWalkers = kFewThreads / H, kWalk = (sizeof(typename T::raw) == 4 ? 4 : 8) * (L > 1 ? 2 : 1);
+  const uint32_t tasks = (uint32_t)(p.width + H * 8 - 1) / (H * 8);
+  for (uint32_t t = gridDim.x - 1 - blockIdx.x; t < tasks * hubs; t += gridDim.x) {
+    const uint32_t row = frequent[t / tasks];
+    int shared;
+    const int chunk = (int)(t % tasks) * H + (int)threadIdx.x % H, at = chunk_at(chunk * 8 < p.width ? chunk : 0, p.width, shared);
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (uint32_t i0 = threadIdx.x / H; i0 < p.count; i0 += kWalk * kWalkers) {
+      bool its[kWalk];
+      raw8<T> g[kWalk];
+#pragma unroll
+      for (int u = 0; u < kWalk; ++u) {
+        const uint32_t i = i0 + u * kWalkers;
+        its[u] = id_at(i < p.count ? i : i0) == (int64_t)row && i < p.count;
+      }
+#pragma unroll
+      for (int u = 0; u < kWalk; ++u) {   // what is not the row's is not used
+        const typename T::raw* from = p.grad + (int64_t)(its[u] ? i0 + u * kWalkers : i0) * p.ldg + at;
+        g[u] = L > 1 || p.width >= 8 ? load_raw<T>(from) : load_raw_narrow<T>(from, p.width);
+      }
+#pragma unroll
+      for (int u = 0; u < kWalk; ++u)
+        if (its[u])
+#pragma unroll
+          for (int j = 0; j < 8; ++j) acc[j] += (float)g[u][j];
+    }
+    join_groups<H>(acc, part);
+    if (threadIdx.x < H && chunk * 8 < p.width) write_row(p.out, p.out_type, p.ldo, row, at, p.width, p.scale, acc, false);
+    __syncthreads();
   }
 }
 
@@ -860,7 +950,8 @@ void launch_few(const FewPlan& f, const void* grad, int64_t ldg, const void* ids
                      scale, out, out_type, ldo, f.owner_bits, f.unit_bits, f.local_rows};
   uint32_t size = kFewThreads;
   while (size < count) size *= 2;
-  const dim3 grid(1u << f.owner_bits);
+  const uint32_t owners = 1u << f.owner_bits;
+  const dim3 grid(count > kSampled && owners < kFrequentBlocks ? kFrequentBlocks : owners);
   const size_t lds = size * sizeof(uint32_t);
   switch (group_lanes(width)) {
     case 1: k_grad_few<T, 1><<<grid, kFewThreads, lds, s>>>(p); break;
