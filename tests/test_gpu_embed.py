@@ -225,6 +225,75 @@ def test_runs_at_every_boundary():
     check_grad(trspmm.embed_grad(grad, ids, 2 * len(lengths)), grad, ids, 2 * len(lengths), 1.0)
 
 
+def sorts(count, rows, width):
+    """That a call of this size sorts its ids, and does not run in one launch."""
+    assert dense.embed_grad_workspace_bytes(count, rows, width) > 0
+
+
+@pytest.mark.parametrize("x", TYPES)
+@pytest.mark.parametrize("o", TYPES)
+@pytest.mark.parametrize("ids_type", [torch.int32, torch.int64])
+def test_types_of_sorted_ids(x, o, ids_type):
+    say("sorted types", x, o, ids_type)
+    sorts(17_003, 300, 72)
+    ids, grad = some_ids(17_003, 300, ids_type, 1), rand((17_003, 72), x, 3)
+    check_grad(trspmm.embed_grad(grad, ids, 300, 1.7, o), grad, ids, 300, 1.7)
+
+
+@pytest.mark.parametrize("width", [1, 2, 3, 4, 5, 6, 7, 8, 9, 11, 12, 13, 15, 16, 17, 31, 33, 64, 65, 100, 127, 129, 250, 257, 511, 512, 513,
+                                   520, 1000, 1023, 1030, 2050])
+@pytest.mark.parametrize("x", [torch.float16, torch.float32])
+def test_widths_of_sorted_ids(width, x):
+    """Each size of a group of lanes, whole and cut last chunks, one and several blocks of columns."""
+    say("sorted width", width, x)
+    for rows in (90, 9001):
+        sorts(17_003, rows, width)
+        ids, grad = some_ids(17_003, rows, torch.int64, width, skew=2), rand((17_003, width), x, 3)
+        check_grad(trspmm.embed_grad(grad, ids, rows, 0.5), grad, ids, rows, 0.5)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("width", [3, 13, 43, 517])
+def test_strides_of_sorted_ids(dtype, width):
+    say("sorted strides", dtype, width)
+    wide, rows, count = width + 18, 700, 17_003
+    sorts(count, rows, width)
+    ids = some_ids(2 * count, rows, torch.int64, 4)[::2]
+    grad = rand((count, wide), dtype, 2)[:, 5:5 + width]
+    buf = torch.full((rows, wide), 9.0, dtype=dtype, device="cuda")
+    out = trspmm.embed_grad(grad, ids, rows, 1.5, out=buf[:, 7:7 + width])
+    check_grad(out, grad, ids, rows, 1.5)
+    assert bool((buf[:, :7] == 9).all()) and bool((buf[:, 7 + width:] == 9).all())
+    g = rand((1, width), dtype, 6).expand(count, width)                    # a broadcast gradient
+    check_grad(trspmm.embed_grad(g, ids, rows, 1.5), g, ids, rows, 1.5)
+
+
+@pytest.mark.parametrize("width", [4, 8, 16, 24, 50, 128, 200, 512, 600, 1030])
+def test_sorted_runs_at_every_boundary(width):
+    """Runs that end just before, at and just after the 16 ids of a piece and the ids of a workgroup (a piece for each of its
+    groups of lanes), and runs over several workgroups, each begun at such a place."""
+    lanes = 1
+    while lanes < 64 and lanes * 8 < width:
+        lanes *= 2
+    piece, block = 16, 256 // lanes * 16
+    lengths = []
+    for unit in (piece, block, 2 * block, 3 * block):
+        for off in (-1, 0, 1, 7):
+            lengths += [unit + off, unit - off] if off else [unit, 1, unit - 1]   # the next one starts on a boundary again
+    lengths += [1, 15, 1, block - 17, 1, block, block, 2, block - 2, piece, block - piece]
+    while sum(lengths) <= 16_400:
+        lengths += [1, 15, 16, 17, 5, 2 * block + 3, block - 1]
+    say("sorted runs", width, sum(lengths))
+    rows = 2 * len(lengths)
+    sorts(sum(lengths), rows, width)
+    ids = torch.cat([torch.full((n,), 2 * i, device="cuda") for i, n in enumerate(lengths)] + [torch.full((5,), -1, device="cuda")])
+    for seed in (0, 1):                                                    # in their order, and not
+        if seed:
+            ids = ids[torch.randperm(ids.shape[0], generator=gen(seed), device="cuda")]
+        grad = rand((ids.shape[0], width), torch.float32, 1)
+        check_grad(trspmm.embed_grad(grad, ids, rows), grad, ids, rows, 1.0)
+
+
 def test_ids_outside_the_table():
     say("outside")
     ids = torch.tensor([0, -1, 4, 5, 2 ** 31, 2 ** 32 + 1, -2 ** 40, 3], device="cuda")
