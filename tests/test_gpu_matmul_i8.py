@@ -194,3 +194,22 @@ def test_refusals():
         call = list(good)
         call[k] = v
         assert lib.trs_matmul_i8(*call) == 1, k
+
+
+def test_an_output_of_another_type_than_asked_for_is_refused():
+    """Every operator that takes both; where no type is asked for, the output's is the one."""
+    say("dtype and out")
+    a, w, sa, sw = codes(4, 32, 1), codes(6, 32, 2), scales(4, 3), scales(6, 4)
+    x, ids, one = torch.randn((6, 32), device="cuda"), torch.tensor([0, 5, 1, 1], device="cuda"), torch.ones(32, device="cuda")
+    calls = [((4, 6), lambda **kw: trspmm.matmul_i8(a, sa, w, sw, **kw)), ((4, 32), lambda **kw: trspmm.embed(x, ids, **kw)),
+             ((9, 32), lambda **kw: trspmm.embed_grad(x[:4], ids, 9, **kw)), ((6, 32), lambda **kw: trspmm.rms_norm(x, one, **kw)[0])]
+    for shape, call in calls:
+        for asked in TYPES:
+            for given in TYPES:
+                out = torch.full(shape, 7.0, dtype=given, device="cuda")
+                if given is not asked:
+                    with pytest.raises(ValueError):
+                        call(out=out, dtype=asked)
+                    assert bool((out == 7).all())
+                kw = {"dtype": asked} if given is asked else {}
+                assert call(out=out, **kw).dtype is given and not bool((out == 7).all())

@@ -77,6 +77,13 @@ Tensor fresh(at::IntArrayRef shape, at::ScalarType type, int64_t dev) {
   return at::empty(shape, at::TensorOptions().dtype(type).device(at::Device(at::kCUDA, (at::DeviceIndex)dev)));
 }
 
+// An output's type: `dtype` or the one that it has by default, and that of the output that is given.
+at::ScalarType type_out(const Given& out, const Type& dtype, at::ScalarType by_default) {
+  if (out && dtype && out->scalar_type() != *dtype)
+    wrong(std::string("out is ") + c10::toString(out->scalar_type()) + ", dtype asks for " + c10::toString(*dtype));
+  return out ? out->scalar_type() : dtype.value_or(by_default);
+}
+
 // The given output, checked, or a new one.
 Tensor output(const char* name, const Given& out, int64_t rows, int64_t width, at::ScalarType type, int64_t dev) {
   if (!out) return fresh({rows, width}, type, dev);
@@ -111,7 +118,7 @@ Tensor embed(const Tensor& table_in, const Tensor& ids_in, double scale, const T
              int64_t stream) {
   const Tensor table = matrix("table", table_in, dev);
   const auto [ids, bits] = ids_of(ids_in, dev);
-  const at::ScalarType type = out_in ? out_in->scalar_type() : dtype.value_or(table.scalar_type());
+  const at::ScalarType type = type_out(out_in, dtype, table.scalar_type());
   const int t_type = type_of("table", table.scalar_type()), o_type = type_of("dtype", type);
   const Tensor out = output("out", out_in, ids.size(0), table.size(1), type, dev);
   ok(trs_embed(table.data_ptr(), t_type, ld(table), table.size(0), ids.data_ptr(), bits, ids.size(0), width_of(table),
@@ -128,7 +135,7 @@ Tensor embed_grad(const Tensor& grad_in, const Tensor& ids_in, int64_t rows, dou
   if (ids.size(0) != count)
     wrong("grad has " + std::to_string(count) + " rows for " + std::to_string(ids.size(0)) + " ids");
   if (rows < 0) wrong("rows must not be negative");
-  const at::ScalarType type = out_in ? out_in->scalar_type() : dtype.value_or(at::kFloat);
+  const at::ScalarType type = type_out(out_in, dtype, at::kFloat);
   const int g_type = type_of("grad", grad.scalar_type()), o_type = type_of("dtype", type);
   const int32_t width = width_of(grad);
   const int64_t need = trs_embed_grad_workspace_bytes(count, rows, width);
@@ -170,7 +177,7 @@ struct NormOperands {
 std::tuple<Tensor, Given> rms_norm(const Tensor& x, const Tensor& weight, const Given& residual, double eps, const Type& dtype,
                                    const Given& out_in, const Given& r_out, int64_t dev, int64_t stream) {
   const NormOperands n(x, weight, residual, r_out, dev);
-  const at::ScalarType type = out_in ? out_in->scalar_type() : dtype.value_or(n.x.scalar_type());
+  const at::ScalarType type = type_out(out_in, dtype, n.x.scalar_type());
   const int y_type = type_of("dtype", type);
   const Tensor out = output("out", out_in, n.rows, n.width, type, dev);
   ok(trs_rms_norm(n.x.data_ptr(), n.x_type, ld(n.x), data(n.residual), n.r_type, n.ldr(), weight.data_ptr(), n.w_type,
@@ -220,7 +227,7 @@ std::tuple<Tensor, Tensor> rms_norm_grad(const Tensor& grad_in, const Tensor& r_
 }
 
 Tensor matmul_i8(const Tensor& a_in, const Tensor& a_scale, const Tensor& w_in, const Tensor& w_scale, const Given& bias,
-                 at::ScalarType dtype, const Given& out_in, int64_t dev, int64_t stream) {
+                 const Type& dtype, const Given& out_in, int64_t dev, int64_t stream) {
   if (a_in.scalar_type() != at::kChar) wrong("a must be int8");
   if (w_in.scalar_type() != at::kChar) wrong("w must be int8");
   const Tensor a = matrix("a", a_in, dev), w = matrix("w", w_in, dev);
@@ -231,7 +238,7 @@ Tensor matmul_i8(const Tensor& a_in, const Tensor& a_scale, const Tensor& w_in, 
   floats("a_scale", a_scale, m, dev);
   floats("w_scale", w_scale, n, dev);
   if (bias) floats("bias", *bias, n, dev);
-  const at::ScalarType type = out_in ? out_in->scalar_type() : dtype;
+  const at::ScalarType type = type_out(out_in, dtype, at::kHalf);
   const int o_type = type_of("dtype", type);
   const Tensor out = output("out", out_in, m, n, type, dev);
   ok(trs_matmul_i8(static_cast<const int8_t*>(a.data_ptr()), ld(a), static_cast<const float*>(a_scale.data_ptr()),

@@ -11,7 +11,8 @@ A layer that serves in 8 bits:
 
 Tensors live on the current GPU; work is enqueued on ``stream`` (default: the current torch stream).
 Matrices are 2-D with unit column stride and any row stride; one with another column stride is copied.
-Outputs and workspaces that are not given are allocated on the launch stream.  Arguments are checked in the
+Outputs that are not given, and workspaces that are not given or too small, are allocated on the launch stream; a given
+output has the type that is asked for, or says which where none is.  Arguments are checked in the
 extension (csrc/ext_dense.cpp); the kernels are libtrspmm.so's, and there is no CPU fallback.
 """
 from __future__ import annotations
@@ -93,9 +94,9 @@ def rms_norm_grad(grad: torch.Tensor, r: torch.Tensor, weight: torch.Tensor, gra
 
 
 def matmul_i8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
-              bias: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.float16,
+              bias: Optional[torch.Tensor] = None, dtype: Optional[torch.dtype] = None,
               out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
-    """out[i, j] = a_scale[i] * w_scale[j] * (a[i] . w[j]) + bias[j] in `dtype`: codes `a` [m, k] with a scale
+    """out[i, j] = a_scale[i] * w_scale[j] * (a[i] . w[j]) + bias[j] in `dtype` (default float16): codes `a` [m, k] with a scale
     for each row (of :func:`rms_norm_i8`), weights `w` [n, k] with a scale for each output channel, both
     int8; scales and bias float32.  The integer sums are exact (k at most 131071)."""
     return _call("matmul_i8", stream, a, a_scale, w, w_scale, bias, dtype, out)
