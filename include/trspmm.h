@@ -477,11 +477,11 @@ int trs_sddmm_f16_kernel_ms(const trs_plan* p, const uint16_t* X, int64_t ldx, c
  * the SpMM.  No reference counterparts (the reference multiplies by the graph only).
  *
  * Matrices are row-major with a leading dimension (elements between rows, at least the width) and
- * start at any element; types are trs_dtype.  Sums, norms and scales are held in 32 bits and
- * rounded once when written.  Calls launch kernels only (no memset nodes, no allocation, no
- * synchronisation), so they can be captured in a HIP graph; equal inputs give equal bits.  They run
- * on the current device, which must hold the operands.  A call with no rows or no width launches
- * nothing it need not.  Rows have at most 2^31 - 65536 columns (trs_rms_norm_grad: 65535 * 2048;
+ * start at any element; types are trs_dtype.  Workspaces start on an 8-byte boundary (TRS_EINVAL
+ * otherwise).  Sums, norms and scales are held in 32 bits and rounded once when written.  Calls
+ * launch kernels only (no memset nodes, no allocation, no synchronisation), so they can be captured
+ * in a HIP graph; equal inputs give equal bits.  They run on the current device, which must hold the
+ * operands.  A call with no rows or no width launches nothing it need not.  Rows have at most 2^31 - 65536 columns (trs_rms_norm_grad: 65535 * 2048;
  * trs_embed_grad where it sorts: 65535 * 512), TRS_ERANGE otherwise.
  * ------------------------------------------------------------------------------------------- */
 /* out[t] = scale * table[ids[t]] for t < count: table [rows, width], out [count, width].  ids are

@@ -114,3 +114,12 @@ def test_gradients_of_more_columns_than_a_grid_are_refused(width, rows):
     lib = nat.lib()
     args = {**NORM_GRAD, "ldg": FAR, "ldr": FAR, "lddr": FAR, "width": width, "rows": rows, "ws_bytes": 1 << 60}
     assert lib.trs_rms_norm_grad(*args.values()) == 5, lib.trs_last_error()
+
+
+@pytest.mark.parametrize("off", [1, 2, 4, 7])
+def test_workspaces_off_8_byte_boundaries_are_refused(off):
+    lib = nat.lib()
+    assert X % 8 == 0
+    args = {**EMBED_GRAD, "count": 100_000, "ws": X + off, "ws_bytes": 1 << 40}
+    assert lib.trs_embed_grad(*args.values()) == 1, lib.trs_last_error()
+    assert lib.trs_rms_norm_grad(*{**NORM_GRAD, "ws": X + off}.values()) == 1, lib.trs_last_error()

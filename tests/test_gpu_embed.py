@@ -428,6 +428,18 @@ def test_large_outputs(o):
         check_grad(trspmm.embed_grad(grad[:900], ids[:900], 90_000, 0.7, o), grad[:900], ids[:900], 90_000, 0.7)
 
 
+@pytest.mark.parametrize("off", [0, 1, 4, 8])
+def test_workspaces_at_any_address(off):
+    """One off the 8-byte boundary is left alone, and another used in its place."""
+    say("workspace", off)
+    ids, grad = some_ids(20_000, 700, torch.int64, 1), rand((20_000, 24), torch.float16, 2)
+    need = dense.embed_grad_workspace_bytes(20_000, 700, 24)
+    ws = torch.full((need + 16,), 171, dtype=torch.uint8, device="cuda")
+    out = trspmm.embed_grad(grad, ids, 700, workspace=ws[off:off + need])
+    check_grad(out, grad, ids, 700, 1.0)
+    assert bool((ws == 171).all()) == (off % 8 != 0)
+
+
 def test_gradient_against_differences():
     """The lookup is linear in the table: <embed(table + v) - embed(table), g> = <embed_grad(g), v>."""
     say("differences")

@@ -43,6 +43,9 @@ inline bool known_type(int32_t t) { return t == TRS_F32 || t == TRS_F16 || t == 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
 
+// Workspaces are read as words of 8 bytes.
+inline bool aligned_workspace(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7) == 0; }
+
 // A launch holds less than 2^32 threads along a dimension.
 inline bool fits_grid(int64_t blocks, int threads = 256) { return blocks <= (int64_t)UINT32_MAX / threads; }
 

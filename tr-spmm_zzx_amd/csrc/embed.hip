@@ -1030,6 +1030,7 @@ extern "C" int trs_embed_grad(const void* grad, int32_t grad_type, int64_t ldg, 
     g = grad_layout(count, rows, width);
     if (!workspace || workspace_bytes < g.bytes)
       return fail(TRS_EINVAL, "trs_embed_grad", "workspace smaller than trs_embed_grad_workspace_bytes");
+    if (!aligned_workspace(workspace)) return fail(TRS_EINVAL, "trs_embed_grad", "workspace off an 8-byte boundary");
   } else {
     g.lanes = group_lanes(width);
   }

@@ -95,12 +95,12 @@ Tensor output(const char* name, const Given& out, int64_t rows, int64_t width, a
   return *out;
 }
 
-// The given workspace, if it is large enough, or a new one.
+// The given workspace, if it is large enough and on the C entries' boundary, or a new one.
 Tensor workspace_of(const Given& workspace, int64_t need, int64_t dev) {
   if (workspace) {
     on_device("workspace", *workspace, dev);
     if (!workspace->is_contiguous()) wrong("workspace must be contiguous");
-    if ((int64_t)workspace->nbytes() >= need) return *workspace;
+    if ((int64_t)workspace->nbytes() >= need && (reinterpret_cast<uintptr_t>(workspace->data_ptr()) & 7) == 0) return *workspace;
   }
   return need > 0 ? fresh({need}, at::kByte, dev) : Tensor();
 }

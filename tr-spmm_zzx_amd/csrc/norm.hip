@@ -704,6 +704,7 @@ extern "C" int trs_rms_norm_grad(const void* grad, int32_t grad_type, int64_t ld
   if (rows > kMostRows || (width > kNormMost && !fits_grid(rows))) return fail(TRS_ERANGE, where, "too many rows");
   if (!workspace || workspace_bytes < trs_rms_norm_grad_workspace_bytes(rows, width))
     return fail(TRS_EINVAL, where, "workspace smaller than trs_rms_norm_grad_workspace_bytes");
+  if (!aligned_workspace(workspace)) return fail(TRS_EINVAL, where, "workspace off an 8-byte boundary");
   if (dr == grad || dr == r) return fail(TRS_EINVAL, where, "dr cannot take the place of grad or r");
   char* ws = static_cast<char*>(workspace);
   const int64_t sums = round_up(grad_blocks(rows, width) * round_up(width, 8) * 4, 256);

@@ -11,8 +11,8 @@ A layer that serves in 8 bits:
 
 Tensors live on the current GPU; work is enqueued on ``stream`` (default: the current torch stream).
 Matrices are 2-D with unit column stride and any row stride; one with another column stride is copied.
-Outputs that are not given, and workspaces that are not given or too small, are allocated on the launch stream; a given
-output has the type that is asked for, or says which where none is.  Arguments are checked in the
+Outputs that are not given, and workspaces that are not given, too small or off an 8-byte boundary, are allocated on the
+launch stream; a given output has the type that is asked for, or says which where none is.  Arguments are checked in the
 extension (csrc/ext_dense.cpp); the kernels are libtrspmm.so's, and there is no CPU fallback.
 """
 from __future__ import annotations
