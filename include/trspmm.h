@@ -481,8 +481,9 @@ int trs_sddmm_f16_kernel_ms(const trs_plan* p, const uint16_t* X, int64_t ldx, c
  * otherwise).  Sums, norms and scales are held in 32 bits and rounded once when written.  Calls
  * launch kernels only (no memset nodes, no allocation, no synchronisation), so they can be captured
  * in a HIP graph; equal inputs give equal bits.  They run on the current device, which must hold the
- * operands.  A call with no rows or no width launches nothing it need not.  Rows have at most 2^31 - 65536 columns (trs_rms_norm_grad: 65535 * 2048;
- * trs_embed_grad where it sorts: 65535 * 512), TRS_ERANGE otherwise.
+ * operands.  A call with no rows or no width launches nothing it need not.  Rows have at most
+ * 2^31 - 65536 columns (trs_rms_norm_grad: 65535 * 2048; trs_embed_grad where it sorts: 65535 * 512),
+ * TRS_ERANGE otherwise.
  * ------------------------------------------------------------------------------------------- */
 /* out[t] = scale * table[ids[t]] for t < count: table [rows, width], out [count, width].  ids are
  * int32 (id_bits 32) or int64 (64); one outside [0, rows) (a padded slot) gives a row of zeros.
@@ -492,8 +493,9 @@ int trs_embed(const void* table, int32_t table_type, int64_t ldt, int64_t rows, 
 
 /* The gradient of trs_embed towards its table: out[v] = scale * sum over t with ids[t] = v of
  * grad[t], for every row v < rows (zeros where no id names it; ids outside [0, rows) take no part).
- * out is written whole.  The ids are sorted in the workspace, equal ones summed in the order they
- * come in, in 32 bits.  count and rows below 2^31 - 1 (TRS_ERANGE otherwise). */
+ * out is written whole.  Sums are in 32 bits and in an order that count, rows, width and the ids
+ * alone decide.  Many ids are sorted in the workspace.  count and rows below 2^31 - 1 (TRS_ERANGE
+ * otherwise). */
 int64_t trs_embed_grad_workspace_bytes(int64_t count, int64_t rows, int32_t width);
 int trs_embed_grad(const void* grad, int32_t grad_type, int64_t ldg, const void* ids, int32_t id_bits, int64_t count,
                    int64_t rows, int32_t width, float scale, void* out, int32_t out_type, int64_t ldo, void* workspace,

@@ -42,7 +42,7 @@ namespace {
 // allocated from a per-thread monotonic arena (released once, after the build) instead of the
 // general heap: freeing and re-allocating them window after window returned memory to the system
 // and faulted it back in, which doubled a first build in a fresh process (grid+hubs 0.76 s against
-// 0.35 s for a second one, R-MAT 0.45 s against 0.26 s on the GPU box host).
+// 0.35 s for a second one, R-MAT 0.45 s against 0.26 s on the MI355X's host).
 template <class T>
 using wvec = std::pmr::vector<T>;
 

@@ -60,8 +60,9 @@ __global__ __launch_bounds__(kThreads) void k_embed(const typename T::raw* __res
 // each block of ids (k_digit_count), turns each digit's counts into offsets (k_digit_offsets) and moves the ids
 // with their positions (k_digit_move).  The order of equal digits is kept: a wave ranks 64 ids at a time with
 // ballots, waves and blocks follow one another.  Ids outside the table are left out in the first pass, whose
-// move writes how many are left (`kept`).  Digits of 11 bits, the most whose counts for each wave fit in LDS, as
-// every pass costs two or three launches.  Bound by their latency and scattered 8-byte writes: 1,000,003 ids of 2^20
+// move writes how many are left (`kept`).  Digits of 11 bits, as every pass costs two or three launches: two digits a
+// thread in the scan, and two workgroups a CU by their 72.5 KB of LDS (12 bits would fit one, in 147.5 KB, and save a pass of
+// tables of 2^22 to 2^24 rows; not measured).  Bound by their latency and scattered 8-byte writes: 1,000,003 ids of 2^20
 // rows, two passes, 52 us (a pass: counts 5, offsets 5, moves 16).
 constexpr int kMaxBits = 11;
 constexpr int kMaxBins = 1 << kMaxBits;
@@ -344,7 +345,7 @@ __global__ __launch_bounds__(kThreads) void k_sum_runs(RunArgs<T> p) {
   constexpr int kGroups = kThreads / L;
   constexpr int kIds = kGroups * kPiece;
   __shared__ float part[kGroups][2][L * 8];
-  __shared__ uint8_t goes_on[kGroups];   // bit 0: the group's last run goes on; bit 1: so does its only run, which came in
+  __shared__ uint8_t goes_on[kGroups];   // whether the group's ids are all of one run, which came in and goes on
   const uint32_t count = p.kept ? *p.kept : 0;
   const uint32_t block = blockIdx.x;
   if (block >= p.groups_blocks) {
@@ -373,7 +374,7 @@ __global__ __launch_bounds__(kThreads) void k_sum_runs(RunArgs<T> p) {
   bool came = some && e0 > 0 && p.sorted[e0 - 1].key == key[0];
   const bool only = came && key[kPiece] == key[0];
   const bool starts_on = some && key[kPiece - 1] < p.rows && key[kPiece] == key[kPiece - 1] && !only;
-  if (lane == 0) goes_on[group] = (uint8_t)((starts_on || only ? 1 : 0) | (only ? 2 : 0));
+  if (lane == 0) goes_on[group] = only;
 
   float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   const bool head = came;
@@ -416,13 +417,13 @@ __global__ __launch_bounds__(kThreads) void k_sum_runs(RunArgs<T> p) {
     const float* from = part[g][which == 0 ? 1 : 0] + lane * 8;
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[j] = from[j];
-    bool on = which == 0 ? true : (goes_on[0] & 2) != 0;
+    bool on = which == 0 || goes_on[0];
     while (on && g + 1 < kGroups) {
       ++g;
       from = part[g][0] + lane * 8;
 #pragma unroll
       for (int j = 0; j < 8; ++j) acc[j] += from[j];
-      on = (goes_on[g] & 2) != 0;
+      on = goes_on[g];
     }
     if (!used) continue;
     if (which == 1 || on) {

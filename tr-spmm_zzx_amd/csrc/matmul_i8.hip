@@ -700,11 +700,20 @@ void launch(const MatArgs& p, hipStream_t s) {
     case 4: return launch_rows<4>(p, odd, s);
   }
   if (p.k <= kDepth) {
-    // Rows that do not come from the MALL (256 MB) are read ahead by k_matmul_panel: 1000003 x 256 x 128: 145 us, with tiles of
-    // 128 x 256 168; x 96: 139, 166; but x 80: 137, 122; 262144 x 512 x 128: 75, 68.
-    // Otherwise, without large outputs' way past the caches: 1000003 x 256 x 128: 240 us with tiles of 64 x 64, 213 of
-    // 128 x 128, 171 of 128 x 256; x 128: 120, 106, 136; x 64: 61, 87, 118.  Below two workgroups a CU the smallest
-    // (2000 x 500 x 128: 4.1, 6.5, 7.0).
+    // k_matmul_panel reads rows ahead, which pays where they come from HBM, and costs its walk's tail where they come from the
+    // MALL (256 MB).  Rows just written by the 8-bit norm do from some 60 M codes down, as the norm's own reads push the others
+    // out: panel against tiles of 128 x 256, us, norm first:
+    //     m x n x k           codes, M   panel  tiles     all rows from HBM     all from the MALL
+    //   524288 x 256 x 64        32       74     62          73     86             74     63
+    //   524288 x 512 x 128       64      151    154         149    180            159    133
+    //   1000003 x 256 x 64       61      139    134         138    164            136    115
+    //   1000003 x 136 x 64       61      126    140         124    141            124    140
+    //   1000003 x 256 x 128     122      148    172         145    167            157    135
+    //   1000003 x 512 x 128     122      288    345         284    343            308    255
+    // Rows off 4-byte boundaries follow (1000003 x 256 x 127, from HBM: 153, 176; x 512: 303, 351), short ones too
+    // (5900001 x 136 x 16, 90 M: 675, 763).
+    // The other tiles' sizes: 1000003 x 256 x 128 240 us with tiles of 64 x 64, 213 of 128 x 128, 171 of 128 x 256; x 128: 120,
+    // 106, 136; x 64: 61, 87, 118.  Below two workgroups a CU the smallest (2000 x 500 x 128: 4.1, 6.5, 7.0).
     if (p.n > 128 && p.n <= 64 * kPanelColumns && p.k >= 16 && p.m * p.k >= (int64_t)90 << 20) launch_panel(p, s);
     else if (p.n > 128 && tiles(p, 128, 256) >= 2 * kCus) launch_once<128, 256, 64, 64>(p, odd, s);
     else if (p.n > 64 && tiles(p, 128, 128) >= 2 * kCus) launch_once<128, 128, 64, 64>(p, odd, s);

@@ -22,8 +22,9 @@ namespace dense {
 namespace {
 
 constexpr int kThreads = 256;
-// Rows are written past the caches from this size on (16384 x 4096 in 16 bits: 97 -> 92 us, its gradient 109 -> 104; half of
-// that, 41 -> 46 and 56 -> 57).
+// Rows are written past the caches from this size on.  In 16 bits, widths of 128, 1024 and 4096, operands that change from call to call:
+// up to 2% either way from 64 to 112 MiB (rows of 1024 gain 2 to 6% from 32 MiB on, float32 sums of 128 to 8-bit codes lose 6%
+// there), 1 to 4% won by the gradient from 128 MiB on (16384 x 4096: 110 -> 106 us) and up to 2% by the norms.
 constexpr int64_t kNormStreams = (int64_t)128 << 20;
 constexpr int kNormMost = kThreads * 8 * 4;   // widths in registers
 constexpr float kSmall = 0x1p-80f;       // brings any finite value's square, summed, into range
@@ -49,7 +50,7 @@ __device__ __forceinline__ void store_any(void* p, int type, int64_t at, int n, 
 }
 
 // Sum (or largest) over a group of G lanes, the same value in each of them and in every run.  `red` is LDS of
-// 4 words for each use of a workgroup-wide group; a use is fenced off from the one before by `flip`.
+// 4 words for each use of a workgroup-wide group: the caller gives each use its own.
 template <int G>
 __device__ __forceinline__ float group_sum(float v, float* red) {
 #pragma unroll
@@ -269,8 +270,9 @@ __global__ __launch_bounds__(kThreads) void k_norm_long(NormArgs p) {
 // ---------------------------------------------------------------------------------------------
 // Gradient.  A workgroup walks a contiguous share of the rows and keeps the weight's gradient of its columns
 // in registers; the workgroups' sums are added in order by k_column_sums.  Bound by memory where there are many rows
-// (16384 x 4096, all bfloat16: 104 us, 0.54 GB, 5.2 TB/s), by the chain of a group's rows where there are few
-// (4099 x 1000, 16 bits: 11 us for 33 MB, and 2.4 for the sums).
+// (16384 x 4096, all bfloat16: 104 us, 0.54 GB, 5.2 TB/s), by how few loads are on their way where there are few
+// (4099 x 1000, 16 bits: 11 us for 33 MB, and 2.4 for the sums: 188 registers a lane leave two waves a SIMD, and 456 workgroups
+// of 4 waves, a group of lanes walking two or three rows, fill less than that).
 struct GradArgs {
   const void *grad, *r, *weight, *grad_r;
   int64_t ldg, ldr, ldgr;
@@ -282,7 +284,7 @@ struct GradArgs {
   bool past;             // dr is written past the caches
   float* dweight;
   float* sums;           // [workgroup][chunks * 8]
-  float* rstd;           // long rows: [rows][2], the norm's factor and the mean of g u
+  float* rstd;           // long rows: [rows][2], the norm's factor and the scale of its values (1 or kSmall)
 };
 
 // Two sums at once.
