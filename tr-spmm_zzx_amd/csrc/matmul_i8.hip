@@ -159,7 +159,7 @@ __device__ __forceinline__ void store_wave(const MatArgs& p, const int16_v (&acc
 // place c ^ (r / 2 & 7), so that the 16-byte reads of neighbouring rows spread over the banks.
 //
 // DIRECT: rows on 16-byte boundaries and k a multiple of 16; the pieces go from memory to LDS without
-// registers.  Otherwise any address, through registers (4096 x 4096 x 4095: 85 us; by 4-byte words, put together as they
+// registers.  Otherwise any address, through registers (4096 x 4096 x 4095: 85 us, where tiles of 256 spill 12 of them; by 4-byte words, put together as they
 // arrive, 134: the products wait for them).  KS groups of waves split a workgroup's steps, each
 // with its own tiles, and the first adds the sums up: for few workgroups and a long k.
 //
@@ -594,7 +594,8 @@ __global__ __launch_bounds__(1024) void k_matmul_rows(MatArgs p, uint32_t blocks
 }
 
 // ---------------------------------------------------------------------------------------------
-// Host side: which kernel.  Times in us measured on the MI355X with operands that change from call to call.
+// Host side: which kernel.  Times in us measured on the MI355X with operands that change from call to call, those below 256 MB
+// in the MALL (from HBM: 32 x 4096 x 4096 9.6, 64 15.9, 256 15.9, 512 20.8, 2048 x 2048 x 2048 19.4).
 constexpr int kCus = 256;
 
 template <int T, int WM, int WN, int KS, bool DIRECT, class Offset>

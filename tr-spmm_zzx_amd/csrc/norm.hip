@@ -271,7 +271,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_long(NormArgs p) {
 // Gradient.  A workgroup walks a contiguous share of the rows and keeps the weight's gradient of its columns
 // in registers; the workgroups' sums are added in order by k_column_sums.  Bound by memory where there are many rows
 // (16384 x 4096, all bfloat16: 104 us, 0.54 GB, 5.2 TB/s), by how few loads are on their way where there are few
-// (4099 x 1000, 16 bits: 11 us for 33 MB, and 2.4 for the sums: 188 registers a lane leave two waves a SIMD, and 456 workgroups
+// (4099 x 1000, 16 bits: 11 us for 33 MB, and 2.4 for the sums: 187 registers a lane leave two waves a SIMD, and 456 workgroups
 // of 4 waves, a group of lanes walking two or three rows, fill less than that).
 struct GradArgs {
   const void *grad, *r, *weight, *grad_r;
