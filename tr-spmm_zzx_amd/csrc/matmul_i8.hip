@@ -159,9 +159,9 @@ __device__ __forceinline__ void store_wave(const MatArgs& p, const int16_v (&acc
 // place c ^ (r / 2 & 7), so that the 16-byte reads of neighbouring rows spread over the banks.
 //
 // DIRECT: rows on 16-byte boundaries and k a multiple of 16; the pieces go from memory to LDS without
-// registers.  Otherwise any address, through registers (4096 x 4096 x 4095: 85 us, where tiles of 256 spill 12 of them; by 4-byte words, put together as they
-// arrive, 134: the products wait for them).  KS groups of waves split a workgroup's steps, each
-// with its own tiles, and the first adds the sums up: for few workgroups and a long k.
+// registers.  Otherwise any address, through registers (4096 x 4096 x 4095: 85 us, where tiles of 256 spill 12 of
+// them; by 4-byte words, put together as they arrive, 134: the products wait for them).  KS groups of waves split a
+// workgroup's steps, each with its own tiles, and the first adds the sums up: for few workgroups and a long k.
 //
 // Bound by arithmetic: 8192 x 8192 x 8192 454 us, 2.42 POP/s, the matrix units busy 75% of the cycles (at the 1.6 GHz that
 // the card holds under them), 2% of the LDS cycles lost to conflicts.  A wave owns 128 x 64 of a 256 x 256 tile; with
