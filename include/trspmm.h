@@ -31,8 +31,9 @@
  * 3: struct_size fields and the stats size argument; 4: the GPU format builder
  * (trs_build_online_device, trs_dformat_*) and plans from its output (trs_plan_create_dformat,
  * trs_plan_create_sddmm_dformat); struct layouts as in 3; 5: the dense operators (trs_embed ..
- * trs_matmul_i8), struct layouts as in 3. */
-#define TRSPMM_ABI_VERSION 5
+ * trs_matmul_i8), struct layouts as in 3; 6: 4-bit codes (trs_quant_mx4, trs_dequant_mx4, trs_rms_norm_mx4,
+ * trs_matmul_mx4) and trs_adamw with its structs, the others as in 3. */
+#define TRSPMM_ABI_VERSION 6
 
 #ifdef __cplusplus
 extern "C" {
@@ -534,6 +535,73 @@ int trs_rms_norm_grad(const void* grad, int32_t grad_type, int64_t ldg, const vo
 int trs_matmul_i8(const int8_t* a, int64_t lda, const float* a_scale, const int8_t* w, int64_t ldw, const float* w_scale,
                   const float* bias, int64_t m, int32_t n, int32_t k, void* out, int32_t out_type, int64_t ldo,
                   void* stream);
+
+/* 4-bit codes with block scales.  A row of `width` numbers is held in ceil(width / 32) blocks of 32: 16 bytes of codes a
+ * block, the lower half of a byte first, and one byte of scale, exponent + 127 of a power of two.  A code is a sign and
+ * one of 0, 0.5, 1, 1.5, 2, 3, 4, 6; its value is that times the scale.  Scale byte 255: all of the block's values are NaN.  Rows of
+ * codes start on 16-byte boundaries (TRS_EINVAL otherwise), ldc >= 16 * blocks in bytes; scales anywhere, lds >= blocks. */
+
+/* x [rows, width] as codes: a block's scale is 2^max(floor(log2 max|x|) - 2, -126), a code the nearest of x / scale (ties to
+ * the even code; 6 beyond 6, so a block's largest value loses a quarter at most).  A block with a NaN or an infinity has
+ * scale byte 255 and codes 0.  The last block is filled up with zeros.  At most 65535 * 2048 columns (TRS_ERANGE). */
+int trs_quant_mx4(const void* x, int32_t x_type, int64_t ldx, int64_t rows, int32_t width, uint8_t* codes, int64_t ldc,
+                  uint8_t* scale, int64_t lds, void* stream);
+
+/* The values of codes and scales, out [rows, width], rounded to out_type.  Limits as above. */
+int trs_dequant_mx4(const uint8_t* codes, int64_t ldc, const uint8_t* scale, int64_t lds, int64_t rows, int32_t width,
+                    void* out, int32_t out_type, int64_t ldo, void* stream);
+
+/* trs_rms_norm with y as 4-bit codes of its 32-bit values (no rounding to 16 bits between). */
+int trs_rms_norm_mx4(const void* x, int32_t x_type, int64_t ldx, const void* residual, int32_t r_type, int64_t ldr,
+                     const void* weight, int32_t w_type, float eps, int64_t rows, int32_t width, uint8_t* codes, int64_t ldc,
+                     uint8_t* scale, int64_t lds, void* r_out, int64_t ldro, void* stream);
+
+/* out[i, j] = sum over the blocks of a's row i times w's row j + bias[j], the values that codes and scales stand for: a
+ * [m, blocks], w [n, blocks]; lda, ldw are rows of codes, ldas, ldws rows of scales, in bytes; bias float32 or NULL.  Codes
+ * past a row's width take part: trs_quant_mx4 and trs_rms_norm_mx4 write zeros there.  Sums in 32 bits, in an order that the
+ * sizes alone decide.  blocks at most 2^26 (TRS_ERANGE). */
+int trs_matmul_mx4(const uint8_t* a, int64_t lda, const uint8_t* a_scale, int64_t ldas, const uint8_t* w, int64_t ldw,
+                   const uint8_t* w_scale, int64_t ldws, const float* bias, int64_t m, int32_t n, int32_t blocks, void* out,
+                   int32_t out_type, int64_t ldo, void* stream);
+
+/* One AdamW step over many tensors in few launches (one for each combination of types and some 40 tensors):
+ *   g = grad * grad_scale
+ *   m = beta1 m + (1 - beta1) g          v = beta2 v + (1 - beta2) g^2
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^step) * m / (sqrt(v / (1 - beta2^step)) + eps)
+ * in 32 bits, in place; p is rounded to its type, and once more to the copy's.  m and v are float32 where m_scale and v_scale
+ * are NULL.  Otherwise they are 8-bit codes (sign, 4 bits of exponent with bias 7, 3 of fraction; 127: NaN) of `count` bytes with one
+ * scale byte (exponent + 127) for each 32 of them, ceil(count / 32) bytes; a new state is all zeros.  Codes are rounded up
+ * or down with the chance that keeps their mean, by bits that seed, step and the element's index in its tensor decide: equal
+ * calls give equal bits.  v > 0 does not become 0.  An element that is not finite is a NaN code and leaves its block's other
+ * elements alone.  The step itself uses m and v before their rounding. */
+typedef struct trs_adamw_tensor {
+  void* param;
+  const void* grad;
+  void *m, *v;
+  uint8_t *m_scale, *v_scale;   /* NULL: m and v are float32 */
+  void* copy;                   /* the new parameters in copy_type, for the next forward pass; NULL: none */
+  int64_t count;
+  float weight_decay;
+  int32_t param_type, grad_type, copy_type;
+} trs_adamw_tensor;
+
+typedef struct trs_adamw_options {
+  int32_t struct_size;               /* sizeof(trs_adamw_options) and of a tensor, set by trs_adamw_options_default */
+  int32_t tensor_size;
+  double lr, beta1, beta2, eps, grad_scale;
+  int64_t step;                      /* counts from 1 */
+  const float* lr_device;            /* where not NULL, these are read on the GPU in place of lr, grad_scale and step, */
+  const float* grad_scale_device;    /* so that a captured call follows them */
+  const int64_t* step_device;
+  const float* skip;                 /* where not NULL and not 0 on the GPU, the call writes nothing */
+  uint32_t seed;
+} trs_adamw_options;
+
+void trs_adamw_options_default(trs_adamw_options* options);
+
+/* TRS_EINVAL also for buffers that are written and overlap (a tensor named twice); gradients must not overlap them
+ * either.  A tensor has at most some 3.4e10 elements (TRS_ERANGE). */
+int trs_adamw(const trs_adamw_tensor* tensors, int64_t count, const trs_adamw_options* options, void* stream);
 
 const char* trs_last_error(void);
 

@@ -1,4 +1,4 @@
-// The dense operators (trs_embed .. trs_matmul_i8) on torch tensors, behind trspmm/dense.py: argument checks,
+// The dense operators (trs_embed .. trs_adamw) on torch tensors, behind trspmm/dense.py: argument checks,
 // outputs and workspaces that are not given, and the call.  Here and not in Python, because a call on a few
 // rows is bound by this path (1 x 4096 x 4096 codes: 10.1 us a call from Python over a kernel of 5.5).
 //
@@ -249,6 +249,190 @@ Tensor matmul_i8(const Tensor& a_in, const Tensor& a_scale, const Tensor& w_in, 
   return out;
 }
 
+// ---------------------------------------------------------------------------------------------
+// 4-bit codes: uint8 [rows, 16 * blocks], and a scale for each block, float8_e8m0fnu [rows, blocks] (or its bytes).
+
+constexpr int64_t kBlock = 32, kBlockBytes = 16;
+int64_t blocks_of(int64_t width) { return (width + kBlock - 1) / kBlock; }
+
+bool is_scale(at::ScalarType t) { return t == at::kFloat8_e8m0fnu || t == at::kByte; }
+
+// Codes [rows, 16 * blocks] whose rows start on 16-byte boundaries: `t` itself, or a copy.
+Tensor codes_of(const char* name, const Tensor& t, int64_t dev) {
+  on_device(name, t, dev);
+  if (t.scalar_type() != at::kByte || t.dim() != 2 || t.size(1) % kBlockBytes != 0)
+    wrong(std::string(name) + " must be a 2-D tensor of uint8 with 16 columns for each block");
+  const Tensor m = matrix(name, t, dev);
+  const bool there = m.numel() == 0 || ((reinterpret_cast<uintptr_t>(m.data_ptr()) | (m.size(0) > 1 ? (uintptr_t)m.stride(0) : 0)) & 15) == 0;
+  return there ? m : m.clone(at::MemoryFormat::Contiguous);
+}
+
+Tensor scales_of(const char* name, const Tensor& t, int64_t rows, int64_t blocks, int64_t dev) {
+  on_device(name, t, dev);
+  if (!is_scale(t.scalar_type()) || t.dim() != 2 || t.size(0) != rows || t.size(1) != blocks)
+    wrong(std::string(name) + " must be a float8_e8m0fnu or uint8 tensor [" + std::to_string(rows) + ", " + std::to_string(blocks) + "]");
+  return matrix(name, t, dev);
+}
+
+// Outputs of a quantisation: those that are given, checked, or new ones.
+struct CodesOut {
+  Tensor codes, scale;
+  CodesOut(const Given& out, const Given& scale_in, int64_t rows, int64_t width, int64_t dev) {
+    const int64_t blocks = blocks_of(width);
+    codes = output("out", out, rows, blocks * kBlockBytes, at::kByte, dev);
+    if (codes.numel() > 0 && ((reinterpret_cast<uintptr_t>(codes.data_ptr()) | (rows > 1 ? (uintptr_t)codes.stride(0) : 0)) & 15) != 0)
+      wrong("rows of out must start on 16-byte boundaries");
+    if (scale_in && !is_scale(scale_in->scalar_type())) wrong("scale must be float8_e8m0fnu or uint8");
+    scale = output("scale", scale_in, rows, blocks, scale_in ? scale_in->scalar_type() : at::kFloat8_e8m0fnu, dev);
+  }
+  uint8_t* codes_at() const { return static_cast<uint8_t*>(codes.data_ptr()); }
+  uint8_t* scale_at() const { return static_cast<uint8_t*>(scale.data_ptr()); }
+};
+
+const uint8_t* bytes(const Tensor& t) { return static_cast<const uint8_t*>(t.data_ptr()); }
+
+std::tuple<Tensor, Tensor> quant_mx4(const Tensor& x_in, const Given& out, const Given& scale, int64_t dev, int64_t stream) {
+  const Tensor x = matrix("x", x_in, dev);
+  const int x_type = type_of("x", x.scalar_type());
+  const CodesOut o(out, scale, x.size(0), x.size(1), dev);
+  ok(trs_quant_mx4(x.data_ptr(), x_type, ld(x), x.size(0), width_of(x), o.codes_at(), ld(o.codes), o.scale_at(), ld(o.scale),
+                   stream_of(stream)),
+     "trs_quant_mx4");
+  return {o.codes, o.scale};
+}
+
+Tensor dequant_mx4(const Tensor& codes_in, const Tensor& scale_in, int64_t width, const Type& dtype, const Given& out_in,
+                   int64_t dev, int64_t stream) {
+  const Tensor codes = codes_of("codes", codes_in, dev);
+  const int64_t rows = codes.size(0), blocks = codes.size(1) / kBlockBytes;
+  if (width < 0 || blocks_of(width) != blocks)
+    wrong("a width of " + std::to_string(width) + " has " + std::to_string(blocks_of(width)) + " blocks, codes have " + std::to_string(blocks));
+  if (width > INT32_MAX) wrong("rows of more than 2^31 - 1 elements");
+  const Tensor scale = scales_of("scale", scale_in, rows, blocks, dev);
+  const at::ScalarType type = type_out(out_in, dtype, at::kHalf);
+  const int o_type = type_of("dtype", type);
+  const Tensor out = output("out", out_in, rows, width, type, dev);
+  ok(trs_dequant_mx4(bytes(codes), ld(codes), bytes(scale), ld(scale), rows, (int32_t)width, out.data_ptr(), o_type, ld(out),
+                     stream_of(stream)),
+     "trs_dequant_mx4");
+  return out;
+}
+
+std::tuple<Tensor, Tensor, Given> rms_norm_mx4(const Tensor& x, const Tensor& weight, const Given& residual, double eps,
+                                               const Given& out, const Given& scale, const Given& r_out, int64_t dev,
+                                               int64_t stream) {
+  const NormOperands n(x, weight, residual, r_out, dev);
+  const CodesOut o(out, scale, n.rows, n.width, dev);
+  ok(trs_rms_norm_mx4(n.x.data_ptr(), n.x_type, ld(n.x), data(n.residual), n.r_type, n.ldr(), weight.data_ptr(), n.w_type,
+                      (float)eps, n.rows, n.width, o.codes_at(), ld(o.codes), o.scale_at(), ld(o.scale), data(n.r), n.ldro(),
+                      stream_of(stream)),
+     "trs_rms_norm_mx4");
+  return {o.codes, o.scale, n.r_given()};
+}
+
+Tensor matmul_mx4(const Tensor& a_in, const Tensor& a_scale_in, const Tensor& w_in, const Tensor& w_scale_in, const Given& bias,
+                  const Type& dtype, const Given& out_in, int64_t dev, int64_t stream) {
+  const Tensor a = codes_of("a", a_in, dev), w = codes_of("w", w_in, dev);
+  const int64_t m = a.size(0), n = w.size(0), blocks = a.size(1) / kBlockBytes;
+  if (w.size(1) != a.size(1))
+    wrong("a has " + std::to_string(blocks) + " blocks in a row and w " + std::to_string(w.size(1) / kBlockBytes));
+  if (n > INT32_MAX || blocks > INT32_MAX) wrong("more than 2^31 - 1 output channels or blocks");
+  const Tensor a_scale = scales_of("a_scale", a_scale_in, m, blocks, dev), w_scale = scales_of("w_scale", w_scale_in, n, blocks, dev);
+  if (bias) floats("bias", *bias, n, dev);
+  const at::ScalarType type = type_out(out_in, dtype, at::kHalf);
+  const int o_type = type_of("dtype", type);
+  const Tensor out = output("out", out_in, m, n, type, dev);
+  ok(trs_matmul_mx4(bytes(a), ld(a), bytes(a_scale), ld(a_scale), bytes(w), ld(w), bytes(w_scale), ld(w_scale),
+                    bias ? static_cast<const float*>(bias->data_ptr()) : nullptr, m, (int32_t)n, (int32_t)blocks, out.data_ptr(),
+                    o_type, ld(out), stream_of(stream)),
+     "trs_matmul_mx4");
+  return out;
+}
+
+// ---------------------------------------------------------------------------------------------
+// A number of the host's or a tensor of one element on the GPU.
+template <class T>
+const T* one_of(const char* name, const py::object& x, at::ScalarType type, int64_t dev) {
+  const Tensor t = x.cast<Tensor>();
+  on_device(name, t, dev);
+  if (t.scalar_type() != type || t.numel() != 1)
+    wrong(std::string(name) + " must be a number or a " + c10::toString(type) + " tensor of one element");
+  return static_cast<const T*>(t.data_ptr());
+}
+
+bool is_tensor(const py::object& x) { return THPVariable_Check(x.ptr()); }
+
+// A tensor that the step writes, or reads beside one: contiguous, of n elements.
+void* flat(const char* name, size_t i, const Tensor& t, int64_t n, int64_t dev) {
+  const std::string which = std::string(name) + "[" + std::to_string(i) + "]";
+  on_device(which.c_str(), t, dev);
+  if (!t.is_contiguous()) wrong(which + " must be contiguous");
+  if (t.numel() != n) wrong(which + " must have " + std::to_string(n) + " elements (it has " + std::to_string(t.numel()) + ")");
+  return t.data_ptr();
+}
+
+void adamw(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const py::sequence& states, const py::object& step,
+           const py::object& lr, std::pair<double, double> betas, double eps, const py::object& decay, const py::object& copies,
+           const py::object& grad_scale, const Given& skip, uint32_t seed, int64_t dev, int64_t stream) {
+  const size_t count = params.size();
+  if (grads.size() != count || states.size() != count)
+    wrong(std::to_string(count) + " params, " + std::to_string(grads.size()) + " grads and " + std::to_string(states.size()) + " states");
+  trs_adamw_options o;
+  trs_adamw_options_default(&o);
+  if (is_tensor(lr)) o.lr_device = one_of<float>("lr", lr, at::kFloat, dev);
+  else o.lr = lr.cast<double>();
+  if (is_tensor(step)) o.step_device = one_of<int64_t>("step", step, at::kLong, dev);
+  else o.step = step.cast<int64_t>();
+  if (is_tensor(grad_scale)) o.grad_scale_device = one_of<float>("grad_scale", grad_scale, at::kFloat, dev);
+  else o.grad_scale = grad_scale.cast<double>();
+  if (skip) o.skip = one_of<float>("skip", py::cast(*skip), at::kFloat, dev);
+  o.beta1 = betas.first, o.beta2 = betas.second, o.eps = eps, o.seed = seed;
+  const bool each = !py::isinstance<py::float_>(decay) && !py::isinstance<py::int_>(decay);
+  const double decay_all = each ? 0.0 : decay.cast<double>();
+  const std::vector<double> decays = each ? decay.cast<std::vector<double>>() : std::vector<double>();
+  if (each && decays.size() != count) wrong("weight_decay must be a number, or one for each of the params");
+  const std::vector<Given> copied = copies.is_none() ? std::vector<Given>() : copies.cast<std::vector<Given>>();
+  if (!copies.is_none() && copied.size() != count) wrong("copies must have one entry for each of the params (None: no copy)");
+  std::vector<trs_adamw_tensor> list(count);
+  std::vector<Tensor> made;   // contiguous copies of gradients
+  for (size_t i = 0; i < count; ++i) {
+    trs_adamw_tensor& t = list[i];
+    const int64_t n = params[i].numel();
+    t = trs_adamw_tensor{};
+    t.count = n;
+    t.weight_decay = (float)(each ? decays[i] : decay_all);
+    t.param = flat("params", i, params[i], n, dev);
+    t.param_type = type_of("params", params[i].scalar_type());
+    const Tensor& g = grads[i];
+    on_device("grads", g, dev);
+    t.grad_type = type_of("grads", g.scalar_type());
+    if (g.sizes() != params[i].sizes()) wrong("grads[" + std::to_string(i) + "] must have its parameter's shape");
+    if (!g.is_contiguous()) made.push_back(g.contiguous());
+    t.grad = g.is_contiguous() ? g.data_ptr() : made.back().data_ptr();
+    const py::sequence state = states[i].cast<py::sequence>();
+    const size_t parts = state.size();
+    if (parts != 2 && (parts != 4 || state[2].is_none() != state[3].is_none())) wrong("a state is (m, v) or (m, v, m_scale, v_scale)");
+    const Tensor m = state[0].cast<Tensor>(), v = state[1].cast<Tensor>();
+    const bool small = parts == 4 && !state[2].is_none();
+    const at::ScalarType type = small ? at::kFloat8_e4m3fn : at::kFloat;
+    if (m.scalar_type() != type || v.scalar_type() != type)
+      wrong(std::string("m and v must be float32, or float8_e4m3fn with scales (states[") + std::to_string(i) + "])");
+    t.m = flat("m of states", i, m, n, dev);
+    t.v = flat("v of states", i, v, n, dev);
+    if (small) {
+      const Tensor ms = state[2].cast<Tensor>(), vs = state[3].cast<Tensor>();
+      if (!is_scale(ms.scalar_type()) || !is_scale(vs.scalar_type())) wrong("scales of states must be float8_e8m0fnu or uint8");
+      t.m_scale = static_cast<uint8_t*>(flat("m_scale of states", i, ms, blocks_of(n), dev));
+      t.v_scale = static_cast<uint8_t*>(flat("v_scale of states", i, vs, blocks_of(n), dev));
+    }
+    if (!copied.empty() && copied[i]) {
+      t.copy = flat("copies", i, *copied[i], n, dev);
+      t.copy_type = type_of("copies", copied[i]->scalar_type());
+    }
+  }
+  ok(trs_adamw(list.data(), (int64_t)count, &o, stream_of(stream)), "trs_adamw");
+}
+
 }  // namespace
 
 void bind_dense(pybind11::module_& m) {
@@ -258,4 +442,9 @@ void bind_dense(pybind11::module_& m) {
   m.def("rms_norm_i8", &rms_norm_i8);
   m.def("rms_norm_grad", &rms_norm_grad);
   m.def("matmul_i8", &matmul_i8);
+  m.def("quant_mx4", &quant_mx4);
+  m.def("dequant_mx4", &dequant_mx4);
+  m.def("rms_norm_mx4", &rms_norm_mx4);
+  m.def("matmul_mx4", &matmul_mx4);
+  m.def("adamw", &adamw);
 }

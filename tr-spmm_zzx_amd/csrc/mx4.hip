@@ -1,0 +1,118 @@
+// 4-bit codes with a power-of-two scale for each block of 32 along a row, and the values that they stand for.
+//
+//   e = max(floor(log2(max|x|)) - 2, -126)       of a block; the scale 2^e as one byte, e + 127
+//   q = x / 2^e to the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 (ties to even codes; 6 beyond 6), with its sign
+//
+// A block with a NaN or an infinity has scale byte 255 and codes 0: all its values are NaN.  The last block of a row whose width 32
+// does not divide is filled up with zeros.  Both kernels move their bytes once and are bound by memory.
+#include "mx.hpp"
+
+namespace trs {
+namespace dense {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int32_t kMostMxWidth = 65535 * kThreads * 8;   // the grid's second dimension
+static_assert(kMostMxWidth <= kMostWidth, "column indexes of 32 bits");
+
+struct QuantArgs {
+  const void* x;       // or the values, to be written
+  int64_t ldx;
+  uint8_t *codes, *scale;
+  int64_t ldc, lds, rows;
+  int width, chunks, shift;   // chunks of 8, four for each block; 2^shift lanes a row
+};
+
+// The row and the chunk of this thread; false: none.  A quad of lanes has a block's four chunks, all of them or none.
+__device__ __forceinline__ bool place_of(const QuantArgs& p, int64_t& row, int& chunk) {
+  row = ((int64_t)blockIdx.x << (8 - p.shift)) + (threadIdx.x >> p.shift);
+  chunk = (int)(blockIdx.y << p.shift) + (threadIdx.x & ((1 << p.shift) - 1));
+  return row < p.rows && chunk < p.chunks;
+}
+
+template <class X>
+__global__ __launch_bounds__(kThreads) void k_quant4(QuantArgs p) {
+  int64_t row;
+  int chunk;
+  if (!place_of(p, row, chunk)) return;
+  const int at = chunk * 8, n = p.width - at;
+  float v[8] = {};
+  if (n > 0) load_chunk<X>(static_cast<const typename X::raw*>(p.x) + row * p.ldx + at, n, v);
+  uint32_t byte;
+  const uint32_t codes = quantise4(v, byte);
+  *reinterpret_cast<uint32_t*>(p.codes + row * p.ldc + chunk * 4) = codes;
+  if ((chunk & 3) == 0) p.scale[row * p.lds + (chunk >> 2)] = (uint8_t)byte;
+}
+
+template <class X>
+__global__ __launch_bounds__(kThreads) void k_dequant4(QuantArgs p) {
+  int64_t row;
+  int chunk;
+  if (!place_of(p, row, chunk)) return;
+  const int at = chunk * 8, n = p.width - at;
+  if (n <= 0) return;
+  const uint32_t codes = *reinterpret_cast<const uint32_t*>(p.codes + row * p.ldc + chunk * 4);
+  const uint32_t byte = p.scale[row * p.lds + (chunk >> 2)];
+  float v[8];
+  // byte 0, 2^-127, is no ordinary float: half of 2^-126
+  values4(codes, scale_of(byte > 0 ? byte : 1), v);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = byte == kNanScale ? __builtin_nanf("") : byte ? v[i] : 0.5f * v[i];
+  store_chunk<X>(static_cast<typename X::raw*>(const_cast<void*>(p.x)) + row * p.ldx + at, n, v);
+}
+
+template <bool QUANT>
+int mx4_call(const char* where, QuantArgs p, int type, void* stream) {
+  if (p.rows < 0 || p.width < 0) return fail(TRS_EINVAL, where, "negative rows or width");
+  if (!known_type(type)) return fail(TRS_EINVAL, where, "unknown element type");
+  if (p.rows == 0 || p.width == 0) return TRS_OK;
+  if (p.width > kMostMxWidth) return fail(TRS_ERANGE, where, "more than 134215680 columns");
+  const int64_t blocks = blocks_of(p.width);
+  if (!p.x || !p.codes || !p.scale) return fail(TRS_EINVAL, where, "NULL operand");
+  if (p.ldx < p.width || p.ldc < blocks * kBlockBytes || p.lds < blocks) return fail(TRS_EINVAL, where, "leading dimension too small");
+  if (!aligned_codes(p.codes, p.ldc)) return fail(TRS_EINVAL, where, "codes off a 16-byte boundary");
+  if (p.rows > (int64_t)1 << 38) return fail(TRS_ERANGE, where, "too many rows");
+  p.chunks = (int)blocks * 4;
+  for (p.shift = 2; p.shift < 8 && (1 << p.shift) < p.chunks;) ++p.shift;
+  const uint32_t y = (uint32_t)ceil_div(p.chunks, (int64_t)1 << p.shift);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const int bytes = type == TRS_F32 ? 4 : 2;
+  // as many rows a launch as it can have workgroups
+  const int64_t slice = (int64_t)(UINT32_MAX / kThreads) << (8 - p.shift);
+  for (int64_t first = 0; first < p.rows; first += slice) {
+    QuantArgs q = p;
+    q.rows = p.rows - first < slice ? p.rows - first : slice;
+    q.x = static_cast<const char*>(p.x) + first * p.ldx * bytes;
+    q.codes = p.codes + first * p.ldc;
+    q.scale = p.scale + first * p.lds;
+    const dim3 grid((uint32_t)ceil_div(q.rows, (int64_t)1 << (8 - p.shift)), y);
+    if constexpr (QUANT) {
+      if (type == TRS_F32) k_quant4<f32_t><<<grid, kThreads, 0, s>>>(q);
+      else if (type == TRS_F16) k_quant4<f16_t><<<grid, kThreads, 0, s>>>(q);
+      else k_quant4<bf16_t><<<grid, kThreads, 0, s>>>(q);
+    } else {
+      if (type == TRS_F32) k_dequant4<f32_t><<<grid, kThreads, 0, s>>>(q);
+      else if (type == TRS_F16) k_dequant4<f16_t><<<grid, kThreads, 0, s>>>(q);
+      else k_dequant4<bf16_t><<<grid, kThreads, 0, s>>>(q);
+    }
+  }
+  return launched(where);
+}
+
+}  // namespace
+}  // namespace dense
+}  // namespace trs
+
+using namespace trs::dense;
+
+extern "C" int trs_quant_mx4(const void* x, int32_t x_type, int64_t ldx, int64_t rows, int32_t width, uint8_t* codes, int64_t ldc,
+                             uint8_t* scale, int64_t lds, void* stream) {
+  return mx4_call<true>("trs_quant_mx4", QuantArgs{x, ldx, codes, scale, ldc, lds, rows, width, 0, 0}, x_type, stream);
+}
+
+extern "C" int trs_dequant_mx4(const uint8_t* codes, int64_t ldc, const uint8_t* scale, int64_t lds, int64_t rows, int32_t width,
+                               void* out, int32_t out_type, int64_t ldo, void* stream) {
+  return mx4_call<false>("trs_dequant_mx4",
+                         QuantArgs{out, ldo, const_cast<uint8_t*>(codes), const_cast<uint8_t*>(scale), ldc, lds, rows, width, 0, 0},
+                         out_type, stream);
+}

@@ -1,9 +1,10 @@
-// Root-mean-square norm with the residual's addition, its 8-bit form, and its gradient.
+// Root-mean-square norm with the residual's addition, its 8-bit and 4-bit forms, and its gradient.
 //
 //   h = x + residual                     32 bits; r = h rounded to the residual's type
 //   s = 1 / sqrt(mean(h^2) + eps)
 //   y = h s w                            trs_rms_norm: rounded once, to y's type
 //   scale = max|y| / 127, q = rint(y / scale)                            trs_rms_norm_i8
+//   4-bit codes of y with a scale for each block of 32 (mx.hpp)          trs_rms_norm_mx4
 //
 //   u = r s, g = dy w                                                    trs_rms_norm_grad
 //   dr = s (g - u mean(g u)) + grad_r,  dw = sum over rows of dy u
@@ -12,7 +13,7 @@
 // output written once: the kernels are bound by memory.  A group of lanes (8 .. 64, or the workgroup) owns a
 // row; 8 elements are one load.  The sum of squares of a row whose values are too large for 32-bit squares
 // is taken again at a smaller scale (kSmall), and so is the gradient's sum of g r where it passes 32 bits.
-#include "dense.hpp"
+#include "mx.hpp"
 
 #include <cfloat>
 #include <type_traits>
@@ -75,10 +76,6 @@ __device__ __forceinline__ uint32_t group_max(uint32_t v, float* red) {
   }
   return v;
 }
-
-// |v| as an integer: ordered like the values, with NaN above infinity.
-__device__ __forceinline__ uint32_t size_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
-constexpr uint32_t kInfBits = 0x7f800000u;
 
 __device__ __forceinline__ void store_codes(int8_t* q, int n, const float (&v)[8], float inv, bool past = false) {
   union { int8_t c[8]; uint64_t w; } u;
@@ -264,6 +261,125 @@ __global__ __launch_bounds__(kThreads) void k_norm_long(NormArgs p) {
     for (int i = 0; i < 8; ++i) h[i] = finite ? (h[i] * f) * s * w[i] : 0.f;
     if constexpr (CODES) store_codes(static_cast<int8_t*>(p.y) + row * p.ldy + at, n, h, inv);
     else store_any(p.y, p.y_type, row * p.ldy + at, n, h);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// 4-bit codes.  Four lanes hold a block's chunks of 8, so chunks start at multiples of 8 here: the last one of a row is
+// narrower, and a block's chunks past the row's end are zeros.
+struct Mx4Args {
+  NormArgs n;          // y: the codes
+  uint8_t* scale;
+  int64_t lds;
+  int chunks;          // four for each block
+};
+
+__device__ __forceinline__ void put_codes(const Mx4Args& p, int64_t row, int chunk, const float (&y)[8]) {
+  uint32_t byte;
+  const uint32_t codes = quantise4(y, byte);
+  if (chunk >= p.chunks) return;
+  *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(p.n.y) + row * p.n.ldy + chunk * 4) = codes;
+  if ((chunk & 3) == 0) p.scale[row * p.lds + (chunk >> 2)] = (uint8_t)byte;
+}
+
+template <class X, class R, int G, int NC>
+__global__ __launch_bounds__(kThreads) void k_norm_mx4(Mx4Args q) {
+  const NormArgs& p = q.n;
+  constexpr int kRows = kThreads / G;
+  __shared__ float red[2][4];
+  const int lane = threadIdx.x % G;
+  const int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / G;
+  if (row >= p.rows) return;   // a whole group
+  constexpr bool kRes = !is_none<R>;
+  raw8<X> x[NC];
+  raw8<typename std::conditional<kRes, R, X>::type> res[NC];
+  float h[NC][8], w[NC][8];
+  // All loads are on their way before the first is waited for.  A lane without a chunk reads the first one and counts
+  // nothing of it.
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int at = (c * G + lane) * 8, n = p.width - at, from = n > 0 ? at : 0, left = n > 0 ? n : p.width;
+    x[c] = load_raw_any<X>(static_cast<const typename X::raw*>(p.x) + row * p.ldx + from, left);
+    if constexpr (kRes) res[c] = load_raw_any<R>(static_cast<const typename R::raw*>(p.res) + row * p.ldr + from, left);
+  }
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int at = (c * G + lane) * 8, n = p.width - at;
+    load_any(p.weight, p.w_type, n > 0 ? at : 0, n > 0 ? n : p.width, w[c]);
+  }
+  float sum = 0.f;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int at = (c * G + lane) * 8, n = p.width - at;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      h[c][i] = (float)x[c][i];
+      if constexpr (kRes) h[c][i] += (float)res[c][i];
+      if (i >= n) h[c][i] = w[c][i] = 0.f;
+      sum += h[c][i] * h[c][i];
+    }
+    if constexpr (kRes)
+      if (n > 0) store_chunk<R>(static_cast<typename R::raw*>(p.r) + row * p.ldro + at, n, h[c], p.past_r);
+  }
+  sum = group_sum<G>(sum, red[0]);
+  float s = rstd_of(sum, p.width, p.eps);
+  float f = 1.f;
+  if (!(sum <= FLT_MAX)) {   // squares beyond 32 bits, or a value that is not finite
+    f = kSmall;
+    sum = 0.f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += (h[c][i] * f) * (h[c][i] * f);
+    sum = group_sum<G>(sum, red[1]);
+    s = rstd_of(sum, p.width, p.eps, f);
+  }
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int chunk = c * G + lane, n = p.width - chunk * 8;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h[c][i] = i < n ? (h[c][i] * f) * s * w[c][i] : 0.f;   // 0 past the row's end, whatever s is
+    put_codes(q, row, chunk, h[c]);
+  }
+}
+
+// Rows too long for registers, read again for each of up to three steps.
+template <class X, class R>
+__global__ __launch_bounds__(kThreads) void k_norm_mx4_long(Mx4Args q) {
+  const NormArgs& p = q.n;
+  __shared__ float red[2][4];
+  const int64_t row = blockIdx.x;
+  float sum = 0.f, h[8], w[8];
+  for (int at = threadIdx.x * 8; at < p.width; at += kThreads * 8) {
+    long_chunk<X, R>(p, row, at, p.width - at, h);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += h[i] * h[i];
+  }
+  sum = group_sum<kThreads>(sum, red[0]);
+  float s = rstd_of(sum, p.width, p.eps), f = 1.f;
+  if (!(sum <= FLT_MAX)) {
+    f = kSmall;
+    sum = 0.f;
+    for (int at = threadIdx.x * 8; at < p.width; at += kThreads * 8) {
+      long_chunk<X, R>(p, row, at, p.width - at, h);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += (h[i] * f) * (h[i] * f);
+    }
+    sum = group_sum<kThreads>(sum, red[1]);
+    s = rstd_of(sum, p.width, p.eps, f);
+  }
+  for (int chunk = threadIdx.x; chunk < q.chunks; chunk += kThreads) {   // a block's four lanes go on or end together
+    const int at = chunk * 8, n = p.width - at;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h[i] = w[i] = 0.f;
+    if (n > 0) {
+      long_chunk<X, R>(p, row, at, n, h);
+      load_any(p.weight, p.w_type, at, n, w);
+      if constexpr (!is_none<R>) store_chunk<R>(static_cast<typename R::raw*>(p.r) + row * p.ldro + at, n, h);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h[i] = i < n ? (h[i] * f) * s * w[i] : 0.f;
+    put_codes(q, row, chunk, h);
   }
 }
 
@@ -546,7 +662,33 @@ void launch_norm(const NormArgs& p, hipStream_t s) {
   else k_norm_long<X, R, CODES><<<blocks(1), kThreads, 0, s>>>(p);
 }
 
+template <class X, class R>
+void launch_mx4(const Mx4Args& p, hipStream_t s) {
+  auto blocks = [&](int rows) { return dim3((uint32_t)ceil_div(p.n.rows, rows)); };
+  const int w = p.n.width;
+  if (w <= 64) k_norm_mx4<X, R, 8, 1><<<blocks(32), kThreads, 0, s>>>(p);
+  else if (w <= 128) k_norm_mx4<X, R, 16, 1><<<blocks(16), kThreads, 0, s>>>(p);
+  else if (w <= 256) k_norm_mx4<X, R, 32, 1><<<blocks(8), kThreads, 0, s>>>(p);
+  else if (w <= 512) k_norm_mx4<X, R, 64, 1><<<blocks(4), kThreads, 0, s>>>(p);
+  else if (w <= 1024 && p.n.rows >= 1024) k_norm_mx4<X, R, 64, 2><<<blocks(4), kThreads, 0, s>>>(p);
+  else if (w <= 2048) k_norm_mx4<X, R, 256, 1><<<blocks(1), kThreads, 0, s>>>(p);
+  else if (w <= 4096) k_norm_mx4<X, R, 256, 2><<<blocks(1), kThreads, 0, s>>>(p);
+  else if (w <= kNormMost) k_norm_mx4<X, R, 256, 4><<<blocks(1), kThreads, 0, s>>>(p);
+  else k_norm_mx4_long<X, R><<<blocks(1), kThreads, 0, s>>>(p);
+}
+
 constexpr int kNoResidual = -1;
+
+template <class X>
+bool launch_mx4_res(const Mx4Args& p, int r_type, hipStream_t s) {
+  if (r_type == kNoResidual) launch_mx4<X, none_t>(p, s);
+  else if (r_type == X::code) launch_mx4<X, X>(p, s);
+  else if (r_type == TRS_F32) launch_mx4<X, f32_t>(p, s);
+  else if constexpr (X::code != TRS_F32) return false;   // two different 16-bit types
+  else if (r_type == TRS_F16) launch_mx4<X, f16_t>(p, s);
+  else launch_mx4<X, bf16_t>(p, s);
+  return true;
+}
 
 template <class X, bool CODES>
 bool launch_norm_res(const NormArgs& p, int r_type, hipStream_t s) {
@@ -605,6 +747,46 @@ int norm_call(const char* where, const NormArgs& p, int x_type, int r_type, void
     const bool known = x_type == TRS_F32   ? launch_norm_res<f32_t, CODES>(q, r_type, s)
                        : x_type == TRS_F16 ? launch_norm_res<f16_t, CODES>(q, r_type, s)
                                            : launch_norm_res<bf16_t, CODES>(q, r_type, s);
+    if (!known) return fail(TRS_EINVAL, where, "x and residual of two different 16-bit types");
+  }
+  return launched(where);
+}
+
+int mx4_call(const Mx4Args& a, int x_type, int r_type, void* stream) {
+  const char* where = "trs_rms_norm_mx4";
+  const NormArgs& p = a.n;
+  if (p.rows < 0 || p.width < 0) return fail(TRS_EINVAL, where, "negative rows or width");
+  if (!known_type(x_type) || !known_type(p.w_type) || (p.res && !known_type(r_type)))
+    return fail(TRS_EINVAL, where, "unknown element type");
+  if (!(p.eps > 0.f) || !std::isfinite(p.eps)) return fail(TRS_EINVAL, where, "eps must be positive and finite");
+  if (p.rows == 0 || p.width == 0) return TRS_OK;
+  if (p.width > kMostWidth) return fail(TRS_ERANGE, where, "more than 2^31 - 65536 columns");
+  const int64_t blocks = blocks_of(p.width);
+  if (!p.x || !p.weight || !p.y || !a.scale) return fail(TRS_EINVAL, where, "NULL operand");
+  if ((p.res == nullptr) != (p.r == nullptr)) return fail(TRS_EINVAL, where, "residual and its output go together");
+  if (p.ldx < p.width || p.ldy < blocks * kBlockBytes || a.lds < blocks || (p.res && (p.ldr < p.width || p.ldro < p.width)))
+    return fail(TRS_EINVAL, where, "leading dimension too small");
+  if (!aligned_codes(p.y, p.ldy)) return fail(TRS_EINVAL, where, "codes off a 16-byte boundary");
+  if (p.rows > kMostRows) return fail(TRS_ERANGE, where, "too many rows");
+  if (!p.res) r_type = kNoResidual;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  // as many rows a launch as it can have workgroups
+  constexpr int64_t kSlice = UINT32_MAX / kThreads;
+  for (int64_t first = 0; first < p.rows; first += kSlice) {
+    Mx4Args q = a;
+    q.chunks = (int)(4 * blocks);
+    q.n.past_r = p.res && streams(p.r, p.ldro, r_type == TRS_F32 ? 4 : 2, p.rows, p.width, kNormStreams);
+    q.n.rows = p.rows - first < kSlice ? p.rows - first : kSlice;
+    q.n.x = at_row(p.x, first * p.ldx, x_type);
+    if (p.res) {
+      q.n.res = at_row(p.res, first * p.ldr, r_type);
+      q.n.r = const_cast<void*>(at_row(p.r, first * p.ldro, r_type));
+    }
+    q.n.y = static_cast<uint8_t*>(p.y) + first * p.ldy;
+    q.scale = a.scale + first * a.lds;
+    const bool known = x_type == TRS_F32   ? launch_mx4_res<f32_t>(q, r_type, s)
+                       : x_type == TRS_F16 ? launch_mx4_res<f16_t>(q, r_type, s)
+                                           : launch_mx4_res<bf16_t>(q, r_type, s);
     if (!known) return fail(TRS_EINVAL, where, "x and residual of two different 16-bit types");
   }
   return launched(where);
@@ -676,6 +858,13 @@ extern "C" int trs_rms_norm_i8(const void* x, int32_t x_type, int64_t ldx, const
                                int64_t ldq, float* scale, void* r_out, int64_t ldro, void* stream) {
   const NormArgs p{x, residual, weight, ldx, ldr, w_type, 0, width, eps, rows, q, ldq, scale, r_out, ldro, false, false};
   return norm_call<true>("trs_rms_norm_i8", p, x_type, r_type, stream);
+}
+
+extern "C" int trs_rms_norm_mx4(const void* x, int32_t x_type, int64_t ldx, const void* residual, int32_t r_type, int64_t ldr,
+                                const void* weight, int32_t w_type, float eps, int64_t rows, int32_t width, uint8_t* codes,
+                                int64_t ldc, uint8_t* scale, int64_t lds, void* r_out, int64_t ldro, void* stream) {
+  const NormArgs p{x, residual, weight, ldx, ldr, w_type, 0, width, eps, rows, codes, ldc, nullptr, r_out, ldro, false, false};
+  return mx4_call(Mx4Args{p, scale, lds, 0}, x_type, r_type, stream);
 }
 
 extern "C" int64_t trs_rms_norm_grad_workspace_bytes(int64_t rows, int32_t width) {

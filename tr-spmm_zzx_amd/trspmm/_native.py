@@ -56,6 +56,17 @@ class MatchStats(ctypes.Structure):
                 ("tc_block_count", c_i64), ("tc_block_max_nnz", c_i64), ("tc_block_min_nnz", c_i64)]
 
 
+class AdamwTensor(ctypes.Structure):
+    _fields_ = [("param", c_p), ("grad", c_p), ("m", c_p), ("v", c_p), ("m_scale", c_p), ("v_scale", c_p), ("copy", c_p),
+                ("count", c_i64), ("weight_decay", c_f32), ("param_type", c_i32), ("grad_type", c_i32), ("copy_type", c_i32)]
+
+
+class AdamwOptions(ctypes.Structure):
+    _fields_ = [("struct_size", c_i32), ("tensor_size", c_i32), ("lr", c_f64), ("beta1", c_f64), ("beta2", c_f64), ("eps", c_f64),
+                ("grad_scale", c_f64), ("step", c_i64), ("lr_device", c_p), ("grad_scale_device", c_p), ("step_device", c_p),
+                ("skip", c_p), ("seed", ctypes.c_uint32)]
+
+
 # name -> (restype, argtypes); every symbol declared in include/trspmm.h
 PROTOTYPES = {
     "trs_build_params_default": (None, [ctypes.POINTER(BuildParams)]),
@@ -117,6 +128,14 @@ PROTOTYPES = {
     "trs_rms_norm_grad": (c_i32, [c_p, c_i32, c_i64, c_p, c_i32, c_i64, c_p, c_i32, c_p, c_i64, c_f32, c_i64, c_i32, c_p,
                                   c_i64, c_p, c_p, c_i64, c_p]),
     "trs_matmul_i8": (c_i32, [c_p, c_i64, c_p, c_p, c_i64, c_p, c_p, c_i64, c_i32, c_i32, c_p, c_i32, c_i64, c_p]),
+    "trs_quant_mx4": (c_i32, [c_p, c_i32, c_i64, c_i64, c_i32, c_p, c_i64, c_p, c_i64, c_p]),
+    "trs_dequant_mx4": (c_i32, [c_p, c_i64, c_p, c_i64, c_i64, c_i32, c_p, c_i32, c_i64, c_p]),
+    "trs_rms_norm_mx4": (c_i32, [c_p, c_i32, c_i64, c_p, c_i32, c_i64, c_p, c_i32, c_f32, c_i64, c_i32, c_p, c_i64, c_p,
+                                 c_i64, c_p, c_i64, c_p]),
+    "trs_matmul_mx4": (c_i32, [c_p, c_i64, c_p, c_i64, c_p, c_i64, c_p, c_i64, c_p, c_i64, c_i32, c_i32, c_p, c_i32, c_i64,
+                               c_p]),
+    "trs_adamw_options_default": (None, [ctypes.POINTER(AdamwOptions)]),
+    "trs_adamw": (c_i32, [ctypes.POINTER(AdamwTensor), c_i64, ctypes.POINTER(AdamwOptions), c_p]),
     "trs_last_error": (ctypes.c_char_p, []),
     "trs_abi_version": (c_i32, []),
 }

@@ -1,6 +1,7 @@
 """The dense operators beside the sparse products: table lookup by ids and its gradient, the
 root-mean-square norm (with the residual's addition, in 16 or 32 bits or in 8 bits with a scale for each
-row) and its gradient, and the product of 8-bit codes with scales.
+row) and its gradient, the product of 8-bit codes with scales, the same in 4-bit codes with a power of two as the scale of
+each 32 numbers, and the AdamW step of a list of tensors.
 
 A layer that serves in 8 bits:
 
@@ -8,6 +9,12 @@ A layer that serves in 8 bits:
     h = plan.spmm(x)                                   # aggregation, float32
     q, s, x = trspmm.rms_norm_i8(h, weight, x)         # x += h; codes and scales of the normed rows
     y = trspmm.matmul_i8(q, s, w_codes, w_scale)       # projection
+
+The same in 4 bits:
+
+    w_codes, w_scale = trspmm.quant_mx4(w)             # once
+    q, s, x = trspmm.rms_norm_mx4(h, weight, x)
+    y = trspmm.matmul_mx4(q, s, w_codes, w_scale)
 
 Tensors live on the current GPU; work is enqueued on ``stream`` (default: the current torch stream).
 Matrices are 2-D with unit column stride and any row stride; one with another column stride is copied.
@@ -17,7 +24,7 @@ extension (csrc/ext_dense.cpp); the kernels are libtrspmm.so's, and there is no 
 """
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -100,3 +107,90 @@ def matmul_i8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: 
     for each row (of :func:`rms_norm_i8`), weights `w` [n, k] with a scale for each output channel, both
     int8; scales and bias float32.  The integer sums are exact (k at most 131071)."""
     return _call("matmul_i8", stream, a, a_scale, w, w_scale, bias, dtype, out)
+
+
+#: Numbers that share a scale in the 4-bit codes and the 8-bit states.
+BLOCK = 32
+
+
+def quant_mx4(x: torch.Tensor, out: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None, stream=None
+              ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(codes, scale) of `x` [rows, width]: blocks of 32 along a row, 16 bytes of codes each (uint8 [rows, 16 * blocks], the
+    lower half of a byte first) and a power of two as their scale (float8_e8m0fnu [rows, blocks]).  A code is the one of 0, 0.5,
+    1, 1.5, 2, 3, 4, 6 with a sign that is nearest to x / scale (ties to the even code, 6 beyond 6); the scale is
+    2^(floor(log2 max|x|) - 2).  A block with a NaN or an infinity has a NaN scale and codes 0; the last block is filled up with
+    zeros.  Rows of a given `out` start on 16-byte boundaries."""
+    return _call("quant_mx4", stream, x, out, scale)
+
+
+def dequant_mx4(codes: torch.Tensor, scale: torch.Tensor, width: int, dtype: Optional[torch.dtype] = None,
+                out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+    """The values [rows, width] that codes and scales of :func:`quant_mx4` stand for, in `dtype` (default float16)."""
+    return _call("dequant_mx4", stream, codes, scale, width, dtype, out)
+
+
+def rms_norm_mx4(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                 out: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None,
+                 r_out: Optional[torch.Tensor] = None, stream=None
+                 ) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
+    """(codes, scale, r): :func:`rms_norm` with y as 4-bit codes of its 32-bit values, as :func:`quant_mx4` makes them."""
+    return _call("rms_norm_mx4", stream, x, weight, residual, eps, out, scale, r_out)
+
+
+def matmul_mx4(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
+               bias: Optional[torch.Tensor] = None, dtype: Optional[torch.dtype] = None,
+               out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+    """out[i, j] = a[i] . w[j] + bias[j] in `dtype` (default float16): codes and scales `a` [m, blocks] (of
+    :func:`rms_norm_mx4` or :func:`quant_mx4`) and weights `w` [n, blocks] (of :func:`quant_mx4`), bias float32.  Sums in 32 bits.
+    Its gradients are those of the product of the values (:func:`dequant_mx4`)."""
+    return _call("matmul_mx4", stream, a, a_scale, w, w_scale, bias, dtype, out)
+
+
+class AdamWState(NamedTuple):
+    """The running means of one parameter's gradient and its square: float32, or float8_e4m3fn codes with a power-of-two
+    scale (float8_e8m0fnu) for each 32 elements in their order."""
+    m: torch.Tensor
+    v: torch.Tensor
+    m_scale: Optional[torch.Tensor] = None
+    v_scale: Optional[torch.Tensor] = None
+
+    def values(self) -> Tuple[torch.Tensor, torch.Tensor]:
+        """(m, v) in float32."""
+        if self.m_scale is None:
+            return self.m, self.v
+
+        def of(codes, scale):
+            scale = scale.view(torch.float8_e8m0fnu).float().repeat_interleave(BLOCK)
+            return codes.float() * scale[:codes.numel()].view(codes.shape)
+        return of(self.m, self.m_scale), of(self.v, self.v_scale)
+
+
+def adamw_state(param: torch.Tensor, bits: int = 32) -> AdamWState:
+    """The state of a parameter before its first step, in 32 or 8 bits an element."""
+    if bits == 32:
+        return AdamWState(*(torch.zeros(param.shape, dtype=torch.float32, device=param.device) for _ in range(2)))
+    if bits != 8:
+        raise ValueError(f"bits must be 32 or 8 (got {bits})")
+    blocks = (param.numel() + BLOCK - 1) // BLOCK
+    codes = [torch.zeros(param.shape, dtype=torch.uint8, device=param.device).view(torch.float8_e4m3fn) for _ in range(2)]
+    scale = [torch.zeros(blocks, dtype=torch.uint8, device=param.device).view(torch.float8_e8m0fnu) for _ in range(2)]
+    return AdamWState(*codes, *scale)
+
+
+def adamw(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], states: Sequence[AdamWState],
+          step: Union[int, torch.Tensor], lr: Union[float, torch.Tensor] = 1e-3, betas: Tuple[float, float] = (0.9, 0.999),
+          eps: float = 1e-8, weight_decay: Union[float, Sequence[float]] = 0.01,
+          copies: Optional[Sequence[Optional[torch.Tensor]]] = None, grad_scale: Union[float, torch.Tensor] = 1.0,
+          skip: Optional[torch.Tensor] = None, seed: int = 0, stream=None) -> None:
+    """One AdamW step over all `params`, in place, in few launches:
+
+        g = grad * grad_scale,  m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2
+        p = p (1 - lr weight_decay) - lr / (1 - beta1^step) * m / (sqrt(v / (1 - beta2^step)) + eps)
+
+    `states`: :func:`adamw_state` of each, in 32 or 8 bits as one likes.  `copies`: tensors that take the new parameters in another
+    type, for the next forward pass (entries may be None).  `weight_decay`: one number, or one for each parameter.  `step`
+    counts from 1.  `step` (int64), `lr` and `grad_scale` (float32) may be tensors of one element on the GPU, such as a clipping
+    factor, and are then read by the kernel; where `skip` (float32, one element) is not 0, nothing is written.  Params, states and
+    copies are contiguous and share no memory; gradients are copied if they are not contiguous.  8-bit states are rounded up
+    or down with the chance that keeps their mean, by bits that `seed` (0 .. 2^32 - 1), step and an element's index decide."""
+    _call("adamw", stream, params, grads, states, step, lr, betas, eps, weight_decay, copies, grad_scale, skip, seed)
