@@ -7,7 +7,7 @@
 // matter; the scales and the bias are applied in 32-bit floats and the result rounded once.
 #include <type_traits>
 
-#include "dense.hpp"
+#include "tiles.hpp"
 
 namespace trs {
 namespace dense {
@@ -15,7 +15,6 @@ namespace {
 
 constexpr int32_t kMostK = 131071;   // 128 * 128 * k stays below 2^31
 
-typedef int int4_v __attribute__((ext_vector_type(4)));
 typedef int int16_v __attribute__((ext_vector_type(16)));
 typedef int4_v int4_u __attribute__((aligned(1)));
 
@@ -74,11 +73,6 @@ __device__ __forceinline__ int4_v load_codes(const int8_t* row, int at, int k) {
   return settle(load16<ODD>(row + start_of(at, k)), at, k);
 }
 
-// A wave's sums, 32 rows and (up to) 64 columns at a time, through LDS (a wave's own part: `lds`, 32 rows of
-// kOutPitch integers), so that a lane holds 8 neighbouring columns of a row, and rows leave in whole vectors.
-template <int FN>
-constexpr int kOutPitch = (FN > 1 ? 64 : 32) + 4;
-
 // The scales of the rows that a lane of store_wave writes, read together: one wait for all.
 template <int FM, int FN>
 struct RowScales {
@@ -95,6 +89,8 @@ struct RowScales {
   }
 };
 
+// A wave's sums, 32 rows and (up to) 64 columns at a time, through LDS (a wave's own part: `lds`, 32 rows of
+// kOutPitch integers), so that a lane holds 8 neighbouring columns of a row, and rows leave in whole vectors.
 template <int FM, int FN>
 __device__ __forceinline__ void store_wave(const MatArgs& p, const int16_v (&acc)[FM][FN], const RowScales<FM, FN>& sa, int* lds,
                                            int64_t m0, int n0, int lane) {
@@ -167,34 +163,6 @@ __device__ __forceinline__ void store_wave(const MatArgs& p, const int16_v (&acc
 // the card holds under them), 2% of the LDS cycles lost to conflicts.  A wave owns 128 x 64 of a 256 x 256 tile; with
 // 64 x 64 (a tile of 256 x 128) it reads more LDS for each product (645 us), 128 x 128 spilled registers (2375).
 constexpr int kDepth = 128;
-
-typedef __attribute__((address_space(3))) void* lds_ptr;
-
-// A barrier that also waits for the wave's own LDS reads: what is written after it (by another wave's copy from
-// memory) must not reach them.  __syncthreads alone has been compiled to a barrier before which reads into
-// registers were still on their way.
-__device__ __forceinline__ void barrier_and_wait() {
-  __builtin_amdgcn_s_waitcnt(0);
-  __syncthreads();
-}
-
-// A buffer that ends with the operand's last code.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t operand(const int8_t* from, int64_t rows, int64_t ld, int k) {
-  const int64_t bytes = (rows - 1) * ld + k;
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(from), 0, (int)(bytes < UINT32_MAX ? bytes : UINT32_MAX), 0x00020000);
-}
-
-// Workgroup b of `total` as a tile: the workgroups of one XCD (b mod 8) take neighbouring tiles, in bands of 8
-// rows of tiles, so that an XCD's L2 serves the operands they share.
-__device__ __forceinline__ void tile_of(uint32_t b, uint32_t tiles_m, uint32_t tiles_n, uint32_t& tm, uint32_t& tn) {
-  const uint32_t total = tiles_m * tiles_n;
-  const uint32_t xcd = b & 7, q = total >> 3, r = total & 7;
-  const uint32_t t = xcd * q + (xcd < r ? xcd : r) + (b >> 3);
-  const uint32_t band = 8 * tiles_n, first = t / band * 8, in = t % band;
-  const uint32_t high = tiles_m - first < 8 ? tiles_m - first : 8;
-  tm = first + in % high;
-  tn = in / high;
-}
 
 template <int TM, int TN, int WM, int WN, int KS, bool DIRECT, class Offset>
 __device__ __forceinline__ void matmul_tile(const MatArgs& p, uint32_t tiles_m, uint32_t tiles_n) {

@@ -6,15 +6,16 @@
 // and its scale as one byte of a register; the sums are 32-bit floats, the result is rounded once.  A block's place along
 // k does not matter as long as both operands agree on it, so a lane takes blocks that follow one another, whose scales
 // are one word.  Codes past the last block are zeros with scale 0, and add nothing.
+#include <algorithm>
 #include <type_traits>
 
 #include "mx.hpp"
+#include "tiles.hpp"
 
 namespace trs {
 namespace dense {
 namespace {
 
-typedef int int4_v __attribute__((ext_vector_type(4)));
 typedef int int8_v __attribute__((ext_vector_type(8)));
 typedef float float4_v __attribute__((ext_vector_type(4)));
 
@@ -117,6 +118,368 @@ __global__ __launch_bounds__(1024) void k_mx4_rows(MatArgs p, uint32_t blocks_n)
   }
 }
 
+// ---------------------------------------------------------------------------------------------
+// Tiles: TM x TN outputs a workgroup, WM x WN a wave, 256 codes of k (8 blocks, 128 bytes of a row) a step, the next step's
+// operands on their way from memory to LDS while this one's are multiplied.  Piece (block) c of row r lies in place
+// c ^ (r / 2 & 7), so that the 16-byte reads of neighbouring rows spread over the banks.  The upper 32 lanes take the step's last four
+// blocks, so a lane's four scales of a step are one word; scales come 16 to a row, for two steps.
+//
+// Bound by arithmetic and by how soon the next step's operands arrive: 8192 x 8192 x 8192 288 us, 3.8 PFLOP/s (without the loads of
+// the steps 243, without LDS reads 260, without either 208, without outputs 265).  Each quarter of a step is read from LDS
+// while the one before is multiplied, scales among the first reads.
+//
+// ALIGNED: scales' rows on 4-byte boundaries; they go from memory to LDS without registers, as the codes do.  KS groups of
+// waves split a workgroup's steps, each with its own tiles, and the first adds the sums up: for few workgroups and a long k.
+constexpr int kDepth = 128;        // bytes of a row in a step
+constexpr int kStepBlocks = kDepth / kBlockBytes, kPair = 2 * kStepBlocks;
+constexpr int kPastEnd = (int)0x80000000u;   // an offset, or a part of one, past every buffer of a tile's rows
+
+typedef float float16_v __attribute__((ext_vector_type(16)));
+
+// 32 x 32 outputs of 64 codes of k.
+template <int J>
+__device__ __forceinline__ float16_v multiply32(int4_v w, int w_scale, int4_v a, int a_scale, float16_v acc) {
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(codes_of(w), codes_of(a), acc, kFp4, kFp4, J, w_scale, J, a_scale);
+}
+
+// 16 scales of a row from block `at` on, at any address; zeros past its end.
+__device__ __forceinline__ int4_v load_scales(const uint8_t* row, int at, int blocks) {
+  typedef int4_v int4_u __attribute__((aligned(1)));
+  if (at + kPair <= blocks) return *reinterpret_cast<const int4_u*>(row + at);
+  union { uint64_t q[2]; int4_v v; } u;
+  u.q[0] = u.q[1] = 0;
+#pragma unroll 1
+  for (int i = blocks - at - 1; i >= 0; --i) {   // from the end, each pushing the others up
+    u.q[1] = u.q[1] << 8 | u.q[0] >> 56;
+    u.q[0] = u.q[0] << 8 | row[at + i];
+  }
+  return u.v;
+}
+
+// A wave's sums, 32 rows and (up to) 64 columns at a time, through LDS (a wave's own part), so that a lane holds 8
+// neighbouring columns of a row, and rows leave in whole vectors.  16-bit outputs are rounded on the way in: half the bytes.
+// Instructions that run once cost a fetch each, so what need not be unrolled is not.
+template <int FN>
+constexpr int kOutBytes = 32 * kOutPitch<FN> * 4;   // of a wave
+
+template <int FM, int FN>
+__device__ __forceinline__ void add_bias(const MatArgs& p, float16_v (&acc)[FM][FN], int n0, int lane) {
+#pragma unroll
+  for (int j = 0; j < FN; ++j)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int n = n0 + j * 32 + 8 * (r / 4) + 4 * (lane >> 5) + r % 4;
+      const float b = p.bias[n < p.n ? n : p.n - 1];
+#pragma unroll
+      for (int i = 0; i < FM; ++i) acc[i][j][r] += b;
+    }
+}
+
+template <class T, int FM, int FN>
+__device__ __forceinline__ void store_wave(const MatArgs& p, const float16_v (&acc)[FM][FN], uint8_t* lds_part, int64_t m0, int n0, int lane) {
+  using raw = typename T::raw;
+  typedef raw four __attribute__((ext_vector_type(4)));
+  constexpr int FJ = FN > 1 ? 2 : 1, kPitch = FJ * 32 + 16 / (int)sizeof(raw);
+  constexpr int kRowLanes = FN > 1 ? 8 : 4, kRows = 64 / kRowLanes, kTurns = 32 / kRows;
+  raw* const lds = reinterpret_cast<raw*>(lds_part);
+  const int first = lane % kRowLanes * 8, row = lane & 31, half = lane >> 5;
+#pragma unroll
+  for (int j0 = 0; j0 < FN; j0 += FJ) {
+    // A lane whose 8 columns the matrix's end cuts takes the last 8 instead, if its wave has them: they are written
+    // twice, the same.
+    const int end = p.n - n0 - j0 * 32;   // columns there are from the part's first on
+    const int column = first + 8 > end && first < end && end >= 8 ? end - 8 : first;
+    const int n = n0 + j0 * 32 + column, left = first < end ? end - column : 0;
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+#pragma unroll
+      for (int j = 0; j < FJ; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float16_v& part = acc[i][j0 + j];
+          const int at = j * 32 + 8 * q + 4 * half;
+          *reinterpret_cast<four*>(lds + row * kPitch + at) =
+              four{(raw)part[4 * q], (raw)part[4 * q + 1], (raw)part[4 * q + 2], (raw)part[4 * q + 3]};
+        }
+      wave_fence();
+#pragma unroll 1
+      for (int t = 0; t < kTurns; ++t) {
+        const int r = t * kRows + lane / kRowLanes;
+        const int64_t m = m0 + i * 32 + r;
+        const raw* from = lds + r * kPitch + column;
+        raw8<T> v;
+        if (column % 8 == 0) {
+          v = *reinterpret_cast<const raw8<T>*>(from);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = from[e];
+        }
+        if (m >= p.m || left <= 0) continue;
+        raw* const to = static_cast<raw*>(p.out) + m * p.ldo + n;
+        if (left >= 8) {
+          typedef raw8<T> any __attribute__((aligned(sizeof(raw))));
+          if (p.past) {
+            keep_apart();
+            __builtin_nontemporal_store(v, reinterpret_cast<any*>(to));
+            keep_apart();
+          } else {
+            *reinterpret_cast<any*>(to) = v;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (e < left) to[e] = v[e];
+        }
+      }
+      wave_fence();
+    }
+  }
+}
+
+template <int TM, int TN, int WM, int WN, int KS, bool ALIGNED>
+__device__ __forceinline__ void mx4_tile(const MatArgs& p, uint32_t tiles_m, uint32_t tiles_n) {
+  constexpr int kWaveRows = TM / WM, kWavesOf = kWaveRows * (TN / WN), kAll = kWavesOf * 64;   // of a group
+  constexpr int FM = WM / 32, FN = WN / 32;
+  constexpr int kLoadsA = TM * 8 / kAll, kLoadsW = TN * 8 / kAll;
+  constexpr int kRows = TM + TN, kBring = (kRows + kAll - 1) / kAll;   // whose scales a thread brings, so many rows each
+  static_assert(TM % 64 == 0 && kRows % 64 == 0 && (kBring == 1 || kRows % kAll == 0), "a wave's rows are of one operand");
+  // of each group: the tiles of a and w of even steps, those of odd steps, the scales of two pairs of steps
+  constexpr int kTile = (TM + TN) * kDepth, kScales = kRows * kPair, kGroup = 2 * kTile + 2 * kScales;
+  __shared__ __align__(1024) uint8_t lds[KS * kGroup];
+  uint32_t tm, tn;
+  tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn);
+  const int64_t m0 = (int64_t)tm * TM;
+  const int n0 = (int)tn * TN;
+  const int any_wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int group = KS > 1 ? any_wave / kWavesOf : 0, wave = any_wave - group * kWavesOf;
+  const int thread = wave * 64 + lane;
+  const int wm = wave % kWaveRows * WM, wn = wave / kWaveRows * WN;
+  lds_bytes const mine_lds = (lds_bytes)lds + group * kGroup, s0 = mine_lds + 2 * kTile;
+
+  // Where this thread's pieces come from: `row0` and every kAll / 8 rows on, which agree in r / 2 & 7.  Rows past the
+  // operand's end are its last row again; their outputs are not stored.
+  const int row0 = thread >> 3, my_piece = (thread & 7) ^ (row0 >> 1 & 7), my_k = my_piece * kBlockBytes;
+  const uint8_t *base_a = p.a + m0 * p.lda, *base_w = p.w + n0 * p.ldw;
+  int at_a[kLoadsA], at_w[kLoadsW];
+#pragma unroll
+  for (int u = 0; u < kLoadsA; ++u) {
+    const int r = u * (kAll / 8) + row0;
+    at_a[u] = (m0 + r < p.m ? r : (int)(p.m - 1 - m0)) * (int)p.lda + my_k;
+  }
+#pragma unroll
+  for (int u = 0; u < kLoadsW; ++u) {
+    const int r = u * (kAll / 8) + row0;
+    at_w[u] = (n0 + r < p.n ? r : p.n - 1 - n0) * (int)p.ldw + my_k;
+  }
+  // The rows whose scales it brings: thread and every kAll on; of a below TM, of w from there on.
+  struct Row { const uint8_t* base; int64_t ld; int at; bool there, of_a; };
+  auto row_of = [&](int u) {
+    const int first = u * kAll + wave * 64, r = first + lane;
+    const bool of_a = first < TM;   // the same in a wave
+    const int at = of_a ? (m0 + r < p.m ? r : (int)(p.m - 1 - m0)) : (n0 + r - TM < p.n ? r - TM : p.n - 1 - n0);
+    return of_a ? Row{p.a_scale + m0 * p.ldas, p.ldas, at, first < kRows, true} : Row{p.w_scale + n0 * p.ldws, p.ldws, at, first < kRows, false};
+  };
+  int4_v held[ALIGNED ? 1 : kBring];
+  // The last step may be short: pieces past a row's end are asked for past the buffer's, which gives zeros.
+  const int steps = (p.blocks + kStepBlocks - 1) / kStepBlocks, last = p.blocks - (steps - 1) * kStepBlocks;   // blocks of the last step
+  // The tile's rows of codes and of scales end with the last row's last byte (scales: with the word that holds it).
+  auto bytes_of = [](int64_t rows, int most, int64_t ld, int row) {
+    return (uint32_t)__builtin_amdgcn_readfirstlane((int)((rows < most ? rows - 1 : most - 1) * ld + row));
+  };
+  const int row_bytes = p.blocks * kBlockBytes, row_words = (p.blocks + 3) & ~3;
+  const uint32_t bytes_a = bytes_of(p.m - m0, TM, p.lda, row_bytes), bytes_w = bytes_of(p.n - n0, TN, p.ldw, row_bytes);
+  const uint32_t bytes_as = bytes_of(p.m - m0, TM, p.ldas, row_words), bytes_ws = bytes_of(p.n - n0, TN, p.ldws, row_words);
+  auto fetch = [&](int odd, int step) {
+    const lds_bytes a = mine_lds + odd * kTile, w = a + TM * kDepth;
+    const int k0 = __builtin_amdgcn_readfirstlane(step * kDepth);   // the same in every lane
+    const __amdgpu_buffer_rsrc_t buf_a = buffer_of(base_a, bytes_a), buf_w = buffer_of(base_w, bytes_w);
+    auto load = [&](int past) {
+#pragma unroll
+      for (int u = 0; u < kLoadsA; ++u)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(buf_a, (lds_ptr)(a + (u * kAll + wave * 64) * 16), 16, at_a[u] | past, k0, 0, 0);
+#pragma unroll
+      for (int u = 0; u < kLoadsW; ++u)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(buf_w, (lds_ptr)(w + (u * kAll + wave * 64) * 16), 16, at_w[u] | past, k0, 0, 0);
+    };
+    if (step + 1 < steps || last == kStepBlocks) load(0);
+    else load(my_piece < last ? 0 : kPastEnd);
+  };
+  // The scales of steps 2 * pair and the next, into the half of the scales' place that the pair's parity names.  What follows a row's
+  // scales comes with them, and is cleared in LDS before a short last step (zeros times a NaN's scale would be NaN).
+  auto fetch_scales = [&](int pair) {
+#pragma unroll
+    for (int u = 0; u < kBring; ++u) {
+      const Row r = row_of(u);
+      if (!r.there) continue;
+      if constexpr (ALIGNED) {
+        const __amdgpu_buffer_rsrc_t buf = buffer_of(r.base, r.of_a ? bytes_as : bytes_ws);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(buf, (lds_ptr)(s0 + ((pair & 1) * kRows + u * kAll + wave * 64) * kPair), 16,
+                                                 r.at * (int)r.ld, __builtin_amdgcn_readfirstlane(pair * kPair), 0, 0);
+      } else {
+        held[u] = load_scales(r.base + r.at * r.ld, pair * kPair, p.blocks);
+      }
+    }
+  };
+  auto place_of_scales = [&](int pair, int u) {
+    return reinterpret_cast<int4_v*>(lds + group * kGroup + 2 * kTile + ((pair & 1) * kRows + u * kAll + thread) * kPair);
+  };
+  auto put_scales = [&](int pair) {
+    if constexpr (!ALIGNED)
+#pragma unroll
+      for (int u = 0; u < kBring; ++u)
+        if (row_of(u).there) *place_of_scales(pair, u) = held[u];
+  };
+
+  auto clear_scales = [&](int step) {
+    if constexpr (ALIGNED)
+#pragma unroll
+      for (int u = 0; u < kBring; ++u)
+        if (row_of(u).there) reinterpret_cast<uint64_t*>(place_of_scales(step >> 1, u))[step & 1] &= ((uint64_t)1 << (8 * last)) - 1;
+  };
+
+  float16_v acc[FM][FN] = {};
+  const int swz = lane >> 1 & 7, row = lane & 31, half = lane >> 5;
+  // Two sets of fragments: one is read from LDS while the other is multiplied.
+  int4_v fa[2][FM] = {}, fw[2][FN] = {};
+  int sa[2][FM] = {}, sw[2][FN] = {};   // of even and odd steps
+  // Where the lane's first pieces and scales lie; the others lie at whole distances, and piece 4 half + h at an exclusive or with h.
+  // `at` hides them from the compiler in each step: it would hold all their sums in registers, which the products need.
+  const int first_piece = ((4 * half) ^ swz) * kBlockBytes;
+  const int of_a = group * kGroup + (wm + row) * kDepth + first_piece, of_w = group * kGroup + (TM + wn + row) * kDepth + first_piece;
+  const int of_sa = group * kGroup + 2 * kTile + (wm + row) * kPair + 4 * half, of_sw = of_sa + (TM + wn - wm) * kPair;
+  struct At { int a, w, sa, sw; };
+  auto places = [&](int odd, int step) {
+    const int scale = (step >> 1 & 1) * kScales + odd * kStepBlocks;
+    At at{of_a + odd * kTile, of_w + odd * kTile, of_sa + scale, of_sw + scale};
+    asm volatile("" : "+v"(at.a), "+v"(at.w), "+v"(at.sa), "+v"(at.sw));
+    return at;
+  };
+  auto read = [&](const At& at, int h) {
+#pragma unroll
+    for (int i = 0; i < FM; ++i) fa[h & 1][i] = *reinterpret_cast<const int4_v*>(lds + (at.a ^ (h * kBlockBytes)) + i * 32 * kDepth);
+#pragma unroll
+    for (int j = 0; j < FN; ++j) fw[h & 1][j] = *reinterpret_cast<const int4_v*>(lds + (at.w ^ (h * kBlockBytes)) + j * 32 * kDepth);
+  };
+  auto read_scales = [&](const At& at, int set) {
+#pragma unroll
+    for (int i = 0; i < FM; ++i) sa[set][i] = *reinterpret_cast<const int*>(lds + at.sa + i * 32 * kPair);
+#pragma unroll
+    for (int j = 0; j < FN; ++j) sw[set][j] = *reinterpret_cast<const int*>(lds + at.sw + j * 32 * kPair);
+  };
+  // The weights are the matrix instruction's first operand, so a lane's registers run along n.
+  auto multiply = [&](auto h, int set) {
+    constexpr int H = decltype(h)::value;
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j) acc[i][j] = multiply32<H>(fw[H & 1][j], sw[set][j], fa[H & 1][i], sa[set][i], acc[i][j]);
+  };
+  // A quarter's order: two reads of LDS after each product as far as they go.
+  auto pace = [&](auto reads) {
+    constexpr int kReads = decltype(reads)::value, kProducts = FM * FN, kEach = kProducts > 1 ? 2 : kReads;
+    constexpr int kGroups = (kReads + kEach - 1) / kEach;
+    static_assert(kGroups <= kProducts, "a product before each group of reads");
+#pragma unroll
+    for (int k = 0; k < kGroups - 1; ++k) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, kEach, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, kReads - (kGroups - 1) * kEach, 0);
+    if constexpr (kProducts > kGroups) __builtin_amdgcn_sched_group_barrier(0x008, kProducts - kGroups, 0);
+  };
+  using std::integral_constant;
+  constexpr integral_constant<int, FM + FN> kCodes;
+  constexpr integral_constant<int, FM + FN + (FM + 1) / 2 + (FN + 1) / 2> kAndScales;   // two words are one read
+  // A step (`set`: whether it is even or odd): each quarter's products while the next quarter is read from LDS.
+  auto step = [&](int set, int t) {
+    const At at = places(set, t);
+    read_scales(at, set);
+    read(at, 0);
+    multiply(integral_constant<int, 3>{}, set ^ 1);      // the step before's last quarter (of nothing at first)
+    pace(kAndScales);
+    read(at, 1);
+    multiply(integral_constant<int, 0>{}, set);
+    pace(kCodes);
+    read(at, 2);
+    multiply(integral_constant<int, 1>{}, set);
+    pace(kCodes);
+    read(at, 3);
+    multiply(integral_constant<int, 2>{}, set);
+    pace(kCodes);
+  };
+
+  // a group's steps start on a pair of them
+  const int turns = KS > 1 ? ((steps + KS - 1) / KS + 1) / 2 * 2 : steps, first = group * turns;
+  const int mine = steps - first < turns ? steps - first : turns;   // this group's; not positive: none
+  if (steps > 0) {
+    if (mine > 0) {
+      fetch(0, first);
+      fetch_scales(first / 2);
+      put_scales(first / 2);
+    }
+    const int short_turn = ALIGNED && last < kStepBlocks ? (steps - 1) % turns : -1;   // a turn that some group's short step is in
+    auto arrived = [&](int t) {
+      barrier_and_wait();
+      if (t != short_turn) return;
+      if (first + t + 1 == steps) clear_scales(first + t);
+      barrier_and_wait();
+    };
+    for (int t = 0;;) {
+      arrived(t);
+      if (t + 1 < mine) fetch(1, first + t + 1);
+      if (KS == 1 || t < mine) step(0, first + t);
+      if (++t == turns) break;
+      arrived(t);
+      if (t + 1 < mine) {
+        fetch(0, first + t + 1);
+        fetch_scales((first + t + 1) / 2);
+      }
+      if (KS == 1 || t < mine) step(1, first + t);
+      if (t + 1 < mine) put_scales((first + t + 1) / 2);
+      if (++t == turns) break;
+    }
+    // the last step's last quarter
+    const bool even = (KS == 1 ? turns : mine) & 1;
+#pragma unroll
+    for (int i = 0; i < FM; ++i) sa[0][i] = even ? sa[0][i] : sa[1][i];
+#pragma unroll
+    for (int j = 0; j < FN; ++j) sw[0][j] = even ? sw[0][j] : sw[1][j];
+    multiply(integral_constant<int, 3>{}, 0);
+  }
+  barrier_and_wait();
+  if constexpr (KS > 1) {
+    // each group's sums in its own tiles, a register of the 64 lanes after the other
+    constexpr int kRegs = FM * FN * 16;
+    static_assert(kRegs * kAll * 4 <= 2 * kTile, "sums fit");
+    auto place = [&](int g, int r) { return reinterpret_cast<float*>(lds + g * kGroup) + r * kAll + thread; };
+    if (group > 0) {
+#pragma unroll
+      for (int r = 0; r < kRegs; ++r) *place(group, r) = acc[r / 16 / FN][r / 16 % FN][r % 16];
+    }
+    barrier_and_wait();
+    if (group > 0) return;
+    for (int g = 1; g < KS; ++g)
+#pragma unroll
+      for (int r = 0; r < kRegs; ++r) acc[r / 16 / FN][r / 16 % FN][r % 16] += *place(g, r);
+  }
+  static_assert(kOutBytes<FN> * kWavesOf <= kGroup, "outputs fit");
+  uint8_t* const part = lds + wave * kOutBytes<FN>;
+  if (p.bias) add_bias<FM, FN>(p, acc, n0 + wn, lane);
+  if (p.out_type == TRS_F32) store_wave<f32_t>(p, acc, part, m0 + wm, n0 + wn, lane);
+  else if (p.out_type == TRS_F16) store_wave<f16_t>(p, acc, part, m0 + wm, n0 + wn, lane);
+  else store_wave<bf16_t>(p, acc, part, m0 + wm, n0 + wn, lane);
+}
+
+template <int TM, int TN, int WM, int WN, int KS, bool ALIGNED>
+__global__ __launch_bounds__((TM / WM) * (TN / WN) * 64 * KS, WM * WN > 8192 ? 1 : 2) void k_mx4_tile(MatArgs p, uint32_t tiles_m, uint32_t tiles_n) {
+  mx4_tile<TM, TN, WM, WN, KS, ALIGNED>(p, tiles_m, tiles_n);
+}
+
+// ---------------------------------------------------------------------------------------------
+// Host side: which kernel.
+constexpr int kCus = 256;
+
 template <int FM>
 void launch_rows(const MatArgs& p, hipStream_t s) {
   const uint32_t bn = (uint32_t)ceil_div(p.n, 16), bm = (uint32_t)ceil_div(p.m, 16 * FM);
@@ -124,8 +487,88 @@ void launch_rows(const MatArgs& p, hipStream_t s) {
   k_mx4_rows<FM><<<dim3(bn * bm), 64 * waves, 0, s>>>(p, bn);
 }
 
-// No code of k: the bias alone.
+// Scales' rows on 4-byte boundaries.
+bool aligned_scales(const MatArgs& p) {
+  return ((reinterpret_cast<uintptr_t>(p.a_scale) | reinterpret_cast<uintptr_t>(p.w_scale) | (uintptr_t)p.ldas | (uintptr_t)p.ldws) & 3) == 0;
+}
+
+template <int T, int WM, int WN, int KS, bool ALIGNED>
+void launch_tile(const MatArgs& p, hipStream_t s) {
+  const uint32_t tm = (uint32_t)ceil_div(p.m, T), tn = (uint32_t)ceil_div(p.n, T);
+  k_mx4_tile<T, T, WM, WN, KS, ALIGNED><<<dim3(tm * tn), (T / WM) * (T / WN) * 64 * KS, 0, s>>>(p, tm, tn);
+}
+
+int64_t tiles(const MatArgs& p, int tm, int tn) { return ceil_div(p.m, tm) * ceil_div(p.n, tn); }
+
+// Microseconds beside a launch's 2, fitted to the sizes below (operands that change from call to call, in the MALL where they fit).
+// Rounds over the CUs: a CU has one workgroup of tiles of 256, two of 128, four of 64, which share its time.
+//   m x n x k              rows 1    2     4   tiles 64  (KS 4)  128    256
+//   1 x 4096 x 4096          3.6   4.0   4.6      6.3     6.7   12.1   25.4
+//   16 x 4096 x 4096         4.4   4.7   5.3      6.4     6.7   12.5
+//   32 x 4096 x 4096         6.7   5.7   6.3      7.3     7.2   13.2
+//   64 x 4096 x 4096        11.1   8.9   8.2      7.3     7.1   13.9
+//   128 x 1000 x 300         3.2   3.5   4.8      4.0     4.9    6.2
+//   300 x 400 x 1000         3.5   3.6   4.7      4.4     5.2    6.9
+//   500 x 1000 x 2010       10.9  10.8  11.1      6.8     7.2    9.7   19.3
+//   512 x 512 x 4096        11.2   9.0   8.4     12.2     8.7   14.7
+//   1000 x 1000 x 2016      18.3                  7.2     7.4   11.9
+//   1024 x 4096 x 4096                           19.6    30.0   18.2   31.3
+//   2048 x 2048 x 2048                           12.3           11.7   19.4
+//   2048 x 4096 x 4096                           38.5           25.3   33.6
+//   4096 x 4096 x 4096                           73.8           46.5   39.5
+//   16384 x 1024 x 512                           16.3           13.0   11.6
+//   8192 x 8192 x 8192                          538            345    288
+struct Choice { double us; int side, groups, rows; };   // rows: of k_mx4_rows, in sixteens; 0: tiles
+
+Choice choose(const MatArgs& p) {
+  const double steps = (p.blocks + kStepBlocks - 1) / kStepBlocks;
+  const bool near = std::max(p.lda, p.ldw) <= INT32_MAX / 256 && std::max(p.ldas, p.ldws) <= INT32_MAX / 256;   // a tile's offsets fit 32 bits
+  const int64_t t64 = ceil_div(tiles(p, 64, 64), kCus), t128 = ceil_div(tiles(p, 128, 128), kCus), t256 = ceil_div(tiles(p, 256, 256), kCus);
+  Choice best{1e300, 0, 0, 0};
+  auto offer = [&](const Choice& c) {
+    const int threads = c.rows || c.groups == 4 ? 1024 : c.side == 256 ? 512 : 256;
+    const bool fits = fits_grid(c.rows ? tiles(p, 16 * c.rows, 16) : tiles(p, c.side, c.side), threads);
+    if (fits && c.us < best.us) best = c;
+  };
+  for (int f : {1, 2, 4}) {
+    const double rows = p.m < 16 * f ? p.m : 16 * f, kb = ceil_div(tiles(p, 16 * f, 16), kCus) * (16 + rows) * p.blocks * 17e-3;
+    offer({std::max(1.4 + 0.2 * f, 0.5 + kb / 32), 0, 0, f});
+  }
+  if (!near) return best;
+  const double rest = t64 % 4;
+  offer({t64 / 4 * (steps + 2.1) + (rest == 0 ? 0 : rest == 1 ? 0.6 * steps + 0.6 : rest == 2 ? 0.65 * steps + 0.8 : 0.85 * steps + 1.5), 64, 1, 0});
+  if (t64 == 1 && steps >= 8) offer({0.36 * steps + 1.4, 64, 4, 0});
+  offer({t128 / 2 * (1.27 * steps + 2.6) + t128 % 2 * (0.9 * steps + 2.4), 128, 1, 0});
+  if (aligned_scales(p)) offer({t256 * (1.96 * steps + 5.8), 256, 1, 0});   // without, the kernel spills: not built
+  return best;
+}
+
+template <bool ALIGNED>
+void launch_tiles(const MatArgs& p, const Choice& c, hipStream_t s) {
+  if constexpr (ALIGNED)
+    if (c.side == 256) return launch_tile<256, 128, 64, 1, true>(p, s);
+  if (c.side == 128) launch_tile<128, 64, 64, 1, ALIGNED>(p, s);
+  else if (c.groups == 4) launch_tile<64, 32, 32, 4, ALIGNED>(p, s);
+  else launch_tile<64, 32, 32, 1, ALIGNED>(p, s);
+}
+
+// The most blocks of a row: 2^30 bytes of codes.
 constexpr int32_t kMostBlocks = 1 << 26;
+constexpr int64_t kMostRows = (int64_t)1 << 34;   // tiles times tiles stay far from 64 bits
+
+// Whether a kernel takes p's sizes; launches it.
+bool launch(const MatArgs& p, hipStream_t s) {
+  const Choice c = choose(p);
+  switch (c.rows) {
+    case 1: launch_rows<1>(p, s); return true;
+    case 2: launch_rows<2>(p, s); return true;
+    case 4: launch_rows<4>(p, s); return true;
+  }
+  if (c.side == 0) return false;
+  if (aligned_scales(p)) launch_tiles<true>(p, c, s);
+  else launch_tiles<false>(p, c, s);
+  return true;
+}
 
 }  // namespace
 }  // namespace dense
@@ -145,10 +588,10 @@ extern "C" int trs_matmul_mx4(const uint8_t* a, int64_t lda, const uint8_t* a_sc
   const int64_t row = (int64_t)blocks * kBlockBytes;
   if (lda < row || ldw < row || ldas < blocks || ldws < blocks || ldo < n) return fail(TRS_EINVAL, where, "leading dimension too small");
   if (blocks > 0 && (!aligned_codes(a, lda) || !aligned_codes(w, ldw))) return fail(TRS_EINVAL, where, "codes off a 16-byte boundary");
-  if (m > (int64_t)1 << 32 || !fits_grid(ceil_div(m, 16) * ceil_div(n, 16), 1024))
-    return fail(TRS_ERANGE, where, "the output needs more workgroups than a launch can have");
+  if (m > kMostRows) return fail(TRS_ERANGE, where, "too many rows");
   const bool past = streams(out, ldo, out_type == TRS_F32 ? 4 : 2, m, n);
   const MatArgs p{a, a_scale, w, w_scale, bias, out, lda, ldas, ldw, ldws, ldo, m, n, blocks, out_type, past};
-  launch_rows<1>(p, static_cast<hipStream_t>(stream));
+  if (!launch(p, static_cast<hipStream_t>(stream)))
+    return fail(TRS_ERANGE, where, "the output needs more workgroups than a launch can have");
   return launched(where);
 }
