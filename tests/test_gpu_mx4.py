@@ -306,7 +306,8 @@ SHAPES = [(1, 1, 1), (1, 1, 32), (1, 16, 33), (2, 17, 64), (1, 4096, 4096), (3, 
           (5, 300, 1000), (31, 64, 513), (32, 2048, 1024), (33, 65, 2010), (64, 64, 64), (64, 100, 4096), (65, 129, 96),
           (100, 100, 100), (127, 255, 257), (128, 128, 256), (129, 257, 288), (200, 1000, 2016), (256, 256, 1056), (257, 300, 3000),
           (500, 1000, 2010), (512, 512, 4096), (700, 130, 256), (1000, 64, 128), (1023, 513, 1600), (4099, 256, 128), (5000, 100, 300),
-          (20_001, 256, 128), (9000, 500, 64), (2049, 2050, 640), (4096, 4096, 512)]
+          (20_001, 256, 128), (9000, 500, 64), (2049, 2050, 640), (4096, 4096, 512), (3000, 3100, 1000),
+          (5000, 3000, 300), (2500, 2500, 1000), (600, 520, 4096)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
@@ -334,7 +335,8 @@ def test_products_of_wide_scales(m, n, k):
     assert torch.equal(got, trspmm.matmul_mx4(a, sa, w, sw, dtype=torch.float32))
 
 
-@pytest.mark.parametrize("m,n,k", [(1, 40, 100), (20, 70, 1100), (130, 140, 520), (600, 700, 290), (3000, 300, 100)])
+@pytest.mark.parametrize("m,n,k", [(1, 40, 100), (20, 70, 1100), (130, 140, 520), (600, 700, 290), (3000, 300, 100), (1500, 1900, 1000),
+                                   (500, 400, 3000)])
 def test_product_strides(m, n, k):
     say("product strides", m, n, k)
     b = blocks_of(k)

@@ -531,13 +531,13 @@ Choice choose(const MatArgs& p) {
     if (fits && c.us < best.us) best = c;
   };
   for (int f : {1, 2, 4}) {
-    const double rows = p.m < 16 * f ? p.m : 16 * f, kb = ceil_div(tiles(p, 16 * f, 16), kCus) * (16 + rows) * p.blocks * 17e-3;
-    offer({std::max(1.4 + 0.2 * f, 0.5 + kb / 32), 0, 0, f});
+    const double rows = p.m < 16 * f ? p.m : 16 * f, kb = (16 + rows) * p.blocks * 17e-3;
+    offer({std::max(1.4 + 0.2 * f, 0.5 + ceil_div(tiles(p, 16 * f, 16), kCus) * std::max(0.3, kb / 32)), 0, 0, f});
   }
   if (!near) return best;
   const double rest = t64 % 4;
-  offer({t64 / 4 * (steps + 2.1) + (rest == 0 ? 0 : rest == 1 ? 0.6 * steps + 0.6 : rest == 2 ? 0.65 * steps + 0.8 : 0.85 * steps + 1.5), 64, 1, 0});
-  if (t64 == 1 && steps >= 8) offer({0.36 * steps + 1.4, 64, 4, 0});
+  offer({t64 / 4 * (steps + 2.1) + (rest == 0 ? 0 : rest == 1 ? 0.58 * steps + 0.4 : rest == 2 ? 0.65 * steps + 0.8 : 0.85 * steps + 1.5), 64, 1, 0});
+  if (t64 == 1 && steps >= 8) offer({0.19 * steps + 3.7, 64, 4, 0});
   offer({t128 / 2 * (1.27 * steps + 2.6) + t128 % 2 * (0.9 * steps + 2.4), 128, 1, 0});
   if (aligned_scales(p)) offer({t256 * (1.96 * steps + 5.8), 256, 1, 0});   // without, the kernel spills: not built
   return best;
