@@ -307,7 +307,9 @@ SHAPES = [(1, 1, 1), (1, 1, 32), (1, 16, 33), (2, 17, 64), (1, 4096, 4096), (3, 
           (100, 100, 100), (127, 255, 257), (128, 128, 256), (129, 257, 288), (200, 1000, 2016), (256, 256, 1056), (257, 300, 3000),
           (500, 1000, 2010), (512, 512, 4096), (700, 130, 256), (1000, 64, 128), (1023, 513, 1600), (4099, 256, 128), (5000, 100, 300),
           (20_001, 256, 128), (9000, 500, 64), (2049, 2050, 640), (4096, 4096, 512), (3000, 3100, 1000),
-          (5000, 3000, 300), (2500, 2500, 1000), (600, 520, 4096)]
+          (5000, 3000, 300), (2500, 2500, 1000), (600, 520, 4096),
+          (9000, 47, 128), (9001, 64, 30), (9001, 128, 33), (40_001, 192, 90), (9000, 320, 160), (20_000, 256, 190), (20_000, 64, 225),
+          (9999, 256, 256), (3001, 33, 100), (40_000, 1, 64)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
@@ -336,7 +338,7 @@ def test_products_of_wide_scales(m, n, k):
 
 
 @pytest.mark.parametrize("m,n,k", [(1, 40, 100), (20, 70, 1100), (130, 140, 520), (600, 700, 290), (3000, 300, 100), (1500, 1900, 1000),
-                                   (500, 400, 3000)])
+                                   (500, 400, 3000), (9000, 128, 120), (9000, 30, 250)])
 def test_product_strides(m, n, k):
     say("product strides", m, n, k)
     b = blocks_of(k)
@@ -360,7 +362,7 @@ def test_product_strides(m, n, k):
     assert torch.equal(trspmm.matmul_mx4(odd, sa, w, sw, dtype=torch.float32), want.float())
 
 
-@pytest.mark.parametrize("m,n,k", [(1, 40, 100), (40, 50, 1100), (300, 400, 1000), (3000, 256, 128)])
+@pytest.mark.parametrize("m,n,k", [(1, 40, 100), (40, 50, 1100), (300, 400, 1000), (3000, 256, 128), (9000, 256, 224), (9000, 64, 30)])
 def test_blocks_of_nan_reach_their_row_and_channel_alone(m, n, k):
     say("nan blocks", m, n, k)
     (a, sa), (w, sw) = operand(m, k, 1), operand(n, k, 3)

@@ -156,11 +156,82 @@ __device__ __forceinline__ int4_v load_scales(const uint8_t* row, int at, int bl
   return u.v;
 }
 
-// A wave's sums, 32 rows and (up to) 64 columns at a time, through LDS (a wave's own part), so that a lane holds 8
-// neighbouring columns of a row, and rows leave in whole vectors.  16-bit outputs are rounded on the way in: half the bytes.
-// Instructions that run once cost a fetch each, so what need not be unrolled is not.
-template <int FN>
-constexpr int kOutBytes = 32 * kOutPitch<FN> * 4;   // of a wave
+// Sums pass through LDS, 32 rows of each wave at a time, so that a lane holds 8 neighbouring columns of a row and rows leave in
+// whole vectors, rounded on the way in.  Instructions that run once cost a fetch each, so what need not be unrolled is not.
+
+// Rows of an output that lie in LDS from `lds` on, `pitch` elements apart, 8 columns (from `first` on) of one of them in this lane, to row
+// m and column n0 + first on.
+template <class T>
+__device__ __forceinline__ void store_piece(const MatArgs& p, const typename T::raw* lds, int first, int64_t m, int n0) {
+  using raw = typename T::raw;
+  // A lane whose 8 columns the matrix's end cuts takes the last 8 instead, if the part has them: they are written twice, the
+  // same.
+  const int end = p.n - n0;   // columns there are from the part's first on
+  const int column = first + 8 > end && first < end && end >= 8 ? end - 8 : first, left = first < end ? end - column : 0;
+  const raw* from = lds + column;
+  raw8<T> v;
+  if (column % 8 == 0) {
+    v = *reinterpret_cast<const raw8<T>*>(from);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = from[e];
+  }
+  if (m >= p.m || left <= 0) return;
+  raw* const to = static_cast<raw*>(p.out) + m * p.ldo + n0 + column;
+  if (left >= 8) {
+    typedef raw8<T> any __attribute__((aligned(sizeof(raw))));
+    if (p.past) {
+      keep_apart();
+      __builtin_nontemporal_store(v, reinterpret_cast<any*>(to));
+      keep_apart();
+    } else {
+      *reinterpret_cast<any*>(to) = v;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < left) to[e] = v[e];
+  }
+}
+
+// A lane's sums of 32 x 32 outputs, a row's columns 4 at a time.
+template <class T>
+__device__ __forceinline__ void put_sums(const float16_v& sums, typename T::raw* row, int half) {
+  using raw = typename T::raw;
+  typedef raw four __attribute__((ext_vector_type(4)));
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    *reinterpret_cast<four*>(row + 8 * q + 4 * half) =
+        four{(raw)sums[4 * q], (raw)sums[4 * q + 1], (raw)sums[4 * q + 2], (raw)sums[4 * q + 3]};
+}
+
+// Elements between rows of `columns` in LDS: 16 bytes more, for the banks.
+template <class T>
+constexpr int pitch_of(int columns) { return columns + 16 / (int)sizeof(typename T::raw); }
+
+// A wave's sums, (up to) 64 columns at a time, through the wave's own part of LDS.
+constexpr int kOutRows = 32, kOutColumns = 64;
+constexpr int kOutBytes = kOutRows * pitch_of<f32_t>(kOutColumns) * 4;
+
+template <class T, int FM, int FN>
+__device__ __forceinline__ void store_wave(const MatArgs& p, const float16_v (&acc)[FM][FN], uint8_t* part, int64_t m0, int n0, int lane) {
+  constexpr int FJ = FN > 1 ? 2 : 1, kPitch = pitch_of<T>(FJ * 32), kPieces = FJ * 4, kRows = 64 / kPieces;
+  typename T::raw* const lds = reinterpret_cast<typename T::raw*>(part);
+#pragma unroll
+  for (int j0 = 0; j0 < FN; j0 += FJ)
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+#pragma unroll
+      for (int j = 0; j < FJ; ++j) put_sums<T>(acc[i][j0 + j], lds + (lane & 31) * kPitch + j * 32, lane >> 5);
+      wave_fence();
+#pragma unroll 1
+      for (int t = 0; t < kOutRows / kRows; ++t) {
+        const int r = t * kRows + lane / kPieces;
+        store_piece<T>(p, lds + r * kPitch, lane % kPieces * 8, m0 + i * 32 + r, n0 + j0 * 32);
+      }
+      wave_fence();
+    }
+}
 
 template <int FM, int FN>
 __device__ __forceinline__ void add_bias(const MatArgs& p, float16_v (&acc)[FM][FN], int n0, int lane) {
@@ -173,67 +244,6 @@ __device__ __forceinline__ void add_bias(const MatArgs& p, float16_v (&acc)[FM][
 #pragma unroll
       for (int i = 0; i < FM; ++i) acc[i][j][r] += b;
     }
-}
-
-template <class T, int FM, int FN>
-__device__ __forceinline__ void store_wave(const MatArgs& p, const float16_v (&acc)[FM][FN], uint8_t* lds_part, int64_t m0, int n0, int lane) {
-  using raw = typename T::raw;
-  typedef raw four __attribute__((ext_vector_type(4)));
-  constexpr int FJ = FN > 1 ? 2 : 1, kPitch = FJ * 32 + 16 / (int)sizeof(raw);
-  constexpr int kRowLanes = FN > 1 ? 8 : 4, kRows = 64 / kRowLanes, kTurns = 32 / kRows;
-  raw* const lds = reinterpret_cast<raw*>(lds_part);
-  const int first = lane % kRowLanes * 8, row = lane & 31, half = lane >> 5;
-#pragma unroll
-  for (int j0 = 0; j0 < FN; j0 += FJ) {
-    // A lane whose 8 columns the matrix's end cuts takes the last 8 instead, if its wave has them: they are written
-    // twice, the same.
-    const int end = p.n - n0 - j0 * 32;   // columns there are from the part's first on
-    const int column = first + 8 > end && first < end && end >= 8 ? end - 8 : first;
-    const int n = n0 + j0 * 32 + column, left = first < end ? end - column : 0;
-#pragma unroll
-    for (int i = 0; i < FM; ++i) {
-#pragma unroll
-      for (int j = 0; j < FJ; ++j)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float16_v& part = acc[i][j0 + j];
-          const int at = j * 32 + 8 * q + 4 * half;
-          *reinterpret_cast<four*>(lds + row * kPitch + at) =
-              four{(raw)part[4 * q], (raw)part[4 * q + 1], (raw)part[4 * q + 2], (raw)part[4 * q + 3]};
-        }
-      wave_fence();
-#pragma unroll 1
-      for (int t = 0; t < kTurns; ++t) {
-        const int r = t * kRows + lane / kRowLanes;
-        const int64_t m = m0 + i * 32 + r;
-        const raw* from = lds + r * kPitch + column;
-        raw8<T> v;
-        if (column % 8 == 0) {
-          v = *reinterpret_cast<const raw8<T>*>(from);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = from[e];
-        }
-        if (m >= p.m || left <= 0) continue;
-        raw* const to = static_cast<raw*>(p.out) + m * p.ldo + n;
-        if (left >= 8) {
-          typedef raw8<T> any __attribute__((aligned(sizeof(raw))));
-          if (p.past) {
-            keep_apart();
-            __builtin_nontemporal_store(v, reinterpret_cast<any*>(to));
-            keep_apart();
-          } else {
-            *reinterpret_cast<any*>(to) = v;
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (e < left) to[e] = v[e];
-        }
-      }
-      wave_fence();
-    }
-  }
 }
 
 template <int TM, int TN, int WM, int WN, int KS, bool ALIGNED>
@@ -463,9 +473,9 @@ __device__ __forceinline__ void mx4_tile(const MatArgs& p, uint32_t tiles_m, uin
 #pragma unroll
       for (int r = 0; r < kRegs; ++r) acc[r / 16 / FN][r / 16 % FN][r % 16] += *place(g, r);
   }
-  static_assert(kOutBytes<FN> * kWavesOf <= kGroup, "outputs fit");
-  uint8_t* const part = lds + wave * kOutBytes<FN>;
+  static_assert(kOutBytes * kWavesOf <= kGroup, "outputs fit into the group's own part");
   if (p.bias) add_bias<FM, FN>(p, acc, n0 + wn, lane);
+  uint8_t* const part = lds + wave * kOutBytes;
   if (p.out_type == TRS_F32) store_wave<f32_t>(p, acc, part, m0 + wm, n0 + wn, lane);
   else if (p.out_type == TRS_F16) store_wave<f16_t>(p, acc, part, m0 + wm, n0 + wn, lane);
   else store_wave<bf16_t>(p, acc, part, m0 + wm, n0 + wn, lane);
@@ -474,6 +484,106 @@ __device__ __forceinline__ void mx4_tile(const MatArgs& p, uint32_t tiles_m, uin
 template <int TM, int TN, int WM, int WN, int KS, bool ALIGNED>
 __global__ __launch_bounds__((TM / WM) * (TN / WN) * 64 * KS, WM * WN > 8192 ? 1 : 2) void k_mx4_tile(MatArgs p, uint32_t tiles_m, uint32_t tiles_n) {
   mx4_tile<TM, TN, WM, WN, KS, ALIGNED>(p, tiles_m, tiles_n);
+}
+
+// ---------------------------------------------------------------------------------------------
+// Short rows (k of at most 256) and many of them: outputs are the bytes that count.  A wave keeps the codes of 64 channels in
+// registers and walks tiles of 32 rows, whose codes go from memory to registers as the matrix instruction takes them, the next tile's on
+// their way while this one's outputs pass through the wave's own part of LDS.  Bound by memory: 2^20 x 256 x 128 100 us, 0.61 GB at 6.0
+// TB/s (tiles of 256: 121); from k = 192 on by the loads' 16-byte pieces of rows (k = 256: 156 us, 4.4 TB/s).  The waves of a workgroup share rows (CW of them,
+// whose loads meet in the L1) or channels; they never wait for one another.  H: blocks of a half of a wave, 2 H for a row.
+constexpr int kPanelWaves = 4, kPanelRows = kOutRows, kPanelColumns = kOutColumns;
+template <int H, int CW>
+__device__ __forceinline__ void mx4_panel(const MatArgs& p, uint32_t tiles_m, uint32_t panels, uint32_t walkers) {
+  __shared__ __align__(16) uint8_t lds[kPanelWaves * kOutBytes];
+  __shared__ __align__(16) float bias[CW * kPanelColumns];
+  constexpr int RW = kPanelWaves / CW;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int row = lane & 31, half = lane >> 5;
+  // The workgroups of an XCD (b mod 8) that share rows follow one another.
+  const uint32_t octet = blockIdx.x >> 3, panel = octet % panels, walker = octet / panels * 8 + (blockIdx.x & 7);
+  const int n0 = (int)(panel * CW + wave % CW) * kPanelColumns;
+  if (p.bias) {
+    if (threadIdx.x < CW * kPanelColumns) {
+      const int n = (int)panel * (CW * kPanelColumns) + (int)threadIdx.x;
+      bias[threadIdx.x] = p.bias[n < p.n ? n : p.n - 1];
+    }
+    __syncthreads();
+  }
+  if (n0 >= p.n) return;
+  // The lane's blocks: H half .. ; the last one may not be there.
+  const int first = H * half;
+  const bool there = first + H <= p.blocks;
+  const int ends = there ? first + H - 1 : p.blocks - 1;   // where to read the last one from
+  auto load = [&](const uint8_t* codes, const uint8_t* scales, int4_v (&c)[H], uint32_t (&s)[H]) {
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      const int b = h + 1 < H ? first + h : ends;
+      c[h] = *reinterpret_cast<const int4_v*>(codes + b * kBlockBytes);
+      s[h] = scales[b];
+    }
+  };
+  auto settle = [&](int4_v (&c)[H], const uint32_t (&s)[H]) {
+    uint32_t word = 0;
+#pragma unroll
+    for (int h = 0; h < H; ++h) word |= (h + 1 < H || there ? s[h] : 0) << (8 * h);
+    if (!there) c[H - 1] = int4_v{0, 0, 0, 0};
+    return (int)word;
+  };
+  int4_v w[2][H];
+  int sw[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int n = n0 + j * 32 + row;
+    const int64_t r = n < p.n ? n : p.n - 1;
+    uint32_t s[H];
+    load(p.w + r * p.ldw, p.w_scale + r * p.ldws, w[j], s);
+    sw[j] = settle(w[j], s);
+  }
+  uint8_t* const part = lds + wave * kOutBytes;
+  const uint32_t step = walkers * RW;
+  int4_v a[H], next[H];
+  uint32_t sa[H], next_s[H];
+  auto fetch = [&](uint32_t tile) {
+    const int64_t m = (int64_t)tile * kPanelRows + row, r = m < p.m ? m : p.m - 1;
+    load(p.a + r * p.lda, p.a_scale + r * p.ldas, next, next_s);
+  };
+  uint32_t tile = walker * RW + wave / CW;
+  if (tile < tiles_m) fetch(tile);
+  for (; tile < tiles_m; tile += step) {
+#pragma unroll
+    for (int h = 0; h < H; ++h) a[h] = next[h], sa[h] = next_s[h];
+    if (tile + step < tiles_m) fetch(tile + step);
+    const int word = settle(a, sa);
+    float16_v acc[1][2] = {};
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      acc[0][j] = multiply32<0>(w[j][0], sw[j], a[0], word, acc[0][j]);
+      if constexpr (H > 1) acc[0][j] = multiply32<1>(w[j][1], sw[j], a[1], word, acc[0][j]);
+      if constexpr (H > 2) acc[0][j] = multiply32<2>(w[j][2], sw[j], a[2], word, acc[0][j]);
+      if constexpr (H > 3) acc[0][j] = multiply32<3>(w[j][3], sw[j], a[3], word, acc[0][j]);
+    }
+    if (p.bias) {
+      const float* b = bias + wave % CW * kPanelColumns + 4 * half;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float4_v v = *reinterpret_cast<const float4_v*>(b + j * 32 + 8 * q);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[0][j][4 * q + e] += v[e];
+        }
+    }
+    const int64_t m0 = (int64_t)tile * kPanelRows;
+    if (p.out_type == TRS_F32) store_wave<f32_t>(p, acc, part, m0, n0, lane);
+    else if (p.out_type == TRS_F16) store_wave<f16_t>(p, acc, part, m0, n0, lane);
+    else store_wave<bf16_t>(p, acc, part, m0, n0, lane);
+  }
+}
+
+template <int H, int CW>
+__global__ __launch_bounds__(kPanelWaves * 64, 4) void k_mx4_panel(MatArgs p, uint32_t tiles_m, uint32_t panels, uint32_t walkers) {
+  mx4_panel<H, CW>(p, tiles_m, panels, walkers);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -500,6 +610,31 @@ void launch_tile(const MatArgs& p, hipStream_t s) {
 
 int64_t tiles(const MatArgs& p, int tm, int tn) { return ceil_div(p.m, tm) * ceil_div(p.n, tn); }
 
+template <int H, int CW>
+void launch_panel(const MatArgs& p, hipStream_t s) {
+  const uint32_t tm = (uint32_t)ceil_div(p.m, (int64_t)kPanelRows), panels = (uint32_t)ceil_div(p.n, CW * kPanelColumns);
+  // four workgroups a CU by their LDS, whole octets of them (one for each XCD), no more than there are tiles
+  const int64_t most = round_up(ceil_div(tm, kPanelWaves / CW), 8), fit = round_up(ceil_div(4 * kCus, panels), 8);
+  const uint32_t walkers = (uint32_t)(most < fit ? most : fit);
+  k_mx4_panel<H, CW><<<dim3(walkers * panels), kPanelWaves * 64, 0, s>>>(p, tm, panels, walkers);
+}
+
+template <int H>
+void launch_panel(const MatArgs& p, hipStream_t s) {
+  if (p.n <= kPanelColumns) launch_panel<H, 1>(p, s);
+  else if (p.n <= 2 * kPanelColumns) launch_panel<H, 2>(p, s);
+  else launch_panel<H, 4>(p, s);
+}
+
+void launch_panel(const MatArgs& p, hipStream_t s) {
+  switch ((p.blocks + 1) / 2) {
+    case 1: return launch_panel<1>(p, s);
+    case 2: return launch_panel<2>(p, s);
+    case 3: return launch_panel<3>(p, s);
+    default: return launch_panel<4>(p, s);
+  }
+}
+
 // Microseconds beside a launch's 2, fitted to the sizes below (operands that change from call to call, in the MALL where they fit).
 // Rounds over the CUs: a CU has one workgroup of tiles of 256, two of 128, four of 64, which share its time.
 //   m x n x k              rows 1    2     4   tiles 64  (KS 4)  128    256
@@ -518,7 +653,19 @@ int64_t tiles(const MatArgs& p, int tm, int tn) { return ceil_div(p.m, tm) * cei
 //   4096 x 4096 x 4096                           73.8           46.5   39.5
 //   16384 x 1024 x 512                           16.3           13.0   11.6
 //   8192 x 8192 x 8192                          538            345    288
-struct Choice { double us; int side, groups, rows; };   // rows: of k_mx4_rows, in sixteens; 0: tiles
+//
+// The panel, us (2 H blocks a row; rows on 64-byte lines, or a wave's columns at most, or the lines that rows share cost twice):
+//   m x n x k              panel   64     128    256
+//   1048576 x 64 x 128       32     50     68    102
+//   1048576 x 256 x 128     100    175    136    121
+//   1048576 x 256 x 192     130    246    179    247
+//   1048576 x 256 x 256     156    283    177    153
+//   1048576 x 300 x 128     342    332    269    265
+//   50000 x 512 x 200        13     22     19     22
+//   2000 x 4096 x 256        11     10      8     10
+//   3000 x 256 x 128        5.1    5.3    5.4    7.9
+struct Choice { double us; int side, groups, rows; };   // rows: of k_mx4_rows, in sixteens; a side of 32: the panel
+constexpr int kPanelSide = 32;
 
 Choice choose(const MatArgs& p) {
   const double steps = (p.blocks + kStepBlocks - 1) / kStepBlocks;
@@ -527,19 +674,27 @@ Choice choose(const MatArgs& p) {
   Choice best{1e300, 0, 0, 0};
   auto offer = [&](const Choice& c) {
     const int threads = c.rows || c.groups == 4 ? 1024 : c.side == 256 ? 512 : 256;
-    const bool fits = fits_grid(c.rows ? tiles(p, 16 * c.rows, 16) : tiles(p, c.side, c.side), threads);
+    const bool fits = c.side == kPanelSide || fits_grid(c.rows ? tiles(p, 16 * c.rows, 16) : tiles(p, c.side, c.side), threads);
     if (fits && c.us < best.us) best = c;
   };
   for (int f : {1, 2, 4}) {
     const double rows = p.m < 16 * f ? p.m : 16 * f, kb = (16 + rows) * p.blocks * 17e-3;
     offer({std::max(1.4 + 0.2 * f, 0.5 + ceil_div(tiles(p, 16 * f, 16), kCus) * std::max(0.3, kb / 32)), 0, 0, f});
   }
+  const int element = p.out_type == TRS_F32 ? 4 : 2;
+  const double mb = ((double)p.m * p.n * element + ((double)p.m + p.n) * p.blocks * 17) * 1e-6;   // 1 TB/s: a microsecond each
+  const int h = (p.blocks + 1) / 2;
+  const bool lines = ((reinterpret_cast<uintptr_t>(p.out) | (uintptr_t)(p.ldo * element)) & 63) == 0;
+  if (h >= 1 && h <= 4 && (lines || p.n <= kPanelColumns) && p.m < (int64_t)kPanelRows << 30) {
+    const double waves = std::min(1.0, ceil_div(p.m, kPanelRows) * ceil_div(p.n, kPanelColumns) / (16.0 * kCus));
+    offer({2.2 + 0.9 * h * waves + mb / (h <= 2 ? 6.0 : h == 3 ? 4.9 : 4.5), kPanelSide, 1, 0});
+  }
   if (!near) return best;
   const double rest = t64 % 4;
   offer({t64 / 4 * (steps + 2.1) + (rest == 0 ? 0 : rest == 1 ? 0.58 * steps + 0.4 : rest == 2 ? 0.65 * steps + 0.8 : 0.85 * steps + 1.5), 64, 1, 0});
   if (t64 == 1 && steps >= 8) offer({0.19 * steps + 3.7, 64, 4, 0});
-  offer({t128 / 2 * (1.27 * steps + 2.6) + t128 % 2 * (0.9 * steps + 2.4), 128, 1, 0});
-  if (aligned_scales(p)) offer({t256 * (1.96 * steps + 5.8), 256, 1, 0});   // without, the kernel spills: not built
+  offer({std::max(mb / 4.7, t128 / 2 * (1.27 * steps + 2.6) + t128 % 2 * (0.9 * steps + 2.4)), 128, 1, 0});
+  if (aligned_scales(p)) offer({std::max(mb / 5, t256 * (1.96 * steps + 5.8)), 256, 1, 0});   // without, the kernel spills: not built
   return best;
 }
 
@@ -565,6 +720,10 @@ bool launch(const MatArgs& p, hipStream_t s) {
     case 4: launch_rows<4>(p, s); return true;
   }
   if (c.side == 0) return false;
+  if (c.side == kPanelSide) {
+    launch_panel(p, s);
+    return true;
+  }
   if (aligned_scales(p)) launch_tiles<true>(p, c, s);
   else launch_tiles<false>(p, c, s);
   return true;
