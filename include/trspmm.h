@@ -588,7 +588,7 @@ typedef struct trs_adamw_tensor {
 typedef struct trs_adamw_options {
   int32_t struct_size;               /* sizeof(trs_adamw_options) and of a tensor, set by trs_adamw_options_default */
   int32_t tensor_size;
-  double lr, beta1, beta2, eps, grad_scale;
+  double lr, beta1, beta2, eps, grad_scale;   /* betas in [0, 1), eps from 2^-126 on */
   int64_t step;                      /* counts from 1 */
   const float* lr_device;            /* where not NULL, these are read on the GPU in place of lr, grad_scale and step, */
   const float* grad_scale_device;    /* so that a captured call follows them */
@@ -600,7 +600,7 @@ typedef struct trs_adamw_options {
 void trs_adamw_options_default(trs_adamw_options* options);
 
 /* TRS_EINVAL also for buffers that are written and overlap (a tensor named twice); gradients must not overlap them
- * either.  A tensor has at most some 3.4e10 elements (TRS_ERANGE). */
+ * either.  A tensor has at most some 1.7e10 elements (TRS_ERANGE). */
 int trs_adamw(const trs_adamw_tensor* tensors, int64_t count, const trs_adamw_options* options, void* stream);
 
 const char* trs_last_error(void);

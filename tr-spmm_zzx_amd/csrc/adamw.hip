@@ -14,7 +14,8 @@
 // m and v are made of single, separately rounded products and sums, so that the codes are a function of the formula as written.
 //
 // Each element's operands are read once and written once: bound by memory.  The tensors' addresses are the launch's arguments, so a
-// call needs no table in memory, no copy and no synchronisation; the tensors of a launch are of the same types.
+// call needs no table in memory, no copy and no synchronisation; the tensors of a launch are of the same types.  2^27 elements, all
+// float32: 660 us, 3.76 GB at 5.7 TB/s; with 8-bit states 407 us, 2.16 GB at 5.3.
 #include <algorithm>
 #include <cfloat>
 #include <new>
@@ -139,7 +140,7 @@ __global__ __launch_bounds__(kThreads) void k_adamw(Args a) {
     root2 = sqrtf(-expm1f((float)step * s.log2));
     key = key_of(s.seed, (uint32_t)step);
   }
-  const float rate = lr / bias1, keep = 1.f - lr * t.decay;
+  const float rate = lr / bias1, keep = 1.f - lr * t.decay, inverse = 1.f / root2;
   const int64_t block_first = (int64_t)(blockIdx.x - a.first_block[k]) * (kThreads * kVec * U) + threadIdx.x * kVec;
   float p[U][kVec], g[U][kVec], m[U][kVec], v[U][kVec];
   uint32_t mc[U], vc[U], ms[U], vs[U];
@@ -175,8 +176,19 @@ __global__ __launch_bounds__(kThreads) void k_adamw(Args a) {
       m[u][i] = s.beta1 * m[u][i] + s.rest1 * x;
       v[u][i] = s.beta2 * v[u][i] + s.rest2 * (x * x);
     }
+    // The hardware's root and reciprocal are off by an ulp each, and take a v below 2^-126 for 0: where a wave has one, the exact
+    // ones.  (With them alone, 2^27 elements in bfloat16 with 8-bit states: 340 us, not 273.)
+    uint32_t least = UINT32_MAX;   // of the bits less 1, so that 0 counts as the largest
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) p[u][i] = p[u][i] * keep - rate * (m[u][i] / (sqrtf(v[u][i]) / root2 + s.eps));
+    for (int i = 0; i < kVec; ++i) least = min(least, __float_as_uint(v[u][i]) - 1);
+    if (__any(least < 0x007fffffu)) {
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) p[u][i] = p[u][i] * keep - rate * (m[u][i] / (sqrtf(v[u][i]) * inverse + s.eps));
+    } else {
+#pragma unroll
+      for (int i = 0; i < kVec; ++i)
+        p[u][i] = p[u][i] * keep - rate * (m[u][i] * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v[u][i]) * inverse + s.eps));
+    }
     store_part<P>(static_cast<typename P::raw*>(t.p) + at, n, p[u]);
     if (t.copy) {
       if (t.copy_type == TRS_F32) store_part<f32_t>(static_cast<float*>(t.copy) + at, n, p[u]);
@@ -219,14 +231,16 @@ __global__ __launch_bounds__(kThreads) void k_adamw(Args a) {
 // ---------------------------------------------------------------------------------------------
 // Host side.
 
-constexpr int kUnroll = 2;
-constexpr int64_t kBlockElements = kThreads * kVec * kUnroll;
+// Rounds of a workgroup: 2 with 8-bit states, whose loads are short (85 M elements in 148 tensors 290 us, 310 with 1), 1 with 32-bit
+// ones (2^27 elements 660 us, 704 with 2, 695 with 4).
+constexpr int unroll_of(bool small) { return small ? 2 : 1; }
+constexpr int64_t elements_of(bool small) { return (int64_t)kThreads * kVec * unroll_of(small); }
 constexpr int64_t kMostBlocks = UINT32_MAX / kThreads;
 
 template <class P, class G>
 void launch_states(const Args& a, bool small, uint32_t blocks, hipStream_t s) {
-  if (small) k_adamw<P, G, true, kUnroll><<<dim3(blocks), kThreads, 0, s>>>(a);
-  else k_adamw<P, G, false, kUnroll><<<dim3(blocks), kThreads, 0, s>>>(a);
+  if (small) k_adamw<P, G, true, unroll_of(true)><<<dim3(blocks), kThreads, 0, s>>>(a);
+  else k_adamw<P, G, false, unroll_of(false)><<<dim3(blocks), kThreads, 0, s>>>(a);
 }
 
 template <class P>
@@ -284,7 +298,7 @@ extern "C" int trs_adamw(const trs_adamw_tensor* tensors, int64_t count, const t
   if (count < 0) return fail(TRS_EINVAL, where, "negative count");
   auto fraction = [](double b) { return b >= 0.0 && b < 1.0; };
   if (!fraction(o->beta1) || !fraction(o->beta2)) return fail(TRS_EINVAL, where, "betas must be in [0, 1)");
-  if (!((float)o->eps > 0.f) || !std::isfinite((float)o->eps)) return fail(TRS_EINVAL, where, "eps must be positive and finite");
+  if (!((float)o->eps >= FLT_MIN) || !std::isfinite((float)o->eps)) return fail(TRS_EINVAL, where, "eps must be positive, at least 2^-126, and finite");
   if (!o->lr_device && !std::isfinite((float)o->lr)) return fail(TRS_EINVAL, where, "lr must be finite");
   if (!o->grad_scale_device && !std::isfinite((float)o->grad_scale)) return fail(TRS_EINVAL, where, "grad_scale must be finite");
   if (!o->step_device && o->step < 1) return fail(TRS_EINVAL, where, "steps count from 1");
@@ -301,7 +315,7 @@ extern "C" int trs_adamw(const trs_adamw_tensor* tensors, int64_t count, const t
     if ((t.m_scale == nullptr) != (t.v_scale == nullptr)) return fail(TRS_EINVAL, where, "the scales of m and v go together");
     if (t.count == 0) continue;
     if (!t.param || !t.grad || !t.m || !t.v) return fail(TRS_EINVAL, where, "NULL operand");
-    if (ceil_div(t.count, kBlockElements) > kMostBlocks) return fail(TRS_ERANGE, where, "a tensor needs more workgroups than a launch can have");
+    if (ceil_div(t.count, elements_of(t.m_scale != nullptr)) > kMostBlocks) return fail(TRS_ERANGE, where, "a tensor needs more workgroups than a launch can have");
     kinds |= 1u << kind_of(t);
     written += 3 + (t.m_scale ? 2 : 0) + (t.copy ? 1 : 0);
   }
@@ -349,7 +363,7 @@ extern "C" int trs_adamw(const trs_adamw_tensor* tensors, int64_t count, const t
         for (int64_t i = 0; i < count; ++i) {
           const trs_adamw_tensor& x = tensors[i];
           if (x.count == 0 || kind_of(x) != kind) continue;
-          const int64_t mine = ceil_div(x.count, kBlockElements);
+          const int64_t mine = ceil_div(x.count, elements_of(small));
           if (a.count == kTensors || blocks + mine > kMostBlocks) {
             launch(a, p_type, g_type, small, blocks, s);
             a.count = 0;
