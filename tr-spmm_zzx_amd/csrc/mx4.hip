@@ -26,54 +26,72 @@ struct QuantArgs {
 };
 
 // A workgroup's chunks lie one after another, a row's after the row's before it: so a wave's loads and stores have no gap
-// between rows, and no lane without a chunk but at the end (250,001 rows of 300 bfloat16 values written: 52 us with a wave a
-// row, whose 600 bytes share their lines with the next).  Long rows: `kSpan` chunks of one.
-constexpr int kSpan = 1024;
+// between rows, and no lane without a chunk but at the end (250,001 rows of 300 bfloat16 values written: 40 us; 52 with a wave a
+// row, whose 600 bytes share their lines with the next).  Long rows: kSpan chunks of one.  A thread's chunks are on their way
+// together.
+constexpr int kTurns = 2, kSpan = kTurns * kThreads;
 
-struct Place { int64_t row; int chunk; };
+struct Place { int64_t row; int chunk; bool there; };
 
-template <class Body>
-__device__ __forceinline__ void each_chunk(const QuantArgs& p, Body body) {
+// The thread's chunk of turn t.  One that is not there stands for the first of the workgroup's, to be read but not written.
+__device__ __forceinline__ Place place_of(const QuantArgs& p, int t) {
   const int64_t first = (int64_t)blockIdx.x * p.share;
+  const int at = t * kThreads + (int)threadIdx.x;
   if (p.chunks > kSpan) {
-    const int begin = (int)blockIdx.y * kSpan, end = begin + kSpan < p.chunks ? begin + kSpan : p.chunks;
-    for (int c = begin + (int)threadIdx.x; c < end; c += kThreads) body(Place{first, c});
-    return;
+    const int chunk = (int)blockIdx.y * kSpan + at;
+    return {first, chunk < p.chunks ? chunk : (int)blockIdx.y * kSpan, chunk < p.chunks};
   }
   const int rows = p.rows - first < p.share ? (int)(p.rows - first) : p.share, all = rows * p.chunks;
-  for (int at = threadIdx.x; at < all; at += kThreads) {
-    const int row = p.chunks == 1 ? at : (int)__umulhi(at, p.inverse);   // at / chunks, exact below 2^16
-    body(Place{first + row, at - row * p.chunks});
-  }
+  if (at >= all) return {first, 0, false};
+  const int row = p.chunks == 1 ? at : (int)__umulhi(at, p.inverse);   // at / chunks, exact below 2^16
+  return {first + row, at - row * p.chunks, true};
 }
 
 template <class X>
 __global__ __launch_bounds__(kThreads) void k_quant4(QuantArgs p) {
-  // a block's four chunks are a quad of lanes': chunks of a row and of a span are a multiple of four
-  each_chunk(p, [&](const Place& k) {
-    const int at = k.chunk * 8, n = p.width - at;
-    float v[8] = {};
-    if (n > 0) load_chunk<X>(static_cast<const typename X::raw*>(p.x) + k.row * p.ldx + at, n, v);
+  // A block's four chunks are a quad of lanes': the chunks of a row and of a span are a multiple of four.
+  raw8<X> x[kTurns];
+  Place k[kTurns];
+#pragma unroll
+  for (int t = 0; t < kTurns; ++t) {
+    k[t] = place_of(p, t);
+    const int at = k[t].chunk * 8, n = p.width - at;   // a block's chunks past the row's end read the row's first
+    x[t] = load_raw_any<X>(static_cast<const typename X::raw*>(p.x) + k[t].row * p.ldx + (n > 0 ? at : 0), n > 0 ? n : p.width);
+  }
+#pragma unroll
+  for (int t = 0; t < kTurns; ++t) {
+    const int n = p.width - k[t].chunk * 8;
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? (float)x[t][i] : 0.f;
     uint32_t byte;
     const uint32_t codes = quantise4(v, byte);
-    *reinterpret_cast<uint32_t*>(p.codes + k.row * p.ldc + k.chunk * 4) = codes;
-    if ((k.chunk & 3) == 0) p.scale[k.row * p.lds + (k.chunk >> 2)] = (uint8_t)byte;
-  });
+    if (!k[t].there) continue;
+    *reinterpret_cast<uint32_t*>(p.codes + k[t].row * p.ldc + k[t].chunk * 4) = codes;
+    if ((k[t].chunk & 3) == 0) p.scale[k[t].row * p.lds + (k[t].chunk >> 2)] = (uint8_t)byte;
+  }
 }
 
 template <class X>
 __global__ __launch_bounds__(kThreads) void k_dequant4(QuantArgs p) {
-  each_chunk(p, [&](const Place& k) {
-    const int at = k.chunk * 8, n = p.width - at;
-    const uint32_t codes = *reinterpret_cast<const uint32_t*>(p.codes + k.row * p.ldc + k.chunk * 4);
-    const uint32_t byte = p.scale[k.row * p.lds + (k.chunk >> 2)];
+  uint32_t codes[kTurns], byte[kTurns];
+  Place k[kTurns];
+#pragma unroll
+  for (int t = 0; t < kTurns; ++t) {
+    k[t] = place_of(p, t);
+    codes[t] = *reinterpret_cast<const uint32_t*>(p.codes + k[t].row * p.ldc + k[t].chunk * 4);
+    byte[t] = p.scale[k[t].row * p.lds + (k[t].chunk >> 2)];
+  }
+#pragma unroll
+  for (int t = 0; t < kTurns; ++t) {
+    const int at = k[t].chunk * 8, n = p.width - at;
     float v[8];
     // byte 0, 2^-127, is no ordinary float: half of 2^-126
-    values4(codes, scale_of(byte > 0 ? byte : 1), v);
+    values4(codes[t], scale_of(byte[t] > 0 ? byte[t] : 1), v);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = byte == kNanScale ? __builtin_nanf("") : byte ? v[i] : 0.5f * v[i];
-    store_chunk<X>(static_cast<typename X::raw*>(const_cast<void*>(p.x)) + k.row * p.ldx + at, n, v);
-  });
+    for (int i = 0; i < 8; ++i) v[i] = byte[t] == kNanScale ? __builtin_nanf("") : byte[t] ? v[i] : 0.5f * v[i];
+    if (k[t].there) store_chunk<X>(static_cast<typename X::raw*>(const_cast<void*>(p.x)) + k[t].row * p.ldx + at, n, v);
+  }
 }
 
 template <bool QUANT>
