@@ -128,7 +128,8 @@ __global__ __launch_bounds__(1024) void k_mx4_rows(MatArgs p, uint32_t blocks_n)
 // the steps 243, without LDS reads 260, without either 208, without outputs 265).  Each quarter of a step is read from LDS
 // while the one before is multiplied, scales among the first reads.
 //
-// ALIGNED: scales' rows on 4-byte boundaries; they go from memory to LDS without registers, as the codes do.  KS groups of
+// ALIGNED: scales' rows on 4-byte boundaries; they go from memory to LDS without registers, as the codes do.  Others come by the
+// words that hold them (loads off those boundaries took a third of the time: 8192^3 with 257 scales between rows 409 us).  KS groups of
 // waves split a workgroup's steps, each with its own tiles, and the first adds the sums up: for few workgroups and a long k.
 constexpr int kDepth = 128;        // bytes of a row in a step
 constexpr int kStepBlocks = kDepth / kBlockBytes, kPair = 2 * kStepBlocks;
@@ -140,20 +141,6 @@ typedef float float16_v __attribute__((ext_vector_type(16)));
 template <int J>
 __device__ __forceinline__ float16_v multiply32(int4_v w, int w_scale, int4_v a, int a_scale, float16_v acc) {
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(codes_of(w), codes_of(a), acc, kFp4, kFp4, J, w_scale, J, a_scale);
-}
-
-// 16 scales of a row from block `at` on, at any address; zeros past its end.
-__device__ __forceinline__ int4_v load_scales(const uint8_t* row, int at, int blocks) {
-  typedef int4_v int4_u __attribute__((aligned(1)));
-  if (at + kPair <= blocks) return *reinterpret_cast<const int4_u*>(row + at);
-  union { uint64_t q[2]; int4_v v; } u;
-  u.q[0] = u.q[1] = 0;
-#pragma unroll 1
-  for (int i = blocks - at - 1; i >= 0; --i) {   // from the end, each pushing the others up
-    u.q[1] = u.q[1] << 8 | u.q[0] >> 56;
-    u.q[0] = u.q[0] << 8 | row[at + i];
-  }
-  return u.v;
 }
 
 // Sums pass through LDS, 32 rows of each wave at a time, so that a lane holds 8 neighbouring columns of a row and rows leave in
@@ -281,24 +268,36 @@ __device__ __forceinline__ void mx4_tile(const MatArgs& p, uint32_t tiles_m, uin
     const int r = u * (kAll / 8) + row0;
     at_w[u] = (n0 + r < p.n ? r : p.n - 1 - n0) * (int)p.ldw + my_k;
   }
-  // The rows whose scales it brings: thread and every kAll on; of a below TM, of w from there on.
-  struct Row { const uint8_t* base; int64_t ld; int at; bool there, of_a; };
-  auto row_of = [&](int u) {
+  // The rows whose scales it brings: thread and every kAll on; of a below TM, of w from there on (the same in a wave).
+  const uint8_t* s_base[kBring];   // with the words that hold its ends: a buffer
+  uint32_t s_bytes[kBring];
+  int s_at[kBring], s_off[kBring];   // where its scales start there, and how far off a word
+  bool s_there[kBring];
+#pragma unroll
+  for (int u = 0; u < kBring; ++u) {
     const int first = u * kAll + wave * 64, r = first + lane;
-    const bool of_a = first < TM;   // the same in a wave
-    const int at = of_a ? (m0 + r < p.m ? r : (int)(p.m - 1 - m0)) : (n0 + r - TM < p.n ? r - TM : p.n - 1 - n0);
-    return of_a ? Row{p.a_scale + m0 * p.ldas, p.ldas, at, first < kRows, true} : Row{p.w_scale + n0 * p.ldws, p.ldws, at, first < kRows, false};
-  };
-  int4_v held[ALIGNED ? 1 : kBring];
+    const bool of_a = first < TM;
+    const int64_t there = of_a ? p.m - m0 : p.n - n0, ld = of_a ? p.ldas : p.ldws;
+    const int at = of_a ? r : r - TM, most = of_a ? TM : TN, mine = at < there ? at : (int)there - 1;
+    const uint8_t* const from = of_a ? p.a_scale + m0 * p.ldas : p.w_scale + n0 * p.ldws;
+    const int off = (int)(reinterpret_cast<uintptr_t>(from) & 3);
+    s_there[u] = first < kRows;
+    s_base[u] = from - off;
+    s_bytes[u] = (uint32_t)__builtin_amdgcn_readfirstlane((int)((off + ((there < most ? there : most) - 1) * ld + p.blocks + 3) & ~3));
+    s_at[u] = off + mine * (int)ld;
+    s_off[u] = s_at[u] & 3;
+    s_at[u] -= s_off[u];
+  }
+  int4_v held[ALIGNED ? 1 : kBring];   // 16 scales lie in five words, from the one that holds the first on
+  int held_end[ALIGNED ? 1 : kBring];
   // The last step may be short: pieces past a row's end are asked for past the buffer's, which gives zeros.
   const int steps = (p.blocks + kStepBlocks - 1) / kStepBlocks, last = p.blocks - (steps - 1) * kStepBlocks;   // blocks of the last step
-  // The tile's rows of codes and of scales end with the last row's last byte (scales: with the word that holds it).
+  // The tile's rows of codes end with the last row's last byte.
   auto bytes_of = [](int64_t rows, int most, int64_t ld, int row) {
     return (uint32_t)__builtin_amdgcn_readfirstlane((int)((rows < most ? rows - 1 : most - 1) * ld + row));
   };
-  const int row_bytes = p.blocks * kBlockBytes, row_words = (p.blocks + 3) & ~3;
+  const int row_bytes = p.blocks * kBlockBytes;
   const uint32_t bytes_a = bytes_of(p.m - m0, TM, p.lda, row_bytes), bytes_w = bytes_of(p.n - n0, TN, p.ldw, row_bytes);
-  const uint32_t bytes_as = bytes_of(p.m - m0, TM, p.ldas, row_words), bytes_ws = bytes_of(p.n - n0, TN, p.ldws, row_words);
   auto fetch = [&](int odd, int step) {
     const lds_bytes a = mine_lds + odd * kTile, w = a + TM * kDepth;
     const int k0 = __builtin_amdgcn_readfirstlane(step * kDepth);   // the same in every lane
@@ -317,16 +316,16 @@ __device__ __forceinline__ void mx4_tile(const MatArgs& p, uint32_t tiles_m, uin
   // The scales of steps 2 * pair and the next, into the half of the scales' place that the pair's parity names.  What follows a row's
   // scales comes with them, and is cleared in LDS before a short last step (zeros times a NaN's scale would be NaN).
   auto fetch_scales = [&](int pair) {
+    const int block = __builtin_amdgcn_readfirstlane(pair * kPair);
 #pragma unroll
     for (int u = 0; u < kBring; ++u) {
-      const Row r = row_of(u);
-      if (!r.there) continue;
+      if (!s_there[u]) continue;
+      const __amdgpu_buffer_rsrc_t buf = buffer_of(s_base[u], s_bytes[u]);
       if constexpr (ALIGNED) {
-        const __amdgpu_buffer_rsrc_t buf = buffer_of(r.base, r.of_a ? bytes_as : bytes_ws);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(buf, (lds_ptr)(s0 + ((pair & 1) * kRows + u * kAll + wave * 64) * kPair), 16,
-                                                 r.at * (int)r.ld, __builtin_amdgcn_readfirstlane(pair * kPair), 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(buf, (lds_ptr)(s0 + ((pair & 1) * kRows + u * kAll + wave * 64) * kPair), 16, s_at[u], block, 0, 0);
       } else {
-        held[u] = load_scales(r.base + r.at * r.ld, pair * kPair, p.blocks);
+        held[u] = __builtin_amdgcn_raw_buffer_load_b128(buf, s_at[u], block, 0);
+        held_end[u] = __builtin_amdgcn_raw_buffer_load_b32(buf, s_at[u] + 16, block, 0);
       }
     }
   };
@@ -336,15 +335,18 @@ __device__ __forceinline__ void mx4_tile(const MatArgs& p, uint32_t tiles_m, uin
   auto put_scales = [&](int pair) {
     if constexpr (!ALIGNED)
 #pragma unroll
-      for (int u = 0; u < kBring; ++u)
-        if (row_of(u).there) *place_of_scales(pair, u) = held[u];
+      for (int u = 0; u < kBring; ++u) {
+        const int4_v& x = held[u];
+        if (s_there[u])
+          *place_of_scales(pair, u) = int4_v{
+              (int)__builtin_amdgcn_alignbyte(x[1], x[0], s_off[u]), (int)__builtin_amdgcn_alignbyte(x[2], x[1], s_off[u]),
+              (int)__builtin_amdgcn_alignbyte(x[3], x[2], s_off[u]), (int)__builtin_amdgcn_alignbyte(held_end[u], x[3], s_off[u])};
+      }
   };
-
   auto clear_scales = [&](int step) {
-    if constexpr (ALIGNED)
 #pragma unroll
-      for (int u = 0; u < kBring; ++u)
-        if (row_of(u).there) reinterpret_cast<uint64_t*>(place_of_scales(step >> 1, u))[step & 1] &= ((uint64_t)1 << (8 * last)) - 1;
+    for (int u = 0; u < kBring; ++u)
+      if (s_there[u]) reinterpret_cast<uint64_t*>(place_of_scales(step >> 1, u))[step & 1] &= ((uint64_t)1 << (8 * last)) - 1;
   };
 
   float16_v acc[FM][FN] = {};
@@ -423,12 +425,14 @@ __device__ __forceinline__ void mx4_tile(const MatArgs& p, uint32_t tiles_m, uin
   const int turns = KS > 1 ? ((steps + KS - 1) / KS + 1) / 2 * 2 : steps, first = group * turns;
   const int mine = steps - first < turns ? steps - first : turns;   // this group's; not positive: none
   if (steps > 0) {
+    const int pairs = (mine + 1) / 2, pair0 = first / 2;   // the group's
     if (mine > 0) {
       fetch(0, first);
-      fetch_scales(first / 2);
-      put_scales(first / 2);
+      fetch_scales(pair0);
+      put_scales(pair0);
+      if (!ALIGNED && pairs > 1) fetch_scales(pair0 + 1);
     }
-    const int short_turn = ALIGNED && last < kStepBlocks ? (steps - 1) % turns : -1;   // a turn that some group's short step is in
+    const int short_turn = last < kStepBlocks ? (steps - 1) % turns : -1;   // a turn that some group's short step is in
     auto arrived = [&](int t) {
       barrier_and_wait();
       if (t != short_turn) return;
@@ -437,16 +441,18 @@ __device__ __forceinline__ void mx4_tile(const MatArgs& p, uint32_t tiles_m, uin
     };
     for (int t = 0;;) {
       arrived(t);
+      // Scales that pass through registers come a step earlier than the others and lie in them for one.
+      if (!ALIGNED && t / 2 + 1 < pairs) put_scales(pair0 + t / 2 + 1);
       if (t + 1 < mine) fetch(1, first + t + 1);
       if (KS == 1 || t < mine) step(0, first + t);
       if (++t == turns) break;
       arrived(t);
       if (t + 1 < mine) {
         fetch(0, first + t + 1);
-        fetch_scales((first + t + 1) / 2);
+        if (ALIGNED) fetch_scales(pair0 + t / 2 + 1);
       }
+      if (!ALIGNED && t / 2 + 2 < pairs) fetch_scales(pair0 + t / 2 + 2);
       if (KS == 1 || t < mine) step(1, first + t);
-      if (t + 1 < mine) put_scales((first + t + 1) / 2);
       if (++t == turns) break;
     }
     // the last step's last quarter
@@ -700,9 +706,8 @@ Choice choose(const MatArgs& p) {
 
 template <bool ALIGNED>
 void launch_tiles(const MatArgs& p, const Choice& c, hipStream_t s) {
-  if constexpr (ALIGNED)
-    if (c.side == 256) return launch_tile<256, 128, 64, 1, true>(p, s);
-  if (c.side == 128) launch_tile<128, 64, 64, 1, ALIGNED>(p, s);
+  if (c.side == 256) launch_tile<256, 128, 64, 1, ALIGNED>(p, s);
+  else if (c.side == 128) launch_tile<128, 64, 64, 1, ALIGNED>(p, s);
   else if (c.groups == 4) launch_tile<64, 32, 32, 4, ALIGNED>(p, s);
   else launch_tile<64, 32, 32, 1, ALIGNED>(p, s);
 }
