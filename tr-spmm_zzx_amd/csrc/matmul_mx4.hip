@@ -122,7 +122,7 @@ __global__ __launch_bounds__(1024) void k_mx4_rows(MatArgs p, uint32_t blocks_n)
 // Tiles: TM x TN outputs a workgroup, WM x WN a wave, 256 codes of k (8 blocks, 128 bytes of a row) a step, the next step's
 // operands on their way from memory to LDS while this one's are multiplied.  Piece (block) c of row r lies in place
 // c ^ (r / 2 & 7), so that the 16-byte reads of neighbouring rows spread over the banks.  The upper 32 lanes take the step's last four
-// blocks, so a lane's four scales of a step are one word; scales come 16 to a row, for two steps.
+// blocks, so a lane's four scales of a step are one word; scales come 32 to a row, for four steps.
 //
 // Bound by arithmetic and by how soon the next step's operands arrive: 8192 x 8192 x 8192 288 us, 3.8 PFLOP/s (without the loads of
 // the steps 243, without LDS reads 260, without either 208, without outputs 265).  Each quarter of a step is read from LDS
@@ -132,7 +132,7 @@ __global__ __launch_bounds__(1024) void k_mx4_rows(MatArgs p, uint32_t blocks_n)
 // words that hold them (loads off those boundaries took a third of the time: 8192^3 with 257 scales between rows 409 us).  KS groups of
 // waves split a workgroup's steps, each with its own tiles, and the first adds the sums up: for few workgroups and a long k.
 constexpr int kDepth = 128;        // bytes of a row in a step
-constexpr int kStepBlocks = kDepth / kBlockBytes, kPair = 2 * kStepBlocks;
+constexpr int kStepBlocks = kDepth / kBlockBytes, kPair = 2 * kStepBlocks, kSlots = 4;
 constexpr int kPastEnd = (int)0x80000000u;   // an offset, or a part of one, past every buffer of a tile's rows
 
 typedef float float16_v __attribute__((ext_vector_type(16)));
@@ -240,8 +240,8 @@ __device__ __forceinline__ void mx4_tile(const MatArgs& p, uint32_t tiles_m, uin
   constexpr int kLoadsA = TM * 8 / kAll, kLoadsW = TN * 8 / kAll;
   constexpr int kRows = TM + TN, kBring = (kRows + kAll - 1) / kAll;   // whose scales a thread brings, so many rows each
   static_assert(TM % 64 == 0 && kRows % 64 == 0 && (kBring == 1 || kRows % kAll == 0), "a wave's rows are of one operand");
-  // of each group: the tiles of a and w of even steps, those of odd steps, the scales of two pairs of steps
-  constexpr int kTile = (TM + TN) * kDepth, kScales = kRows * kPair, kGroup = 2 * kTile + 2 * kScales;
+  // of each group: the tiles of a and w of even steps, those of odd steps, the scales of four pairs of steps
+  constexpr int kTile = (TM + TN) * kDepth, kScales = kRows * kPair, kGroup = 2 * kTile + kSlots * kScales;
   __shared__ __align__(1024) uint8_t lds[KS * kGroup];
   uint32_t tm, tn;
   tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn);
@@ -288,10 +288,13 @@ __device__ __forceinline__ void mx4_tile(const MatArgs& p, uint32_t tiles_m, uin
     s_off[u] = s_at[u] & 3;
     s_at[u] -= s_off[u];
   }
-  int4_v held[ALIGNED ? 1 : kBring];   // 16 scales lie in five words, from the one that holds the first on
-  int held_end[ALIGNED ? 1 : kBring];
+  int4_v held[ALIGNED ? 1 : 2][ALIGNED ? 1 : kBring];   // 16 scales lie in five words, from the one that holds the first on
+  int held_end[ALIGNED ? 1 : 2][ALIGNED ? 1 : kBring];
   // The last step may be short: pieces past a row's end are asked for past the buffer's, which gives zeros.
   const int steps = (p.blocks + kStepBlocks - 1) / kStepBlocks, last = p.blocks - (steps - 1) * kStepBlocks;   // blocks of the last step
+  // a group's steps start on a pair of them
+  const int turns = KS > 1 ? ((steps + KS - 1) / KS + 1) / 2 * 2 : steps, first = group * turns;
+  const int mine = steps - first < turns ? steps - first : turns;   // this group's; not positive: none
   // The tile's rows of codes end with the last row's last byte.
   auto bytes_of = [](int64_t rows, int most, int64_t ld, int row) {
     return (uint32_t)__builtin_amdgcn_readfirstlane((int)((rows < most ? rows - 1 : most - 1) * ld + row));
@@ -313,40 +316,46 @@ __device__ __forceinline__ void mx4_tile(const MatArgs& p, uint32_t tiles_m, uin
     if (step + 1 < steps || last == kStepBlocks) load(0);
     else load(my_piece < last ? 0 : kPastEnd);
   };
-  // The scales of steps 2 * pair and the next, into the half of the scales' place that the pair's parity names.  What follows a row's
-  // scales comes with them, and is cleared in LDS before a short last step (zeros times a NaN's scale would be NaN).
+  // The scales of two pairs of steps, `pair` (of the group's) and the next: the memory's line that holds a row's is read once for both.
+  // What follows a row's scales comes with them, and is cleared in LDS before a short last step (zeros times a NaN's scale would be NaN).
+  auto place_of_scales = [&](int pair, int u) {
+    return reinterpret_cast<int4_v*>(lds + group * kGroup + 2 * kTile + ((pair & (kSlots - 1)) * kRows + u * kAll + thread) * kPair);
+  };
   auto fetch_scales = [&](int pair) {
-    const int block = __builtin_amdgcn_readfirstlane(pair * kPair);
+    const int block = __builtin_amdgcn_readfirstlane((first / 2 + pair) * kPair);
 #pragma unroll
     for (int u = 0; u < kBring; ++u) {
       if (!s_there[u]) continue;
       const __amdgpu_buffer_rsrc_t buf = buffer_of(s_base[u], s_bytes[u]);
-      if constexpr (ALIGNED) {
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(buf, (lds_ptr)(s0 + ((pair & 1) * kRows + u * kAll + wave * 64) * kPair), 16, s_at[u], block, 0, 0);
-      } else {
-        held[u] = __builtin_amdgcn_raw_buffer_load_b128(buf, s_at[u], block, 0);
-        held_end[u] = __builtin_amdgcn_raw_buffer_load_b32(buf, s_at[u] + 16, block, 0);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        if constexpr (ALIGNED) {
+          const lds_bytes to = s0 + (((pair + k) & (kSlots - 1)) * kRows + u * kAll + wave * 64) * kPair;
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(buf, (lds_ptr)to, 16, s_at[u], block + k * kPair, 0, 0);
+        } else {
+          held[k][u] = __builtin_amdgcn_raw_buffer_load_b128(buf, s_at[u], block + k * kPair, 0);
+          held_end[k][u] = __builtin_amdgcn_raw_buffer_load_b32(buf, s_at[u] + 16, block + k * kPair, 0);
+        }
       }
     }
-  };
-  auto place_of_scales = [&](int pair, int u) {
-    return reinterpret_cast<int4_v*>(lds + group * kGroup + 2 * kTile + ((pair & 1) * kRows + u * kAll + thread) * kPair);
   };
   auto put_scales = [&](int pair) {
     if constexpr (!ALIGNED)
 #pragma unroll
-      for (int u = 0; u < kBring; ++u) {
-        const int4_v& x = held[u];
-        if (s_there[u])
-          *place_of_scales(pair, u) = int4_v{
-              (int)__builtin_amdgcn_alignbyte(x[1], x[0], s_off[u]), (int)__builtin_amdgcn_alignbyte(x[2], x[1], s_off[u]),
-              (int)__builtin_amdgcn_alignbyte(x[3], x[2], s_off[u]), (int)__builtin_amdgcn_alignbyte(held_end[u], x[3], s_off[u])};
-      }
+      for (int u = 0; u < kBring; ++u)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int4_v& x = held[k][u];
+          if (s_there[u])
+            *place_of_scales(pair + k, u) = int4_v{
+                (int)__builtin_amdgcn_alignbyte(x[1], x[0], s_off[u]), (int)__builtin_amdgcn_alignbyte(x[2], x[1], s_off[u]),
+                (int)__builtin_amdgcn_alignbyte(x[3], x[2], s_off[u]), (int)__builtin_amdgcn_alignbyte(held_end[k][u], x[3], s_off[u])};
+        }
   };
-  auto clear_scales = [&](int step) {
+  auto clear_scales = [&](int t) {
 #pragma unroll
     for (int u = 0; u < kBring; ++u)
-      if (s_there[u]) reinterpret_cast<uint64_t*>(place_of_scales(step >> 1, u))[step & 1] &= ((uint64_t)1 << (8 * last)) - 1;
+      if (s_there[u]) reinterpret_cast<uint64_t*>(place_of_scales(t >> 1, u))[t & 1] &= ((uint64_t)1 << (8 * last)) - 1;
   };
 
   float16_v acc[FM][FN] = {};
@@ -360,8 +369,8 @@ __device__ __forceinline__ void mx4_tile(const MatArgs& p, uint32_t tiles_m, uin
   const int of_a = group * kGroup + (wm + row) * kDepth + first_piece, of_w = group * kGroup + (TM + wn + row) * kDepth + first_piece;
   const int of_sa = group * kGroup + 2 * kTile + (wm + row) * kPair + 4 * half, of_sw = of_sa + (TM + wn - wm) * kPair;
   struct At { int a, w, sa, sw; };
-  auto places = [&](int odd, int step) {
-    const int scale = (step >> 1 & 1) * kScales + odd * kStepBlocks;
+  auto places = [&](int odd, int t) {
+    const int scale = (t >> 1 & (kSlots - 1)) * kScales + odd * kStepBlocks;
     At at{of_a + odd * kTile, of_w + odd * kTile, of_sa + scale, of_sw + scale};
     asm volatile("" : "+v"(at.a), "+v"(at.w), "+v"(at.sa), "+v"(at.sw));
     return at;
@@ -421,38 +430,31 @@ __device__ __forceinline__ void mx4_tile(const MatArgs& p, uint32_t tiles_m, uin
     pace(kCodes);
   };
 
-  // a group's steps start on a pair of them
-  const int turns = KS > 1 ? ((steps + KS - 1) / KS + 1) / 2 * 2 : steps, first = group * turns;
-  const int mine = steps - first < turns ? steps - first : turns;   // this group's; not positive: none
   if (steps > 0) {
-    const int pairs = (mine + 1) / 2, pair0 = first / 2;   // the group's
+    const int pairs = (mine + 1) / 2;   // the group's
     if (mine > 0) {
       fetch(0, first);
-      fetch_scales(pair0);
-      put_scales(pair0);
-      if (!ALIGNED && pairs > 1) fetch_scales(pair0 + 1);
+      fetch_scales(0);
+      put_scales(0);
     }
     const int short_turn = last < kStepBlocks ? (steps - 1) % turns : -1;   // a turn that some group's short step is in
     auto arrived = [&](int t) {
       barrier_and_wait();
       if (t != short_turn) return;
-      if (first + t + 1 == steps) clear_scales(first + t);
+      if (first + t + 1 == steps) clear_scales(t);
       barrier_and_wait();
     };
     for (int t = 0;;) {
       arrived(t);
-      // Scales that pass through registers come a step earlier than the others and lie in them for one.
-      if (!ALIGNED && t / 2 + 1 < pairs) put_scales(pair0 + t / 2 + 1);
+      // Scales that pass through registers lie in them for a step.
+      if (!ALIGNED && t % 4 == 2 && t / 2 + 1 < pairs) put_scales(t / 2 + 1);
       if (t + 1 < mine) fetch(1, first + t + 1);
-      if (KS == 1 || t < mine) step(0, first + t);
+      if (KS == 1 || t < mine) step(0, t);
       if (++t == turns) break;
       arrived(t);
-      if (t + 1 < mine) {
-        fetch(0, first + t + 1);
-        if (ALIGNED) fetch_scales(pair0 + t / 2 + 1);
-      }
-      if (!ALIGNED && t / 2 + 2 < pairs) fetch_scales(pair0 + t / 2 + 2);
-      if (KS == 1 || t < mine) step(1, first + t);
+      if (t + 1 < mine) fetch(0, first + t + 1);
+      if (t % 4 == 1 && t / 2 + 2 < pairs) fetch_scales(t / 2 + 2);
+      if (KS == 1 || t < mine) step(1, t);
       if (++t == turns) break;
     }
     // the last step's last quarter
