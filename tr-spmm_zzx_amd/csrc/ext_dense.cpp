@@ -362,18 +362,40 @@ const T* one_of(const char* name, const py::object& x, at::ScalarType type, int6
 
 bool is_tensor(const py::object& x) { return THPVariable_Check(x.ptr()); }
 
-// A tensor that the step writes, or reads beside one: contiguous, of n elements.
-void* flat(const char* name, size_t i, const Tensor& t, int64_t n, int64_t dev) {
-  const std::string which = std::string(name) + "[" + std::to_string(i) + "]";
-  on_device(which.c_str(), t, dev);
-  if (!t.is_contiguous()) wrong(which + " must be contiguous");
-  if (t.numel() != n) wrong(which + " must have " + std::to_string(n) + " elements (it has " + std::to_string(t.numel()) + ")");
+// A sequence's items without a cast of each: a list of some hundred tensors is walked in every step.
+class Items {
+ public:
+  Items(const char* name, const py::handle& x) : fast_(py::reinterpret_steal<py::object>(PySequence_Fast(x.ptr(), name))) {
+    if (!fast_) throw py::error_already_set();
+  }
+  size_t size() const { return (size_t)PySequence_Fast_GET_SIZE(fast_.ptr()); }
+  PyObject* operator[](size_t i) const { return PySequence_Fast_GET_ITEM(fast_.ptr(), (Py_ssize_t)i); }
+
+ private:
+  py::object fast_;
+};
+
+std::string at_index(const char* name, size_t i) { return std::string(name) + "[" + std::to_string(i) + "]"; }
+
+const Tensor& tensor_at(const char* name, size_t i, PyObject* x, int64_t dev) {
+  if (!THPVariable_Check(x)) wrong(at_index(name, i) + " must be a tensor");
+  const Tensor& t = THPVariable_Unpack(x);
+  if (!t.is_cuda() || t.get_device() != dev) on_device(at_index(name, i).c_str(), t, dev);
+  return t;
+}
+
+// A tensor that the step writes: contiguous, of n elements.
+void* flat(const char* name, size_t i, const Tensor& t, int64_t n) {
+  if (!t.is_contiguous()) wrong(at_index(name, i) + " must be contiguous");
+  if (t.numel() != n) wrong(at_index(name, i) + " must have " + std::to_string(n) + " elements (it has " + std::to_string(t.numel()) + ")");
   return t.data_ptr();
 }
 
-void adamw(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const py::sequence& states, const py::object& step,
-           const py::object& lr, std::pair<double, double> betas, double eps, const py::object& decay, const py::object& copies,
+void adamw(const py::object& params_in, const py::object& grads_in, const py::object& states_in, const py::object& step,
+           const py::object& lr, std::pair<double, double> betas, double eps, const py::object& decay, const py::object& copies_in,
            const py::object& grad_scale, const Given& skip, uint32_t seed, int64_t dev, int64_t stream) {
+  const Items params("params must be a sequence of tensors", params_in), grads("grads must be a sequence of tensors", grads_in),
+      states("states must be a sequence", states_in);
   const size_t count = params.size();
   if (grads.size() != count || states.size() != count)
     wrong(std::to_string(count) + " params, " + std::to_string(grads.size()) + " grads and " + std::to_string(states.size()) + " states");
@@ -391,43 +413,49 @@ void adamw(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, 
   const double decay_all = each ? 0.0 : decay.cast<double>();
   const std::vector<double> decays = each ? decay.cast<std::vector<double>>() : std::vector<double>();
   if (each && decays.size() != count) wrong("weight_decay must be a number, or one for each of the params");
-  const std::vector<Given> copied = copies.is_none() ? std::vector<Given>() : copies.cast<std::vector<Given>>();
-  if (!copies.is_none() && copied.size() != count) wrong("copies must have one entry for each of the params (None: no copy)");
+  std::optional<Items> copies;
+  if (!copies_in.is_none()) copies.emplace("copies must be a sequence of tensors", copies_in);
+  if (copies && copies->size() != count) wrong("copies must have one entry for each of the params (None: no copy)");
   std::vector<trs_adamw_tensor> list(count);
   std::vector<Tensor> made;   // contiguous copies of gradients
   for (size_t i = 0; i < count; ++i) {
     trs_adamw_tensor& t = list[i];
-    const int64_t n = params[i].numel();
     t = trs_adamw_tensor{};
+    const Tensor& p = tensor_at("params", i, params[i], dev);
+    const int64_t n = p.numel();
     t.count = n;
     t.weight_decay = (float)(each ? decays[i] : decay_all);
-    t.param = flat("params", i, params[i], n, dev);
-    t.param_type = type_of("params", params[i].scalar_type());
-    const Tensor& g = grads[i];
-    on_device("grads", g, dev);
+    t.param = flat("params", i, p, n);
+    t.param_type = type_of("params", p.scalar_type());
+    const Tensor& g = tensor_at("grads", i, grads[i], dev);
     t.grad_type = type_of("grads", g.scalar_type());
-    if (g.sizes() != params[i].sizes()) wrong("grads[" + std::to_string(i) + "] must have its parameter's shape");
-    if (!g.is_contiguous()) made.push_back(g.contiguous());
-    t.grad = g.is_contiguous() ? g.data_ptr() : made.back().data_ptr();
-    const py::sequence state = states[i].cast<py::sequence>();
+    if (g.sizes() != p.sizes()) wrong(at_index("grads", i) + " must have its parameter's shape");
+    if (g.is_contiguous()) {
+      t.grad = g.data_ptr();
+    } else {
+      made.push_back(g.contiguous());
+      t.grad = made.back().data_ptr();
+    }
+    const Items state("a state is (m, v) or (m, v, m_scale, v_scale)", states[i]);
     const size_t parts = state.size();
-    if (parts != 2 && (parts != 4 || state[2].is_none() != state[3].is_none())) wrong("a state is (m, v) or (m, v, m_scale, v_scale)");
-    const Tensor m = state[0].cast<Tensor>(), v = state[1].cast<Tensor>();
-    const bool small = parts == 4 && !state[2].is_none();
+    if (parts != 2 && (parts != 4 || (state[2] == Py_None) != (state[3] == Py_None))) wrong("a state is (m, v) or (m, v, m_scale, v_scale)");
+    const Tensor &m = tensor_at("m of states", i, state[0], dev), &v = tensor_at("v of states", i, state[1], dev);
+    const bool small = parts == 4 && state[2] != Py_None;
     const at::ScalarType type = small ? at::kFloat8_e4m3fn : at::kFloat;
     if (m.scalar_type() != type || v.scalar_type() != type)
-      wrong(std::string("m and v must be float32, or float8_e4m3fn with scales (states[") + std::to_string(i) + "])");
-    t.m = flat("m of states", i, m, n, dev);
-    t.v = flat("v of states", i, v, n, dev);
+      wrong("m and v must be float32, or float8_e4m3fn with scales (" + at_index("states", i) + ")");
+    t.m = flat("m of states", i, m, n);
+    t.v = flat("v of states", i, v, n);
     if (small) {
-      const Tensor ms = state[2].cast<Tensor>(), vs = state[3].cast<Tensor>();
+      const Tensor &ms = tensor_at("m_scale of states", i, state[2], dev), &vs = tensor_at("v_scale of states", i, state[3], dev);
       if (!is_scale(ms.scalar_type()) || !is_scale(vs.scalar_type())) wrong("scales of states must be float8_e8m0fnu or uint8");
-      t.m_scale = static_cast<uint8_t*>(flat("m_scale of states", i, ms, blocks_of(n), dev));
-      t.v_scale = static_cast<uint8_t*>(flat("v_scale of states", i, vs, blocks_of(n), dev));
+      t.m_scale = static_cast<uint8_t*>(flat("m_scale of states", i, ms, blocks_of(n)));
+      t.v_scale = static_cast<uint8_t*>(flat("v_scale of states", i, vs, blocks_of(n)));
     }
-    if (!copied.empty() && copied[i]) {
-      t.copy = flat("copies", i, *copied[i], n, dev);
-      t.copy_type = type_of("copies", copied[i]->scalar_type());
+    if (copies && (*copies)[i] != Py_None) {
+      const Tensor& c = tensor_at("copies", i, (*copies)[i], dev);
+      t.copy = flat("copies", i, c, n);
+      t.copy_type = type_of("copies", c.scalar_type());
     }
   }
   ok(trs_adamw(list.data(), (int64_t)count, &o, stream_of(stream)), "trs_adamw");
