@@ -124,8 +124,7 @@ __global__ __launch_bounds__(1024) void k_mx4_rows(MatArgs p, uint32_t blocks_n)
 // c ^ (r / 2 & 7), so that the 16-byte reads of neighbouring rows spread over the banks.  The upper 32 lanes take the step's last four
 // blocks, so a lane's four scales of a step are one word; scales come 32 to a row, for four steps.
 //
-// Bound by arithmetic and by how soon the next step's operands arrive: 8192 x 8192 x 8192 288 us, 3.8 PFLOP/s (without the loads of
-// the steps 243, without LDS reads 260, without either 208, without outputs 265).  Each quarter of a step is read from LDS
+// Bound by arithmetic and by how soon the next step's operands arrive: 8192 x 8192 x 8192 253 to 262 us by card, 4.2 PFLOP/s.  Each quarter of a step is read from LDS
 // while the one before is multiplied, scales among the first reads.
 //
 // ALIGNED: scales' rows on 4-byte boundaries; they go from memory to LDS without registers, as the codes do.  Others come by the
@@ -646,21 +645,25 @@ void launch_panel(const MatArgs& p, hipStream_t s) {
 // Microseconds beside a launch's 2, fitted to the sizes below (operands that change from call to call, in the MALL where they fit).
 // Rounds over the CUs: a CU has one workgroup of tiles of 256, two of 128, four of 64, which share its time.
 //   m x n x k              rows 1    2     4   tiles 64  (KS 4)  128    256
-//   1 x 4096 x 4096          3.6   4.0   4.6      6.3     6.7   12.1   25.4
-//   16 x 4096 x 4096         4.4   4.7   5.3      6.4     6.7   12.5
-//   32 x 4096 x 4096         6.7   5.7   6.3      7.3     7.2   13.2
-//   64 x 4096 x 4096        11.1   8.9   8.2      7.3     7.1   13.9
-//   128 x 1000 x 300         3.2   3.5   4.8      4.0     4.9    6.2
-//   300 x 400 x 1000         3.5   3.6   4.7      4.4     5.2    6.9
-//   500 x 1000 x 2010       10.9  10.8  11.1      6.8     7.2    9.7   19.3
-//   512 x 512 x 4096        11.2   9.0   8.4     12.2     8.7   14.7
-//   1000 x 1000 x 2016      18.3                  7.2     7.4   11.9
-//   1024 x 4096 x 4096                           19.6    30.0   18.2   31.3
-//   2048 x 2048 x 2048                           12.3           11.7   19.4
-//   2048 x 4096 x 4096                           38.5           25.3   33.6
-//   4096 x 4096 x 4096                           73.8           46.5   39.5
-//   16384 x 1024 x 512                           16.3           13.0   11.6
-//   8192 x 8192 x 8192                          538            345    288
+//   1 x 4096 x 4096          4.1   4.4   4.9      6.9     6.8   10.8   23.5
+//   16 x 4096 x 4096         4.8   5.0   5.7      7.0     6.8   10.8   23.5
+//   32 x 4096 x 4096         6.7   5.9   6.6      7.7     7.0   11.4
+//   64 x 4096 x 4096        11.0   9.1   8.4      8.2     7.3   11.8
+//   300 x 400 x 1000         4.2   4.2   5.0      4.2     5.5    5.7   10.0
+//   200 x 200 x 8192         7.4   9.7  14.0     11.9     9.6   18.8   43.1
+//   500 x 1000 x 2016       10.8  10.6  11.0      5.7     6.5    8.1   15.7
+//   512 x 512 x 4096        11.0   9.0   8.2      7.4     7.1   11.2   24.0
+//   256 x 4096 x 4096       37.8  29.6  26.0     10.5     8.4   13.7   25.7
+//   512 x 4096 x 4096       72.9  56.4  49.0     11.4    15.1   14.1   26.0
+//   1024 x 4096 x 4096                           19.1    28.3   16.0   26.4
+//   3000 x 768 x 6400                            19.0    30.0   21.1   37.9
+//   2048 x 2048 x 2048                           12.4            9.9   16.3
+//   2048 x 4096 x 4096                           33.2           21.8   27.1
+//   9000 x 3008 x 4800                            151            100     81
+//   4096 x 4096 x 4096                           63.6           41.8   37.1
+//   16384 x 1024 x 512                           14.1           10.9   10.7
+//   8192 x 8192 x 8192                            460            293    253
+// (With scales off 4-byte boundaries tiles of 256 take up to a quarter longer, the others 2 to 5%.)
 //
 // The panel, us (2 H blocks a row; rows on 64-byte lines, or a wave's columns at most, or the lines that rows share cost twice):
 //   m x n x k              panel   64     128    256
@@ -698,11 +701,12 @@ Choice choose(const MatArgs& p) {
     offer({2.2 + 0.9 * h * waves + mb / (h <= 2 ? 6.0 : h == 3 ? 4.9 : 4.5), kPanelSide, 1, 0});
   }
   if (!near) return best;
-  const double rest = t64 % 4;
-  offer({t64 / 4 * (steps + 2.1) + (rest == 0 ? 0 : rest == 1 ? 0.58 * steps + 0.4 : rest == 2 ? 0.65 * steps + 0.8 : 0.85 * steps + 1.5), 64, 1, 0});
-  if (t64 == 1 && steps >= 8) offer({0.19 * steps + 3.7, 64, 4, 0});
-  offer({std::max(mb / 4.7, t128 / 2 * (1.27 * steps + 2.6) + t128 % 2 * (0.9 * steps + 2.4)), 128, 1, 0});
-  if (aligned_scales(p)) offer({std::max(mb / 5, t256 * (1.96 * steps + 5.8)), 256, 1, 0});   // without, the kernel spills: not built
+  const double rest = t64 % 4, fill = std::min(1.0, tiles(p, 64, 64) / (double)kCus);
+  offer({t64 / 4 * (0.83 * steps + 2.2) + (rest == 0 ? 0 : rest == 1 ? (0.28 + 0.25 * fill) * steps + 0.6 : rest == 2 ? 0.55 * steps + 0.6 : 0.65 * steps + 0.8),
+         64, 1, 0});
+  if (t64 == 1 && steps >= 8) offer({2.9 + (0.13 + 0.11 * fill) * steps, 64, 4, 0});
+  offer({std::max(mb / 4.7, t128 / 2 * (1.03 * steps + 3.2) + t128 % 2 * (0.73 * steps + 2.1)), 128, 1, 0});
+  offer({std::max(mb / 5, t256 * (1.8 * steps + 5)), 256, 1, 0});
   return best;
 }
 
