@@ -309,7 +309,9 @@ SHAPES = [(1, 1, 1), (1, 1, 32), (1, 16, 33), (2, 17, 64), (1, 4096, 4096), (3, 
           (20_001, 256, 128), (9000, 500, 64), (2049, 2050, 640), (4096, 4096, 512), (3000, 3100, 1000),
           (5000, 3000, 300), (2500, 2500, 1000), (600, 520, 4096),
           (9000, 47, 128), (9001, 64, 30), (9001, 128, 33), (40_001, 192, 90), (9000, 320, 160), (20_000, 256, 190), (20_000, 64, 225),
-          (9999, 256, 256), (3001, 33, 100), (40_000, 1, 64)]
+          (9999, 256, 256), (3001, 33, 100), (40_000, 1, 64),
+          (50_001, 100, 128), (50_001, 172, 90), (40_000, 300, 128), (40_001, 301, 60), (30_000, 500, 64), (30_003, 255, 190),
+          (20_000, 257, 250), (20_000, 443, 33)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
@@ -338,7 +340,7 @@ def test_products_of_wide_scales(m, n, k):
 
 
 @pytest.mark.parametrize("m,n,k", [(1, 40, 100), (20, 70, 1100), (130, 140, 520), (600, 700, 290), (3000, 300, 100), (1500, 1900, 1000),
-                                   (500, 400, 3000), (9000, 128, 120), (9000, 30, 250)])
+                                   (500, 400, 3000), (9000, 128, 120), (9000, 30, 250), (30_000, 172, 100), (20_000, 400, 64)])
 def test_product_strides(m, n, k):
     say("product strides", m, n, k)
     b = blocks_of(k)
@@ -362,7 +364,7 @@ def test_product_strides(m, n, k):
     assert torch.equal(trspmm.matmul_mx4(odd, sa, w, sw, dtype=torch.float32), want.float())
 
 
-@pytest.mark.parametrize("m,n,k", [(1, 40, 100), (40, 50, 1100), (300, 400, 1000), (3000, 256, 128), (9000, 256, 224), (9000, 64, 30)])
+@pytest.mark.parametrize("m,n,k", [(1, 40, 100), (40, 50, 1100), (300, 400, 1000), (3000, 256, 128), (9000, 256, 224), (9000, 64, 30), (40_000, 300, 90)])
 def test_blocks_of_nan_reach_their_row_and_channel_alone(m, n, k):
     say("nan blocks", m, n, k)
     (a, sa), (w, sw) = operand(m, k, 1), operand(n, k, 3)

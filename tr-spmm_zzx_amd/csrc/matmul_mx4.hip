@@ -500,6 +500,82 @@ __global__ __launch_bounds__((TM / WM) * (TN / WN) * 64 * KS, WM * WN > 8192 ? 1
 // TB/s (tiles of 256: 121); from k = 192 on by the loads' 16-byte pieces of rows (k = 256: 156 us, 4.4 TB/s).  The waves of a workgroup share rows (CW of them,
 // whose loads meet in the L1) or channels; they never wait for one another.  H: blocks of a half of a wave, 2 H for a row.
 constexpr int kPanelWaves = 4, kPanelRows = kOutRows, kPanelColumns = kOutColumns;
+// The blocks of a row that a lane takes: H of them from H half on; the last one may not be there.
+template <int H>
+struct LaneBlocks {
+  int first, ends;   // ends: where to read the last one from
+  bool there;
+  int4_v codes[H];
+  uint32_t scales[H];
+  __device__ __forceinline__ LaneBlocks(int half, int blocks)
+      : first(H * half), ends(H * half + H <= blocks ? H * half + H - 1 : blocks - 1), there(H * half + H <= blocks) {}
+  __device__ __forceinline__ void load(const uint8_t* row, const uint8_t* row_scales) {
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      const int b = h + 1 < H ? first + h : ends;
+      codes[h] = *reinterpret_cast<const int4_v*>(row + b * kBlockBytes);
+      scales[h] = row_scales[b];
+    }
+  }
+  // The scales as one word; zeros in the place of what is not there.
+  __device__ __forceinline__ int settle() {
+    uint32_t word = 0;
+#pragma unroll
+    for (int h = 0; h < H; ++h) word |= (h + 1 < H || there ? scales[h] : 0) << (8 * h);
+    if (!there) codes[H - 1] = int4_v{0, 0, 0, 0};
+    return (int)word;
+  }
+};
+
+template <int H>
+__device__ __forceinline__ float16_v multiply_blocks(const int4_v (&w)[H], int sw, const int4_v (&a)[H], int sa) {
+  float16_v acc = {};
+  acc = multiply32<0>(w[0], sw, a[0], sa, acc);
+  if constexpr (H > 1) acc = multiply32<1>(w[1], sw, a[1], sa, acc);
+  if constexpr (H > 2) acc = multiply32<2>(w[2], sw, a[2], sa, acc);
+  if constexpr (H > 3) acc = multiply32<3>(w[3], sw, a[3], sa, acc);
+  return acc;
+}
+
+// 64 channels' codes, and their biases from LDS.
+template <int H>
+struct Channels {
+  int4_v codes[2][H];
+  int scales[2];
+  __device__ __forceinline__ void load(const MatArgs& p, int n0, int row, int half) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int n = n0 + j * 32 + row;
+      const int64_t r = n < p.n ? n : p.n - 1;
+      LaneBlocks<H> x(half, p.blocks);
+      x.load(p.w + r * p.ldw, p.w_scale + r * p.ldws);
+      scales[j] = x.settle();
+#pragma unroll
+      for (int h = 0; h < H; ++h) codes[j][h] = x.codes[h];
+    }
+  }
+  __device__ __forceinline__ void multiply(const LaneBlocks<H>& a, int a_scale, const float* bias, int half, float16_v (&acc)[1][2]) const {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      acc[0][j] = multiply_blocks<H>(codes[j], scales[j], a.codes, a_scale);
+      if (!bias) continue;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float4_v v = *reinterpret_cast<const float4_v*>(bias + j * 32 + 8 * q + 4 * half);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[0][j][4 * q + e] += v[e];
+      }
+    }
+  }
+};
+
+// The biases of `columns` channels from n0 on, into LDS.
+__device__ __forceinline__ void bring_bias(const MatArgs& p, int n0, int columns, float* bias) {
+  if (!p.bias) return;
+  for (int c = threadIdx.x; c < columns; c += kPanelWaves * 64) bias[c] = p.bias[n0 + c < p.n ? n0 + c : p.n - 1];
+  __syncthreads();
+}
+
 template <int H, int CW>
 __device__ __forceinline__ void mx4_panel(const MatArgs& p, uint32_t tiles_m, uint32_t panels, uint32_t walkers) {
   __shared__ __align__(16) uint8_t lds[kPanelWaves * kOutBytes];
@@ -510,77 +586,26 @@ __device__ __forceinline__ void mx4_panel(const MatArgs& p, uint32_t tiles_m, ui
   // The workgroups of an XCD (b mod 8) that share rows follow one another.
   const uint32_t octet = blockIdx.x >> 3, panel = octet % panels, walker = octet / panels * 8 + (blockIdx.x & 7);
   const int n0 = (int)(panel * CW + wave % CW) * kPanelColumns;
-  if (p.bias) {
-    if (threadIdx.x < CW * kPanelColumns) {
-      const int n = (int)panel * (CW * kPanelColumns) + (int)threadIdx.x;
-      bias[threadIdx.x] = p.bias[n < p.n ? n : p.n - 1];
-    }
-    __syncthreads();
-  }
+  bring_bias(p, (int)panel * (CW * kPanelColumns), CW * kPanelColumns, bias);
   if (n0 >= p.n) return;
-  // The lane's blocks: H half .. ; the last one may not be there.
-  const int first = H * half;
-  const bool there = first + H <= p.blocks;
-  const int ends = there ? first + H - 1 : p.blocks - 1;   // where to read the last one from
-  auto load = [&](const uint8_t* codes, const uint8_t* scales, int4_v (&c)[H], uint32_t (&s)[H]) {
-#pragma unroll
-    for (int h = 0; h < H; ++h) {
-      const int b = h + 1 < H ? first + h : ends;
-      c[h] = *reinterpret_cast<const int4_v*>(codes + b * kBlockBytes);
-      s[h] = scales[b];
-    }
-  };
-  auto settle = [&](int4_v (&c)[H], const uint32_t (&s)[H]) {
-    uint32_t word = 0;
-#pragma unroll
-    for (int h = 0; h < H; ++h) word |= (h + 1 < H || there ? s[h] : 0) << (8 * h);
-    if (!there) c[H - 1] = int4_v{0, 0, 0, 0};
-    return (int)word;
-  };
-  int4_v w[2][H];
-  int sw[2];
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int n = n0 + j * 32 + row;
-    const int64_t r = n < p.n ? n : p.n - 1;
-    uint32_t s[H];
-    load(p.w + r * p.ldw, p.w_scale + r * p.ldws, w[j], s);
-    sw[j] = settle(w[j], s);
-  }
+  Channels<H> w;
+  w.load(p, n0, row, half);
   uint8_t* const part = lds + wave * kOutBytes;
+  const float* const my_bias = p.bias ? bias + wave % CW * kPanelColumns : nullptr;
   const uint32_t step = walkers * RW;
-  int4_v a[H], next[H];
-  uint32_t sa[H], next_s[H];
+  LaneBlocks<H> next(half, p.blocks);
   auto fetch = [&](uint32_t tile) {
     const int64_t m = (int64_t)tile * kPanelRows + row, r = m < p.m ? m : p.m - 1;
-    load(p.a + r * p.lda, p.a_scale + r * p.ldas, next, next_s);
+    next.load(p.a + r * p.lda, p.a_scale + r * p.ldas);
   };
   uint32_t tile = walker * RW + wave / CW;
   if (tile < tiles_m) fetch(tile);
   for (; tile < tiles_m; tile += step) {
-#pragma unroll
-    for (int h = 0; h < H; ++h) a[h] = next[h], sa[h] = next_s[h];
+    LaneBlocks<H> a = next;
     if (tile + step < tiles_m) fetch(tile + step);
-    const int word = settle(a, sa);
-    float16_v acc[1][2] = {};
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      acc[0][j] = multiply32<0>(w[j][0], sw[j], a[0], word, acc[0][j]);
-      if constexpr (H > 1) acc[0][j] = multiply32<1>(w[j][1], sw[j], a[1], word, acc[0][j]);
-      if constexpr (H > 2) acc[0][j] = multiply32<2>(w[j][2], sw[j], a[2], word, acc[0][j]);
-      if constexpr (H > 3) acc[0][j] = multiply32<3>(w[j][3], sw[j], a[3], word, acc[0][j]);
-    }
-    if (p.bias) {
-      const float* b = bias + wave % CW * kPanelColumns + 4 * half;
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float4_v v = *reinterpret_cast<const float4_v*>(b + j * 32 + 8 * q);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[0][j][4 * q + e] += v[e];
-        }
-    }
+    const int a_scale = a.settle();
+    float16_v acc[1][2];
+    w.multiply(a, a_scale, my_bias, half, acc);
     const int64_t m0 = (int64_t)tile * kPanelRows;
     if (p.out_type == TRS_F32) store_wave<f32_t>(p, acc, part, m0, n0, lane);
     else if (p.out_type == TRS_F16) store_wave<f16_t>(p, acc, part, m0, n0, lane);
@@ -591,6 +616,72 @@ __device__ __forceinline__ void mx4_panel(const MatArgs& p, uint32_t tiles_m, ui
 template <int H, int CW>
 __global__ __launch_bounds__(kPanelWaves * 64, 4) void k_mx4_panel(MatArgs p, uint32_t tiles_m, uint32_t panels, uint32_t walkers) {
   mx4_panel<H, CW>(p, tiles_m, panels, walkers);
+}
+
+// The same for rows of up to 256 GW outputs that do not start on 64-byte lines.  Lines that a row shares with the next are written in
+// parts, which costs a read of them if the other part does not follow at once: so a workgroup has whole rows of outputs in LDS and
+// its waves write them one after another (2^20 x 300 x 128: 64 columns at a time 342 us).
+template <class T, int H, int GW>
+__device__ __forceinline__ void store_rows(const MatArgs& p, const float16_v (&acc)[GW][1][2], uint8_t* lds_bytes_, int64_t m0, int wave, int lane,
+                                           int pieces, uint32_t inverse) {
+  constexpr int kPitch = pitch_of<T>(GW * kPanelWaves * kPanelColumns);
+  typename T::raw* const lds = reinterpret_cast<typename T::raw*>(lds_bytes_);
+#pragma unroll
+  for (int u = 0; u < GW; ++u)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      put_sums<T>(acc[u][0][j], lds + (lane & 31) * kPitch + (u * kPanelWaves + wave) * kPanelColumns + j * 32, lane >> 5);
+  __syncthreads();
+  for (int at = threadIdx.x; at < kPanelRows * pieces; at += kPanelWaves * 64) {
+    const int r = (int)__umulhi(at, inverse);   // at / pieces
+    store_piece<T>(p, lds + r * kPitch, (at - r * pieces) * 8, m0 + r, 0);
+  }
+  __syncthreads();
+}
+
+template <int H, int GW, int BYTES>
+__device__ __forceinline__ void mx4_rows_panel(const MatArgs& p, uint32_t tiles_m, uint32_t inverse) {
+  constexpr int kColumns = GW * kPanelWaves * kPanelColumns;
+  __shared__ __align__(16) uint8_t lds[kPanelRows * (kColumns * BYTES + 16)];
+  __shared__ __align__(16) float bias[kColumns];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int row = lane & 31, half = lane >> 5;
+  bring_bias(p, 0, kColumns, bias);
+  Channels<H> w[GW];
+#pragma unroll
+  for (int u = 0; u < GW; ++u) w[u].load(p, (u * kPanelWaves + wave) * kPanelColumns, row, half);
+  const int pieces = (p.n + 7) / 8;
+  LaneBlocks<H> next(half, p.blocks);
+  auto fetch = [&](uint32_t tile) {
+    const int64_t m = (int64_t)tile * kPanelRows + row, r = m < p.m ? m : p.m - 1;
+    next.load(p.a + r * p.lda, p.a_scale + r * p.ldas);
+  };
+  uint32_t tile = blockIdx.x;
+  if (tile < tiles_m) fetch(tile);
+  for (; tile < tiles_m; tile += gridDim.x) {   // the same tiles in every wave
+    LaneBlocks<H> a = next;
+    if (tile + gridDim.x < tiles_m) fetch(tile + gridDim.x);
+    const int a_scale = a.settle();
+    float16_v acc[GW][1][2];
+#pragma unroll
+    for (int u = 0; u < GW; ++u)
+      w[u].multiply(a, a_scale, p.bias ? bias + (u * kPanelWaves + wave) * kPanelColumns : nullptr, half, acc[u]);
+    const int64_t m0 = (int64_t)tile * kPanelRows;
+    if constexpr (BYTES == 4) {
+      store_rows<f32_t, H, GW>(p, acc, lds, m0, wave, lane, pieces, inverse);
+    } else {
+      if (p.out_type == TRS_F16) store_rows<f16_t, H, GW>(p, acc, lds, m0, wave, lane, pieces, inverse);
+      else store_rows<bf16_t, H, GW>(p, acc, lds, m0, wave, lane, pieces, inverse);
+    }
+  }
+}
+
+// Workgroups that a CU holds, by their LDS and registers.
+constexpr int rows_panels(int gw, int bytes) { return gw == 1 ? 4 : bytes == 2 ? 3 : 2; }
+
+template <int H, int GW, int BYTES>
+__global__ __launch_bounds__(kPanelWaves * 64, rows_panels(GW, BYTES)) void k_mx4_rows_panel(MatArgs p, uint32_t tiles_m, uint32_t inverse) {
+  mx4_rows_panel<H, GW, BYTES>(p, tiles_m, inverse);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -633,7 +724,43 @@ void launch_panel(const MatArgs& p, hipStream_t s) {
   else launch_panel<H, 4>(p, s);
 }
 
+constexpr int kMostWhole = 2 * kPanelWaves * kPanelColumns;   // outputs of a row that a workgroup has together
+
+template <int H, int GW, int BYTES>
+void launch_rows_panel(const MatArgs& p, hipStream_t s) {
+  const uint32_t tm = (uint32_t)ceil_div(p.m, (int64_t)kPanelRows), pieces = (uint32_t)ceil_div(p.n, 8);
+  const uint32_t fit = kCus * rows_panels(GW, BYTES);
+  k_mx4_rows_panel<H, GW, BYTES><<<dim3(tm < fit ? tm : fit), kPanelWaves * 64, 0, s>>>(
+      p, tm, (uint32_t)((((uint64_t)1 << 32) + pieces - 1) / pieces));
+}
+
+template <int H>
+void launch_rows_panel(const MatArgs& p, hipStream_t s) {
+  const bool wide = p.n > kMostWhole / 2;
+  if (p.out_type == TRS_F32) {
+    if (wide) launch_rows_panel<H, 2, 4>(p, s);
+    else launch_rows_panel<H, 1, 4>(p, s);
+  } else {
+    if (wide) launch_rows_panel<H, 2, 2>(p, s);
+    else launch_rows_panel<H, 1, 2>(p, s);
+  }
+}
+
+// Whether rows of outputs start on 64-byte lines.
+bool on_lines(const MatArgs& p) {
+  const int bytes = p.out_type == TRS_F32 ? 4 : 2;
+  return ((reinterpret_cast<uintptr_t>(p.out) | (uintptr_t)(p.ldo * bytes)) & 63) == 0;
+}
+
 void launch_panel(const MatArgs& p, hipStream_t s) {
+  if (!on_lines(p) && p.n > kPanelColumns && p.n <= kMostWhole) {
+    switch ((p.blocks + 1) / 2) {
+      case 1: return launch_rows_panel<1>(p, s);
+      case 2: return launch_rows_panel<2>(p, s);
+      case 3: return launch_rows_panel<3>(p, s);
+      default: return launch_rows_panel<4>(p, s);
+    }
+  }
   switch ((p.blocks + 1) / 2) {
     case 1: return launch_panel<1>(p, s);
     case 2: return launch_panel<2>(p, s);
@@ -665,13 +792,16 @@ void launch_panel(const MatArgs& p, hipStream_t s) {
 //   8192 x 8192 x 8192                            460            293    253
 // (With scales off 4-byte boundaries tiles of 256 take up to a quarter longer, the others 2 to 5%.)
 //
-// The panel, us (2 H blocks a row; rows on 64-byte lines, or a wave's columns at most, or the lines that rows share cost twice):
+// The panel, us (k_mx4_rows_panel where rows are off 64-byte lines):
 //   m x n x k              panel   64     128    256
 //   1048576 x 64 x 128       32     50     68    102
 //   1048576 x 256 x 128     100    175    136    121
 //   1048576 x 256 x 192     130    246    179    247
 //   1048576 x 256 x 256     156    283    177    153
-//   1048576 x 300 x 128     342    332    269    265
+//   1048576 x 172 x 128     101    179    159    127
+//   1048576 x 300 x 128     162    288    239    231
+//   1048576 x 500 x 64      200    443    310    318
+//   1048576 x 257 x 256     265    277    236    236
 //   50000 x 512 x 200        13     22     19     22
 //   2000 x 4096 x 256        11     10      8     10
 //   3000 x 256 x 128        5.1    5.3    5.4    7.9
@@ -692,21 +822,21 @@ Choice choose(const MatArgs& p) {
     const double rows = p.m < 16 * f ? p.m : 16 * f, kb = (16 + rows) * p.blocks * 17e-3;
     offer({std::max(1.4 + 0.2 * f, 0.5 + ceil_div(tiles(p, 16 * f, 16), kCus) * std::max(0.3, kb / 32)), 0, 0, f});
   }
-  const int element = p.out_type == TRS_F32 ? 4 : 2;
-  const double mb = ((double)p.m * p.n * element + ((double)p.m + p.n) * p.blocks * 17) * 1e-6;   // 1 TB/s: a microsecond each
+  const bool lines = on_lines(p);
+  const double mb = ((double)p.m * p.n * (p.out_type == TRS_F32 ? 4 : 2) + ((double)p.m + p.n) * p.blocks * 17) * 1e-6;   // 1 TB/s: a microsecond each
   const int h = (p.blocks + 1) / 2;
-  const bool lines = ((reinterpret_cast<uintptr_t>(p.out) | (uintptr_t)(p.ldo * element)) & 63) == 0;
-  if (h >= 1 && h <= 4 && (lines || p.n <= kPanelColumns) && p.m < (int64_t)kPanelRows << 30) {
+  if (h >= 1 && h <= 4 && (lines || p.n <= kMostWhole) && p.m < (int64_t)kPanelRows << 30) {
     const double waves = std::min(1.0, ceil_div(p.m, kPanelRows) * ceil_div(p.n, kPanelColumns) / (16.0 * kCus));
-    offer({2.2 + 0.9 * h * waves + mb / (h <= 2 ? 6.0 : h == 3 ? 4.9 : 4.5), kPanelSide, 1, 0});
+    const double rate = lines || p.n <= kPanelColumns ? (h <= 2 ? 6.0 : h == 3 ? 4.9 : 4.5) : (h == 1 ? 5.0 : h == 2 ? 4.2 : h == 3 ? 3.6 : 2.8);
+    offer({2.2 + 0.9 * h * waves + mb / rate, kPanelSide, 1, 0});
   }
   if (!near) return best;
   const double rest = t64 % 4, fill = std::min(1.0, tiles(p, 64, 64) / (double)kCus);
   offer({t64 / 4 * (0.83 * steps + 2.2) + (rest == 0 ? 0 : rest == 1 ? (0.28 + 0.25 * fill) * steps + 0.6 : rest == 2 ? 0.55 * steps + 0.6 : 0.65 * steps + 0.8),
          64, 1, 0});
   if (t64 == 1 && steps >= 8) offer({2.9 + (0.13 + 0.11 * fill) * steps, 64, 4, 0});
-  offer({std::max(mb / 4.7, t128 / 2 * (1.03 * steps + 3.2) + t128 % 2 * (0.73 * steps + 2.1)), 128, 1, 0});
-  offer({std::max(mb / 5, t256 * (1.8 * steps + 5)), 256, 1, 0});
+  offer({std::max(mb / (lines ? 4.7 : 2.9), t128 / 2 * (1.03 * steps + 3.2) + t128 % 2 * (0.73 * steps + 2.1)), 128, 1, 0});
+  offer({std::max(mb / (lines ? 5 : 3.1), t256 * (1.8 * steps + 5)), 256, 1, 0});
   return best;
 }
 
