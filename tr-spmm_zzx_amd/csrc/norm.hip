@@ -662,15 +662,26 @@ void launch_norm(const NormArgs& p, hipStream_t s) {
   else k_norm_long<X, R, CODES><<<blocks(1), kThreads, 0, s>>>(p);
 }
 
+// Rows of more than 1024 values: a wave walks a whole row where its chunks leave registers for enough other waves, four
+// waves share it otherwise.  A row of four waves waits for its loads, for the others' sums and for its stores one after the
+// other, and no more than 8 rows are on a unit.  262144 rows, us, four waves / one:
+//   float16 x 1030   350 / 199    1374  364 / 215    2040  340 / 282    2500  525 / 424    4096  562 / 664
+//   float32 x 1030   363 / 261    1374  399 / 310    2040  439 / 465    2500  651 / 584    4096  910 / 906
+//   float16 + residual x 1374  556 / 445    2040  658 / 646 (16384 rows: 34 / 38)
+//   float32 + residual x 1374  884 / 876    2040 1271 / 1300
 template <class X, class R>
 void launch_mx4(const Mx4Args& p, hipStream_t s) {
   auto blocks = [&](int rows) { return dim3((uint32_t)ceil_div(p.n.rows, rows)); };
   const int w = p.n.width;
+  constexpr bool one = is_none<R>;
   if (w <= 64) k_norm_mx4<X, R, 8, 1><<<blocks(32), kThreads, 0, s>>>(p);
   else if (w <= 128) k_norm_mx4<X, R, 16, 1><<<blocks(16), kThreads, 0, s>>>(p);
   else if (w <= 256) k_norm_mx4<X, R, 32, 1><<<blocks(8), kThreads, 0, s>>>(p);
   else if (w <= 512) k_norm_mx4<X, R, 64, 1><<<blocks(4), kThreads, 0, s>>>(p);
   else if (w <= 1024 && p.n.rows >= 1024) k_norm_mx4<X, R, 64, 2><<<blocks(4), kThreads, 0, s>>>(p);
+  else if (w > 1024 && w <= 1536) k_norm_mx4<X, R, 64, 3><<<blocks(4), kThreads, 0, s>>>(p);
+  else if (w > 1536 && w <= 2048 && one && sizeof(typename X::raw) == 2) k_norm_mx4<X, R, 64, 4><<<blocks(4), kThreads, 0, s>>>(p);
+  else if (w > 2048 && w <= 2560 && one) k_norm_mx4<X, R, 64, 5><<<blocks(4), kThreads, 0, s>>>(p);
   else if (w <= 2048) k_norm_mx4<X, R, 256, 1><<<blocks(1), kThreads, 0, s>>>(p);
   else if (w <= 4096) k_norm_mx4<X, R, 256, 2><<<blocks(1), kThreads, 0, s>>>(p);
   else if (w <= kNormMost) k_norm_mx4<X, R, 256, 4><<<blocks(1), kThreads, 0, s>>>(p);
