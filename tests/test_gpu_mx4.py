@@ -405,6 +405,25 @@ def test_another_stream_and_a_graph():
         assert all(torch.equal(a, b) for a, b in zip(held, want)), turn
 
 
+def test_more_channels_than_a_walk_can_have():
+    """600,000,001 channels of one block: weights of 9.6 GB, addresses past 32 bits, more strips than a grid of panels holds."""
+    say("many channels")
+    n = 600_000_001
+    if torch.cuda.mem_get_info()[0] < 24e9:
+        pytest.skip("not enough memory")
+    w, sw = torch.zeros((n, 16), dtype=torch.uint8, device="cuda"), torch.full((n, 1), 127, dtype=torch.uint8, device="cuda")
+    a, sa = operand(2, 32, 1)
+    ends, scale = operand(300, 32, 3)
+    for at in (0, 268_435_300, n - 300):
+        w[at:at + 300], sw[at:at + 300] = ends, scale.view(torch.uint8)
+    got = trspmm.matmul_mx4(a, sa, w, sw, dtype=torch.float32)
+    want = product(a, sa, ends, scale).float()
+    for at in (0, 268_435_300, n - 300):
+        assert torch.equal(got[:, at:at + 300], want), at
+        got[:, at:at + 300] = 0
+    assert not bool(got.any())
+
+
 def test_equal_inputs_give_equal_bits():
     say("again")
     for m, n, k in [(1, 500, 4000), (50, 500, 4000), (900, 800, 700), (5000, 256, 128)]:

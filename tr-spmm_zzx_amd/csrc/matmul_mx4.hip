@@ -708,20 +708,32 @@ void launch_tile(const MatArgs& p, hipStream_t s) {
 
 int64_t tiles(const MatArgs& p, int tm, int tn) { return ceil_div(p.m, tm) * ceil_div(p.n, tn); }
 
+// Waves of a workgroup that share rows in the panel, and the workgroups that walk down the rows of `panels` such strips: four a CU by
+// their LDS, whole octets of them (one for each XCD), no more than there are tiles.
+int panel_waves(int n) { return n <= kPanelColumns ? 1 : n <= 2 * kPanelColumns ? 2 : 4; }
+int64_t panel_walkers(int64_t tiles_m, int cw, int64_t panels) {
+  const int64_t most = round_up(ceil_div(tiles_m, kPanelWaves / cw), 8), fit = round_up(ceil_div(4 * kCus, panels), 8);
+  return most < fit ? most : fit;
+}
+int64_t panel_blocks(int64_t tiles_m, int n) {
+  const int64_t panels = ceil_div(n, panel_waves(n) * kPanelColumns);
+  return panel_walkers(tiles_m, panel_waves(n), panels) * panels;
+}
+
 template <int H, int CW>
 void launch_panel(const MatArgs& p, hipStream_t s) {
   const uint32_t tm = (uint32_t)ceil_div(p.m, (int64_t)kPanelRows), panels = (uint32_t)ceil_div(p.n, CW * kPanelColumns);
-  // four workgroups a CU by their LDS, whole octets of them (one for each XCD), no more than there are tiles
-  const int64_t most = round_up(ceil_div(tm, kPanelWaves / CW), 8), fit = round_up(ceil_div(4 * kCus, panels), 8);
-  const uint32_t walkers = (uint32_t)(most < fit ? most : fit);
+  const uint32_t walkers = (uint32_t)panel_walkers(tm, CW, panels);
   k_mx4_panel<H, CW><<<dim3(walkers * panels), kPanelWaves * 64, 0, s>>>(p, tm, panels, walkers);
 }
 
 template <int H>
 void launch_panel(const MatArgs& p, hipStream_t s) {
-  if (p.n <= kPanelColumns) launch_panel<H, 1>(p, s);
-  else if (p.n <= 2 * kPanelColumns) launch_panel<H, 2>(p, s);
-  else launch_panel<H, 4>(p, s);
+  switch (panel_waves(p.n)) {
+    case 1: return launch_panel<H, 1>(p, s);
+    case 2: return launch_panel<H, 2>(p, s);
+    default: return launch_panel<H, 4>(p, s);
+  }
 }
 
 constexpr int kMostWhole = 2 * kPanelWaves * kPanelColumns;   // outputs of a row that a workgroup has together
@@ -825,7 +837,8 @@ Choice choose(const MatArgs& p) {
   const bool lines = on_lines(p);
   const double mb = ((double)p.m * p.n * (p.out_type == TRS_F32 ? 4 : 2) + ((double)p.m + p.n) * p.blocks * 17) * 1e-6;   // 1 TB/s: a microsecond each
   const int h = (p.blocks + 1) / 2;
-  if (h >= 1 && h <= 4 && (lines || p.n <= kMostWhole) && p.m < (int64_t)kPanelRows << 30) {
+  const bool fits = fits_grid(panel_blocks(ceil_div(p.m, kPanelRows), p.n));
+  if (fits && h >= 1 && h <= 4 && (lines || p.n <= kMostWhole) && p.m < (int64_t)kPanelRows << 30) {
     const double waves = std::min(1.0, ceil_div(p.m, kPanelRows) * ceil_div(p.n, kPanelColumns) / (16.0 * kCus));
     const double rate = lines || p.n <= kPanelColumns ? (h <= 2 ? 6.0 : h == 3 ? 4.9 : 4.5) : (h == 1 ? 5.0 : h == 2 ? 4.2 : h == 3 ? 3.6 : 2.8);
     offer({2.2 + 0.9 * h * waves + mb / rate, kPanelSide, 1, 0});
@@ -883,6 +896,7 @@ extern "C" int trs_matmul_mx4(const uint8_t* a, int64_t lda, const uint8_t* a_sc
   if (m < 0 || n < 0 || blocks < 0) return fail(TRS_EINVAL, where, "negative m, n or blocks");
   if (!known_type(out_type)) return fail(TRS_EINVAL, where, "unknown element type");
   if (blocks > kMostBlocks) return fail(TRS_ERANGE, where, "more than 2^26 blocks");
+  if (n > kMostWidth) return fail(TRS_ERANGE, where, "more than 2^31 - 65536 columns");
   if (m == 0 || n == 0) return TRS_OK;
   if (!out || (blocks > 0 && (!a || !w || !a_scale || !w_scale))) return fail(TRS_EINVAL, where, "NULL operand");
   const int64_t row = (int64_t)blocks * kBlockBytes;
