@@ -557,7 +557,7 @@ int trs_rms_norm_mx4(const void* x, int32_t x_type, int64_t ldx, const void* res
                      uint8_t* scale, int64_t lds, void* r_out, int64_t ldro, void* stream);
 
 /* out[i, j] = sum over the blocks of a's row i times w's row j + bias[j], the values that codes and scales stand for: a
- * [m, blocks], w [n, blocks]; lda, ldw are rows of codes, ldas, ldws rows of scales, in bytes; bias float32 or NULL.  Codes
+ * [m, blocks], w [n, blocks]; lda, ldw are rows of codes, ldas, ldws rows of scales, in bytes; bias float32 or NULL; n at most 2^31 - 65536.  Codes
  * past a row's width take part: trs_quant_mx4 and trs_rms_norm_mx4 write zeros there.  Sums in 32 bits, in an order that the
  * sizes alone decide.  blocks at most 2^26 (TRS_ERANGE). */
 int trs_matmul_mx4(const uint8_t* a, int64_t lda, const uint8_t* a_scale, int64_t ldas, const uint8_t* w, int64_t ldw,
@@ -599,8 +599,7 @@ typedef struct trs_adamw_options {
 
 void trs_adamw_options_default(trs_adamw_options* options);
 
-/* TRS_EINVAL also for buffers that are written and overlap (a tensor named twice); gradients must not overlap them
- * either.  A tensor has at most some 1.7e10 elements (TRS_ERANGE). */
+/* TRS_EINVAL also for buffers that are written and overlap each other (a tensor named twice) or a gradient.  A tensor has at most some 1.7e10 elements (TRS_ERANGE). */
 int trs_adamw(const trs_adamw_tensor* tensors, int64_t count, const trs_adamw_options* options, void* stream);
 
 const char* trs_last_error(void);

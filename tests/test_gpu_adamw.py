@@ -347,13 +347,16 @@ def test_refusals():
                        (([p], [g], [s]), {"copies": []}), (([p], [g], [s]), {"copies": [half.int()]}),
                        (([p], [g], [s]), {"lr": torch.ones(2, device="cuda")}), (([p], [g], [s]), {"lr": half[:1]}),
                        (([p], [g], [s]), {"skip": torch.ones(1, dtype=torch.int32, device="cuda")}),
-                       (([p], [g], [s]), {"grad_scale": torch.ones(1)})]:
+                       (([p], [g], [s]), {"grad_scale": torch.ones(1)}), (([p], [None], [s]), {}), (([p], [g], [s]), {"seed": -1}),
+                       (([p], [g], [s]), {"seed": 2 ** 32}), (([p], [g], [s]), {"lr": "1"}), (([p], [g], [s]), {"weight_decay": "1"}),
+                       (([p], [g], [s]), {"weight_decay": [None]})]:
         with pytest.raises(ValueError):
             trspmm.adamw(*args, 1, **more)
     other = trspmm.adamw_state(p)
     for args, more in [(([p, p], [g, g], [s, other]), {}), (([p, half], [g, g], [s, s]), {}), (([p], [g], [(s.m, s.m)]), {}),
                        (([p[:60], p[40:]], [g[:60], g[40:]], [trspmm.adamw_state(p[:60]), trspmm.adamw_state(p[40:])]), {}),
-                       (([p], [g], [s]), {"copies": [p]}), (([p], [g], [s]), {"betas": (1.0, 0.9)}), (([p], [g], [s]), {"betas": (0.9, -0.1)}),
+                       (([p], [g], [s]), {"copies": [p]}), (([p], [g], [s]), {"copies": [g]}), (([p], [p], [s]), {}), (([p], [s.v], [s]), {}),
+                       (([p], [g], [s]), {"betas": (1.0, 0.9)}), (([p], [g], [s]), {"betas": (0.9, -0.1)}),
                        (([p], [g], [s]), {"eps": 0.0}), (([p], [g], [s]), {"lr": float("nan")}), (([p], [g], [s]), {"weight_decay": float("inf")}),
                        (([p], [g], [s]), {"grad_scale": float("inf")})]:
         with pytest.raises(nat.TrsError):
@@ -363,5 +366,34 @@ def test_refusals():
     with pytest.raises(ValueError):
         trspmm.adamw([p], [g], [s], torch.ones(1, device="cuda"))
     with pytest.raises(ValueError):
+        trspmm.adamw([p], [g], [s], 1.5)
+    with pytest.raises(ValueError):
         trspmm.adamw_state(p, 16)
     assert bool((p == 1).all()) and bool((s.m == 0).all())
+
+
+def test_numbers_of_other_kinds_and_a_shared_gradient():
+    say("numpy numbers, shared gradient")
+    g = rand((1000,), torch.float32, 1)
+    first, second, third = (rand((1000,), torch.float32, 2) for _ in range(3))
+    states = [trspmm.adamw_state(first) for _ in range(3)]
+    trspmm.adamw([first, second], [g, g], states[:2], np.int64(1), np.float32(0.125), weight_decay=np.float32(0.25), grad_scale=np.float64(0.5))
+    trspmm.adamw((third,), (g,), states[2:], 1, 0.125, weight_decay=(0.25,), grad_scale=0.5)
+    assert torch.equal(first, third) and torch.equal(second, third)
+
+
+def test_autograd_sees_the_change():
+    """A backward pass through what was saved of a parameter before the step is refused, as after torch's own in-place operations."""
+    say("versions")
+    p = rand((64,), torch.float32, 1).requires_grad_()
+    copy = p.detach().clone().requires_grad_()
+    loss, other = (p * p).sum(), (copy * copy).sum()
+    g = torch.ones(64, device="cuda")
+    trspmm.adamw([p], [g], [trspmm.adamw_state(p)], 1, copies=[copy])
+    for x in (loss, other):
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            x.backward()
+    with torch.inference_mode():
+        q = torch.ones(64, device="cuda")
+        trspmm.adamw([q], [g], [trspmm.adamw_state(q)], 1)
+    assert bool((q != 1).all())

@@ -52,7 +52,7 @@ def test_columns_past_the_grid_or_32_bits_are_refused(width):
         assert lib.trs_rms_norm_mx4(*{**NORM, **wide, "ldx": FAR, "ldr": FAR, "ldro": FAR}.values()) == 5
 
 
-@pytest.mark.parametrize("m,n", [(1 << 41, 2 ** 31 - 1), (1 << 62, 2 ** 31 - 1), (1 << 40, 1), (64, 2 ** 31 - 1), (1 << 36, 64)])
+@pytest.mark.parametrize("m,n", [(1 << 41, 2 ** 31 - 1), (1 << 62, 2 ** 31 - 1), (1 << 40, 1), (64, 2 ** 31 - 1), (1 << 36, 64), (1, 2 ** 31 - 65535)])
 def test_products_past_a_launch_are_refused(m, n):
     lib = nat.lib()
     assert lib.trs_matmul_mx4(*{**MATMUL, "m": m, "n": n, "ldo": n}.values()) == 5, lib.trs_last_error()
@@ -118,11 +118,14 @@ def test_adamw_overlaps_refused():
     far = dict(param=X + 4096, m=X + 8192, v=X + 12288)
     for tensors in ([tensor(), tensor()], [tensor(), tensor(**{**far, "param": X + 36})], [tensor(m=X + 36)], [tensor(v=X)],
                     [tensor(copy=X + 39)], [tensor(m_scale=X + 513, v_scale=X + 4096)], [tensor(m_scale=X + 4096, v_scale=X + 4096)],
-                    [tensor(), tensor(**{**far, "m": X + 1063})]):
+                    [tensor(), tensor(**{**far, "m": X + 1063})], [tensor(grad=X + 36)], [tensor(grad=X + 1063)], [tensor(copy=X + 295)],
+                    [tensor(), tensor(**far, grad=X + 4000, count=100)]):
         assert adamw(tensors, options()) == 1
         assert b"overlaps" in nat.lib().trs_last_error()
     many = [tensor(param=X + 100_000 * i, m=X + 100_000 * i + 400, v=X + 100_000 * i + 800) for i in range(400)]
     many[399].v = many[7].m + 4
+    assert adamw(many, options()) == 1 and b"overlaps" in nat.lib().trs_last_error()
+    many[399].v, many[5].grad = many[398].v + 100_000, many[300].m + 39
     assert adamw(many, options()) == 1 and b"overlaps" in nat.lib().trs_last_error()
 
 

@@ -261,12 +261,12 @@ int bytes_of(int type) { return type == TRS_F32 ? 4 : 2; }
 int kind_of(int p_type, int g_type, bool small) { return (p_type * 3 + g_type) * 2 + small; }
 int kind_of(const trs_adamw_tensor& t) { return kind_of(t.param_type, t.grad_type, t.m_scale != nullptr); }
 
-// Whether two of the buffers that the call writes share a byte.  Sorted by their first byte, as a call over hundreds of tensors
+// Whether two of the n buffers that the call writes share a byte, or one of them and one that it only reads.  Sorted by their first byte, as a call over hundreds of tensors
 // is bound by what the host does: by 11 bits of the distance from the lowest at a time, in steps of 2^(bits - 33), then what those steps left.
 struct Range { uintptr_t first, end; };
 constexpr int kDigit = 11, kDigits = 3;
 
-bool overlap(Range* r, Range* spare, int64_t n) {
+bool overlap(Range* r, Range* spare, int64_t n, const Range* read, int64_t reads) {
   auto before = [](const Range& x, const Range& y) { return x.first < y.first; };
   if (n <= 64) {
     std::sort(r, r + n, before);
@@ -289,6 +289,10 @@ bool overlap(Range* r, Range* spare, int64_t n) {
   }
   for (int64_t i = 1; i < n; ++i)
     if (r[i].first < r[i - 1].end) return true;
+  for (int64_t i = 0; i < reads; ++i) {   // the last one that starts before its end
+    const Range* after = std::lower_bound(r, r + n, read[i].end, [](const Range& x, uintptr_t at) { return x.first < at; });
+    if (after > r && after[-1].end > read[i].first) return true;
+  }
   return false;
 }
 
@@ -325,7 +329,7 @@ extern "C" int trs_adamw(const trs_adamw_tensor* tensors, int64_t count, const t
   if (!o->step_device && o->step < 1) return fail(TRS_EINVAL, where, "steps count from 1");
   if (count == 0) return TRS_OK;
   if (!tensors) return fail(TRS_EINVAL, where, "NULL tensors");
-  int64_t written = 0;
+  int64_t written = 0, read = 0;
   uint32_t kinds = 0;   // the combinations of types there are
   for (int64_t i = 0; i < count; ++i) {
     const trs_adamw_tensor& t = tensors[i];
@@ -339,32 +343,35 @@ extern "C" int trs_adamw(const trs_adamw_tensor* tensors, int64_t count, const t
     if (ceil_div(t.count, elements_of(t.m_scale != nullptr)) > kMostBlocks) return fail(TRS_ERANGE, where, "a tensor needs more workgroups than a launch can have");
     kinds |= 1u << kind_of(t);
     written += 3 + (t.m_scale ? 2 : 0) + (t.copy ? 1 : 0);
+    ++read;
   }
   if (written == 0) return TRS_OK;
-  Range few[64];
-  Range* ranges = written <= 64 ? few : new (std::nothrow) Range[2 * written];
+  Range few[64];   // the written ones, the read ones, and room to sort more than 64
+  const bool small_call = written + read <= 64;
+  Range* ranges = small_call ? few : new (std::nothrow) Range[2 * written + read];
   if (!ranges) return fail(TRS_ENOMEM, where, "out of memory");
-  int64_t r = 0;
-  auto add = [&](const void* p, int64_t bytes) {
+  int64_t w = 0, r = written;
+  auto range = [](const void* p, int64_t bytes) {
     const uintptr_t a = reinterpret_cast<uintptr_t>(p);
-    ranges[r++] = Range{a, a + (uintptr_t)bytes};
+    return Range{a, a + (uintptr_t)bytes};
   };
   for (int64_t i = 0; i < count; ++i) {
     const trs_adamw_tensor& t = tensors[i];
     if (t.count == 0) continue;
     const int state = t.m_scale ? 1 : 4;
-    add(t.param, t.count * bytes_of(t.param_type));
-    add(t.m, t.count * state);
-    add(t.v, t.count * state);
+    ranges[w++] = range(t.param, t.count * bytes_of(t.param_type));
+    ranges[w++] = range(t.m, t.count * state);
+    ranges[w++] = range(t.v, t.count * state);
     if (t.m_scale) {
-      add(t.m_scale, blocks_of(t.count));
-      add(t.v_scale, blocks_of(t.count));
+      ranges[w++] = range(t.m_scale, blocks_of(t.count));
+      ranges[w++] = range(t.v_scale, blocks_of(t.count));
     }
-    if (t.copy) add(t.copy, t.count * bytes_of(t.copy_type));
+    if (t.copy) ranges[w++] = range(t.copy, t.count * bytes_of(t.copy_type));
+    ranges[r++] = range(t.grad, t.count * bytes_of(t.grad_type));
   }
-  const bool shared = overlap(ranges, ranges + written, r);
-  if (ranges != few) delete[] ranges;
-  if (shared) return fail(TRS_EINVAL, where, "a parameter, state or copy is named twice or overlaps another");
+  const bool shared = overlap(ranges, ranges + written + read, written, ranges + written, read);
+  if (!small_call) delete[] ranges;
+  if (shared) return fail(TRS_EINVAL, where, "a parameter, state or copy is named twice, or overlaps another or a gradient");
 
   const double t = (double)o->step;
   Args a;

@@ -360,6 +360,16 @@ const T* one_of(const char* name, const py::object& x, at::ScalarType type, int6
   return static_cast<const T*>(t.data_ptr());
 }
 
+template <class T>
+T number(const char* name, const char* what, const py::object& x) {
+  try {
+    return x.cast<T>();
+  } catch (const py::cast_error&) {
+    wrong(std::string(name) + " must be " + what);
+  }
+  return T();
+}
+
 bool is_tensor(const py::object& x) { return THPVariable_Check(x.ptr()); }
 
 // A sequence's items without a cast of each: a list of some hundred tensors is walked in every step.
@@ -393,7 +403,7 @@ void* flat(const char* name, size_t i, const Tensor& t, int64_t n) {
 
 void adamw(const py::object& params_in, const py::object& grads_in, const py::object& states_in, const py::object& step,
            const py::object& lr, std::pair<double, double> betas, double eps, const py::object& decay, const py::object& copies_in,
-           const py::object& grad_scale, const Given& skip, uint32_t seed, int64_t dev, int64_t stream) {
+           const py::object& grad_scale, const Given& skip, int64_t seed, int64_t dev, int64_t stream) {
   const Items params("params must be a sequence of tensors", params_in), grads("grads must be a sequence of tensors", grads_in),
       states("states must be a sequence", states_in);
   const size_t count = params.size();
@@ -402,16 +412,19 @@ void adamw(const py::object& params_in, const py::object& grads_in, const py::ob
   trs_adamw_options o;
   trs_adamw_options_default(&o);
   if (is_tensor(lr)) o.lr_device = one_of<float>("lr", lr, at::kFloat, dev);
-  else o.lr = lr.cast<double>();
+  else o.lr = number<double>("lr", "a number or a tensor", lr);
   if (is_tensor(step)) o.step_device = one_of<int64_t>("step", step, at::kLong, dev);
-  else o.step = step.cast<int64_t>();
+  else o.step = number<int64_t>("step", "an integer or a tensor", step);
   if (is_tensor(grad_scale)) o.grad_scale_device = one_of<float>("grad_scale", grad_scale, at::kFloat, dev);
-  else o.grad_scale = grad_scale.cast<double>();
+  else o.grad_scale = number<double>("grad_scale", "a number or a tensor", grad_scale);
   if (skip) o.skip = one_of<float>("skip", py::cast(*skip), at::kFloat, dev);
-  o.beta1 = betas.first, o.beta2 = betas.second, o.eps = eps, o.seed = seed;
-  const bool each = !py::isinstance<py::float_>(decay) && !py::isinstance<py::int_>(decay);
-  const double decay_all = each ? 0.0 : decay.cast<double>();
-  const std::vector<double> decays = each ? decay.cast<std::vector<double>>() : std::vector<double>();
+  o.beta1 = betas.first, o.beta2 = betas.second, o.eps = eps;
+  if (seed < 0 || seed > (int64_t)UINT32_MAX) wrong("seed must be in 0 .. 2^32 - 1");
+  o.seed = (uint32_t)seed;
+  const bool each = PySequence_Check(decay.ptr());
+  const char* const numbers = "a number, or one for each of the params";
+  const double decay_all = each ? 0.0 : number<double>("weight_decay", numbers, decay);
+  const std::vector<double> decays = each ? number<std::vector<double>>("weight_decay", numbers, decay) : std::vector<double>();
   if (each && decays.size() != count) wrong("weight_decay must be a number, or one for each of the params");
   std::optional<Items> copies;
   if (!copies_in.is_none()) copies.emplace("copies must be a sequence of tensors", copies_in);
@@ -459,6 +472,15 @@ void adamw(const py::object& params_in, const py::object& grads_in, const py::ob
     }
   }
   ok(trs_adamw(list.data(), (int64_t)count, &o, stream_of(stream)), "trs_adamw");
+  // Autograd refuses a backward pass through what it saved of them before.
+  auto changed = [](PyObject* x) {
+    const Tensor& t = THPVariable_Unpack(x);
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  };
+  for (size_t i = 0; i < count; ++i) {
+    changed(params[i]);
+    if (copies && (*copies)[i] != Py_None) changed((*copies)[i]);
+  }
 }
 
 }  // namespace
