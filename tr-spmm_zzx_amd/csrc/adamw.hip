@@ -231,8 +231,8 @@ __global__ __launch_bounds__(kThreads) void k_adamw(Args a) {
 // ---------------------------------------------------------------------------------------------
 // Host side.
 
-// Rounds of a workgroup: 2 with 8-bit states, whose loads are short (85 M elements in 148 tensors 290 us, 310 with 1), 1 with 32-bit
-// ones (2^27 elements 660 us, 704 with 2, 695 with 4).
+// Rounds of a workgroup: 2 with 8-bit states, whose loads are short (85 M elements in 148 tensors 290 us, 310 with 1), 1 with
+// 32-bit ones (2^27 elements 660 us, 704 with 2, 695 with 4).
 constexpr int unroll_of(bool small) { return small ? 2 : 1; }
 constexpr int64_t elements_of(bool small) { return (int64_t)kThreads * kVec * unroll_of(small); }
 constexpr int64_t kMostBlocks = UINT32_MAX / kThreads;
@@ -261,8 +261,9 @@ int bytes_of(int type) { return type == TRS_F32 ? 4 : 2; }
 int kind_of(int p_type, int g_type, bool small) { return (p_type * 3 + g_type) * 2 + small; }
 int kind_of(const trs_adamw_tensor& t) { return kind_of(t.param_type, t.grad_type, t.m_scale != nullptr); }
 
-// Whether two of the n buffers that the call writes share a byte, or one of them and one that it only reads.  Sorted by their first byte, as a call over hundreds of tensors
-// is bound by what the host does: by 11 bits of the distance from the lowest at a time, in steps of 2^(bits - 33), then what those steps left.
+// Whether two of the n buffers that the call writes share a byte, or one of them and one that it only reads.  Sorted by their
+// first byte, as a call over hundreds of tensors is bound by what the host does: by 11 bits of the distance from the lowest at a
+// time, in steps of 2^(bits - 33), then what those steps left.
 struct Range { uintptr_t first, end; };
 constexpr int kDigit = 11, kDigits = 3;
 

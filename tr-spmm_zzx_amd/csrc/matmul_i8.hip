@@ -73,6 +73,11 @@ __device__ __forceinline__ int4_v load_codes(const int8_t* row, int at, int k) {
   return settle(load16<ODD>(row + start_of(at, k)), at, k);
 }
 
+// A wave's sums, 32 rows and (up to) 64 columns at a time, through LDS (a wave's own part: `lds`, 32 rows of
+// kOutPitch integers), so that a lane holds 8 neighbouring columns of a row, and rows leave in whole vectors.
+template <int FN>
+constexpr int kOutPitch = (FN > 1 ? 64 : 32) + 4;
+
 // The scales of the rows that a lane of store_wave writes, read together: one wait for all.
 template <int FM, int FN>
 struct RowScales {
@@ -89,8 +94,6 @@ struct RowScales {
   }
 };
 
-// A wave's sums, 32 rows and (up to) 64 columns at a time, through LDS (a wave's own part: `lds`, 32 rows of
-// kOutPitch integers), so that a lane holds 8 neighbouring columns of a row, and rows leave in whole vectors.
 template <int FM, int FN>
 __device__ __forceinline__ void store_wave(const MatArgs& p, const int16_v (&acc)[FM][FN], const RowScales<FM, FN>& sa, int* lds,
                                            int64_t m0, int n0, int lane) {
@@ -163,6 +166,12 @@ __device__ __forceinline__ void store_wave(const MatArgs& p, const int16_v (&acc
 // the card holds under them), 2% of the LDS cycles lost to conflicts.  A wave owns 128 x 64 of a 256 x 256 tile; with
 // 64 x 64 (a tile of 256 x 128) it reads more LDS for each product (645 us), 128 x 128 spilled registers (2375).
 constexpr int kDepth = 128;
+
+// A buffer that ends with the operand's last code.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t operand(const int8_t* from, int64_t rows, int64_t ld, int k) {
+  const int64_t bytes = (rows - 1) * ld + k;
+  return buffer_of(from, (uint32_t)(bytes < UINT32_MAX ? bytes : UINT32_MAX));
+}
 
 template <int TM, int TN, int WM, int WN, int KS, bool DIRECT, class Offset>
 __device__ __forceinline__ void matmul_tile(const MatArgs& p, uint32_t tiles_m, uint32_t tiles_n) {

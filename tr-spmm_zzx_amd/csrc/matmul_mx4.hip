@@ -120,16 +120,17 @@ __global__ __launch_bounds__(1024) void k_mx4_rows(MatArgs p, uint32_t blocks_n)
 
 // ---------------------------------------------------------------------------------------------
 // Tiles: TM x TN outputs a workgroup, WM x WN a wave, 256 codes of k (8 blocks, 128 bytes of a row) a step, the next step's
-// operands on their way from memory to LDS while this one's are multiplied.  Piece (block) c of row r lies in place
-// c ^ (r / 2 & 7), so that the 16-byte reads of neighbouring rows spread over the banks.  The upper 32 lanes take the step's last four
+// operands on their way from memory to LDS while this one's are multiplied.  Piece (block) c of row r lies in place c ^ (r / 2 &
+// 7), so that the 16-byte reads of neighbouring rows spread over the banks.  The upper 32 lanes take the step's last four
 // blocks, so a lane's four scales of a step are one word; scales come 32 to a row, for four steps.
 //
-// Bound by arithmetic and by how soon the next step's operands arrive: 8192 x 8192 x 8192 253 to 262 us by card, 4.2 PFLOP/s.  Each quarter of a step is read from LDS
-// while the one before is multiplied, scales among the first reads.
+// Bound by arithmetic and by how soon the next step's operands arrive: 8192 x 8192 x 8192 253 to 262 us by card, 4.2 PFLOP/s.
+// Each quarter of a step is read from LDS while the one before is multiplied, scales among the first reads.
 //
 // ALIGNED: scales' rows on 4-byte boundaries; they go from memory to LDS without registers, as the codes do.  Others come by the
-// words that hold them (loads off those boundaries took a third of the time: 8192^3 with 257 scales between rows 409 us).  KS groups of
-// waves split a workgroup's steps, each with its own tiles, and the first adds the sums up: for few workgroups and a long k.
+// words that hold them (loads off those boundaries took a third of the time: 8192^3 with 257 scales between rows 409 us).  KS
+// groups of waves split a workgroup's steps, each with its own tiles, and the first adds the sums up: for few workgroups and a
+// long k.
 constexpr int kDepth = 128;        // bytes of a row in a step
 constexpr int kStepBlocks = kDepth / kBlockBytes, kPair = 2 * kStepBlocks, kSlots = 4;
 constexpr int kPastEnd = (int)0x80000000u;   // an offset, or a part of one, past every buffer of a tile's rows
@@ -145,8 +146,8 @@ __device__ __forceinline__ float16_v multiply32(int4_v w, int w_scale, int4_v a,
 // Sums pass through LDS, 32 rows of each wave at a time, so that a lane holds 8 neighbouring columns of a row and rows leave in
 // whole vectors, rounded on the way in.  Instructions that run once cost a fetch each, so what need not be unrolled is not.
 
-// Rows of an output that lie in LDS from `lds` on, `pitch` elements apart, 8 columns (from `first` on) of one of them in this lane, to row
-// m and column n0 + first on.
+// Rows of an output that lie in LDS from `lds` on, `pitch` elements apart, 8 columns (from `first` on) of one of them in this
+// lane, to row m and column n0 + first on.
 template <class T>
 __device__ __forceinline__ void store_piece(const MatArgs& p, const typename T::raw* lds, int first, int64_t m, int n0) {
   using raw = typename T::raw;
@@ -315,8 +316,9 @@ __device__ __forceinline__ void mx4_tile(const MatArgs& p, uint32_t tiles_m, uin
     if (step + 1 < steps || last == kStepBlocks) load(0);
     else load(my_piece < last ? 0 : kPastEnd);
   };
-  // The scales of two pairs of steps, `pair` (of the group's) and the next: the memory's line that holds a row's is read once for both.
-  // What follows a row's scales comes with them, and is cleared in LDS before a short last step (zeros times a NaN's scale would be NaN).
+  // The scales of two pairs of steps, `pair` (of the group's) and the next: the memory's line that holds a row's is read once
+  // for both. What follows a row's scales comes with them, and is cleared in LDS before a short last step (zeros times a NaN's
+  // scale would be NaN).
   auto place_of_scales = [&](int pair, int u) {
     return reinterpret_cast<int4_v*>(lds + group * kGroup + 2 * kTile + ((pair & (kSlots - 1)) * kRows + u * kAll + thread) * kPair);
   };
@@ -362,8 +364,8 @@ __device__ __forceinline__ void mx4_tile(const MatArgs& p, uint32_t tiles_m, uin
   // Two sets of fragments: one is read from LDS while the other is multiplied.
   int4_v fa[2][FM] = {}, fw[2][FN] = {};
   int sa[2][FM] = {}, sw[2][FN] = {};   // of even and odd steps
-  // Where the lane's first pieces and scales lie; the others lie at whole distances, and piece 4 half + h at an exclusive or with h.
-  // `at` hides them from the compiler in each step: it would hold all their sums in registers, which the products need.
+  // Where the lane's first pieces and scales lie; the others lie at whole distances, and piece 4 half + h at an exclusive or
+  // with h. `at` hides them from the compiler in each step: it would hold all their sums in registers, which the products need.
   const int first_piece = ((4 * half) ^ swz) * kBlockBytes;
   const int of_a = group * kGroup + (wm + row) * kDepth + first_piece, of_w = group * kGroup + (TM + wn + row) * kDepth + first_piece;
   const int of_sa = group * kGroup + 2 * kTile + (wm + row) * kPair + 4 * half, of_sw = of_sa + (TM + wn - wm) * kPair;
@@ -495,10 +497,11 @@ __global__ __launch_bounds__((TM / WM) * (TN / WN) * 64 * KS, WM * WN > 8192 ? 1
 
 // ---------------------------------------------------------------------------------------------
 // Short rows (k of at most 256) and many of them: outputs are the bytes that count.  A wave keeps the codes of 64 channels in
-// registers and walks tiles of 32 rows, whose codes go from memory to registers as the matrix instruction takes them, the next tile's on
-// their way while this one's outputs pass through the wave's own part of LDS.  Bound by memory: 2^20 x 256 x 128 100 us, 0.61 GB at 6.0
-// TB/s (tiles of 256: 121); from k = 192 on by the loads' 16-byte pieces of rows (k = 256: 156 us, 4.4 TB/s).  The waves of a workgroup share rows (CW of them,
-// whose loads meet in the L1) or channels; they never wait for one another.  H: blocks of a half of a wave, 2 H for a row.
+// registers and walks tiles of 32 rows, whose codes go from memory to registers as the matrix instruction takes them, the next
+// tile's on their way while this one's outputs pass through the wave's own part of LDS.  Bound by memory: 2^20 x 256 x 128 100
+// us, 0.61 GB at 6.0 TB/s (tiles of 256: 121); from k = 192 on by the loads' 16-byte pieces of rows (k = 256: 156 us, 4.4
+// TB/s).  The waves of a workgroup share rows (CW of them, whose loads meet in the L1) or channels; they never wait for one
+// another.  H: blocks of a half of a wave, 2 H for a row.
 constexpr int kPanelWaves = 4, kPanelRows = kOutRows, kPanelColumns = kOutColumns;
 // The blocks of a row that a lane takes: H of them from H half on; the last one may not be there.
 template <int H>
@@ -618,9 +621,9 @@ __global__ __launch_bounds__(kPanelWaves * 64, 4) void k_mx4_panel(MatArgs p, ui
   mx4_panel<H, CW>(p, tiles_m, panels, walkers);
 }
 
-// The same for rows of up to 256 GW outputs that do not start on 64-byte lines.  Lines that a row shares with the next are written in
-// parts, which costs a read of them if the other part does not follow at once: so a workgroup has whole rows of outputs in LDS and
-// its waves write them one after another (2^20 x 300 x 128: 64 columns at a time 342 us).
+// The same for rows of up to 256 GW outputs that do not start on 64-byte lines.  Lines that a row shares with the next are
+// written in parts, which costs a read of them if the other part does not follow at once: so a workgroup has whole rows of
+// outputs in LDS and its waves write them one after another (2^20 x 300 x 128: 64 columns at a time 342 us).
 template <class T, int H, int GW>
 __device__ __forceinline__ void store_rows(const MatArgs& p, const float16_v (&acc)[GW][1][2], uint8_t* lds_bytes_, int64_t m0, int wave, int lane,
                                            int pieces, uint32_t inverse) {
@@ -708,8 +711,8 @@ void launch_tile(const MatArgs& p, hipStream_t s) {
 
 int64_t tiles(const MatArgs& p, int tm, int tn) { return ceil_div(p.m, tm) * ceil_div(p.n, tn); }
 
-// Waves of a workgroup that share rows in the panel, and the workgroups that walk down the rows of `panels` such strips: four a CU by
-// their LDS, whole octets of them (one for each XCD), no more than there are tiles.
+// Waves of a workgroup that share rows in the panel, and the workgroups that walk down the rows of `panels` such strips: four a
+// CU by their LDS, whole octets of them (one for each XCD), no more than there are tiles.
 int panel_waves(int n) { return n <= kPanelColumns ? 1 : n <= 2 * kPanelColumns ? 2 : 4; }
 int64_t panel_walkers(int64_t tiles_m, int cw, int64_t panels) {
   const int64_t most = round_up(ceil_div(tiles_m, kPanelWaves / cw), 8), fit = round_up(ceil_div(4 * kCus, panels), 8);

@@ -22,11 +22,6 @@ __device__ __forceinline__ void barrier_and_wait() {
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void* from, uint32_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(from), 0, (int)bytes, 0x00020000);
 }
-// One of `rows` rows of `bytes` bytes that ends with the last row's last byte.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t operand(const void* from, int64_t rows, int64_t ld, int bytes) {
-  const int64_t all = (rows - 1) * ld + bytes;
-  return buffer_of(from, (uint32_t)(all < UINT32_MAX ? all : UINT32_MAX));
-}
 
 // Workgroup b of `total` as a tile: the workgroups of one XCD (b mod 8) take neighbouring tiles, in bands of 8
 // rows of tiles, so that an XCD's L2 serves the operands they share.
@@ -39,10 +34,6 @@ __device__ __forceinline__ void tile_of(uint32_t b, uint32_t tiles_m, uint32_t t
   tm = first + in % high;
   tn = in / high;
 }
-
-// A wave's sums pass through LDS 32 rows and (up to) 64 columns at a time, in rows of kOutPitch words.
-template <int FN>
-constexpr int kOutPitch = (FN > 1 ? 64 : 32) + 4;
 
 }  // namespace dense
 }  // namespace trs
