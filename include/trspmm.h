@@ -12,7 +12,7 @@
  * hipStream_t (NULL = the default stream).  fp16 data is passed as uint16_t bit patterns.
  *
  * Versioning
- *   Parameter structs (trs_build_params, trs_reorder_params, trs_plan_options) start with
+ *   Parameter structs (trs_build_params, trs_reorder_params, trs_plan_options, trs_adamw_options) start with
  *   `struct_size`, which their *_default initialiser sets to sizeof the struct of this header.
  *   Every entry point that reads such a struct refuses a struct_size other than the library's
  *   with TRS_EINVAL, before it reads anything past that first field, so a caller compiled against
@@ -558,8 +558,8 @@ int trs_rms_norm_mx4(const void* x, int32_t x_type, int64_t ldx, const void* res
 
 /* out[i, j] = sum over the blocks of a's row i times w's row j + bias[j], the values that codes and scales stand for: a
  * [m, blocks], w [n, blocks]; lda, ldw are rows of codes, ldas, ldws rows of scales, in bytes; bias float32 or NULL; n at most 2^31 - 65536.  Codes
- * past a row's width take part: trs_quant_mx4 and trs_rms_norm_mx4 write zeros there.  Sums in 32 bits, in an order that the
- * sizes alone decide.  blocks at most 2^26 (TRS_ERANGE). */
+ * past a row's width take part: trs_quant_mx4 and trs_rms_norm_mx4 write zeros there.  Sums in 32 bits, in an order that
+ * sizes, types, strides and addresses' alignment decide.  blocks at most 2^26 (TRS_ERANGE). */
 int trs_matmul_mx4(const uint8_t* a, int64_t lda, const uint8_t* a_scale, int64_t ldas, const uint8_t* w, int64_t ldw,
                    const uint8_t* w_scale, int64_t ldws, const float* bias, int64_t m, int32_t n, int32_t blocks, void* out,
                    int32_t out_type, int64_t ldo, void* stream);

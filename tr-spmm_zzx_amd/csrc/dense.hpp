@@ -1,5 +1,5 @@
-// Shared by the dense operators beside the sparse products (embed.hip, norm.hip, matmul_i8.hip):
-// element types, eight-element chunks of a row at any address, argument checks.
+// Shared by the dense operators beside the sparse products (embed.hip, norm.hip, matmul_i8.hip, mx4.hip,
+// matmul_mx4.hip, adamw.hip): element types, eight-element chunks of a row at any address, argument checks.
 //
 // Rows are handled in chunks of 8 elements.  A row whose width 8 does not divide ends in a chunk that
 // starts at width - 8 and overlaps its neighbour: both compute the same values for the shared
