@@ -244,13 +244,13 @@ MIXES = [(x, r) for x in TYPES for r in [None, *TYPES] if r is None or r is x or
 @pytest.mark.parametrize("w_type", TYPES)
 def test_norm_types(x_type, r_type, w_type):
     say("norm types", x_type, r_type, w_type)
-    for rows, width in [(37, 96), (9, 1000), (5, 1800), (6, 2300)]:
+    for rows, width in [(37, 96), (9, 1000), (5, 1800), (6, 2300), (5, 4500)]:
         x, w = rand((rows, width), x_type, 1), (1 + 0.2 * rand((width,), torch.float32, 2)).to(w_type)
         res = None if r_type is None else rand((rows, width), r_type, 3, 2.0)
         check_norm(x, w, res, *trspmm.rms_norm_mx4(x, w, res, EPS))
 
 
-@pytest.mark.parametrize("width", [*WIDTHS, 127, 512, 513, 1023, 1024, 1025, 1374, 1536, 1537, 2100, 2560, 2561, 4097, 8191, 8192, 8193, 12_001, 20_000])
+@pytest.mark.parametrize("width", [*WIDTHS, 127, 512, 513, 1023, 1024, 1025, 1374, 1536, 1537, 2100, 2560, 2561, 2900, 3060, 3100, 4097, 6144, 6145, 8191, 8192, 8193, 12_001, 20_000])
 def test_norm_widths(width):
     say("norm width", width)
     for rows in (1, 33, 1025):
@@ -266,7 +266,7 @@ def test_norm_widths(width):
         check_norm(x, w, res, codes, scale, r)
 
 
-@pytest.mark.parametrize("width", [40, 300, 1400, 2000, 2400, 5000, 9000])
+@pytest.mark.parametrize("width", [40, 300, 1400, 2000, 2400, 5000, 7000, 9000])
 def test_norm_of_large_values_and_of_none(width):
     say("norm extremes", width)
     w = torch.ones(width, device="cuda")

@@ -59,7 +59,7 @@ __device__ __forceinline__ float group_sum(float v, float* red) {
   if constexpr (G > 64) {
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
-    v = (red[0] + red[1]) + (red[2] + red[3]);
+    v = G == 128 ? red[0] + red[1] : (red[0] + red[1]) + (red[2] + red[3]);
   }
   return v;
 }
@@ -283,10 +283,13 @@ __device__ __forceinline__ void put_codes(const Mx4Args& p, int64_t row, int chu
   if ((chunk & 3) == 0) p.scale[row * p.lds + (chunk >> 2)] = (uint8_t)byte;
 }
 
+// A workgroup is one group of lanes, or 256 lanes of smaller ones.
+constexpr int mx4_threads(int g) { return g > 64 ? g : kThreads; }
+
 template <class X, class R, int G, int NC>
-__global__ __launch_bounds__(kThreads) void k_norm_mx4(Mx4Args q) {
+__global__ __launch_bounds__(mx4_threads(G)) void k_norm_mx4(Mx4Args q) {
   const NormArgs& p = q.n;
-  constexpr int kRows = kThreads / G;
+  constexpr int kRows = mx4_threads(G) / G;
   __shared__ float red[2][4];
   const int lane = threadIdx.x % G;
   const int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / G;
@@ -663,30 +666,56 @@ void launch_norm(const NormArgs& p, hipStream_t s) {
   else k_norm_long<X, R, CODES><<<blocks(1), kThreads, 0, s>>>(p);
 }
 
-// Rows of more than 1024 values: a wave walks a whole row where its chunks leave registers for enough other waves, four
-// waves share it otherwise.  A row of four waves waits for its loads, for the others' sums and for its stores one after the
-// other, and no more than 8 rows are on a unit.  262144 rows, us, four waves / one:
-//   float16 x 1030   350 / 199    1374  364 / 215    2040  340 / 282    2500  525 / 424    4096  562 / 664
-//   float32 x 1030   363 / 261    1374  399 / 310    2040  439 / 465    2500  651 / 584    4096  910 / 906
-//   float16 + residual x 1374  556 / 445    2040  658 / 646 (16384 rows: 34 / 38)
-//   float32 + residual x 1374  884 / 876    2040 1271 / 1300
+// Rows of more than 1024 values: one wave, two or four of them share a row, with up to three chunks a lane in the first two (more
+// leave registers for too few other waves).  A row of four waves waits for its loads, for the others' sums and for its stores one
+// after the other, and no more than 8 rows are on a unit.  131072 rows, us (lanes of a row, chunks of a lane):
+//   float16                 (64, 3)  (128, 2)  (128, 3)  (256, 1)  (256, 2)  (256, 3)  (256, 4)
+//     1400                    103       128                 182
+//     2000                              142                 170
+//     2560                                        188                 241
+//     4096                                                            279 (128, 4: 275, 16384 rows 39 for 36)
+//     5120                                                                     372       448
+//   float16, residual
+//     1400                    214       218                 278
+//     2000                              338                 322
+//     2560                                        376                 392
+//   float32
+//     1400                    155       160                 200
+//     2000                              223                 220
+//     2560                                        280                 310
+//     5120                                                                     570       634
+//   float32, residual
+//     1400                    436       457                 442
+//     2560 (16384 rows)                           102                  98
 template <class X, class R>
 void launch_mx4(const Mx4Args& p, hipStream_t s) {
-  auto blocks = [&](int rows) { return dim3((uint32_t)ceil_div(p.n.rows, rows)); };
   const int w = p.n.width;
-  constexpr bool one = is_none<R>;
-  if (w <= 64) k_norm_mx4<X, R, 8, 1><<<blocks(32), kThreads, 0, s>>>(p);
-  else if (w <= 128) k_norm_mx4<X, R, 16, 1><<<blocks(16), kThreads, 0, s>>>(p);
-  else if (w <= 256) k_norm_mx4<X, R, 32, 1><<<blocks(8), kThreads, 0, s>>>(p);
-  else if (w <= 512) k_norm_mx4<X, R, 64, 1><<<blocks(4), kThreads, 0, s>>>(p);
-  else if (w <= 1024 && p.n.rows >= 1024) k_norm_mx4<X, R, 64, 2><<<blocks(4), kThreads, 0, s>>>(p);
-  else if (w > 1024 && w <= 1536) k_norm_mx4<X, R, 64, 3><<<blocks(4), kThreads, 0, s>>>(p);
-  else if (w > 1536 && w <= 2048 && one && sizeof(typename X::raw) == 2) k_norm_mx4<X, R, 64, 4><<<blocks(4), kThreads, 0, s>>>(p);
-  else if (w > 2048 && w <= 2560 && one) k_norm_mx4<X, R, 64, 5><<<blocks(4), kThreads, 0, s>>>(p);
-  else if (w <= 2048) k_norm_mx4<X, R, 256, 1><<<blocks(1), kThreads, 0, s>>>(p);
-  else if (w <= 4096) k_norm_mx4<X, R, 256, 2><<<blocks(1), kThreads, 0, s>>>(p);
-  else if (w <= kNormMost) k_norm_mx4<X, R, 256, 4><<<blocks(1), kThreads, 0, s>>>(p);
-  else k_norm_mx4_long<X, R><<<blocks(1), kThreads, 0, s>>>(p);
+  constexpr bool kOne = is_none<R>, kShort = sizeof(typename X::raw) == 2;
+  auto run = [&](auto lanes, auto chunks) {
+    constexpr int G = decltype(lanes)::value, NC = decltype(chunks)::value, kTogether = mx4_threads(G);
+    k_norm_mx4<X, R, G, NC><<<dim3((uint32_t)ceil_div(p.n.rows, kTogether / G)), kTogether, 0, s>>>(p);
+  };
+  using std::integral_constant;
+  integral_constant<int, 1> one;
+  integral_constant<int, 2> two;
+  integral_constant<int, 3> three;
+  integral_constant<int, 4> four;
+  integral_constant<int, 64> wave;
+  integral_constant<int, 128> waves2;
+  integral_constant<int, 256> waves4;
+  if (w <= 64) run(integral_constant<int, 8>{}, one);
+  else if (w <= 128) run(integral_constant<int, 16>{}, one);
+  else if (w <= 256) run(integral_constant<int, 32>{}, one);
+  else if (w <= 512) run(wave, one);
+  else if (w <= 1024 && p.n.rows >= 1024) run(wave, two);
+  else if (w > 1024 && w <= 1536) run(wave, three);
+  else if (w > 1536 && w <= 2048 && kOne && kShort) run(waves2, two);
+  else if (w <= 2048) run(waves4, one);
+  else if (w <= 3 * 1024 && (kOne || kShort)) run(waves2, three);
+  else if (w <= 4096) run(waves4, two);
+  else if (w <= 6144) run(waves4, three);
+  else if (w <= kNormMost) run(waves4, four);
+  else k_norm_mx4_long<X, R><<<dim3((uint32_t)p.n.rows), kThreads, 0, s>>>(p);
 }
 
 constexpr int kNoResidual = -1;
