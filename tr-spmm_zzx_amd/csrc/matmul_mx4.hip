@@ -28,6 +28,7 @@ struct MatArgs {
   bool past;   // out is written past the caches
 };
 
+constexpr int kCus = 256;
 constexpr int kFp4 = 4;   // the matrix instructions' name for these codes
 
 __device__ __forceinline__ int8_v codes_of(int4_v v) { return int8_v{v[0], v[1], v[2], v[3], 0, 0, 0, 0}; }
@@ -124,7 +125,7 @@ __global__ __launch_bounds__(1024) void k_mx4_rows(MatArgs p, uint32_t blocks_n)
 // 7), so that the 16-byte reads of neighbouring rows spread over the banks.  The upper 32 lanes take the step's last four
 // blocks, so a lane's four scales of a step are one word; scales come 32 to a row, for four steps.
 //
-// Bound by arithmetic and by how soon the next step's operands arrive: 8192 x 8192 x 8192 253 to 262 us by card, 4.2 PFLOP/s.
+// Bound by arithmetic and by how soon the next step's operands arrive: 8192 x 8192 x 8192 247 to 253 us by card, 4.4 PFLOP/s.
 // Each quarter of a step is read from LDS while the one before is multiplied, scales among the first reads.
 //
 // ALIGNED: scales' rows on 4-byte boundaries; they go from memory to LDS without registers, as the codes do.  Others come by the
@@ -233,6 +234,22 @@ __device__ __forceinline__ void add_bias(const MatArgs& p, float16_v (&acc)[FM][
     }
 }
 
+// The workgroup's tile.  An XCD starts its walk over its tiles (tile_of) as many eighths of them on as its number says: XCDs in step
+// write outputs that lie a whole part of the matrix apart, often a power of two and then in the same memory channels (8192 x 8192 x
+// 1024, tiles of 256: 65 us from their first tiles on, 56 so).
+__device__ __forceinline__ void spread_tile_of(uint32_t b, uint32_t tiles_m, uint32_t tiles_n, uint32_t& tm, uint32_t& tn) {
+  const uint32_t total = tiles_m * tiles_n, xcd = b & 7, mine = (total >> 3) + (xcd < (total & 7) ? 1 : 0);
+  uint32_t at = (b >> 3) + mine * xcd / 8;
+  if (at >= mine) at -= mine;
+  tile_of(at * 8 + xcd, tiles_m, tiles_n, tm, tn);
+}
+
+// Two workgroups of a CU that walk many tiles in step have taken up to twice the time of two that do not (tiles of 128, 16384 x
+// 4096 x 1024: 111 us, 57 so; 8192 x 8192 x 2048: 144 and 91; not on every card), so the second of the first ones starts 2 us later.
+__device__ __forceinline__ void start_apart(uint32_t b, uint32_t total) {
+  if (total > 2 * kCus && b >= kCus && b < 2 * kCus) __builtin_amdgcn_s_sleep(60);
+}
+
 template <int TM, int TN, int WM, int WN, int KS, bool ALIGNED>
 __device__ __forceinline__ void mx4_tile(const MatArgs& p, uint32_t tiles_m, uint32_t tiles_n) {
   constexpr int kWaveRows = TM / WM, kWavesOf = kWaveRows * (TN / WN), kAll = kWavesOf * 64;   // of a group
@@ -244,7 +261,8 @@ __device__ __forceinline__ void mx4_tile(const MatArgs& p, uint32_t tiles_m, uin
   constexpr int kTile = (TM + TN) * kDepth, kScales = kRows * kPair, kGroup = 2 * kTile + kSlots * kScales;
   __shared__ __align__(1024) uint8_t lds[KS * kGroup];
   uint32_t tm, tn;
-  tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn);
+  spread_tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn);
+  if constexpr (TM == 128) start_apart(blockIdx.x, gridDim.x);
   const int64_t m0 = (int64_t)tm * TM;
   const int n0 = (int)tn * TN;
   const int any_wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -689,8 +707,6 @@ __global__ __launch_bounds__(kPanelWaves * 64, rows_panels(GW, BYTES)) void k_mx
 
 // ---------------------------------------------------------------------------------------------
 // Host side: which kernel.
-constexpr int kCus = 256;
-
 template <int FM>
 void launch_rows(const MatArgs& p, hipStream_t s) {
   const uint32_t bn = (uint32_t)ceil_div(p.n, 16), bm = (uint32_t)ceil_div(p.m, 16 * FM);
@@ -802,9 +818,12 @@ void launch_panel(const MatArgs& p, hipStream_t s) {
 //   2048 x 2048 x 2048                           12.4            9.9   16.3
 //   2048 x 4096 x 4096                           33.2           21.8   27.1
 //   9000 x 3008 x 4800                            151            100     81
-//   4096 x 4096 x 4096                           63.6           41.8   37.1
-//   16384 x 1024 x 512                           14.1           10.9   10.7
-//   8192 x 8192 x 8192                            460            293    253
+//   4096 x 4096 x 1024                           21.9           16.4   14.9
+//   4096 x 4096 x 4096                           63.1           42.1   36.7
+//   16384 x 1024 x 512                           15.0           11.3   10.7
+//   16384 x 4096 x 1024                          76.0           56.0   53.2
+//   8192 x 8192 x 2048                            128           89.5   81.0
+//   8192 x 8192 x 8192                            460            294    250
 // (With scales off 4-byte boundaries tiles of 256 take up to a quarter longer, the others 2 to 5%.)
 //
 // The panel, us (k_mx4_rows_panel where rows are off 64-byte lines):
@@ -852,7 +871,7 @@ Choice choose(const MatArgs& p) {
          64, 1, 0});
   if (t64 == 1 && steps >= 8) offer({2.9 + (0.13 + 0.11 * fill) * steps, 64, 4, 0});
   offer({std::max(mb / (lines ? 4.7 : 2.9), t128 / 2 * (1.03 * steps + 3.2) + t128 % 2 * (0.73 * steps + 2.1)), 128, 1, 0});
-  offer({std::max(mb / (lines ? 5 : 3.1), t256 * (1.8 * steps + 5)), 256, 1, 0});
+  offer({std::max(mb / (lines ? 5 : 3.1), t256 * (1.75 * steps + 6.2)), 256, 1, 0});
   return best;
 }
 
