@@ -397,3 +397,33 @@ def test_autograd_sees_the_change():
         q = torch.ones(64, device="cuda")
         trspmm.adamw([q], [g], [trspmm.adamw_state(q)], 1)
     assert bool((q != 1).all())
+
+
+def test_an_index_past_32_bits():
+    """2^32 + 5000 elements: those with a gradient, at the start, around 2^31 and at the end, are stepped as in a tensor of their own."""
+    say("long tensor")
+    n = 2 ** 32 + 5000
+    if torch.cuda.mem_get_info()[0] < 80e9:
+        pytest.skip("not enough memory")
+    p, g = (torch.zeros(n, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    state = trspmm.adamw_state(p, 8)
+    parts = [slice(0, 640), slice(2 ** 31 - 320, 2 ** 31 + 320), slice(2 ** 32 - 320, 2 ** 32 + 320), slice(n - 584, n)]
+    alone = []
+    for i, at in enumerate(parts):
+        count = at.stop - at.start
+        mine, grad = (rand((count,), torch.bfloat16, 10 * i + k) for k in range(2))
+        p[at], g[at] = mine, grad
+        alone.append((mine, trspmm.adamw_state(mine, 8)))
+        trspmm.adamw([mine], [grad], [alone[-1][1]], 1, lr=0.5)
+    trspmm.adamw([p], [g], [state], 1, lr=0.5)
+    for at, (mine, its) in zip(parts, alone):
+        assert torch.equal(p[at], mine), at
+        blocks = slice(at.start // 32, (at.stop + 31) // 32)
+        for long, short in ((state.m_scale, its.m_scale), (state.v_scale, its.v_scale)):
+            assert torch.equal(long[blocks].view(torch.uint8), short.view(torch.uint8)), at
+        # codes: one of the same two neighbours, by other bits
+        for long, short in ((state.m, its.m), (state.v, its.v)):
+            off = long[at].view(torch.uint8).int() - short.view(torch.uint8).int()
+            assert int(off.abs().max()) <= 1
+        p[at] = 0
+    assert not bool(p.any())

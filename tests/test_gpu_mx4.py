@@ -424,6 +424,31 @@ def test_more_channels_than_a_walk_can_have():
     assert not bool(got.any())
 
 
+def test_offsets_past_32_bits():
+    """2.2 million rows of 1000: elements of x, of the residual's sum and of the product past 2^31; the last rows are those of a call of their own."""
+    say("long offsets")
+    rows, width = 2_200_001, 1000
+    if torch.cuda.mem_get_info()[0] < 40e9:
+        pytest.skip("not enough memory")
+    x = torch.ones((rows, width), dtype=torch.float16, device="cuda")
+    last = slice(rows - 301, rows)
+    x[last] = rand((301, width), torch.float16, 1)
+    weight = 1 + 0.1 * rand((width,), torch.float32, 2)
+
+    def same(got, want):
+        assert all(torch.equal(a[last].view(torch.uint8) if a.dtype == E8M0 else a[last], b.view(torch.uint8) if b.dtype == E8M0 else b)
+                   for a, b in zip(got, want))
+    codes, scale = trspmm.quant_mx4(x)
+    same((codes, scale), trspmm.quant_mx4(x[last].clone()))
+    same((trspmm.dequant_mx4(codes, scale, width),), (trspmm.dequant_mx4(codes[last].clone(), scale[last].clone(), width),))
+    same(trspmm.rms_norm_mx4(x, weight, x, EPS), trspmm.rms_norm_mx4(x[last].clone(), weight, x[last].clone(), EPS))
+    del x
+    w, sw = operand(width, width, 3)
+    a, sa = operand(301, width, 5)
+    codes[last], scale.view(torch.uint8)[last] = a, sa.view(torch.uint8)
+    same((trspmm.matmul_mx4(codes, scale, w, sw, dtype=torch.bfloat16),), (product(a, sa, w, sw).to(torch.bfloat16),))
+
+
 def test_equal_inputs_give_equal_bits():
     say("again")
     for m, n, k in [(1, 500, 4000), (50, 500, 4000), (900, 800, 700), (5000, 256, 128)]:
