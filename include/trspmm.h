@@ -592,7 +592,7 @@ typedef struct trs_adamw_options {
   int64_t step;                      /* counts from 1 */
   const float* lr_device;            /* where not NULL, these are read on the GPU in place of lr, grad_scale and step, */
   const float* grad_scale_device;    /* so that a captured call follows them */
-  const int64_t* step_device;
+  const int64_t* step_device;        /* where it is below 1 on the GPU, the call writes nothing */
   const float* skip;                 /* where not NULL and not 0 on the GPU, the call writes nothing */
   uint32_t seed;
 } trs_adamw_options;

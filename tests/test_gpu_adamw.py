@@ -427,3 +427,33 @@ def test_an_index_past_32_bits():
             assert int(off.abs().max()) <= 1
         p[at] = 0
     assert not bool(p.any())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_step_from_the_gpu_below_1_writes_nothing(bits):
+    """Steps count from 1; a counter that is raised behind the call starts at 0, where the bias corrections divide by 0."""
+    say("step below 1", bits)
+    for step in (0, -1, -2 ** 40):
+        c = Case(900, torch.float32, torch.bfloat16, bits, torch.float16, 3)
+        step_all([c], torch.tensor(step, device="cuda"))
+        now = c.host()
+        assert np.array_equal(now[0], c.before[0]) and all(np.array_equal(a, b) for a, b in zip(now[2], c.before[2]))
+        assert bool((c.copy == 0).all())
+
+
+def test_a_captured_step_that_counts_behind_the_call():
+    say("graph, counted behind")
+    c, twin = (Case(3000, torch.float32, torch.float32, 8, torch.bfloat16, 3) for _ in range(2))
+    step = torch.tensor([0], device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        step_all([c], step, seed=4)
+        step.add_(1)
+    for turn in range(4):
+        graph.replay()
+        if turn > 0:
+            step_all([twin], torch.tensor([turn], device="cuda"), seed=4)
+        torch.cuda.synchronize()
+        assert torch.equal(c.p, twin.p) and torch.equal(c.copy, twin.copy), turn
+        assert all(torch.equal(s.view(torch.uint8), t.view(torch.uint8)) for s, t in zip(c.state, twin.state))

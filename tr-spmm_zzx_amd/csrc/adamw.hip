@@ -136,6 +136,7 @@ __global__ __launch_bounds__(kThreads) void k_adamw(Args a) {
   if (s.grad_scale_at) grad_scale = *s.grad_scale_at;
   if (s.step_at) {
     const int64_t step = *s.step_at;
+    if (step < 1) return;   // nothing to correct the bias by; the host refuses such a number
     bias1 = -expm1f((float)step * s.log1);
     root2 = sqrtf(-expm1f((float)step * s.log2));
     key = key_of(s.seed, (uint32_t)step);
