@@ -570,7 +570,7 @@ int trs_matmul_mx4(const uint8_t* a, int64_t lda, const uint8_t* a_scale, int64_
  *   p = p (1 - lr weight_decay) - lr / (1 - beta1^step) * m / (sqrt(v / (1 - beta2^step)) + eps)
  * in 32 bits, in place; p is rounded to its type, and once more to the copy's.  m and v are float32 where m_scale and v_scale
  * are NULL.  Otherwise they are 8-bit codes (sign, 4 bits of exponent with bias 7, 3 of fraction; 127: NaN) of `count` bytes with one
- * scale byte (exponent + 127) for each 32 of them, ceil(count / 32) bytes; a new state is all zeros.  Codes are rounded up
+ * scale byte (exponent + 127; 255: the 32 values are NaN) for each 32 of them, ceil(count / 32) bytes; a new state is all zeros.  Codes are rounded up
  * or down with the chance that keeps their mean, by bits that seed, step and the element's index in its tensor decide: equal
  * calls give equal bits.  v > 0 does not become 0.  An element that is not finite is a NaN code and leaves its block's other
  * elements alone.  The step itself uses m and v before their rounding. */

@@ -457,3 +457,32 @@ def test_a_captured_step_that_counts_behind_the_call():
         torch.cuda.synchronize()
         assert torch.equal(c.p, twin.p) and torch.equal(c.copy, twin.copy), turn
         assert all(torch.equal(s.view(torch.uint8), t.view(torch.uint8)) for s, t in zip(c.state, twin.state))
+
+
+@pytest.mark.parametrize("byte", [0, 1, 200, 254])
+def test_states_with_every_scale(byte):
+    """Scale byte b stands for 2^(b - 127), also where that is no ordinary float: a state that was written elsewhere may hold it."""
+    say("scale", byte)
+    c = Case(640, torch.float32, torch.float32, 8, None, 3)
+    for codes, scale in ((c.state.m, c.state.m_scale), (c.state.v, c.state.v_scale)):
+        scale.view(torch.uint8).fill_(byte)
+        codes.view(torch.uint8).clamp_(max=0x3F if byte == 254 else 0x78)      # 2^127 times 1.875 is finite
+    c.g.zero_()
+    c.before = c.host()
+    assert all(np.array_equal(decoded(c.before[2][k], c.before[2][2 + k]), x.cpu().numpy()) for k, x in enumerate(c.state.values()))
+    step_all([c], 2)
+    c.check(2)
+    if byte == 0:       # 0.9 and 0.999 of values up to 2^-119: they live on at the smallest scale that is written
+        assert bool((c.state.m.view(torch.uint8) & 127 > 0).any()) and bool((c.state.v.view(torch.uint8) > 0).any())
+
+
+def test_a_nan_scale_is_a_block_of_nan():
+    say("nan scale")
+    c = Case(640, torch.float32, torch.float32, 8, None, 3)
+    for scale in (c.state.m_scale, c.state.v_scale):
+        scale.view(torch.uint8)[3] = 255
+    c.state.m.view(torch.uint8)[96:128] = torch.arange(32, dtype=torch.uint8, device="cuda")
+    step_all([c], 2)
+    assert torch.nonzero(torch.isnan(c.p)).flatten().tolist() == list(range(96, 128))
+    for codes in (c.state.m, c.state.v):
+        assert torch.nonzero(torch.isnan(codes.float())).flatten().tolist() == list(range(96, 128))

@@ -117,7 +117,8 @@ __device__ __forceinline__ void store_codes(uint8_t* p, int n, uint32_t x) {
 __device__ __forceinline__ void values8(uint32_t codes, uint32_t byte, float (&v)[4]) {
   typedef float pair __attribute__((ext_vector_type(2)));
   const pair a = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, true);
-  const float scale = scale_of(byte);
+  // byte 0 is 2^-127, no ordinary float; 255 makes each value of its block NaN
+  const float scale = byte == kNanScale ? __builtin_nanf("") : byte ? scale_of(byte) : 0x1p-127f;
   v[0] = a[0] * scale, v[1] = a[1] * scale, v[2] = b[0] * scale, v[3] = b[1] * scale;
 }
 

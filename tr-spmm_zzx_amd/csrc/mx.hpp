@@ -1,6 +1,7 @@
 // Blocks of 32 numbers with a power of two as their scale, shared by mx4.hip (4-bit codes), norm.hip (a norm's output as
-// such codes) and adamw.hip (8-bit states): a scale is one byte, exponent + 127; 255 marks a block that holds a NaN or an
-// infinity.
+// such codes) and adamw.hip (8-bit states): a scale is one byte, exponent + 127; the values of a block with byte 255 are NaN.
+// 4-bit codes are written so where a block holds a NaN or an infinity; 8-bit ones have a NaN of their own, and their scales are
+// written as 1 .. 247 (0 in a new state).
 #pragma once
 #include "dense.hpp"
 
