@@ -539,7 +539,8 @@ int trs_matmul_i8(const int8_t* a, int64_t lda, const float* a_scale, const int8
 /* 4-bit codes with block scales.  A row of `width` numbers is held in ceil(width / 32) blocks of 32: 16 bytes of codes a
  * block, the lower half of a byte first, and one byte of scale, exponent + 127 of a power of two.  A code is a sign and
  * one of 0, 0.5, 1, 1.5, 2, 3, 4, 6; its value is that times the scale.  Scale byte 255: all of the block's values are NaN.  Rows of
- * codes start on 16-byte boundaries (TRS_EINVAL otherwise), ldc >= 16 * blocks in bytes; scales anywhere, lds >= blocks. */
+ * codes start on 16-byte boundaries (TRS_EINVAL otherwise; of a single row only its address counts), ldc >= 16 * blocks in bytes;
+ * scales anywhere, lds >= blocks. */
 
 /* x [rows, width] as codes: a block's scale is 2^max(floor(log2 max|x|) - 2, -126), a code the nearest of x / scale (ties to
  * the even code; 6 beyond 6, so a block's largest value loses a quarter at most).  A block with a NaN or an infinity has

@@ -483,3 +483,29 @@ def test_refusals():
         trspmm.rms_norm_mx4(x, w, eps=0.0)
     with pytest.raises(nat.TrsError):
         trspmm.rms_norm_mx4(x, w, x.bfloat16())
+
+
+@pytest.mark.parametrize("blocks", [1, 3, 16, 33])
+def test_a_single_rows_stride_says_nothing(blocks):
+    """One row of codes with its scales behind it, 17 bytes a block: it starts on a 16-byte boundary, whatever follows it."""
+    say("one row", blocks)
+    k = 32 * blocks
+    x, weight = rand((1, k), torch.float16, 1), 1 + 0.1 * rand((k,), torch.float32, 2)
+
+    def packed():
+        row = torch.full((1, 17 * blocks + 5), 9, dtype=torch.uint8, device="cuda")
+        assert row[:, :16 * blocks].stride(0) % 16 != 0
+        return row, row[:, :16 * blocks], row[:, 16 * blocks:17 * blocks]
+
+    for quantise in (lambda **out: trspmm.quant_mx4(x, **out), lambda **out: trspmm.rms_norm_mx4(x, weight, eps=EPS, **out)):
+        want, byte = (t.view(torch.uint8) for t in quantise()[:2])
+        row, codes, scale = packed()
+        got = quantise(out=codes, scale=scale)
+        assert got[0].data_ptr() == codes.data_ptr() and got[1].data_ptr() == scale.data_ptr()
+        assert torch.equal(codes, want) and torch.equal(scale, byte) and bool((row[:, 17 * blocks:] == 9).all())
+    assert torch.equal(trspmm.dequant_mx4(codes, scale, k), trspmm.dequant_mx4(want, byte, k))
+    for rows in (1, 40, 3000):
+        b, sb = operand(rows, k, 3)
+        # the packed row as the rows and as the channels
+        assert torch.equal(trspmm.matmul_mx4(codes, scale, b, sb), trspmm.matmul_mx4(want, byte, b, sb))
+        assert torch.equal(trspmm.matmul_mx4(b, sb, codes, scale), trspmm.matmul_mx4(b, sb, want, byte))

@@ -135,3 +135,16 @@ def test_adamw_of_nothing():
     lib = nat.lib()
     assert lib.trs_adamw(None, 1, options(), None) == 1 and lib.trs_adamw(None, 0, options(), None) == 0
     assert lib.trs_adamw(None, 0, None, None) == 1 and adamw([tensor()], options(), count=-1) == 1
+
+
+def test_a_single_rows_distance_says_nothing():
+    """One row on a 16-byte boundary is taken whatever the next would be at: these calls are refused for what is checked behind it."""
+    lib = nat.lib()
+    assert lib.trs_rms_norm_mx4(*{**NORM, "rows": 1, "ldc": 33, "x_type": 1, "r_type": 2}.values()) == 1
+    assert b"16-bit types" in lib.trs_last_error()
+    assert lib.trs_matmul_mx4(*{**MATMUL, "m": 1 << 40, "n": 1, "ldw": 33, "ldo": 1}.values()) == 5
+    for name, args in [("trs_quant_mx4", {**QUANT, "rows": 1, "codes": X + 8}), ("trs_quant_mx4", {**QUANT, "rows": 1, "ldc": 31}),
+                       ("trs_dequant_mx4", {**DEQUANT, "rows": 1, "codes": X + 1}), ("trs_rms_norm_mx4", {**NORM, "rows": 1, "codes": X + 4}),
+                       ("trs_matmul_mx4", {**MATMUL, "m": 1, "a": X + 8}), ("trs_matmul_mx4", {**MATMUL, "n": 1, "w": X + 8}),
+                       ("trs_matmul_mx4", {**MATMUL, "m": 1, "lda": 31}), ("trs_quant_mx4", {**QUANT, "rows": 2, "ldc": 33})]:
+        assert getattr(lib, name)(*args.values()) == 1, name

@@ -923,7 +923,7 @@ extern "C" int trs_matmul_mx4(const uint8_t* a, int64_t lda, const uint8_t* a_sc
   if (!out || (blocks > 0 && (!a || !w || !a_scale || !w_scale))) return fail(TRS_EINVAL, where, "NULL operand");
   const int64_t row = (int64_t)blocks * kBlockBytes;
   if (lda < row || ldw < row || ldas < blocks || ldws < blocks || ldo < n) return fail(TRS_EINVAL, where, "leading dimension too small");
-  if (blocks > 0 && (!aligned_codes(a, lda) || !aligned_codes(w, ldw))) return fail(TRS_EINVAL, where, "codes off a 16-byte boundary");
+  if (blocks > 0 && (!aligned_codes(a, lda, m) || !aligned_codes(w, ldw, n))) return fail(TRS_EINVAL, where, "codes off a 16-byte boundary");
   if (m > kMostRows) return fail(TRS_ERANGE, where, "too many rows");
   const bool past = streams(out, ldo, out_type == TRS_F32 ? 4 : 2, m, n);
   const MatArgs p{a, a_scale, w, w_scale, bias, out, lda, ldas, ldw, ldws, ldo, m, n, blocks, out_type, past};

@@ -65,8 +65,10 @@ __device__ __forceinline__ void values4(uint32_t codes, float scale, float (&v)[
   v[0] = a[0], v[1] = a[1], v[2] = b[0], v[3] = b[1], v[4] = c[0], v[5] = c[1], v[6] = d[0], v[7] = d[1];
 }
 
-// Host: what the entry points ask of codes (blocks of 16 bytes on 16-byte boundaries).
-inline bool aligned_codes(const void* p, int64_t ld) { return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)ld) & 15) == 0; }
+// Host: what the entry points ask of codes (rows on 16-byte boundaries; a single one's distance to the next says nothing).
+inline bool aligned_codes(const void* p, int64_t ld, int64_t rows) {
+  return ((reinterpret_cast<uintptr_t>(p) | (rows > 1 ? (uintptr_t)ld : 0)) & 15) == 0;
+}
 inline int64_t blocks_of(int64_t width) { return ceil_div(width, kBlock); }
 
 }  // namespace dense

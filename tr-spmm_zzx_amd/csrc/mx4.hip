@@ -104,7 +104,7 @@ int mx4_call(const char* where, QuantArgs p, int type, void* stream) {
   const int64_t blocks = blocks_of(p.width);
   if (!p.x || !p.codes || !p.scale) return fail(TRS_EINVAL, where, "NULL operand");
   if (p.ldx < p.width || p.ldc < blocks * kBlockBytes || p.lds < blocks) return fail(TRS_EINVAL, where, "leading dimension too small");
-  if (!aligned_codes(p.codes, p.ldc)) return fail(TRS_EINVAL, where, "codes off a 16-byte boundary");
+  if (!aligned_codes(p.codes, p.ldc, p.rows)) return fail(TRS_EINVAL, where, "codes off a 16-byte boundary");
   if (p.rows > (int64_t)1 << 38) return fail(TRS_ERANGE, where, "too many rows");
   p.chunks = QUANT ? (int)blocks * 4 : (int)ceil_div(p.width, 8);
   p.share = p.chunks > kSpan ? 1 : kSpan / p.chunks;

@@ -807,7 +807,7 @@ int mx4_call(const Mx4Args& a, int x_type, int r_type, void* stream) {
   if ((p.res == nullptr) != (p.r == nullptr)) return fail(TRS_EINVAL, where, "residual and its output go together");
   if (p.ldx < p.width || p.ldy < blocks * kBlockBytes || a.lds < blocks || (p.res && (p.ldr < p.width || p.ldro < p.width)))
     return fail(TRS_EINVAL, where, "leading dimension too small");
-  if (!aligned_codes(p.y, p.ldy)) return fail(TRS_EINVAL, where, "codes off a 16-byte boundary");
+  if (!aligned_codes(p.y, p.ldy, p.rows)) return fail(TRS_EINVAL, where, "codes off a 16-byte boundary");
   if (p.rows > kMostRows) return fail(TRS_ERANGE, where, "too many rows");
   if (!p.res) r_type = kNoResidual;
   hipStream_t s = static_cast<hipStream_t>(stream);
