@@ -600,7 +600,8 @@ typedef struct trs_adamw_options {
 
 void trs_adamw_options_default(trs_adamw_options* options);
 
-/* TRS_EINVAL also for buffers that are written and overlap each other (a tensor named twice) or a gradient.  A tensor has at most some 1.7e10 elements (TRS_ERANGE). */
+/* TRS_EINVAL also for buffers that are written and overlap each other (a tensor named twice), a gradient or one of the numbers
+ * that are read on the GPU.  A tensor has at most some 1.7e10 elements (TRS_ERANGE). */
 int trs_adamw(const trs_adamw_tensor* tensors, int64_t count, const trs_adamw_options* options, void* stream);
 
 const char* trs_last_error(void);

@@ -486,3 +486,22 @@ def test_a_nan_scale_is_a_block_of_nan():
     assert torch.nonzero(torch.isnan(c.p)).flatten().tolist() == list(range(96, 128))
     for codes in (c.state.m, c.state.v):
         assert torch.nonzero(torch.isnan(codes.float())).flatten().tolist() == list(range(96, 128))
+
+
+def test_numbers_on_the_gpu_that_the_step_would_write():
+    """A factor, a rate, a step or a flag inside of what is written would be read by some workgroups before the write and by others
+    after it."""
+    say("overlapping numbers")
+    p, g = torch.ones(5000, device="cuda"), torch.ones(5000, device="cuda")
+    s, s8 = trspmm.adamw_state(p), trspmm.adamw_state(p, 8)
+    copy = torch.zeros(5000, device="cuda")
+    for state, more in [(s, {"lr": p[7:8]}), (s, {"grad_scale": s.m[4999:]}), (s, {"skip": s.v[:1]}), (s, {"skip": copy[3:4], "copies": [copy]}),
+                        (s8, {"lr": s8.v.view(torch.uint8)[8:12].view(torch.float32)}),
+                        (s8, {"skip": s8.m_scale.view(torch.uint8)[8:12].view(torch.float32)})]:
+        with pytest.raises(nat.TrsError, match="overlaps"):
+            trspmm.adamw([p], [g], [state], 1, **more)
+    with pytest.raises(nat.TrsError, match="overlaps"):
+        trspmm.adamw([p], [g], [s], s.m[:2].view(torch.int64))
+    assert bool((p == 1).all()) and bool((s.m == 0).all())
+    trspmm.adamw([p], [g], [s], 1, lr=g[:1])      # one that is only read
+    assert bool((p < 1).all())

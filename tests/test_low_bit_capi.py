@@ -148,3 +148,11 @@ def test_a_single_rows_distance_says_nothing():
                        ("trs_matmul_mx4", {**MATMUL, "m": 1, "a": X + 8}), ("trs_matmul_mx4", {**MATMUL, "n": 1, "w": X + 8}),
                        ("trs_matmul_mx4", {**MATMUL, "m": 1, "lda": 31}), ("trs_quant_mx4", {**QUANT, "rows": 2, "ldc": 33})]:
         assert getattr(lib, name)(*args.values()) == 1, name
+
+
+@pytest.mark.parametrize("field", ["lr_device", "grad_scale_device", "step_device", "skip"])
+def test_adamw_numbers_inside_of_what_is_written(field):
+    size = 8 if field == "step_device" else 4
+    for at in (X, X + 36, X + 40 - size, X + 512, X + 1024 + 40 - size):
+        assert adamw([tensor()], options(**{field: at})) == 1
+        assert b"overlaps" in nat.lib().trs_last_error()

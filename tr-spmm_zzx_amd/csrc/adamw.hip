@@ -349,6 +349,9 @@ extern "C" int trs_adamw(const trs_adamw_tensor* tensors, int64_t count, const t
     ++read;
   }
   if (written == 0) return TRS_OK;
+  // numbers that the kernel reads: inside of what is written, some workgroups would read them before the write and others after it
+  const struct { const void* at; int64_t bytes; } numbers[] = {{o->lr_device, 4}, {o->grad_scale_device, 4}, {o->step_device, 8}, {o->skip, 4}};
+  for (const auto& x : numbers) read += x.at != nullptr;
   Range few[64];   // the written ones, the read ones, and room to sort more than 64
   const bool small_call = written + read <= 64;
   Range* ranges = small_call ? few : new (std::nothrow) Range[2 * written + read];
@@ -372,9 +375,11 @@ extern "C" int trs_adamw(const trs_adamw_tensor* tensors, int64_t count, const t
     if (t.copy) ranges[w++] = range(t.copy, t.count * bytes_of(t.copy_type));
     ranges[r++] = range(t.grad, t.count * bytes_of(t.grad_type));
   }
+  for (const auto& x : numbers)
+    if (x.at) ranges[r++] = range(x.at, x.bytes);
   const bool shared = overlap(ranges, ranges + written + read, written, ranges + written, read);
   if (!small_call) delete[] ranges;
-  if (shared) return fail(TRS_EINVAL, where, "a parameter, state or copy is named twice, or overlaps another or a gradient");
+  if (shared) return fail(TRS_EINVAL, where, "a parameter, state or copy is named twice, or overlaps another, a gradient or a number on the GPU");
 
   const double t = (double)o->step;
   Args a;
