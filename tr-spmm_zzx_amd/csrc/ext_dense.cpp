@@ -105,6 +105,17 @@ Tensor workspace_of(const Given& workspace, int64_t need, int64_t dev) {
   return need > 0 ? fresh({need}, at::kByte, dev) : Tensor();
 }
 
+// Autograd refuses a backward pass through what it saved of them before.
+void changed(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+// Of a call that has gone well: the outputs that were given.
+void changed(std::initializer_list<const Given*> outputs) {
+  for (const Given* t : outputs)
+    if (*t) changed(**t);
+}
+
 void* data(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 std::pair<Tensor, int32_t> ids_of(const Tensor& ids, int64_t dev) {
@@ -124,6 +135,7 @@ Tensor embed(const Tensor& table_in, const Tensor& ids_in, double scale, const T
   ok(trs_embed(table.data_ptr(), t_type, ld(table), table.size(0), ids.data_ptr(), bits, ids.size(0), width_of(table),
                (float)scale, out.data_ptr(), o_type, ld(out), stream_of(stream)),
      "trs_embed");
+  changed({&out_in});
   return out;
 }
 
@@ -144,6 +156,7 @@ Tensor embed_grad(const Tensor& grad_in, const Tensor& ids_in, int64_t rows, dou
   ok(trs_embed_grad(grad.data_ptr(), g_type, ld(grad), ids.data_ptr(), bits, count, rows, width, (float)scale,
                     out.data_ptr(), o_type, ld(out), data(ws), need, stream_of(stream)),
      "trs_embed_grad");
+  changed({&out_in});
   return out;
 }
 
@@ -183,6 +196,7 @@ std::tuple<Tensor, Given> rms_norm(const Tensor& x, const Tensor& weight, const 
   ok(trs_rms_norm(n.x.data_ptr(), n.x_type, ld(n.x), data(n.residual), n.r_type, n.ldr(), weight.data_ptr(), n.w_type,
                   (float)eps, n.rows, n.width, out.data_ptr(), y_type, ld(out), data(n.r), n.ldro(), stream_of(stream)),
      "trs_rms_norm");
+  changed({&out_in, &r_out});
   return {out, n.r_given()};
 }
 
@@ -197,6 +211,7 @@ std::tuple<Tensor, Tensor, Given> rms_norm_i8(const Tensor& x, const Tensor& wei
                      (float)eps, n.rows, n.width, static_cast<int8_t*>(out.data_ptr()), ld(out),
                      static_cast<float*>(scale.data_ptr()), data(n.r), n.ldro(), stream_of(stream)),
      "trs_rms_norm_i8");
+  changed({&out_in, &scale_in, &r_out});
   return {out, scale, n.r_given()};
 }
 
@@ -223,6 +238,7 @@ std::tuple<Tensor, Tensor> rms_norm_grad(const Tensor& grad_in, const Tensor& r_
                        more.defined() ? ld(more) : 0, (float)eps, rows, width, out.data_ptr(), ld(out),
                        static_cast<float*>(dweight.data_ptr()), data(ws), need, stream_of(stream)),
      "trs_rms_norm_grad");
+  changed({&out_in, &dweight_in});
   return {out, dweight};
 }
 
@@ -246,6 +262,7 @@ Tensor matmul_i8(const Tensor& a_in, const Tensor& a_scale, const Tensor& w_in, 
                    bias ? static_cast<const float*>(bias->data_ptr()) : nullptr, m, (int32_t)n, width_of(a), out.data_ptr(),
                    o_type, ld(out), stream_of(stream)),
      "trs_matmul_i8");
+  changed({&out_in});
   return out;
 }
 
@@ -298,6 +315,7 @@ std::tuple<Tensor, Tensor> quant_mx4(const Tensor& x_in, const Given& out, const
   ok(trs_quant_mx4(x.data_ptr(), x_type, ld(x), x.size(0), width_of(x), o.codes_at(), ld(o.codes), o.scale_at(), ld(o.scale),
                    stream_of(stream)),
      "trs_quant_mx4");
+  changed({&out, &scale});
   return {o.codes, o.scale};
 }
 
@@ -315,6 +333,7 @@ Tensor dequant_mx4(const Tensor& codes_in, const Tensor& scale_in, int64_t width
   ok(trs_dequant_mx4(bytes(codes), ld(codes), bytes(scale), ld(scale), rows, (int32_t)width, out.data_ptr(), o_type, ld(out),
                      stream_of(stream)),
      "trs_dequant_mx4");
+  changed({&out_in});
   return out;
 }
 
@@ -327,6 +346,7 @@ std::tuple<Tensor, Tensor, Given> rms_norm_mx4(const Tensor& x, const Tensor& we
                       (float)eps, n.rows, n.width, o.codes_at(), ld(o.codes), o.scale_at(), ld(o.scale), data(n.r), n.ldro(),
                       stream_of(stream)),
      "trs_rms_norm_mx4");
+  changed({&out, &scale, &r_out});
   return {o.codes, o.scale, n.r_given()};
 }
 
@@ -346,6 +366,7 @@ Tensor matmul_mx4(const Tensor& a_in, const Tensor& a_scale_in, const Tensor& w_
                     bias ? static_cast<const float*>(bias->data_ptr()) : nullptr, m, (int32_t)n, (int32_t)blocks, out.data_ptr(),
                     o_type, ld(out), stream_of(stream)),
      "trs_matmul_mx4");
+  changed({&out_in});
   return out;
 }
 
@@ -472,14 +493,12 @@ void adamw(const py::object& params_in, const py::object& grads_in, const py::ob
     }
   }
   ok(trs_adamw(list.data(), (int64_t)count, &o, stream_of(stream)), "trs_adamw");
-  // Autograd refuses a backward pass through what it saved of them before.
-  auto changed = [](PyObject* x) {
-    const Tensor& t = THPVariable_Unpack(x);
-    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
-  };
   for (size_t i = 0; i < count; ++i) {
-    changed(params[i]);
-    if (copies && (*copies)[i] != Py_None) changed((*copies)[i]);
+    changed(THPVariable_Unpack(params[i]));
+    if (copies && (*copies)[i] != Py_None) changed(THPVariable_Unpack((*copies)[i]));
+    const Items state("a state", states[i]);
+    for (size_t k = 0; k < state.size(); ++k)
+      if (state[k] != Py_None) changed(THPVariable_Unpack(state[k]));
   }
 }
 

@@ -18,6 +18,7 @@ The same in 4 bits:
 
 Tensors live on the current GPU; work is enqueued on ``stream`` (default: the current torch stream).
 Matrices are 2-D with unit column stride and any row stride; one with another column stride is copied.
+For autograd, outputs that are given count as changed in place.
 Outputs that are not given, and workspaces that are not given, too small or off an 8-byte boundary, are allocated on the
 launch stream; a given output has the type that is asked for, or says which where none is.  Arguments are checked in the
 extension (csrc/ext_dense.cpp); the kernels are libtrspmm.so's, and there is no CPU fallback.
@@ -193,5 +194,5 @@ def adamw(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], states:
     factor, and are then read by the kernel; where `skip` (float32, one element) is not 0 or such a `step` is below 1, nothing is
     written.  Params, states and copies are contiguous and share no memory with each other, a gradient or such a number; gradients
     are copied if they are not contiguous.  8-bit states are rounded up or down with the chance that keeps their mean, by bits that `seed` (0 .. 2^32 - 1), step
-    and an element's index decide.  For autograd, params and copies count as changed in place."""
+    and an element's index decide.  For autograd, params, states and copies count as changed in place."""
     _call("adamw", stream, params, grads, states, step, lr, betas, eps, weight_decay, copies, grad_scale, skip, seed)
