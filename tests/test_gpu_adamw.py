@@ -505,18 +505,3 @@ def test_numbers_on_the_gpu_that_the_step_would_write():
     assert bool((p == 1).all()) and bool((s.m == 0).all())
     trspmm.adamw([p], [g], [s], 1, lr=g[:1])      # one that is only read
     assert bool((p < 1).all())
-
-
-def test_states_count_as_changed():
-    say("versions of states")
-    p, g = torch.ones(64, device="cuda"), torch.ones(64, device="cuda")
-    for bits in (32, 8):
-        state = trspmm.adamw_state(p, bits)
-        before = [t._version for t in state if t is not None]
-        trspmm.adamw([p], [g], [state], 1)
-        assert all(t._version > b for t, b in zip((t for t in state if t is not None), before))
-    m = state.m.float().requires_grad_()
-    loss = (m * m).sum()
-    trspmm.adamw([p], [g], [(m, torch.zeros(64, device="cuda"))], 1)
-    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
-        loss.backward()

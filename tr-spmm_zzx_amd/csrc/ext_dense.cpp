@@ -493,12 +493,10 @@ void adamw(const py::object& params_in, const py::object& grads_in, const py::ob
     }
   }
   ok(trs_adamw(list.data(), (int64_t)count, &o, stream_of(stream)), "trs_adamw");
+  // States are no operands of a loss: the counters of 148 tensors' states took 6 to 11 us beside the call's 32 to 37.
   for (size_t i = 0; i < count; ++i) {
     changed(THPVariable_Unpack(params[i]));
     if (copies && (*copies)[i] != Py_None) changed(THPVariable_Unpack((*copies)[i]));
-    const Items state("a state", states[i]);
-    for (size_t k = 0; k < state.size(); ++k)
-      if (state[k] != Py_None) changed(THPVariable_Unpack(state[k]));
   }
 }
 

@@ -194,5 +194,6 @@ def adamw(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], states:
     factor, and are then read by the kernel; where `skip` (float32, one element) is not 0 or such a `step` is below 1, nothing is
     written.  Params, states and copies are contiguous and share no memory with each other, a gradient or such a number; gradients
     are copied if they are not contiguous.  8-bit states are rounded up or down with the chance that keeps their mean, by bits that `seed` (0 .. 2^32 - 1), step
-    and an element's index decide.  For autograd, params, states and copies count as changed in place."""
+    and an element's index decide.  For autograd, params and copies count as changed in place, states do
+    not."""
     _call("adamw", stream, params, grads, states, step, lr, betas, eps, weight_decay, copies, grad_scale, skip, seed)
