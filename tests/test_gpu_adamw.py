@@ -505,3 +505,70 @@ def test_numbers_on_the_gpu_that_the_step_would_write():
     assert bool((p == 1).all()) and bool((s.m == 0).all())
     trspmm.adamw([p], [g], [s], 1, lr=g[:1])      # one that is only read
     assert bool((p < 1).all())
+
+
+def words_from(first, n, seed, step):
+    """The rounding bits of n elements from index `first` on."""
+    key = (seed * 0x6A09E667 + step * 0xB7E15163) & MASK
+    key = ((key ^ key >> 16) * 0xBB67AE85) & MASK
+    out = np.empty(n, np.uint64)
+    for i in range(n):
+        at = first + i
+        x = (key + at * 0x9E3779B9 + (at >> 32) * 0x243F6A89) & MASK
+        x = ((x ^ x >> 15) * 0xBB67AE85) & MASK
+        out[i] = x ^ x >> 16
+    return out
+
+
+def test_rounding_bits_past_32_bits():
+    """Codes around element 2^32 and at the end are those of the formula, whose bits depend on the index's upper half."""
+    say("long tensor's codes")
+    n = 2 ** 32 + 5000
+    if torch.cuda.mem_get_info()[0] < 80e9:
+        pytest.skip("not enough memory")
+    assert np.array_equal(words_from(0, 100, 5, 9), words(100, 5, 9))
+    p, g = (torch.zeros(n, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    state = trspmm.adamw_state(p, 8)
+    parts = [slice(0, 640), slice(2 ** 31 - 320, 2 ** 31 + 320), slice(2 ** 32 - 320, 2 ** 32 + 320), slice(n - 584, n)]
+    for i, at in enumerate(parts):
+        g[at] = rand((at.stop - at.start,), torch.bfloat16, 10 + i)
+    step = 2 ** 32 + 3
+    trspmm.adamw([p], [g], [state], step, seed=6)
+    f = np.float32
+    for at in parts:
+        x = g[at].float().cpu().numpy()
+        w = words_from(at.start, x.size, 6, step)
+        blocks = slice(at.start // 32, (at.stop + 31) // 32)
+        for codes, scale, y, chance, floor in ((state.m, state.m_scale, f(1 - 0.9) * x, w >> np.uint64(16), False),
+                                               (state.v, state.v_scale, f(1 - 0.999) * (x * x), w & np.uint64(0xFFFF), True)):
+            want, byte = encoded(y, chance.astype(np.float64), floor)
+            assert np.array_equal(scale[blocks].view(torch.uint8).cpu().numpy(), byte), at
+            assert np.array_equal(codes[at].view(torch.uint8).cpu().numpy(), want), at
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("step", [2 ** 32, 2 ** 32 + 3, 2 ** 40 + 7])
+def test_steps_past_32_bits(step, bits):
+    """The hash takes the step modulo 2^32, the bias corrections the step itself."""
+    say("step", step, bits)
+    for number in (step, torch.tensor([step], device="cuda")):
+        c = Case(700, torch.float32, torch.float32, bits, None, 3)
+        step_all([c], number, betas=(0.9, 1 - 2.0 ** -30), seed=8)
+        c.check(step, betas=(0.9, 1 - 2.0 ** -30), seed=8)
+
+
+def test_a_second_moment_far_below_its_blocks_largest():
+    """v below 2^-17 of its block's largest is held at the smallest code, 2^-9 of the scale, 2^-17 to 2^-16 of the largest: never
+    0, no longer its mean, and the parameter's change is smaller by the root of that."""
+    say("v's floor")
+    n = 32
+    p, g = torch.zeros(n, device="cuda"), torch.full((n,), 2.0 ** -20, device="cuda")
+    g[0] = 1.0
+    state = trspmm.adamw_state(p, 8)
+    for step in range(1, 6):
+        trspmm.adamw([p], [g], [state], step, weight_decay=0.0, seed=1)
+        v = state.values()[1]
+        unit = 2.0 ** (int(state.v_scale.view(torch.uint8)[0]) - 127)
+        assert bool((v[1:] == unit * 2.0 ** -9).all())
+        share = float(v[1] / v[0])
+        assert 2.0 ** -17.2 <= share <= 2.0 ** -16

@@ -509,3 +509,40 @@ def test_a_single_rows_stride_says_nothing(blocks):
         # the packed row as the rows and as the channels
         assert torch.equal(trspmm.matmul_mx4(codes, scale, b, sb), trspmm.matmul_mx4(want, byte, b, sb))
         assert torch.equal(trspmm.matmul_mx4(b, sb, codes, scale), trspmm.matmul_mx4(b, sb, want, byte))
+
+
+def test_the_terms_of_wide_scales_are_all_there():
+    """One block of a row far above the others, by 2^13: what rounds is the largest term's share, so the sum has to be within
+    k 2^-23 of the sum of the products' sizes, and without its largest block within that of the rest."""
+    say("largest term")
+    for m, n, k in [(1, 300, 5000), (300, 400, 4096), (9000, 64, 250)]:
+        (a, sa), (w, sw) = operand(m, k, 1), operand(n, k, 3)
+        high = sa.view(torch.uint8).clone()
+        high[:, 0] += 13
+        got = trspmm.matmul_mx4(a, high, w, sw, dtype=torch.float32).double()
+        rest = a.clone()
+        rest[:, :16] = 0
+        less = trspmm.matmul_mx4(rest, high, w, sw, dtype=torch.float32).double()
+        for value, codes in ((got, a), (less, rest)):
+            size = torch.mm(values(codes, high).abs(), values(w, sw).abs().t().contiguous())
+            assert bool(((value - product(codes, high, w, sw)).abs() <= k * 2.0 ** -23 * size).all())
+
+
+def test_every_pair_of_scales():
+    """One product of codes for each pair of scale bytes, from 2^-254 on, 255 among them: a 32-bit float as the product rounds to
+    it, zeros and infinities too."""
+    say("pairs of scales")
+    byte = torch.arange(256, dtype=torch.int64, device="cuda")
+    exponent = byte[:, None] + byte[None, :] - 254
+    bad = (byte == 255)[:, None] | (byte == 255)[None, :]
+    for rows, blocks in ((256, 1), (256, 16), (10_240, 1), (4096, 16)):
+        times = rows // 256
+        a, w = (torch.zeros((r, 16 * blocks), dtype=torch.uint8, device="cuda") for r in (rows, 256))
+        sa, sw = (torch.full((r, blocks), 127, dtype=torch.uint8, device="cuda") for r in (rows, 256))
+        sa[:, 0], sw[:, 0] = byte.repeat(times).to(torch.uint8), byte.to(torch.uint8)
+        w[:, 0] = 2
+        for code, size in ((0, 0.0), (2, 1.0), (10, -1.0)):
+            a[:, 0] = code
+            got = trspmm.matmul_mx4(a, sa, w, sw, dtype=torch.float32).view(times, 256, 256)
+            want = torch.where(bad, float("nan"), power(exponent) * size).float()
+            assert bool(((got == want) | (torch.isnan(got) & torch.isnan(want))).all()), (rows, blocks, code)
