@@ -573,7 +573,8 @@ int trs_matmul_mx4(const uint8_t* a, int64_t lda, const uint8_t* a_scale, int64_
  * are NULL.  Otherwise they are 8-bit codes (sign, 4 bits of exponent with bias 7, 3 of fraction; 127: NaN) of `count` bytes with one
  * scale byte (exponent + 127; 255: the 32 values are NaN) for each 32 of them, ceil(count / 32) bytes; a new state is all zeros.  Codes are rounded up
  * or down with the chance that keeps their mean, by bits that seed, step and the element's index in its tensor decide: equal
- * calls give equal bits.  v > 0 does not become 0.  An element that is not finite is a NaN code and leaves its block's other
+ * calls give equal bits, and equal places of all tensors round alike.  v > 0 does not become 0: it is at least 2^-9 of its block's
+ * scale, 2^-17 to 2^-16 of the block's largest v, and below that its mean is not kept (it is too large, the element's steps too small).  An element that is not finite is a NaN code and leaves its block's other
  * elements alone.  The step itself uses m and v before their rounding. */
 typedef struct trs_adamw_tensor {
   void* param;

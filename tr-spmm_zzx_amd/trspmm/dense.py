@@ -193,7 +193,8 @@ def adamw(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], states:
     counts from 1.  `step` (int64), `lr` and `grad_scale` (float32) may be tensors of one element on the GPU, such as a clipping
     factor, and are then read by the kernel; where `skip` (float32, one element) is not 0 or such a `step` is below 1, nothing is
     written.  Params, states and copies are contiguous and share no memory with each other, a gradient or such a number; gradients
-    are copied if they are not contiguous.  8-bit states are rounded up or down with the chance that keeps their mean, by bits that `seed` (0 .. 2^32 - 1), step
-    and an element's index decide.  For autograd, params and copies count as changed in place, states do
-    not."""
+    are copied if they are not contiguous.  8-bit states are rounded up or down with the chance that keeps their mean, by
+    bits that `seed` (0 .. 2^32 - 1), step and an element's index in its tensor decide.  A v of less than 2^-17 to 2^-16 of the largest
+    of its 32 elements is held at that size: the steps of elements whose gradients are smaller than their neighbours' by more than
+    256 to 362 are smaller than with 32 bits.  For autograd, params and copies count as changed in place, states do not."""
     _call("adamw", stream, params, grads, states, step, lr, betas, eps, weight_decay, copies, grad_scale, skip, seed)
