@@ -509,7 +509,7 @@ __device__ __forceinline__ void mx4_tile(const MatArgs& p, uint32_t tiles_m, uin
 }
 
 template <int TM, int TN, int WM, int WN, int KS, bool ALIGNED>
-__global__ __launch_bounds__((TM / WM) * (TN / WN) * 64 * KS, WM * WN > 8192 ? 1 : 2) void k_mx4_tile(MatArgs p, uint32_t tiles_m, uint32_t tiles_n) {
+__global__ __launch_bounds__((TM / WM) * (TN / WN) * 64 * KS, 2) void k_mx4_tile(MatArgs p, uint32_t tiles_m, uint32_t tiles_n) {
   mx4_tile<TM, TN, WM, WN, KS, ALIGNED>(p, tiles_m, tiles_n);
 }
 
@@ -642,7 +642,7 @@ __global__ __launch_bounds__(kPanelWaves * 64, 4) void k_mx4_panel(MatArgs p, ui
 // The same for rows of up to 256 GW outputs that do not start on 64-byte lines.  Lines that a row shares with the next are
 // written in parts, which costs a read of them if the other part does not follow at once: so a workgroup has whole rows of
 // outputs in LDS and its waves write them one after another (2^20 x 300 x 128: 64 columns at a time 342 us).
-template <class T, int H, int GW>
+template <class T, int GW>
 __device__ __forceinline__ void store_rows(const MatArgs& p, const float16_v (&acc)[GW][1][2], uint8_t* lds_bytes_, int64_t m0, int wave, int lane,
                                            int pieces, uint32_t inverse) {
   constexpr int kPitch = pitch_of<T>(GW * kPanelWaves * kPanelColumns);
@@ -689,10 +689,10 @@ __device__ __forceinline__ void mx4_rows_panel(const MatArgs& p, uint32_t tiles_
       w[u].multiply(a, a_scale, p.bias ? bias + (u * kPanelWaves + wave) * kPanelColumns : nullptr, half, acc[u]);
     const int64_t m0 = (int64_t)tile * kPanelRows;
     if constexpr (BYTES == 4) {
-      store_rows<f32_t, H, GW>(p, acc, lds, m0, wave, lane, pieces, inverse);
+      store_rows<f32_t, GW>(p, acc, lds, m0, wave, lane, pieces, inverse);
     } else {
-      if (p.out_type == TRS_F16) store_rows<f16_t, H, GW>(p, acc, lds, m0, wave, lane, pieces, inverse);
-      else store_rows<bf16_t, H, GW>(p, acc, lds, m0, wave, lane, pieces, inverse);
+      if (p.out_type == TRS_F16) store_rows<f16_t, GW>(p, acc, lds, m0, wave, lane, pieces, inverse);
+      else store_rows<bf16_t, GW>(p, acc, lds, m0, wave, lane, pieces, inverse);
     }
   }
 }

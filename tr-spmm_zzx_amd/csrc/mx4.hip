@@ -13,7 +13,7 @@ namespace dense {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int32_t kMostMxWidth = 65535 * 2048;   // the grid's second dimension, and columns' indexes of 32 bits
+constexpr int32_t kMostMxWidth = 65535 * 2048;   // of the interface; kernels have room beyond it
 static_assert(kMostMxWidth <= kMostWidth, "column indexes of 32 bits");
 
 struct QuantArgs {
@@ -31,6 +31,7 @@ struct QuantArgs {
 // row, whose 600 bytes share their lines with the next).  Long rows: kSpan chunks of one.  A thread's chunks are on their way
 // together.
 constexpr int kTurns = 2, kSpan = kTurns * kThreads;
+static_assert(kMostMxWidth / 8 / kSpan < 65535, "the grid's second dimension");
 
 struct Place { int64_t row; int chunk; bool there; };
 
