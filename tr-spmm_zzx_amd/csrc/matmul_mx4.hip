@@ -245,7 +245,8 @@ __device__ __forceinline__ void spread_tile_of(uint32_t b, uint32_t tiles_m, uin
 }
 
 // Two workgroups of a CU that walk many tiles in step have taken up to twice the time of two that do not (tiles of 128, 16384 x
-// 4096 x 1024: 111 us, 57 so; 8192 x 8192 x 2048: 144 and 91; not on every card), so the second of the first ones starts 2 us later.
+// 4096 x 1024: 111 us, 57 so; 8192 x 8192 x 2048: 144 and 91; not on every card, and there it costs its 2 us, which `choose` does not
+// count), so the second of the first ones starts 2 us later.
 __device__ __forceinline__ void start_apart(uint32_t b, uint32_t total) {
   if (total > 2 * kCus && b >= kCus && b < 2 * kCus) __builtin_amdgcn_s_sleep(60);
 }
@@ -517,7 +518,8 @@ __global__ __launch_bounds__((TM / WM) * (TN / WN) * 64 * KS, 2) void k_mx4_tile
 // Short rows (k of at most 256) and many of them: outputs are the bytes that count.  A wave keeps the codes of 64 channels in
 // registers and walks tiles of 32 rows, whose codes go from memory to registers as the matrix instruction takes them, the next
 // tile's on their way while this one's outputs pass through the wave's own part of LDS.  Bound by memory: 2^20 x 256 x 128 100
-// us, 0.61 GB at 6.0 TB/s (tiles of 256: 121); from k = 192 on by the loads' 16-byte pieces of rows (k = 256: 156 us, 4.4
+// us, 0.61 GB at 6.0 TB/s (tiles of 256: 121), and 120 to 130 right behind the norm that makes its codes, whose 0.34 GB are still on their
+// way to memory; from k = 192 on by the loads' 16-byte pieces of rows (k = 256: 156 us, 4.4
 // TB/s).  The waves of a workgroup share rows (CW of them, whose loads meet in the L1) or channels; they never wait for one
 // another.  H: blocks of a half of a wave, 2 H for a row.
 constexpr int kPanelWaves = 4, kPanelRows = kOutRows, kPanelColumns = kOutColumns;
@@ -697,7 +699,8 @@ __device__ __forceinline__ void mx4_rows_panel(const MatArgs& p, uint32_t tiles_
   }
 }
 
-// Workgroups that a CU holds, by their LDS and registers.
+// Workgroups that a CU holds, by their LDS and registers.  (Four blocks to a half of a wave, two groups of columns and 16 bits pass the
+// registers of three: 16 to 20 are spilled.)
 constexpr int rows_panels(int gw, int bytes) { return gw == 1 ? 4 : bytes == 2 ? 3 : 2; }
 
 template <int H, int GW, int BYTES>
