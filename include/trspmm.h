@@ -558,11 +558,12 @@ int trs_rms_norm_mx4(const void* x, int32_t x_type, int64_t ldx, const void* res
                      uint8_t* scale, int64_t lds, void* r_out, int64_t ldro, void* stream);
 
 /* out[i, j] = sum over the blocks of a's row i times w's row j + bias[j], the values that codes and scales stand for: a
- * [m, blocks], w [n, blocks]; lda, ldw are rows of codes, ldas, ldws rows of scales, in bytes; bias float32 or NULL; n at most 2^31 - 65536.  Codes
+ * [m, blocks], w [n, blocks]; lda, ldw are rows of codes, ldas, ldws rows of scales, in bytes; bias float32 or NULL.  Codes
  * past a row's width take part: trs_quant_mx4 and trs_rms_norm_mx4 write zeros there.  Sums in 32 bits, in an order that
- * sizes, types, strides and addresses' alignment decide.  TRS_ERANGE: blocks past 2^26, m past 2^34, or an output of more workgroups
- * than a launch can have: past 2^39 outputs, m and n rounded up to 256 (rows of at most 8 blocks, which need no tiles, apart), or, where rows
- * of codes or scales lie 8 MB and more apart, past 2^32, m rounded up to 64 (2^26 channels of up to 16 rows). */
+ * sizes, types, strides and addresses' alignment decide.  TRS_ERANGE: n past 2^31 - 65536, blocks past 2^26, m past 2^34, or
+ * an output of more workgroups than a launch can have: past 2^39 outputs, m and n rounded up to 256 (rows of at most 8 blocks,
+ * which need no tiles, apart), or, where rows of codes or scales lie 8 MB and more apart, past 2^32, m rounded up to 64 (2^26
+ * channels of up to 16 rows). */
 int trs_matmul_mx4(const uint8_t* a, int64_t lda, const uint8_t* a_scale, int64_t ldas, const uint8_t* w, int64_t ldw,
                    const uint8_t* w_scale, int64_t ldws, const float* bias, int64_t m, int32_t n, int32_t blocks, void* out,
                    int32_t out_type, int64_t ldo, void* stream);

@@ -10,8 +10,8 @@
 // The scale is a power of two so that the codes' values stay where they are while the block's largest value moves: an
 // element that does not change keeps its code, and the noise is that of the changes alone.  v > 0 never becomes 0, for m / eps
 // would follow: it is at least the smallest code, 2^-9 of a scale whose block's largest value lies in [2^7, 2^8].  So a v below
-// some 2^-17 of its block's largest (a gradient smaller by 256 to 362) is held too large, and its steps are smaller for it.  Equal places of
-// all tensors have the same rounding bits in a step.  The step itself takes m and v before their rounding.
+// some 2^-17 of its block's largest (a gradient smaller by 256 to 362) is held too large, and its steps are smaller for it.  Equal
+// places of all tensors have the same rounding bits in a step.  The step itself takes m and v before their rounding.
 //
 // m and v are made of single, separately rounded products and sums, so that the codes are a function of the formula as written.
 //
